@@ -1,0 +1,228 @@
+"""CPU checks of include/tbq_kv.h: rotation plans against 64-bit formulas,
+the page pool, and what the calls refuse (fake, aligned device pointers:
+every check comes before the first HIP call, so nothing is dereferenced)."""
+import ctypes as C
+import random
+
+import pytest
+
+import trailblaze_amd as tb
+from paged_ref import frequencies
+from trailblaze_amd import paged
+
+FAKE = 1 << 20
+
+
+@pytest.mark.parametrize("rot", [8, 64, 128])
+@pytest.mark.parametrize("kw", [dict(), dict(scaling="linear", factor=4.0),
+                                dict(scaling="yarn", factor=4.0, orig_ctx=32768),
+                                dict(scaling="yarn", factor=32.0, orig_ctx=4096, beta_fast=16.0, beta_slow=2.0)])
+def test_rope_plan(rot, kw):
+    r = paged.rope(rot, 1e6, **kw)
+    f, m = frequencies(rot, 1e6, **kw)
+    assert r.rot_dim == rot and r.mscale == pytest.approx(m, rel=1e-15)
+    assert list(r.freq)[:rot // 2] == pytest.approx(f.tolist(), rel=1e-13)   # a few 64-bit roundings
+
+
+def test_rope_plan_factors():
+    fac = [1.0 + 0.5 * j for j in range(32)]
+    r = paged.rope(64, 5e5, layout="interleaved", factors=fac)
+    assert list(r.freq)[:32] == pytest.approx(frequencies(64, 5e5, factors=fac)[0].tolist(), rel=1e-13)
+
+
+@pytest.mark.parametrize("a", [(0, 0, 1e4, 0, 1.0, 0), (12, 0, 1e4, 0, 1.0, 0), (136, 0, 1e4, 0, 1.0, 0),
+                               (64, 2, 1e4, 0, 1.0, 0), (64, 0, 1.0, 0, 1.0, 0), (64, 0, float("inf"), 0, 1.0, 0),
+                               (64, 0, 1e4, 3, 1.0, 0), (64, 0, 1e4, 1, 0.5, 0), (64, 0, 1e4, 2, 4.0, 0),
+                               (64, 0, 1e4, 1, float("nan"), 0)])
+def test_rope_plan_refusals(a):
+    r = paged.Rope()
+    assert tb.lib().tbq_rope_init(C.byref(r), *a, 0.0, 0.0, None) == 0
+    assert b"tbq_rope_init" in tb.lib().tbq_last_error()
+
+
+# ---- pool --------------------------------------------------------------------
+def test_pool_against_a_model():
+    """Random calls against a plain list of holders."""
+    rng = random.Random(4)
+    n = 40
+    pool, model = paged.PagePool(n), [0] * n
+    for _ in range(2000):
+        op, used = rng.randrange(4), [i for i in range(n) if model[i]]
+        if op == 0:
+            m = rng.randrange(0, 8)
+            free = [i for i in range(n) if not model[i]]
+            if m > len(free):
+                with pytest.raises(tb.TbqError):
+                    pool.alloc(m)
+            else:
+                got = pool.alloc(m)
+                assert got == free[:m]
+                for i in got:
+                    model[i] = 1
+        elif op == 1 and used:
+            some = [rng.choice(used) for _ in range(3)]
+            pool.share(some)
+            for i in some:
+                model[i] += 1
+        elif op == 2 and used:
+            some = [rng.choice(used) for _ in range(rng.randrange(1, 5))]
+            if all(some.count(i) <= model[i] for i in some):
+                pool.release(some)
+                for i in some:
+                    model[i] -= 1
+            else:
+                with pytest.raises(tb.TbqError):
+                    pool.release(some)
+        elif op == 3 and rng.random() < 0.2:
+            most = rng.choice([0, 3, n])
+            moves = pool.defrag(most)
+            assert len(moves) <= most
+            for s, d in moves:
+                assert model[s] and not model[d] and d < s
+                model[d], model[s] = model[s], 0
+            if len(moves) < most:
+                assert all(model[:sum(m > 0 for m in model)])
+        assert pool.free_pages() == model.count(0)
+        assert [pool.holders(i) for i in range(n)] == model
+    pool.close()
+
+
+@pytest.mark.parametrize("positions,page", [(0, 16), (1, 16), (16, 16), (40, 16), (48, 16)])
+def test_pool_fork(positions, page):
+    pool = paged.PagePool(8)
+    n = -(-positions // page)
+    mine = pool.alloc(n)
+    child, copy = pool.fork(positions, page, mine)
+    if positions % page:
+        assert copy == (mine[-1], n) and child == mine[:-1] + [n]
+        assert pool.holders(mine[-1]) == 1 and pool.holders(n) == 1
+    else:
+        assert copy is None and child == mine
+    assert all(pool.holders(p) == 2 for p in mine[:positions // page])
+    pool.release(child)
+    pool.release(mine)
+    assert pool.free_pages() == 8
+
+
+def test_pool_refusals():
+    with pytest.raises(tb.TbqError):
+        paged.PagePool(0)
+    pool = paged.PagePool(2)
+    mine = pool.alloc(2)
+    with pytest.raises(tb.TbqError):        # no page for the partly filled one, and nothing shared
+        pool.fork(17, 16, mine)
+    assert [pool.holders(p) for p in (0, 1, 2, -1)] == [1, 1, -1, -1]
+    for bad in ([2], [-1], [0, 0]):
+        with pytest.raises(tb.TbqError):
+            pool.release(bad)
+    with pytest.raises(tb.TbqError):
+        pool.share([5])
+    assert pool.defrag(4) == [] and pool.free_pages() == 0
+
+
+# ---- refusals ------------------------------------------------------------------
+def cache(**kw):
+    d = dict(n_layers=2, n_pages=8, n_kv_heads=2, page_size=16, head_dim=128, type=1, k=FAKE, v=FAKE)
+    d.update(kw)
+    return paged.KvCache(*[d[n] for n, _ in paged.KvCache._fields_])
+
+
+def batch(**kw):
+    d = dict(n_seqs=2, n_tokens=3, max_pages=4, max_q=0, max_kv=0, q_start=FAKE, kv_len=FAKE, page_table=FAKE)
+    d.update(kw)
+    return paged.KvBatch(*[d[n] for n, _ in paged.KvBatch._fields_])
+
+
+def refused(ok, words):
+    assert ok == 0
+    msg = tb.lib().tbq_last_error().decode()
+    assert words in msg, msg
+
+
+CACHES = [(dict(type=0), "cache type"), (dict(type=12), "cache type"), (dict(head_dim=96), "head_dim"),
+          (dict(page_size=24), "page_size"), (dict(page_size=8), "page_size"), (dict(n_layers=0), "layers"),
+          (dict(n_pages=0), "pages"), (dict(n_kv_heads=0), "kv heads"), (dict(k=None), "null or misaligned"),
+          (dict(v=FAKE + 8), "null or misaligned")]
+BATCHES = [(dict(n_seqs=-1), "sequences"), (dict(n_tokens=-1), "tokens"), (dict(max_pages=0), "pages"),
+           (dict(max_q=-1), "max_q"), (dict(q_start=None), "null batch"), (dict(page_table=None), "null batch")]
+
+
+def append(c, b, layer=0, heads=4, rope=None, in_type=1, q=FAKE, qs=512, k=FAKE, ks=256, v=FAKE, vs=256, q_type=1,
+           q_out=2 * FAKE, qn=None):
+    return tb.lib().tbq_kv_append(C.byref(c), layer, C.byref(b), heads, None if rope is None else C.byref(rope), qn, None,
+                                  1e-6, None, in_type, q, qs, k, ks, v, vs, q_type, q_out, None)
+
+
+def attn(c, b, layer=0, heads=4, q_type=1, q=FAKE, qs=512, out=FAKE, window=0, sinks=0, scale=0.0, ws=FAKE,
+         wsb=1 << 40):
+    return tb.lib().tbq_attn_paged(C.byref(c), layer, C.byref(b), heads, q_type, q, qs, out, window, sinks, scale, ws,
+                                   wsb, None)
+
+
+@pytest.mark.parametrize("kw,words", CACHES)
+def test_cache_refusals(kw, words):
+    c, b = cache(**kw), batch()
+    refused(append(c, b), words)
+    refused(attn(c, b), words)
+    one = (C.c_int * 1)(0)
+    refused(tb.lib().tbq_kv_copy_pages(C.byref(c), one, one, 1, None), words)
+    refused(tb.lib().tbq_kv_compact(C.byref(c), 1, FAKE, 4, FAKE, FAKE, None), words)
+    assert tb.lib().tbq_attn_paged_workspace_size(C.byref(c), C.byref(b), 4, 1) == 0
+
+
+@pytest.mark.parametrize("kw,words", BATCHES)
+def test_batch_refusals(kw, words):
+    refused(append(cache(), batch(**kw)), words)
+    refused(attn(cache(), batch(**kw)), words)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(layer=2), "layer"), (dict(layer=-1), "layer"), (dict(in_type=30), "in_type"), (dict(in_type=12), "in_type"),
+    (dict(q_type=0), "q_type"), (dict(q_type=30), "q_type"), (dict(q=None), "go together"), (dict(q_out=None), "go together"),
+    (dict(heads=0), "n_heads"), (dict(k=None), "null k or v"), (dict(v=FAKE + 2), "misaligned"), (dict(q=FAKE + 8), "misaligned"),
+    (dict(qn=FAKE + 4), "misaligned"), (dict(ks=260), "strides"), (dict(vs=128), "shorter"), (dict(qs=504), "shorter"),
+    (dict(q_out=FAKE, qs=1024), "q_out is q"), (dict(in_type=0, q_out=FAKE), "q_out is q"),
+    (dict(rope=paged.Rope(12, 0, 1.0)), "rot_dim"), (dict(rope=paged.Rope(136, 0, 1.0)), "rot_dim"),
+    (dict(rope=paged.Rope(64, 7, 1.0)), "rope layout")])
+def test_append_refusals(kw, words):
+    refused(append(cache(), batch(), **kw), words)
+
+
+def test_append_rotation_longer_than_the_head():
+    refused(append(cache(head_dim=64), batch(), rope=paged.rope(128, 1e4)), "rot_dim")
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(layer=2), "layer"), (dict(heads=3), "n_heads"), (dict(heads=0), "n_heads"), (dict(q_type=30), "q_type"),
+    (dict(window=-1), "window"), (dict(sinks=-1), "sinks"), (dict(scale=-1.0), "scale"), (dict(scale=float("nan")), "scale"),
+    (dict(scale=float("inf")), "scale"), (dict(q=None), "null"), (dict(out=FAKE + 8), "misaligned"), (dict(qs=500), "q_stride"),
+    (dict(qs=256), "q_stride")])
+def test_attention_refusals(kw, words):
+    refused(attn(cache(), batch(), **kw), words)
+
+
+def test_attention_f32_needs_an_f16_cache():
+    refused(attn(cache(type=30), batch(), q_type=0), "q_type")
+
+
+@pytest.mark.parametrize("src,dst,words", [([0], [8], "pair 0"), ([-1], [1], "pair 0"), ([0, 1], [2, 2], "written twice"),
+                                           ([0, 1], [1, 2], "read and written"), ([3], [3], "read and written")])
+def test_copy_refusals(src, dst, words):
+    a = lambda v: (C.c_int * len(v))(*v)   # noqa: E731
+    refused(tb.lib().tbq_kv_copy_pages(C.byref(cache()), a(src), a(dst), len(src), None), words)
+
+
+def test_compact_refusals():
+    c = cache()
+    refused(tb.lib().tbq_kv_compact(C.byref(c), -1, FAKE, 4, FAKE, FAKE, None), "sequences")
+    refused(tb.lib().tbq_kv_compact(C.byref(c), 1, FAKE, 0, FAKE, FAKE, None), "pages")
+    refused(tb.lib().tbq_kv_compact(C.byref(c), 1, None, 4, FAKE, FAKE, None), "null")
+
+
+def test_nothing_to_do_is_done():
+    """Empty batches and lists, without a device."""
+    c = cache()
+    for b in (batch(n_seqs=0), batch(n_tokens=0)):
+        assert append(c, b) == 1 and attn(c, b) == 1
+    assert tb.lib().tbq_kv_copy_pages(C.byref(c), None, None, 0, None) == 1
+    assert tb.lib().tbq_kv_compact(C.byref(c), 0, None, 4, None, None, None) == 1

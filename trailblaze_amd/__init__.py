@@ -25,8 +25,8 @@ TBQ_MOE_I8 = 2
 TBQ_MV_AUTO, TBQ_MV_FMA, TBQ_MV_INTDOT, TBQ_MV_KQ = 0, 1, 2, 3
 
 # (name, restype, argtypes) for every symbol declared in include/tbq.h,
-# include/tbq_gguf.h and include/tb_gguf_dequant.h.
-_vp, _i, _sz, _f = C.c_void_p, C.c_int, C.c_size_t, C.c_float
+# include/tbq_kv.h, include/tbq_gguf.h and include/tb_gguf_dequant.h.
+_vp, _i, _sz, _f, _d, _ll = C.c_void_p, C.c_int, C.c_size_t, C.c_float, C.c_double, C.c_longlong
 SYMBOLS = {
     # include/tbq.h
     "tbq_init": (_i, []),
@@ -61,6 +61,22 @@ SYMBOLS = {
     "tbq_expf_device": (_i, [_vp, _vp, _sz, _vp]),
     "tbq_expf_host": (_f, [_f]),
     "tbq_gemm_plan": (_i, [_i, _i, _i, _i, _i, _vp]),
+    # include/tbq_kv.h
+    "tbq_rope_init": (_i, [_vp, _i, _i, _d, _i, _d, _i, _d, _d, _vp]),
+    "tbq_kv_append": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp, _f, _vp, _i, _vp, _ll, _vp, _ll, _vp, _ll, _i, _vp, _vp]),
+    "tbq_attn_paged_workspace_size": (_sz, [_vp, _vp, _i, _i]),
+    "tbq_attn_paged": (_i, [_vp, _i, _vp, _i, _i, _vp, _ll, _vp, _i, _i, _f, _vp, _sz, _vp]),
+    "tbq_kv_copy_pages": (_i, [_vp, _vp, _vp, _i, _vp]),
+    "tbq_kv_compact": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp]),
+    "tbq_kv_pool_create": (_vp, [_i]),
+    "tbq_kv_pool_destroy": (None, [_vp]),
+    "tbq_kv_pool_free_pages": (_i, [_vp]),
+    "tbq_kv_pool_holders": (_i, [_vp, _i]),
+    "tbq_kv_pool_alloc": (_i, [_vp, _i, _vp]),
+    "tbq_kv_pool_share": (_i, [_vp, _i, _vp]),
+    "tbq_kv_pool_release": (_i, [_vp, _i, _vp]),
+    "tbq_kv_pool_fork": (_i, [_vp, _i, _i, _vp, _vp, _vp]),
+    "tbq_kv_pool_defrag": (_i, [_vp, _i, _vp, _vp]),
     # include/tbq_gguf.h
     "tbq_gguf_open": (_vp, [C.c_char_p]),
     "tbq_gguf_close": (None, [_vp]),

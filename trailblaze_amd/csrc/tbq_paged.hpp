@@ -1,0 +1,115 @@
+// tbq_paged.hpp -- what the kernels over the paged key/value cache share
+// (include/tbq_kv.h): the arguments that describe cache and batch, and the
+// lookups of a token's sequence and of a position's row.
+#pragma once
+
+#include "tbq_device.hpp"
+#include "../../include/tbq_kv.h"
+
+namespace tbq {
+
+// One layer of a cache, and a batch.
+struct PgArgs {
+    void *k, *v;           // the layer's [n_pages][NKV][1 << shift][D]
+    int n_pages, NKV, shift;
+    int n_seqs, n_tokens, max_pages, max_q, max_kv;
+    const int *q_start, *kv_len, *table;
+};
+
+struct PgRope {
+    int rot, interleaved;
+    float mscale;
+    double turns[64];      // freq[j] / 2 pi
+};
+
+inline void pg_rope(const tbq_rope &r, PgRope &o) {
+    o.rot = r.rot_dim;
+    o.interleaved = r.layout == TBQ_ROPE_INTERLEAVED;
+    o.mscale = (float)r.mscale;
+    for (int j = 0; j < r.rot_dim / 2; j++) o.turns[j] = r.freq[j] * 0.15915494309189533577;
+}
+
+struct PgAppend {
+    PgArgs pg;
+    const void *q, *k, *v;             // heads of row t side by side at base + t * stride
+    long long qs, ks, vs;
+    void *qo;                          // [n_tokens][NQ][D]
+    const float *qn, *kn;              // norm weights, or null
+    const int *positions;              // rotation positions, or null
+    float eps;
+    int NQ;                            // 0: k and v only
+    // the dense prefill's products: row t is scaled by 1 / rs[t], and the rows
+    // are nsl split-K slices (slice z at base + z * slstride)
+    const float *rs;
+    int nsl;
+    long long slstride;
+    PgRope rope;
+};
+
+struct PgAttn {
+    PgArgs pg;
+    const void *q;         // heads of row t side by side at base + t * stride
+    long long qs;
+    void *out;             // [n_tokens][NQ][D]
+    int NQ, window, sinks;
+    float scale;           // of q . k, times log2(e): the softmax is in powers of two
+};
+
+constexpr int PG_PAIRS = 128;   // page copies per launch, 1 KiB of kernel arguments
+struct PgPairs {
+    int src[PG_PAIRS], dst[PG_PAIRS];
+};
+
+// The sequence of token row t: the number of sequences that end at or before
+// it (n_seqs: none).  The whole wave calls it; uniform.
+__device__ __forceinline__ int pg_seq_of(const int *__restrict__ q_start, int n_seqs, int t) {
+    const int lane = threadIdx.x & 63;
+    int s = 0;
+    for (int i = 0; i < n_seqs; i += 64) {
+        const bool ends = i + lane < n_seqs && q_start[i + lane + 1] <= t;
+        s += __builtin_popcountll(__builtin_amdgcn_ballot_w64(ends));
+    }
+    return s;
+}
+
+// The page of position p (>= 0) of sequence s, -1 where it has none.
+__device__ __forceinline__ int pg_page(const PgArgs &a, int s, int p) {
+    const int e = p >> a.shift;
+    if (e >= a.max_pages) return -1;
+    const int page = a.table[(long long)s * a.max_pages + e];
+    return (unsigned)page < (unsigned)a.n_pages ? page : -1;
+}
+
+// Elements before row (p mod page size) of kv head h in a page.
+template <int D>
+__device__ __forceinline__ long long pg_row(const PgArgs &a, int page, int h, int p) {
+    return ((((long long)page * a.NKV + h) << a.shift) + (p & ((1 << a.shift) - 1))) * D;
+}
+
+typedef uint32_t pg_u4 __attribute__((ext_vector_type(4)));   // 16 bytes moved as they are
+typedef __bf16 pg_bf16;
+typedef _Float16 pg_f16;
+
+// Four elements as floats, and back (one rounding, to nearest even).
+template <typename T>
+__device__ __forceinline__ float4 pg_ld4(const T *p) {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    const v4 v = *reinterpret_cast<const v4 *>(p);
+    return make_float4((float)v[0], (float)v[1], (float)v[2], (float)v[3]);
+}
+template <typename T>
+__device__ __forceinline__ void pg_st4(T *p, float4 f) {
+    typedef T v4 __attribute__((ext_vector_type(4)));
+    *reinterpret_cast<v4 *>(p) = v4{(T)f.x, (T)f.y, (T)f.z, (T)f.w};
+}
+
+// Launchers (tbq_paged.hip, tbq_paged_attn.hip).
+hipError_t launch_pg_append(const PgAppend &a, int D, int in_type, int q_type, int c_type, hipStream_t st);
+hipError_t launch_pg_copy(void *k, void *v, int n_layers, long long pbytes, long long lbytes, const PgPairs &pairs, int n,
+                          hipStream_t st);
+hipError_t launch_pg_compact(void *k, void *v, int n_layers, long long lelems, int D, const PgArgs &a, const int *keep_start,
+                             const int *keep, hipStream_t st);
+size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32);
+hipError_t launch_pg_attn(const PgAttn &a, int D, int q_type, int c_type, void *ws, size_t ws_bytes, hipStream_t st);
+
+}  // namespace tbq
