@@ -184,6 +184,7 @@ static int check_attn(const char *who, const tbq_kv_cache *c, const tbq_kv_batch
     if (!check_cache(who, c) || !check_batch(who, b)) return 0;
     if (n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv_heads)
         return fail("%s: n_heads %d, a multiple of the %d kv heads", who, n_heads, c->n_kv_heads);
+    if ((long long)b->n_tokens * n_heads >= 1ll << 30) return fail("%s: %d tokens of %d heads", who, b->n_tokens, n_heads);
     if (q_type != c->type && !(q_type == TBQ_KV_F32 && c->type == TBQ_KV_F16))
         return fail("%s: q_type %d with cache type %d (the cache's type, or F32 with an F16 cache)", who, q_type, c->type);
     return 1;
@@ -213,10 +214,10 @@ int tbq_attn_paged(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int 
     a.qs = qs;
     a.out = out;
     a.NQ = n_heads;
-    a.window = window;
-    a.sinks = window > 0 ? sinks : 0;
+    a.window = window < (1 << 30) ? window : 1 << 30;   // differences of positions stay in 32 bits
+    a.sinks = window > 0 ? (sinks < (1 << 30) ? sinks : 1 << 30) : 0;
     a.scale = (scale > 0 ? scale : 1.0f / sqrtf((float)c->head_dim)) * 1.4426950408889634f;
-    return hip_ok(launch_pg_attn(a, c->head_dim, q_type, c->type, ws, ws_bytes, S(stream)), "paged attention launch");
+    return hip_ok(launch_pg_attn(a, c->head_dim, q_type, c->type, ws, S(stream)), "paged attention launch");
 }
 
 int tbq_kv_copy_pages(const tbq_kv_cache *c, const int *src, const int *dst, int n, void *stream) {

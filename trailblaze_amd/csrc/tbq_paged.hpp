@@ -110,6 +110,6 @@ hipError_t launch_pg_copy(void *k, void *v, int n_layers, long long pbytes, long
 hipError_t launch_pg_compact(void *k, void *v, int n_layers, long long lelems, int D, const PgArgs &a, const int *keep_start,
                              const int *keep, hipStream_t st);
 size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32);
-hipError_t launch_pg_attn(const PgAttn &a, int D, int q_type, int c_type, void *ws, size_t ws_bytes, hipStream_t st);
+hipError_t launch_pg_attn(const PgAttn &a, int D, int q_type, int c_type, void *ws, hipStream_t st);
 
 }  // namespace tbq

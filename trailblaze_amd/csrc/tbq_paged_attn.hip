@@ -1,63 +1,852 @@
 // tbq_paged_attn.hip -- causal attention of new tokens over the paged
 // key/value cache (include/tbq_kv.h) on gfx950.
+//
+// The query heads that share a kv head are rows of one product: row r of a
+// sequence's kv head is token r / G, head r % G of its G.  Sequences with few
+// rows (single tokens) go to k_pg_attn_rows, bound by the cache's bytes; the
+// others to k_pg_attn_chunk, bound by MFMA and the softmax.  Both are one pass
+// over the visible positions with the softmax's running maximum and sum (in
+// powers of two), and both form S^T = K Q^T, so that a lane holds scores of one
+// row only and the probabilities are, without any exchange, the operand of
+// O^T += V^T P^T when the products' positions are taken in the order that the
+// accumulators have.
+//
+// F32 rows (HL): q, scaled by the power of two that puts its largest element in
+// [2^13, 2^14), and the probabilities are each taken as two halves, x = hi + lo,
+// which keeps ~22 bits; the keys and values are halves already.  16-bit rows
+// round the probabilities to the cache's type.  Half probabilities are scaled by
+// 2^14, so those that a half cannot hold are below 2^-38 of the largest.
+//
+// What a row does not see must not reach it, NaN and infinities included.
+// Scores are replaced before the maximum.  In the product with V an unseen
+// position's weight is 0, but 0 times a NaN is a NaN: values of positions that
+// no row of the block sees are made zero in the tiles on the edges, and a row
+// whose outputs are not all finite at the end is formed again in a way that
+// multiplies only what the row sees.
+#include <algorithm>
+#include <type_traits>
+
+#include "tbq_dma.hpp"
 #include "tbq_kernels.h"
 #include "tbq_paged.hpp"
 
 namespace tbq {
 
-// One wave per token and query head, a position at a time with the running
-// maximum and sum of the softmax: lane l holds elements l and l + 64 of the
-// head.
+constexpr float PG_LOW = -3.402823466e38f;   // the running maximum before any score
+
+template <typename T>
+struct PgVec;
+template <>
+struct PgVec<pg_f16> {
+    typedef pg_f16 h8 __attribute__((ext_vector_type(8)));
+    static constexpr float SHIFT = 14.f;
+};
+template <>
+struct PgVec<pg_bf16> {
+    typedef pg_bf16 h8 __attribute__((ext_vector_type(8)));
+    static constexpr float SHIFT = 0.f;
+};
+typedef float pg_f4 __attribute__((ext_vector_type(4)));
+typedef float pg_f16x __attribute__((ext_vector_type(16)));
+
+__device__ __forceinline__ pg_f4 pg_mfma16(PgVec<pg_f16>::h8 a, PgVec<pg_f16>::h8 b, pg_f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ pg_f4 pg_mfma16(PgVec<pg_bf16>::h8 a, PgVec<pg_bf16>::h8 b, pg_f4 c) {
+    return __builtin_amdgcn_mfma_f32_16x16x32_bf16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ pg_f16x pg_mfma32(PgVec<pg_f16>::h8 a, PgVec<pg_f16>::h8 b, pg_f16x c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0);
+}
+__device__ __forceinline__ pg_f16x pg_mfma32(PgVec<pg_bf16>::h8 a, PgVec<pg_bf16>::h8 b, pg_f16x c) {
+    return __builtin_amdgcn_mfma_f32_32x32x16_bf16(a, b, c, 0, 0, 0);
+}
+
+// The tiles of TS positions that tokens at plo .. phi see any part of: first
+// the sinks' tiles in front of the window, then the window's.
+struct PgTiles {
+    int sinks, first, n;
+    __device__ __forceinline__ int at(int it) const { return it < sinks ? it : first + it - sinks; }
+};
+template <int TS>
+__device__ __forceinline__ PgTiles pg_tiles(int plo, int phi, int window, int sinks, int max_kv) {
+    phi = min(phi, max_kv - 1);
+    if (phi < 0) return {0, 0, 0};
+    const int lo = window > 0 ? max(0, plo - window + 1) : 0;
+    if (lo > phi) return {0, 0, 0};
+    const int first = lo / TS, ns = min((min(sinks, phi + 1) + TS - 1) / TS, first);
+    return {ns, first, ns + phi / TS - first + 1};
+}
+
+// Bit k: whether position k0 + k of 64 is in (lo, hi] or, up to hi, below sinks.
+__device__ __forceinline__ uint64_t pg_upto(int k) { return k < 0 ? 0ull : k >= 63 ? ~0ull : (2ull << k) - 1ull; }
+__device__ __forceinline__ uint64_t pg_seen(int k0, int lo, int hi, int sinks) {
+    return pg_upto(hi - k0) & (~pg_upto(lo - k0) | pg_upto(sinks - 1 - k0));
+}
+// All ones where bit c of m is set.
+__device__ __forceinline__ uint32_t pg_ones(uint32_t m, int c) { return (uint32_t)__builtin_amdgcn_sbfe((int)m, c, 1); }
+// s where its mask is ones, -infinity where it is 0.
+__device__ __forceinline__ float pg_hide(float s, uint32_t ones) {
+    return __builtin_bit_cast(float, (__builtin_bit_cast(uint32_t, s) & ones) | (0xFF800000u & ~ones));
+}
+
+// The page of a 16-position block, -1 where there is none to read: blocks past
+// the last visible position are not looked up.
+__device__ __forceinline__ int pg_block_page(const PgArgs &a, int s, int pos, int last) {
+    return pos <= last ? pg_page(a, s, pos) : -1;
+}
+
+// Power of two that puts a row's largest element in [2^13, 2^14).
+__device__ __forceinline__ int pg_row_shift(float amax) {
+    int e = 0;
+    frexpf(amax, &e);
+    const int sh = amax > 0.f ? 14 - e : 0;
+    return min(max(sh, -126), 126);
+}
+
+// The halves of v, or zeros, by a mask of ones or 0.
+template <typename V>
+__device__ __forceinline__ V pg_keep(V v, uint32_t ones) {
+    typedef uint32_t w __attribute__((ext_vector_type(sizeof(V) / 4)));
+    w x = __builtin_bit_cast(w, v);
+#pragma unroll
+    for (int i = 0; i < (int)(sizeof(V) / 4); i++) x[i] &= ones;
+    return __builtin_bit_cast(V, x);
+}
+
+// One row by one wave, 64 positions at a time, from what the row sees only: lane
+// i scores position i of the tile, then the wave adds p V for the seen positions
+// in turn, lane l the dims l and l + 64.  *m, *l: maximum and sum.
 template <typename TA, typename TC, int D>
-__global__ __launch_bounds__(64) void k_pg_attn_row(const PgAttn a) {
-    const int h = blockIdx.x, t = blockIdx.y, lane = threadIdx.x;
+__device__ __forceinline__ void pg_slow_row(const PgArgs &pg, const TA *q, float cs, int s, int kvh, int pos, int back,
+                                         int sinks, PgTiles tiles, int it0, int it1, float (&o)[D / 64], float *m,
+                                         float *l) {
+    const int lane = threadIdx.x & 63, last = min(pos, pg.max_kv - 1);
+#pragma unroll
+    for (int i = 0; i < D / 64; i++) o[i] = 0.f;
+    *m = PG_LOW;
+    *l = 0.f;
+    for (int it = it0; it < it1; it++) {
+        const int k0 = tiles.at(it) * 64, key = k0 + lane;
+        const int page = pg_block_page(pg, s, key, last);
+        const long long at = pg_row<D>(pg, max(page, 0), kvh, key);
+        const bool sees = page >= 0 && ((pg_seen(k0, pos - back, last, sinks) >> lane) & 1);
+        float dot = 0.f;
+        for (int d = 0; d < D; d += 4) {
+            const float4 x = pg_ld4(q + d), y = pg_ld4((const TC *)pg.k + at + d);
+            dot = fmaf(x.x, y.x, fmaf(x.y, y.y, fmaf(x.z, y.z, fmaf(x.w, y.w, dot))));
+        }
+        dot = sees ? dot * cs : -__builtin_huge_valf();
+        const float mn = fmaxf(*m, wave_max(dot)), corr = __builtin_amdgcn_exp2f(*m - mn);
+        const float p = __builtin_amdgcn_exp2f(dot - mn);
+        *m = mn;
+        *l = *l * corr + group_sum<64>(p);
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) o[i] *= corr;
+        for (unsigned long long left = __builtin_amdgcn_ballot_w64(sees); left; left &= left - 1) {
+            const int k = __builtin_ctzll(left);
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), k));
+            const long long row = pg_row<D>(pg, __builtin_amdgcn_readlane(page, k), kvh, k0 + k);
+#pragma unroll
+            for (int i = 0; i < D / 64; i++) o[i] = fmaf(w, (float)((const TC *)pg.v)[row + lane + 64 * i], o[i]);
+        }
+    }
+}
+
+constexpr int pg_rec(int D) { return D + 4; }   // floats of a split's record: D outputs, max, sum, padding
+
+// ---------------------------------------------------------------------------
+// Few rows.  A workgroup has one sequence, one kv head, RB = 16 rows (8 as F32:
+// their hi halves are the MFMA's columns 0-7, their lo halves 8-15) and a range
+// of tiles of 32 positions, dealt to its four waves, which keep maxima, sums
+// and outputs of their own until the end.  K and V go from memory to registers
+// only: lane l holds row l % 16 of each 16 keys as the MFMA's A operand wants
+// them; of V it loads 8 (4) dims, D / 16 * (l % 16) on, of the 8 positions
+// whose probabilities it computed, and the 8 x 8 halves, transposed in
+// registers, are the A operands of D / 16 products, product j giving the dims
+// congruent to j.  A tile's loads are issued a tile ahead.
+// ---------------------------------------------------------------------------
+constexpr int PR_WAVES = 4, PR_TS = 32;
+#ifndef TBQ_PG_RMAX
+#define TBQ_PG_RMAX 16
+#endif
+constexpr int PR_MAX = TBQ_PG_RMAX;   // rows up to which a sequence is one of few rows
+
+template <typename TC, int D, bool HL>
+__global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pg_attn_rows(
+    const PgAttn a, int nrb, int tps, int nsplit, float *__restrict__ part) {
+    typedef typename PgVec<TC>::h8 h8;
+    typedef TC hv __attribute__((ext_vector_type(D / 16)));
+    constexpr int RB = HL ? 8 : 16, NS = D / 32, ND = D / 16, OST = D + 4;
+    constexpr float SH = PgVec<TC>::SHIFT;
+    __shared__ __attribute__((aligned(16))) float os[PR_WAVES][16 * OST];
+    __shared__ float ms[PR_WAVES][16], ls[PR_WAVES][16];
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, h = lane >> 4;
+    const int kvh = blockIdx.x % a.pg.NKV, r0 = blockIdx.x / a.pg.NKV * RB, s = blockIdx.z, G = a.NQ / a.pg.NKV;
+    const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
+    if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
+    const int rows = qn * G;
+    if (rows > PR_MAX || r0 >= rows) return;
+    const int base = a.pg.kv_len[s] - qn;   // position of the first token
+    const int t0 = r0 / G, t1 = (min(r0 + RB, rows) - 1) / G;   // the block's tokens
+    const int plo = base + t0, phi = base + t1, last = min(phi, a.pg.max_kv - 1);
+    const int back = a.window > 0 ? a.window : 0x40000000;   // a token at p sees the positions > p - back
+    const PgTiles tiles = pg_tiles<PR_TS>(plo, phi, a.window, a.sinks, a.pg.max_kv);
+    const int z = blockIdx.y, nz = (tiles.n + tps - 1) / tps, it0 = z * tps, it1 = min(it0 + tps, tiles.n);
+    if (z > 0 && it0 >= it1) return;
+    const int row = r0 + (HL ? li & 7 : li), rc = min(row, rows - 1), tok = rc / G, pos = base + tok;
+    // Q^T's columns
+    h8 qf[NS];
+    float cs = a.scale;
+    {
+        const long long off = (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * h;
+        if constexpr (HL) {
+            const float *q = (const float *)a.q + off;
+            float4 x[NS][2];
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float4 v = x[i][j] = pg_ld4(q + 32 * i + 4 * j);
+                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                }
+            mx = swap32_max(swap16_max(mx));
+            const int sh = pg_row_shift(mx);
+            const float f = ldexpf(1.f, sh);
+            cs *= ldexpf(1.f, -sh);
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float v[4] = {x[i][j].x * f, x[i][j].y * f, x[i][j].z * f, x[i][j].w * f};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        const TC hi = (TC)v[e];
+                        qf[i][4 * j + e] = li < 8 ? hi : (TC)(v[e] - (float)hi);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; i++) qf[i] = *reinterpret_cast<const h8 *>((const TC *)a.q + off + 32 * i);
+        }
+    }
+    const long long hstride = (long long)D << a.pg.shift;   // elements of a kv head in a page
+    const uint32_t koff = (uint32_t)(li * D + 8 * h), voff = (uint32_t)(4 * h * D + ND * li);
+    int pages = -1;   // lane i: the page of block i % 2 of the wave's tile i / 2 (of 32 tiles)
+    auto tile_at = [&](int n) { return tiles.at(it0 + wave + PR_WAVES * n) * PR_TS; };
+    auto page_of = [&](int n, int b) { return __builtin_amdgcn_readlane(pages, 2 * (n & 31) + b); };
+    const int nt = (it1 - it0 - wave + PR_WAVES - 1) / PR_WAVES;   // this wave's tiles
+    auto look_up = [&](int n) {
+        const int k = n + (lane >> 1);
+        pages = k < nt ? pg_block_page(a.pg, s, tile_at(k) + 16 * (lane & 1), last) : -1;
+    };
+    h8 kf[2][2][NS];
+    hv vf[2][8];
+    auto load = [&](int buf, int n) {
+        if ((n & 31) == 0) look_up(n);
+        const int k0 = tile_at(n);
+#pragma unroll
+        for (int b = 0; b < 2; b++) {
+            const int in = (k0 + 16 * b) & ((1 << a.pg.shift) - 1);
+            const long long off = ((long long)max(page_of(n, b), 0) * a.pg.NKV + kvh) * hstride + (long long)in * D;
+            const TC *kp = (const TC *)a.pg.k + off, *vp = (const TC *)a.pg.v + off;
+#pragma unroll
+            for (int i = 0; i < NS; i++) kf[buf][b][i] = *reinterpret_cast<const h8 *>(kp + koff + 32 * i);
+#pragma unroll
+            for (int i = 0; i < 4; i++) vf[buf][4 * b + i] = *reinterpret_cast<const hv *>(vp + voff + i * D);
+        }
+    };
+    pg_f4 o[ND];
+    float m, l;
+    // b: whether the block has a page
+    auto compute = [&](int buf, int n, bool safe) {
+        const int k0 = tile_at(n);
+        const bool pg0 = page_of(n, 0) >= 0, pg1 = page_of(n, 1) >= 0;
+        const bool whole = pg0 && pg1 && k0 + PR_TS - 1 <= min(plo, a.pg.max_kv - 1) &&
+                           (k0 > phi - back || k0 + PR_TS <= a.sinks);
+        const uint32_t has = (pg0 ? 0xFFFFu : 0u) | (pg1 ? 0xFFFF0000u : 0u);
+        // the lane's positions that tokens at lo .. hi see: element e is bit 16 (e / 4) + e % 4
+        auto seen = [&](int lo, int hi) {
+            return ((uint32_t)pg_seen(k0, lo - back, min(hi, last), a.sinks) & has) >> (4 * h);
+        };
+        pg_f4 sc[2] = {pg_f4{}, pg_f4{}};
+#pragma unroll
+        for (int i = 0; i < NS; i++)
+#pragma unroll
+            for (int b = 0; b < 2; b++) sc[b] = pg_mfma16(kf[buf][b][i], qf[i], sc[b]);
+        if constexpr (HL) {
+#pragma unroll
+            for (int b = 0; b < 2; b++)
+#pragma unroll
+                for (int r = 0; r < 4; r++) sc[b][r] += dpp_f32<0x128>(sc[b][r]);   // row_ror:8
+        }
+        auto bit = [](int e) { return 16 * (e / 4) + e % 4; };
+        if (!whole) {
+            const uint32_t mine = seen(pos, pos);
+#pragma unroll
+            for (int e = 0; e < 8; e++) sc[e / 4][e % 4] = pg_hide(sc[e / 4][e % 4], pg_ones(mine, bit(e)));
+        }
+        float mx = sc[0][0];
+#pragma unroll
+        for (int e = 1; e < 8; e++) mx = fmaxf(mx, sc[e / 4][e % 4]);
+        mx = swap32_max(swap16_max(mx)) * cs;
+        if (__builtin_amdgcn_ballot_w64(mx > m)) {
+            const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
+            m = mn;
+            l *= corr;
+#pragma unroll
+            for (int j = 0; j < ND; j++) o[j] *= corr;
+        }
+        h8 pf;
+        const float mb = SH - m;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][e % 4], cs, mb));
+            l += p;
+            const TC hi = (TC)p;
+            if constexpr (HL) pf[e] = li < 8 ? hi : (TC)(p - (float)hi);
+            else pf[e] = hi;
+        }
+        if (!whole) {   // values that no row of the block sees
+            const uint32_t any = seen(plo, phi);
+#pragma unroll
+            for (int e = 0; e < 8; e++) vf[buf][e] = pg_keep(vf[buf][e], pg_ones(any, bit(e)));
+        }
+        if (whole || !safe) {
+#pragma unroll
+            for (int j = 0; j < ND; j++) {
+                h8 v;
+#pragma unroll
+                for (int e = 0; e < 8; e++) v[e] = vf[buf][e][j];
+                o[j] = pg_mfma16(v, pf, o[j]);
+            }
+        } else {
+            for (int t = t0; t <= t1; t++) {
+                const uint32_t its = seen(base + t, base + t);
+                hv w[8];
+#pragma unroll
+                for (int e = 0; e < 8; e++) w[e] = pg_keep(vf[buf][e], pg_ones(its, bit(e)));
+#pragma unroll
+                for (int j = 0; j < ND; j++) {
+                    h8 v;
+#pragma unroll
+                    for (int e = 0; e < 8; e++) v[e] = w[e][j];
+                    const pg_f4 u = pg_mfma16(v, pf, o[j]);
+                    if (tok == t) o[j] = u;
+                }
+            }
+        }
+    };
+    for (int safe = 0;; safe = 1) {
+        m = PG_LOW;
+        l = 0.f;
+#pragma unroll
+        for (int j = 0; j < ND; j++) o[j] = pg_f4{};
+        if (nt > 0) load(0, 0);
+        for (int n = 0; n < nt; n += 2) {
+            if (n + 1 < nt) load(1, n + 1);
+            compute(0, n, safe);
+            if (n + 1 >= nt) break;
+            if (n + 2 < nt && ((n + 2) & 31) != 0) load(0, n + 2);
+            compute(1, n + 1, safe);
+            if (n + 2 < nt && ((n + 2) & 31) == 0) load(0, n + 2);   // the pages of 32 tiles are used up first
+        }
+        float sum = 0.f;
+#pragma unroll
+        for (int j = 0; j < ND; j++) sum += (o[j][0] - o[j][0]) + (o[j][1] - o[j][1]) + (o[j][2] - o[j][2]) + (o[j][3] - o[j][3]);
+        if (safe || !__builtin_amdgcn_ballot_w64(row < rows && sum != 0.f)) break;   // no NaN or infinity
+    }
+    l = swap32_sum(swap16_sum(l));
+    // accumulator register r of lane (li, h): row li, dims ND (4 h + r) + j
+#pragma unroll
+    for (int r = 0; r < 4; r++)
+#pragma unroll
+        for (int j = 0; j < ND; j += 4)
+            *reinterpret_cast<float4 *>(&os[wave][li * OST + ND * (4 * h + r) + j]) =
+                make_float4(o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]);
+    if (h == 0) {
+        ms[wave][li] = m;
+        ls[wave][li] = l;
+    }
+    __syncthreads();
+    for (int i = threadIdx.x; i < RB * D / 4; i += 64 * PR_WAVES) {
+        const int c = i / (D / 4), d = i % (D / 4) * 4, r = r0 + c;
+        if (r >= rows) break;
+        float M = ms[0][c];
+#pragma unroll
+        for (int w = 1; w < PR_WAVES; w++) M = fmaxf(M, ms[w][c]);
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f;
+#pragma unroll
+        for (int w = 0; w < PR_WAVES; w++) {
+            const float f = __builtin_amdgcn_exp2f(ms[w][c] - M);
+            float4 y = *reinterpret_cast<const float4 *>(&os[w][c * OST + d]);
+            if constexpr (HL) {
+                const float4 y2 = *reinterpret_cast<const float4 *>(&os[w][(c + 8) * OST + d]);
+                y = make_float4(y.x + y2.x, y.y + y2.y, y.z + y2.z, y.w + y2.w);
+            }
+            x = make_float4(fmaf(f, y.x, x.x), fmaf(f, y.y, x.y), fmaf(f, y.z, x.z), fmaf(f, y.w, x.w));
+            den = fmaf(f, ls[w][c], den);
+        }
+        if (nz <= 1) {
+            const float inv = den == 0.f ? 0.f : 1.0f / den;   // a row that sees nothing is 0
+            const long long at = ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D + d;
+            x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+            if constexpr (HL) pg_st4((float *)a.out + at, x);
+            else pg_st4((TC *)a.out + at, x);
+        } else {
+            float *rec = part + ((((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit + z) * pg_rec(D);
+            *reinterpret_cast<float4 *>(rec + d) = x;
+            if (d == 0) {
+                rec[D] = M;
+                rec[D + 1] = den;
+            }
+        }
+    }
+}
+
+// Joins the splits of a row: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z, in
+// split order.  grid = (NKV * rows of few-row sequences, n_seqs), D threads.
+template <typename TC, int D, bool HL>
+__global__ __launch_bounds__(D) void k_pg_join_rows(const PgAttn a, int nrb, int tps, int nsplit,
+                                                    const float *__restrict__ part) {
+    constexpr int RB = HL ? 8 : 16;
+    const int s = blockIdx.y, kvh = blockIdx.x % a.pg.NKV, r = blockIdx.x / a.pg.NKV, G = a.NQ / a.pg.NKV, d = threadIdx.x;
+    const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
+    if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
+    const int rows = qn * G;
+    if (rows > PR_MAX || r >= rows) return;
+    const int base = a.pg.kv_len[s] - qn, r0 = r / RB * RB;
+    const int nz = (pg_tiles<PR_TS>(base + r0 / G, base + (min(r0 + RB, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n +
+                    tps - 1) / tps;
+    if (nz <= 1) return;
+    const float *rec = part + (((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit * pg_rec(D);
+    float M = PG_LOW;
+    for (int i = 0; i < nz; i++) M = fmaxf(M, rec[i * pg_rec(D) + D]);
+    float num = 0.f, den = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < nz; i++) {
+        const float f = __builtin_amdgcn_exp2f(rec[i * pg_rec(D) + D] - M);
+        num = fmaf(f, rec[i * pg_rec(D) + d], num);
+        den = fmaf(f, rec[i * pg_rec(D) + D + 1], den);
+    }
+    const float x = den == 0.f ? 0.f : num / den;
+    const long long at = ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D + d;
+    if constexpr (HL) ((float *)a.out)[at] = x;
+    else ((TC *)a.out)[at] = (TC)x;
+}
+
+// ---------------------------------------------------------------------------
+// Many rows.  A workgroup has one kv head and 128 of a sequence's rows, 32 a
+// wave, and goes through K and V 64 positions at a time in LDS, copied there
+// directly a tile ahead, each 16 positions from their page.  A wave forms S^T
+// (64 positions x its 32 rows) with v_mfma_f32_32x32x16: lane l holds of row l %
+// 32 the positions 32 b + 8 (r / 4) + 4 (l / 32) + r % 4.  V stays as the cache
+// has it, [position][dim]: ds_read_b64_tr_b16 gives 16 lanes 4 positions of 16
+// dims transposed, which are the A operand's positions in the order of the
+// probabilities.  The 16-byte segments of LDS rows are XOR-swizzled by the
+// copies' source addresses: K's by row, V's so that the four positions of a
+// transposing read lie in different banks.
+//
+// Blocks are numbered over the batch (a sequence's last one first, its rows see
+// most); blockIdx.y takes a share of the block's tiles where there are few
+// blocks.
+// ---------------------------------------------------------------------------
+constexpr int PC_WAVES = 4, PC_TS = 64, PC_ROWS = 32 * PC_WAVES;
+
+template <int D>
+struct PcLds {
+    unsigned char k[2][PC_TS * D * 2], v[2][PC_TS * D * 2];
+};
+
+typedef short pg_s4 __attribute__((ext_vector_type(4)));
+__device__ __forceinline__ pg_s4 pg_read_tr(uint32_t addr) {
+    return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pg_s4 *)(uintptr_t)addr);
+}
+
+// Block y of the batch: its sequence (-1: there is none) and its number in it.
+__device__ __forceinline__ int pg_chunk_block(const PgArgs &a, int G, int y, int *yb) {
+    const int lane = threadIdx.x & 63;
+    for (int i = 0; i < a.n_seqs; i += 64) {
+        long long rows = 0;
+        if (i + lane < a.n_seqs) rows = (long long)(a.q_start[i + lane + 1] - a.q_start[i + lane]) * G;
+        const int nb = rows > PR_MAX ? (int)((rows + PC_ROWS - 1) / PC_ROWS) : 0;
+        int sum = nb;   // inclusive over the lanes
+#pragma unroll
+        for (int d = 1; d < 64; d *= 2) {
+            const int o = __shfl_up(sum, d);
+            if (lane >= d) sum += o;
+        }
+        const unsigned long long past = __builtin_amdgcn_ballot_w64(sum > y);
+        if (past) {
+            const int f = __builtin_ctzll(past);
+            const int end = __builtin_amdgcn_readlane(sum, f);
+            *yb = end - 1 - y;   // the last block first
+            return i + f;
+        }
+        y -= __builtin_amdgcn_readlane(sum, 63);
+    }
+    return -1;
+}
+
+template <typename TC, int D, bool HL>
+__global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pg_attn_chunk(
+    const PgAttn a, int nsplit, float *__restrict__ part) {
+    typedef typename PgVec<TC>::h8 h8;
+    constexpr int NT = D / 32, NS = D / 16, SEG = D / 8, NP = HL ? 2 : 1, RPC = 64 / SEG;   // rows per copy
+    constexpr int CPW = PC_TS / RPC / PC_WAVES;                                                 // copies per wave
+    constexpr float SH = PgVec<TC>::SHIFT;
+    extern __shared__ __attribute__((aligned(1024))) unsigned char pc_lds[];
+    PcLds<D> *st = reinterpret_cast<PcLds<D> *>(pc_lds);
+    const int kvh = blockIdx.x % a.pg.NKV, G = a.NQ / a.pg.NKV;
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, h = lane >> 5;
+    int yb = 0;
+    const int s = pg_chunk_block(a.pg, G, blockIdx.x / a.pg.NKV, &yb);
+    if (s < 0) return;
+    const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
+    if (q0 < 0 || qn > a.pg.n_tokens - q0) return;
+    const int rows = qn * G, base = a.pg.kv_len[s] - qn;
+    const int r0 = yb * PC_ROWS, r1 = min(r0 + PC_ROWS, rows) - 1;
+    const int plo = base + r0 / G, phi = base + r1 / G, last = min(phi, a.pg.max_kv - 1);
+    const int back = a.window > 0 ? a.window : 0x40000000;   // a token at p sees the positions > p - back
+    const PgTiles tiles = pg_tiles<PC_TS>(plo, phi, a.window, a.sinks, a.pg.max_kv);
+    const int tps = max((tiles.n + nsplit - 1) / nsplit, 1), it0 = blockIdx.y * tps, it1 = min(it0 + tps, tiles.n);
+    const int nz = (tiles.n + tps - 1) / tps;
+    if (blockIdx.y > 0 && it0 >= it1) return;
+    const int row = r0 + wave * 32 + li, rc = min(row, rows - 1), tok = rc / G, pos = base + tok;
+    // the wave's tokens
+    const int w0 = min(r0 + wave * 32, rows - 1) / G, w1 = min(r0 + wave * 32 + 31, rows - 1) / G;
+    // Q^T's columns: dim step i, lane half h has dims 16 i + 8 h .. + 8
+    h8 qf[NP][NS];
+    float cs = a.scale;
+    {
+        const long long off = (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * h;
+        if constexpr (HL) {
+            const float *q = (const float *)a.q + off;
+            float4 x[NS][2];
+            float mx = 0.f;
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float4 v = x[i][j] = pg_ld4(q + 16 * i + 4 * j);
+                    mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
+                }
+            const int sh = pg_row_shift(swap32_max(mx));
+            const float f = ldexpf(1.f, sh);
+            cs *= ldexpf(1.f, -sh);
+#pragma unroll
+            for (int i = 0; i < NS; i++)
+#pragma unroll
+                for (int j = 0; j < 2; j++) {
+                    const float v[4] = {x[i][j].x * f, x[i][j].y * f, x[i][j].z * f, x[i][j].w * f};
+#pragma unroll
+                    for (int e = 0; e < 4; e++) {
+                        qf[0][i][4 * j + e] = (TC)v[e];
+                        qf[NP - 1][i][4 * j + e] = (TC)(v[e] - (float)qf[0][i][4 * j + e]);
+                    }
+                }
+        } else {
+#pragma unroll
+            for (int i = 0; i < NS; i++) qf[0][i] = *reinterpret_cast<const h8 *>((const TC *)a.q + off + 16 * i);
+        }
+    }
+    // copies: copy c = wave + 4 i takes rows RPC c .. + RPC of the tile, which lie in one
+    // 16-position block of it
+    auto kswz = [](int r) { return SEG == 16 ? r & 15 : (r & 7) ^ ((r >> 3) & 1); };
+    auto vswz = [](int r) { return SEG == 16 ? (r & 3) << 2 : ((r >> 1) & 1) << 2; };
+    uint32_t ko[CPW], vo[CPW];
+#pragma unroll
+    for (int i = 0; i < CPW; i++) {
+        const int r = (wave + PC_WAVES * i) * RPC + lane / SEG;
+        ko[i] = (uint32_t)((r & 15) * D * 2 + 16 * ((lane % SEG) ^ kswz(r)));
+        vo[i] = (uint32_t)((r & 15) * D * 2 + 16 * ((lane % SEG) ^ vswz(r)));
+    }
+    const uint32_t lk = lds_addr(st->k[0]), lv = lds_addr(st->v[0]);
+    int pages = -1;   // lane i: the page of block i % 4 of tile i / 4 (of 16 tiles)
+    auto look_up = [&](int n) {
+        const int it = it0 + n + (lane >> 2);
+        pages = it < it1 ? pg_block_page(a.pg, s, tiles.at(it) * PC_TS + 16 * (lane & 3), last) : -1;
+    };
+    const long long hbytes = (long long)(2 * D) << a.pg.shift;   // bytes of a kv head in a page
+    auto copy = [&](int buf, int n) {
+        const int k0 = tiles.at(it0 + n) * PC_TS;
+#pragma unroll
+        for (int i = 0; i < CPW; i++) {
+            const int c = wave + PC_WAVES * i, blk = c * RPC / 16;
+            const int page = max(__builtin_amdgcn_readlane(pages, 4 * (n & 15) + blk), 0);
+            const int in = (k0 + 16 * blk) & ((1 << a.pg.shift) - 1);
+            const long long off = ((long long)page * a.pg.NKV + kvh) * hbytes + (long long)in * (2 * D);
+            dma16(lk + buf * (PC_TS * D * 2) + c * 1024, ko[i], dma_rsrc((const uint8_t *)a.pg.k + off, 32 * D), 0);
+            dma16(lv + buf * (PC_TS * D * 2) + c * 1024, vo[i], dma_rsrc((const uint8_t *)a.pg.v + off, 32 * D), 0);
+        }
+    };
+    // V's transposing reads: lane l of 16 addresses position kk = l / 4 of 4, dims 4 (l % 4) .. + 4
+    // of 16; of dim block j the address is voff[j] + the step's rows
+    uint32_t voff[NT];
+    {
+        const int kk = (lane & 15) >> 2;
+#pragma unroll
+        for (int j = 0; j < NT; j++) {
+            const int seg = 4 * j + 2 * ((lane >> 4) & 1) + ((lane & 3) >> 1);
+            voff[j] = (uint32_t)((4 * h + kk) * D * 2 + 16 * (seg ^ vswz(kk)) + 8 * (lane & 1));
+        }
+    }
+    pg_f16x o[NT];
+    float m, l;
+    const int ksw = kswz(li);
+    {
+        m = PG_LOW;
+        l = 0.f;
+#pragma unroll
+        for (int j = 0; j < NT; j++) o[j] = pg_f16x{};
+        const int nt = it1 - it0;
+        if (nt > 0) {
+            look_up(0);
+            copy(0, 0);
+        }
+        dma_wait_barrier();
+        for (int n = 0, buf = 0; n < nt; n++, buf ^= 1) {
+            const int k0 = tiles.at(it0 + n) * PC_TS;
+            uint64_t has = 0;   // positions of the tile that have a page
+#pragma unroll
+            for (int b = 0; b < 4; b++)
+                has |= __builtin_amdgcn_readlane(pages, 4 * (n & 15) + b) >= 0 ? 0xFFFFull << (16 * b) : 0ull;
+            if (n + 1 < nt) {
+                if (((n + 1) & 15) == 0) look_up(n + 1);
+                copy(buf ^ 1, n + 1);
+            }
+            // values that no row of the block sees are made zero
+            const uint64_t dead = ~(pg_seen(k0, plo - back, last, a.sinks) & has);
+            if (dead) {   // uniform
+#pragma unroll
+                for (int i = 0; i < PC_TS * SEG / (64 * PC_WAVES); i++) {
+                    const int f = threadIdx.x + 64 * PC_WAVES * i;
+                    if ((dead >> (f / SEG)) & 1) *reinterpret_cast<pg_u4 *>(st->v[buf] + 16 * f) = pg_u4{};
+                }
+                __syncthreads();
+            }
+            const int wlo = base + w0, whi = base + w1;
+            if (k0 <= whi && (k0 + PC_TS > wlo - back || k0 < a.sinks)) {   // the wave's rows see some of it
+                const bool whole = has == ~0ull && k0 + PC_TS - 1 <= min(wlo, a.pg.max_kv - 1) &&
+                                   (k0 > whi - back || k0 + PC_TS <= a.sinks);
+                // the positions that tokens at lo .. hi see, from the lane's 4 h on
+                auto seen = [&](int lo, int hi) {
+                    return (pg_seen(k0, lo - back, min(hi, last), a.sinks) & has) >> (4 * h);
+                };
+                const unsigned char *Kb = st->k[buf] + li * (D * 2);
+                pg_f16x sc[2] = {pg_f16x{}, pg_f16x{}};
+#pragma unroll
+                for (int i = 0; i < NS; i++)
+#pragma unroll
+                    for (int b = 0; b < 2; b++) {
+                        const h8 x = *reinterpret_cast<const h8 *>(Kb + b * (32 * D * 2) + 16 * ((2 * i + h) ^ ksw));
+#pragma unroll
+                        for (int p = 0; p < NP; p++) sc[b] = pg_mfma32(x, qf[p][i], sc[b]);
+                    }
+                if (!whole) {
+                    const uint64_t mine = seen(pos, pos);
+#pragma unroll
+                    for (int e = 0; e < 32; e++)
+                        sc[e / 16][e % 16] = pg_hide(sc[e / 16][e % 16], pg_ones((uint32_t)(mine >> (e / 16 * 32)),
+                                                                                 8 * (e % 16 / 4) + e % 4));
+                }
+                float mx = sc[0][0];
+#pragma unroll
+                for (int e = 1; e < 32; e++) mx = fmaxf(mx, sc[e / 16][e % 16]);
+                mx = swap32_max(mx) * cs;
+                if (__builtin_amdgcn_ballot_w64(mx > m)) {
+                    const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
+                    m = mn;
+                    l *= corr;
+#pragma unroll
+                    for (int j = 0; j < NT; j++) o[j] *= corr;
+                }
+                h8 pf[NP][4];
+                const float mb = SH - m;
+                float sum = 0.f;
+#pragma unroll
+                for (int e = 0; e < 32; e++) {
+                    const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 16][e % 16], cs, mb));
+                    sum += p;
+                    pf[0][e / 8][e % 8] = (TC)p;
+                    if constexpr (HL) pf[NP - 1][e / 8][e % 8] = (TC)(p - (float)pf[0][e / 8][e % 8]);
+                }
+                l += sum;
+                const uint32_t vb = lv + buf * (PC_TS * D * 2);
+                auto vfrag = [&](int u, int j) {
+                    const pg_s4 x = pg_read_tr(vb + voff[j] + 16 * u * (D * 2)), y = pg_read_tr(vb + voff[j] + (16 * u + 8) * (D * 2));
+                    return __builtin_shufflevector(x, y, 0, 1, 2, 3, 4, 5, 6, 7);
+                };
+#pragma unroll
+                for (int u = 0; u < 4; u++)
+#pragma unroll
+                    for (int j = 0; j < NT; j++) {
+                        const h8 x = __builtin_bit_cast(h8, vfrag(u, j));
+#pragma unroll
+                        for (int p = 0; p < NP; p++) o[j] = pg_mfma32(x, pf[p][u], o[j]);
+                    }
+            }
+            dma_wait_barrier();
+        }
+    }
+    l = swap32_sum(l);
+    // rows with an output that is not finite are formed again, one at a time
+    float odd = 0.f;   // NaN where an output is NaN or infinite
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int r = 0; r < 16; r++) odd += o[j][r] - o[j][r];
+    odd += __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * (lane ^ 32), __builtin_bit_cast(int, odd)));
+    const bool again = row < rows && !(odd == 0.f);
+    for (unsigned long long left = __builtin_amdgcn_ballot_w64(again && h == 0); left; left &= left - 1) {
+        typedef typename std::conditional<HL, float, TC>::type TA;
+        const int c = __builtin_ctzll(left), r = r0 + wave * 32 + c, t = r / G;
+        float so[D / 64], sm, sl;
+        pg_slow_row<TA, TC, D>(a.pg, (const TA *)a.q + (long long)(q0 + t) * a.qs + (long long)(kvh * G + r % G) * D, a.scale,
+                               s, kvh, base + t, back, a.sinks, tiles, it0, it1, so, &sm, &sl);
+        const long long to = (long long)(q0 + t) * a.NQ + kvh * G + r % G;
+        float *rec = part + (to * nsplit + blockIdx.y) * pg_rec(D);
+#pragma unroll
+        for (int i = 0; i < D / 64; i++) {
+            if (nz <= 1) ((TA *)a.out)[to * D + lane + 64 * i] = (TA)(sl == 0.f ? 0.f : so[i] / sl);
+            else rec[lane + 64 * i] = so[i];
+        }
+        if (nz > 1 && lane == 0) {
+            rec[D] = sm;
+            rec[D + 1] = sl;
+        }
+    }
+    if (again) return;
+    if (row >= rows) return;
+    const long long at = ((long long)(q0 + tok) * a.NQ + kvh * G + row % G);
+    if (nz <= 1) {
+        const float inv = l == 0.f ? 0.f : 1.0f / l;   // a row that sees nothing is 0
+#pragma unroll
+        for (int j = 0; j < NT; j++)
+#pragma unroll
+            for (int r = 0; r < 4; r++) {
+                const float4 x = make_float4(o[j][4 * r] * inv, o[j][4 * r + 1] * inv, o[j][4 * r + 2] * inv, o[j][4 * r + 3] * inv);
+                const long long d = at * D + 32 * j + 8 * r + 4 * h;
+                if constexpr (HL) pg_st4((float *)a.out + d, x);
+                else pg_st4((TC *)a.out + d, x);
+            }
+        return;
+    }
+    float *rec = part + (at * nsplit + blockIdx.y) * pg_rec(D);
+#pragma unroll
+    for (int j = 0; j < NT; j++)
+#pragma unroll
+        for (int r = 0; r < 4; r++)
+            *reinterpret_cast<float4 *>(rec + 32 * j + 8 * r + 4 * h) =
+                make_float4(o[j][4 * r], o[j][4 * r + 1], o[j][4 * r + 2], o[j][4 * r + 3]);
+    if (h == 0) {
+        rec[D] = m;
+        rec[D + 1] = l;
+    }
+}
+
+// Joins the splits of the many-row sequences' rows.  grid = NQ * n_tokens, D threads.
+template <typename TC, int D, bool HL>
+__global__ __launch_bounds__(D) void k_pg_join_chunk(const PgAttn a, int nsplit, const float *__restrict__ part) {
+    const int hd = blockIdx.x % a.NQ, t = blockIdx.x / a.NQ, d = threadIdx.x, G = a.NQ / a.pg.NKV;
     const int s = pg_seq_of(a.pg.q_start, a.pg.n_seqs, t);
     if (s >= a.pg.n_seqs || t < a.pg.q_start[s]) return;
-    const int pos = a.pg.kv_len[s] - a.pg.q_start[s + 1] + t;
-    const int kvh = h / (a.NQ / a.pg.NKV);
-    const TA *q = (const TA *)a.q + t * a.qs + h * D;
-    float qv[D / 64], o[D / 64] = {}, m = -3.402823466e38f, l = 0.f;
-#pragma unroll
-    for (int i = 0; i < D / 64; i++) qv[i] = (float)q[lane + 64 * i];
-    const int lo = a.window > 0 ? pos - a.window + 1 : 0;
-    for (int p = 0; p <= pos; p++) {
-        if (p < lo && p >= a.sinks) p = lo;
-        const int page = pg_page(a.pg, s, p);
-        if (page < 0) continue;
-        const long long row = pg_row<D>(a.pg, page, kvh, p);
-        float dot = 0.f;
-#pragma unroll
-        for (int i = 0; i < D / 64; i++) dot += qv[i] * (float)((const TC *)a.pg.k)[row + lane + 64 * i];
-        dot = group_sum<64>(dot) * a.scale;
-        const float mn = fmaxf(m, dot), corr = __builtin_amdgcn_exp2f(m - mn), w = __builtin_amdgcn_exp2f(dot - mn);
-        m = mn;
-        l = l * corr + w;
-#pragma unroll
-        for (int i = 0; i < D / 64; i++) o[i] = o[i] * corr + w * (float)((const TC *)a.pg.v)[row + lane + 64 * i];
+    const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
+    if (q0 < 0 || qn > a.pg.n_tokens - q0 || (long long)qn * G <= PR_MAX) return;
+    const int rows = qn * G, base = a.pg.kv_len[s] - qn, r0 = ((t - q0) * G + hd % G) / PC_ROWS * PC_ROWS;
+    const int n = pg_tiles<PC_TS>(base + r0 / G, base + (min(r0 + PC_ROWS, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n;
+    const int tps = max((n + nsplit - 1) / nsplit, 1), nz = (n + tps - 1) / tps;
+    if (nz <= 1) return;
+    const long long at = (long long)t * a.NQ + hd;
+    const float *rec = part + at * nsplit * pg_rec(D);
+    float M = PG_LOW;
+    for (int i = 0; i < nz; i++) M = fmaxf(M, rec[i * pg_rec(D) + D]);
+    float num = 0.f, den = 0.f;
+#pragma unroll 4
+    for (int i = 0; i < nz; i++) {
+        const float f = __builtin_amdgcn_exp2f(rec[i * pg_rec(D) + D] - M);
+        num = fmaf(f, rec[i * pg_rec(D) + d], num);
+        den = fmaf(f, rec[i * pg_rec(D) + D + 1], den);
     }
-    TA *out = (TA *)a.out + ((long long)t * a.NQ + h) * D;
-#pragma unroll
-    for (int i = 0; i < D / 64; i++) out[lane + 64 * i] = (TA)(l > 0.f ? o[i] / l : l);
+    const float x = den == 0.f ? 0.f : num / den;
+    if constexpr (HL) ((float *)a.out)[at * D + d] = x;
+    else ((TC *)a.out)[at * D + d] = (TC)x;
 }
 
+// ---------------------------------------------------------------------------
+// Host side: the splits, by what the host knows (max_q, max_kv, n_tokens).
+// ---------------------------------------------------------------------------
+struct PgPlan {
+    int nrb, row_tps, row_splits;   // few rows: row blocks, tiles of a split, splits
+    bool chunks;                    // whether a sequence can have many rows
+    int blocks, chunk_splits;
+    size_t rows_bytes, bytes;       // workspace: the few rows' records, then the others'
+};
+
+static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32) {
+    PgPlan p{};
+    const int G = NQ / a.NKV, RB = f32 ? 8 : 16, cu = 256;
+    const long long most = std::min((long long)a.max_q * G, (long long)PR_MAX);
+    p.nrb = (int)((most + RB - 1) / RB);
+    // positions that one block can see
+    long long seen = a.max_kv;
+    if (window > 0) seen = std::min(seen, (long long)window + sinks + 2 * PC_TS + std::min(a.max_q, PC_ROWS));
+    const long long tiles = (seen + PR_TS - 1) / PR_TS + 1;
+    const long long wgs = (long long)a.NKV * p.nrb * a.n_seqs;
+    long long want = std::max(1ll, (4 * cu + wgs - 1) / wgs);
+    long long tps = (tiles + want - 1) / want;
+    tps = std::max(4ll, (tps + 3) / 4 * 4);
+    p.row_tps = (int)tps;
+    p.row_splits = (int)((tiles + tps - 1) / tps);
+    if (p.row_splits > 1) p.rows_bytes = (size_t)a.n_seqs * a.NKV * p.nrb * RB * p.row_splits * pg_rec(D) * 4;
+    p.chunks = (long long)a.max_q * G > PR_MAX;
+    p.bytes = p.rows_bytes;
+    if (p.chunks) {
+        p.blocks = (int)(((long long)a.n_tokens * G + PC_ROWS - 1) / PC_ROWS) + a.n_seqs;
+        const long long w = (long long)a.NKV * (((long long)a.n_tokens * G + PC_ROWS - 1) / PC_ROWS);
+        const long long t = (seen + PC_TS - 1) / PC_TS;
+        p.chunk_splits = (int)std::max(1ll, std::min(std::min(8ll, (2 * cu + w - 1) / w), t / 2));
+        if (p.chunk_splits > 1) p.bytes += (size_t)a.n_tokens * NQ * p.chunk_splits * pg_rec(D) * 4;
+    }
+    return p;
+}
+
+// Without the window: a plan with one sees no more positions, so it has no more
+// tiles, but may split them less; its records fit.
 size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32) {
-    (void)a; (void)D; (void)NQ; (void)f32;
-    return 0;
+    if (a.n_seqs == 0 || a.n_tokens == 0) return 0;
+    return pg_plan(a, D, NQ, 0, 0, f32).bytes;
 }
 
-hipError_t launch_pg_attn(const PgAttn &a, int D, int q_type, int c_type, void *ws, size_t ws_bytes, hipStream_t st) {
-    (void)ws; (void)ws_bytes;
-    const dim3 grid(a.NQ, a.pg.n_tokens);
-#define TBQ_AT(TA, TC)                                                                              \
-    do {                                                                                            \
-        if (D == 128) hipLaunchKernelGGL((k_pg_attn_row<TA, TC, 128>), grid, dim3(64), 0, st, a);   \
-        else hipLaunchKernelGGL((k_pg_attn_row<TA, TC, 64>), grid, dim3(64), 0, st, a);             \
-        return hipGetLastError();                                                                   \
-    } while (0)
-    if (q_type == TBQ_KV_F32) TBQ_AT(float, pg_f16);
-    if (c_type == TBQ_KV_F16) TBQ_AT(pg_f16, pg_f16);
-    TBQ_AT(pg_bf16, pg_bf16);
-#undef TBQ_AT
+template <typename TC, int D, bool HL>
+static hipError_t pg_attn(const PgAttn &a, float *ws, hipStream_t st) {
+    const PgPlan p = pg_plan(a.pg, D, a.NQ, a.window, a.sinks, HL);
+    constexpr int RB = HL ? 8 : 16;
+    hipLaunchKernelGGL((k_pg_attn_rows<TC, D, HL>), dim3(a.pg.NKV * p.nrb, p.row_splits, a.pg.n_seqs), dim3(64 * PR_WAVES),
+                       0, st, a, p.nrb, p.row_tps, p.row_splits, ws);
+    if (p.row_splits > 1)
+        hipLaunchKernelGGL((k_pg_join_rows<TC, D, HL>), dim3(a.pg.NKV * std::min(p.nrb * RB, PR_MAX), a.pg.n_seqs), dim3(D), 0,
+                           st, a, p.nrb, p.row_tps, p.row_splits, ws);
+    if (p.chunks) {
+        static const hipError_t e = hipFuncSetAttribute((const void *)k_pg_attn_chunk<TC, D, HL>,
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PcLds<D>));
+        if (e != hipSuccess) return e;
+        float *part = ws + p.rows_bytes / 4;
+        hipLaunchKernelGGL((k_pg_attn_chunk<TC, D, HL>), dim3(a.pg.NKV * p.blocks, p.chunk_splits), dim3(64 * PC_WAVES),
+                           sizeof(PcLds<D>), st, a, p.chunk_splits, part);
+        if (p.chunk_splits > 1)
+            hipLaunchKernelGGL((k_pg_join_chunk<TC, D, HL>), dim3(a.NQ * a.pg.n_tokens), dim3(D), 0, st, a, p.chunk_splits, part);
+    }
+    return hipGetLastError();
+}
+
+hipError_t launch_pg_attn(const PgAttn &a, int D, int q_type, int c_type, void *ws, hipStream_t st) {
+    float *w = (float *)ws;
+    if (q_type == TBQ_KV_F32) return D == 128 ? pg_attn<pg_f16, 128, true>(a, w, st) : pg_attn<pg_f16, 64, true>(a, w, st);
+    if (c_type == TBQ_KV_F16) return D == 128 ? pg_attn<pg_f16, 128, false>(a, w, st) : pg_attn<pg_f16, 64, false>(a, w, st);
+    return D == 128 ? pg_attn<pg_bf16, 128, false>(a, w, st) : pg_attn<pg_bf16, 64, false>(a, w, st);
 }
 
 }  // namespace tbq
