@@ -49,6 +49,8 @@ int check_cache(const char *who, const tbq_kv_cache *c) {
         return fail("%s: page_size %d (16, 32, 64, 128 or 256)", who, c->page_size);
     if (c->n_layers < 1 || c->n_layers > 16384 || c->n_pages < 1 || c->n_kv_heads < 1 || c->n_kv_heads > 65535)
         return fail("%s: cache of %d layers, %d pages, %d kv heads", who, c->n_layers, c->n_pages, c->n_kv_heads);
+    if ((long long)c->n_pages * c->n_kv_heads * c->page_size > 0x7FFFFFFF)
+        return fail("%s: more than 2^31 - 1 rows of kv heads in a layer", who);
     if (!c->k || !c->v || !aligned(c->k, 16) || !aligned(c->v, 16)) return fail("%s: null or misaligned cache", who);
     return 1;
 }

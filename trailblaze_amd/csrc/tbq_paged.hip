@@ -167,48 +167,76 @@ hipError_t launch_pg_copy(void *k, void *v, int n_layers, long long pbytes, long
 
 // ---------------------------------------------------------------------------
 // Compaction, in place: row j of a sequence becomes its row keep[j] >= j, keep
-// ascending.  A workgroup has one sequence, layer, K or V, and kv head (no
-// other workgroup touches these rows) and goes through the kept rows CO_ROWS at
-// a time: all of a step's rows are loaded before any is stored, and a step's
-// stores reach no row that a later step loads (keep[j'] >= j' > j).
+// ascending.  A workgroup has one sequence, layer, K or V, hpw kv heads and a
+// 128-byte column of their rows (no other workgroup touches it) and goes through
+// the kept rows a step at a time: all of a step's rows have arrived in every
+// wave before any is stored, and a step's stores reach no row that a later step
+// loads (keep[j'] >= j' > j), so the next step's rows are loaded before this
+// one's are stored, and its page lookups before those.
 // ---------------------------------------------------------------------------
-constexpr int CO_THREADS = 256, CO_V = 8;
+constexpr int CO_THREADS = 256, CO_V = 8, CO_UNITS = CO_THREADS / 8 * CO_V;   // rows of one head in a step
 template <int D>
 __global__ __launch_bounds__(CO_THREADS) void k_pg_compact(uint16_t *k, uint16_t *v, long long lelems, const PgArgs a,
-                                                           const int *keep_start, const int *keep) {
-    constexpr int LPR = D / 8, RPV = CO_THREADS / LPR, ROWS = RPV * CO_V;   // 16 bytes a lane
-    const int h = blockIdx.x, s = blockIdx.z, l = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
-    uint16_t *base = (blockIdx.y & 1 ? v : k) + (blockIdx.y >> 1) * lelems;
+                                                           const int *__restrict__ keep_start,
+                                                           const int *__restrict__ keep, int hpw) {
+    constexpr int SL = D / 64;   // 128-byte columns of a row
+    const int s = blockIdx.z, l = threadIdx.x % 8, u0 = threadIdx.x / 8;
+    const int col = blockIdx.x % SL, h0 = blockIdx.x / SL * hpw, jr = CO_UNITS / hpw;   // rows of a step
+    uint16_t *base = (blockIdx.y & 1 ? v : k) + (blockIdx.y >> 1) * lelems + 64 * col + 8 * l;
     const int at = keep_start[s], n = keep_start[s + 1] - at;
-    for (int j0 = 0; j0 < n; j0 += ROWS) {   // uniform
-        pg_u4 r[CO_V];
-        long long dst[CO_V];   // elements into the layer, -1: nothing to store
+    int src[2][CO_V], dst[2][CO_V];   // rows from `base` on, dst -1: nothing to store
+    pg_u4 r[2][CO_V];
+    auto find = [&](int b, int j0) {
 #pragma unroll
         for (int i = 0; i < CO_V; i++) {
-            const int j = min(j0 + i * RPV + r0, n - 1), from = keep[at + j], p = max(from, 0);
-            const int ps = pg_page(a, s, p), pd = pg_page(a, s, j);
-            const bool moves = j0 + i * RPV + r0 < n && from >= 0 && p != j && ps >= 0 && pd >= 0;
+            const int u = i * (CO_THREADS / 8) + u0, h = u / jr;
+            const int j = j0 + u % jr, jc = min(j, n - 1), from = keep[at + jc], p = max(from, 0);
+            const int ps = pg_page(a, s, p), pd = pg_page(a, s, jc);
+            const bool moves = j < n && h < hpw && from >= 0 && p != j && ps >= 0 && pd >= 0;
             // a row that does not move is loaded from where it is (or page 0) and not stored
-            r[i] = *reinterpret_cast<const pg_u4 *>(base + pg_row<D>(a, max(ps, 0), h, p) + 8 * l);
-            dst[i] = moves ? pg_row<D>(a, pd, h, j) + 8 * l : -1;
+            src[b][i] = (int)(pg_row<D>(a, max(ps, 0), h0 + min(h, hpw - 1), p) / D);
+            dst[b][i] = moves ? (int)(pg_row<D>(a, pd, h0 + h, jc) / D) : -1;
         }
-        // every wave's rows have arrived
-        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+    };
+    auto load = [&](int b) {
+#pragma unroll
+        for (int i = 0; i < CO_V; i++) r[b][i] = *reinterpret_cast<const pg_u4 *>(base + (long long)src[b][i] * D);
+    };
+    auto store = [&](int b) {
 #pragma unroll
         for (int i = 0; i < CO_V; i++)
-            if (dst[i] >= 0) *reinterpret_cast<pg_u4 *>(base + dst[i]) = r[i];
+            if (dst[b][i] >= 0) *reinterpret_cast<pg_u4 *>(base + (long long)dst[b][i] * D) = r[b][i];
+    };
+    if (n <= 0) return;
+    auto step = [&](int b, int j0) {
+        if (j0 + jr < n) find(b ^ 1, j0 + jr);
+        // every wave's rows have arrived
+        asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
+        if (j0 + jr < n) load(b ^ 1);
+        store(b);
+    };
+    find(0, 0);
+    load(0);
+    for (int j0 = 0; j0 < n; j0 += 2 * jr) {   // uniform
+        step(0, j0);
+        if (j0 + jr < n) step(1, j0 + jr);
     }
 }
 
+// Heads of a workgroup: all, or as many as leave about four workgroups a CU
+// (many short sequences: one step does it all, and the page lookups are shared).
 hipError_t launch_pg_compact(void *k, void *v, int n_layers, long long lelems, int D, const PgArgs &a, const int *keep_start,
                              const int *keep, hipStream_t st) {
-    const dim3 grid(a.NKV, 2 * n_layers, a.n_seqs);
+    int hpw = 1;
+    for (int h = 2; h <= a.NKV && h <= 32; h++)
+        if (a.NKV % h == 0 && (long long)a.n_seqs * 2 * n_layers * (a.NKV / h) * (D / 64) >= 1024) hpw = h;
+    const dim3 grid(a.NKV / hpw * (D / 64), 2 * n_layers, a.n_seqs);
     if (D == 128)
         hipLaunchKernelGGL(k_pg_compact<128>, grid, dim3(CO_THREADS), 0, st, (uint16_t *)k, (uint16_t *)v, lelems, a,
-                           keep_start, keep);
+                           keep_start, keep, hpw);
     else
         hipLaunchKernelGGL(k_pg_compact<64>, grid, dim3(CO_THREADS), 0, st, (uint16_t *)k, (uint16_t *)v, lelems, a,
-                           keep_start, keep);
+                           keep_start, keep, hpw);
     return hipGetLastError();
 }
 

@@ -14,8 +14,9 @@
 // F32 rows (HL): q, scaled by the power of two that puts its largest element in
 // [2^13, 2^14), and the probabilities are each taken as two halves, x = hi + lo,
 // which keeps ~22 bits; the keys and values are halves already.  16-bit rows
-// round the probabilities to the cache's type.  Half probabilities are scaled by
-// 2^14, so those that a half cannot hold are below 2^-38 of the largest.
+// round the probabilities to the cache's type.  Half probabilities are scaled up
+// (by 2^14, or 2^7 where the running maximum may lag 2^8 behind), so those that
+// a half cannot hold are below 2^-31 of the largest.
 //
 // What a row does not see must not reach it, NaN and infinities included.
 // Scores are replaced before the maximum.  In the product with V an unseen
@@ -167,22 +168,29 @@ constexpr int pg_rec(int D) { return D + 4; }   // floats of a split's record: D
 // congruent to j.  A tile's loads are issued a tile ahead.
 // ---------------------------------------------------------------------------
 constexpr int PR_WAVES = 4, PR_TS = 32;
-#ifndef TBQ_PG_RMAX
-#define TBQ_PG_RMAX 16
-#endif
-constexpr int PR_MAX = TBQ_PG_RMAX;   // rows up to which a sequence is one of few rows
+// Rows up to which a sequence is one of few rows: 8 tokens of 4 heads a kv head
+// after 4000 positions 13.8 us as two row blocks, 28.6 as one of many; 16 tokens
+// of 8 sequences after 2000 40.0 us as four, 33.4 as many.
+constexpr int PR_MAX = 32;
+constexpr int PR_MIN = 4, PR_LONG = 64;   // tiles of a split: one a wave at least, 2048 positions at most
 
-template <typename TC, int D, bool HL>
-__global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pg_attn_rows(
-    const PgAttn a, int nrb, int tps, int nsplit, float *__restrict__ part) {
+template <int D>
+struct PrLds {
+    float o[PR_WAVES][16 * (D + 4)], m[PR_WAVES][16], l[PR_WAVES][16];
+};
+
+// x: kv head + NKV * row block; z: split; s: sequence.  ONCE: one row block reads the values,
+// whole lines at a time, which then need not stay in the caches (64 sequences of up to 8192:
+// 242 -> 228 us; keys, whose lines take two loads, are slower so).
+template <typename TC, int D, bool HL, bool ONCE>
+__device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int nsplit, float *__restrict__ part, int x, int z,
+                                        int s, PrLds<D> *lds) {
     typedef typename PgVec<TC>::h8 h8;
     typedef TC hv __attribute__((ext_vector_type(D / 16)));
     constexpr int RB = HL ? 8 : 16, NS = D / 32, ND = D / 16, OST = D + 4;
     constexpr float SH = PgVec<TC>::SHIFT;
-    __shared__ __attribute__((aligned(16))) float os[PR_WAVES][16 * OST];
-    __shared__ float ms[PR_WAVES][16], ls[PR_WAVES][16];
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, h = lane >> 4;
-    const int kvh = blockIdx.x % a.pg.NKV, r0 = blockIdx.x / a.pg.NKV * RB, s = blockIdx.z, G = a.NQ / a.pg.NKV;
+    const int kvh = x % a.pg.NKV, r0 = x / a.pg.NKV * RB, G = a.NQ / a.pg.NKV;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
     if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
     const int rows = qn * G;
@@ -192,7 +200,7 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2
     const int plo = base + t0, phi = base + t1, last = min(phi, a.pg.max_kv - 1);
     const int back = a.window > 0 ? a.window : 0x40000000;   // a token at p sees the positions > p - back
     const PgTiles tiles = pg_tiles<PR_TS>(plo, phi, a.window, a.sinks, a.pg.max_kv);
-    const int z = blockIdx.y, nz = (tiles.n + tps - 1) / tps, it0 = z * tps, it1 = min(it0 + tps, tiles.n);
+    const int nz = (tiles.n + tps - 1) / tps, it0 = z * tps, it1 = min(it0 + tps, tiles.n);
     if (z > 0 && it0 >= it1) return;
     const int row = r0 + (HL ? li & 7 : li), rc = min(row, rows - 1), tok = rc / G, pos = base + tok;
     // Q^T's columns
@@ -254,7 +262,11 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
             for (int i = 0; i < NS; i++) kf[buf][b][i] = *reinterpret_cast<const h8 *>(kp + koff + 32 * i);
 #pragma unroll
-            for (int i = 0; i < 4; i++) vf[buf][4 * b + i] = *reinterpret_cast<const hv *>(vp + voff + i * D);
+            for (int i = 0; i < 4; i++) {
+                const hv *v = reinterpret_cast<const hv *>(vp + voff + i * D);
+                if constexpr (ONCE) vf[buf][4 * b + i] = __builtin_nontemporal_load(v);
+                else vf[buf][4 * b + i] = *v;
+            }
         }
     };
     pg_f4 o[ND];
@@ -363,41 +375,41 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2
     for (int r = 0; r < 4; r++)
 #pragma unroll
         for (int j = 0; j < ND; j += 4)
-            *reinterpret_cast<float4 *>(&os[wave][li * OST + ND * (4 * h + r) + j]) =
+            *reinterpret_cast<float4 *>(&lds->o[wave][li * OST + ND * (4 * h + r) + j]) =
                 make_float4(o[j][r], o[j + 1][r], o[j + 2][r], o[j + 3][r]);
     if (h == 0) {
-        ms[wave][li] = m;
-        ls[wave][li] = l;
+        lds->m[wave][li] = m;
+        lds->l[wave][li] = l;
     }
     __syncthreads();
     for (int i = threadIdx.x; i < RB * D / 4; i += 64 * PR_WAVES) {
         const int c = i / (D / 4), d = i % (D / 4) * 4, r = r0 + c;
         if (r >= rows) break;
-        float M = ms[0][c];
+        float M = lds->m[0][c];
 #pragma unroll
-        for (int w = 1; w < PR_WAVES; w++) M = fmaxf(M, ms[w][c]);
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        for (int w = 1; w < PR_WAVES; w++) M = fmaxf(M, lds->m[w][c]);
+        float4 sum = make_float4(0.f, 0.f, 0.f, 0.f);
         float den = 0.f;
 #pragma unroll
         for (int w = 0; w < PR_WAVES; w++) {
-            const float f = __builtin_amdgcn_exp2f(ms[w][c] - M);
-            float4 y = *reinterpret_cast<const float4 *>(&os[w][c * OST + d]);
+            const float f = __builtin_amdgcn_exp2f(lds->m[w][c] - M);
+            float4 y = *reinterpret_cast<const float4 *>(&lds->o[w][c * OST + d]);
             if constexpr (HL) {
-                const float4 y2 = *reinterpret_cast<const float4 *>(&os[w][(c + 8) * OST + d]);
+                const float4 y2 = *reinterpret_cast<const float4 *>(&lds->o[w][(c + 8) * OST + d]);
                 y = make_float4(y.x + y2.x, y.y + y2.y, y.z + y2.z, y.w + y2.w);
             }
-            x = make_float4(fmaf(f, y.x, x.x), fmaf(f, y.y, x.y), fmaf(f, y.z, x.z), fmaf(f, y.w, x.w));
-            den = fmaf(f, ls[w][c], den);
+            sum = make_float4(fmaf(f, y.x, sum.x), fmaf(f, y.y, sum.y), fmaf(f, y.z, sum.z), fmaf(f, y.w, sum.w));
+            den = fmaf(f, lds->l[w][c], den);
         }
         if (nz <= 1) {
             const float inv = den == 0.f ? 0.f : 1.0f / den;   // a row that sees nothing is 0
             const long long at = ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D + d;
-            x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-            if constexpr (HL) pg_st4((float *)a.out + at, x);
-            else pg_st4((TC *)a.out + at, x);
+            sum = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
+            if constexpr (HL) pg_st4((float *)a.out + at, sum);
+            else pg_st4((TC *)a.out + at, sum);
         } else {
             float *rec = part + ((((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit + z) * pg_rec(D);
-            *reinterpret_cast<float4 *>(rec + d) = x;
+            *reinterpret_cast<float4 *>(rec + d) = sum;
             if (d == 0) {
                 rec[D] = M;
                 rec[D + 1] = den;
@@ -406,13 +418,28 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2
     }
 }
 
-// Joins the splits of a row: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z, in
-// split order.  grid = (NKV * rows of few-row sequences, n_seqs), D threads.
+template <typename TC, int D, bool HL, bool ONCE>
+__global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pg_attn_rows(
+    const PgAttn a, int nrb, int tps, int nsplit, float *__restrict__ part) {
+    __shared__ __attribute__((aligned(16))) PrLds<D> lds;
+    pg_rows<TC, D, HL, ONCE>(a, nrb, tps, nsplit, part, blockIdx.x, blockIdx.y, blockIdx.z, &lds);
+}
+
+// Joins the splits of a row: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.
+// One workgroup a row.  GROUPS groups of D / 4
+// lanes each add every GROUPS-th split, then the groups are added in order:
+// a row's records (hundreds for one token over a long context) are read by as
+// many lanes as there are, 8 in flight each.
+constexpr int PJ_THREADS = 256, PJ_MAX = 1024;   // most splits (pg_plan)
+// x: kv head + NKV * row; s: sequence.
 template <typename TC, int D, bool HL>
-__global__ __launch_bounds__(D) void k_pg_join_rows(const PgAttn a, int nrb, int tps, int nsplit,
-                                                    const float *__restrict__ part) {
-    constexpr int RB = HL ? 8 : 16;
-    const int s = blockIdx.y, kvh = blockIdx.x % a.pg.NKV, r = blockIdx.x / a.pg.NKV, G = a.NQ / a.pg.NKV, d = threadIdx.x;
+__device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, int nsplit, const float *__restrict__ part,
+                                             int xx, int s) {
+    constexpr int RB = HL ? 8 : 16, GROUPS = PJ_THREADS / (D / 4), REC = pg_rec(D);
+    __shared__ float fs[PJ_MAX];
+    __shared__ float red[2][PJ_THREADS / 64];
+    __shared__ __attribute__((aligned(16))) float os[GROUPS][D];
+    const int kvh = xx % a.pg.NKV, r = xx / a.pg.NKV, G = a.NQ / a.pg.NKV, tid = threadIdx.x;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
     if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
     const int rows = qn * G;
@@ -421,20 +448,58 @@ __global__ __launch_bounds__(D) void k_pg_join_rows(const PgAttn a, int nrb, int
     const int nz = (pg_tiles<PR_TS>(base + r0 / G, base + (min(r0 + RB, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n +
                     tps - 1) / tps;
     if (nz <= 1) return;
-    const float *rec = part + (((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit * pg_rec(D);
-    float M = PG_LOW;
-    for (int i = 0; i < nz; i++) M = fmaxf(M, rec[i * pg_rec(D) + D]);
-    float num = 0.f, den = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < nz; i++) {
-        const float f = __builtin_amdgcn_exp2f(rec[i * pg_rec(D) + D] - M);
-        num = fmaf(f, rec[i * pg_rec(D) + d], num);
-        den = fmaf(f, rec[i * pg_rec(D) + D + 1], den);
+    const float *rec = part + (((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit * REC;
+    float mz[PJ_MAX / PJ_THREADS], lz[PJ_MAX / PJ_THREADS], M = PG_LOW;
+#pragma unroll
+    for (int i = 0; i < PJ_MAX / PJ_THREADS; i++) {
+        const int z = tid + PJ_THREADS * i;
+        const float2 ml = *reinterpret_cast<const float2 *>(rec + (long long)min(z, nz - 1) * REC + D);
+        mz[i] = z < nz ? ml.x : PG_LOW;
+        lz[i] = z < nz ? ml.y : 0.f;
+        M = fmaxf(M, mz[i]);
     }
-    const float x = den == 0.f ? 0.f : num / den;
-    const long long at = ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D + d;
-    if constexpr (HL) ((float *)a.out)[at] = x;
-    else ((TC *)a.out)[at] = (TC)x;
+    M = wave_max(M);
+    if ((tid & 63) == 0) red[0][tid >> 6] = M;
+    __syncthreads();
+#pragma unroll
+    for (int i = 0; i < PJ_THREADS / 64; i++) M = fmaxf(M, red[0][i]);
+    float den = 0.f;
+#pragma unroll
+    for (int i = 0; i < PJ_MAX / PJ_THREADS; i++) {
+        const float f = __builtin_amdgcn_exp2f(mz[i] - M);
+        fs[tid + PJ_THREADS * i] = f;
+        den = fmaf(f, lz[i], den);
+    }
+    den = group_sum<64>(den);
+    if ((tid & 63) == 0) red[1][tid >> 6] = den;
+    __syncthreads();
+    const int g = tid / (D / 4), d = tid % (D / 4) * 4;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int z = g; z < nz; z += 8 * GROUPS) {
+        float4 y[8];
+#pragma unroll
+        for (int i = 0; i < 8; i++)   // past the last: the last again, weighed 0
+            y[i] = *reinterpret_cast<const float4 *>(rec + (long long)min(z + i * GROUPS, nz - 1) * REC + d);
+#pragma unroll
+        for (int i = 0; i < 8; i++) {
+            if (z + i * GROUPS >= nz) continue;
+            const float f = fs[z + i * GROUPS];
+            x = make_float4(fmaf(f, y[i].x, x.x), fmaf(f, y[i].y, x.y), fmaf(f, y[i].z, x.z), fmaf(f, y[i].w, x.w));
+        }
+    }
+    *reinterpret_cast<float4 *>(&os[g][d]) = x;
+    __syncthreads();
+    if (tid >= D) return;
+    den = 0.f;
+#pragma unroll
+    for (int i = 0; i < PJ_THREADS / 64; i++) den += red[1][i];
+    float num = os[0][tid];
+#pragma unroll
+    for (int i = 1; i < GROUPS; i++) num += os[i][tid];
+    const float out = den == 0.f ? 0.f : num / den;
+    const long long at = ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D + tid;
+    if constexpr (HL) ((float *)a.out)[at] = out;
+    else ((TC *)a.out)[at] = (TC)out;
 }
 
 // ---------------------------------------------------------------------------
@@ -490,19 +555,20 @@ __device__ __forceinline__ int pg_chunk_block(const PgArgs &a, int G, int y, int
     return -1;
 }
 
+// x: kv head + NKV * block; z: split.
 template <typename TC, int D, bool HL>
-__global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_pg_attn_chunk(
-    const PgAttn a, int nsplit, float *__restrict__ part) {
+__device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__restrict__ part, int x, int z,
+                                         PcLds<D> *st) {
     typedef typename PgVec<TC>::h8 h8;
     constexpr int NT = D / 32, NS = D / 16, SEG = D / 8, NP = HL ? 2 : 1, RPC = 64 / SEG;   // rows per copy
     constexpr int CPW = PC_TS / RPC / PC_WAVES;                                                 // copies per wave
-    constexpr float SH = PgVec<TC>::SHIFT;
-    extern __shared__ __attribute__((aligned(1024))) unsigned char pc_lds[];
-    PcLds<D> *st = reinterpret_cast<PcLds<D> *>(pc_lds);
-    const int kvh = blockIdx.x % a.pg.NKV, G = a.NQ / a.pg.NKV;
+    // a running maximum that lags by up to LAG spares most of the rescalings of o (a wave's 32 rows
+    // rarely all keep theirs): 350 -> 340 us for 2048 tokens after 8192, 32 / 8 heads of 128
+    constexpr float LAG = 8.f, SH = PgVec<TC>::SHIFT - (PgVec<TC>::SHIFT > 0.f ? 7.f : 0.f);
+    const int kvh = x % a.pg.NKV, G = a.NQ / a.pg.NKV;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, h = lane >> 5;
     int yb = 0;
-    const int s = pg_chunk_block(a.pg, G, blockIdx.x / a.pg.NKV, &yb);
+    const int s = pg_chunk_block(a.pg, G, x / a.pg.NKV, &yb);
     if (s < 0) return;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
     if (q0 < 0 || qn > a.pg.n_tokens - q0) return;
@@ -511,9 +577,9 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
     const int plo = base + r0 / G, phi = base + r1 / G, last = min(phi, a.pg.max_kv - 1);
     const int back = a.window > 0 ? a.window : 0x40000000;   // a token at p sees the positions > p - back
     const PgTiles tiles = pg_tiles<PC_TS>(plo, phi, a.window, a.sinks, a.pg.max_kv);
-    const int tps = max((tiles.n + nsplit - 1) / nsplit, 1), it0 = blockIdx.y * tps, it1 = min(it0 + tps, tiles.n);
+    const int tps = max((tiles.n + nsplit - 1) / nsplit, 1), it0 = z * tps, it1 = min(it0 + tps, tiles.n);
     const int nz = (tiles.n + tps - 1) / tps;
-    if (blockIdx.y > 0 && it0 >= it1) return;
+    if (z > 0 && it0 >= it1) return;
     const int row = r0 + wave * 32 + li, rc = min(row, rows - 1), tok = rc / G, pos = base + tok;
     // the wave's tokens
     const int w0 = min(r0 + wave * 32, rows - 1) / G, w1 = min(r0 + wave * 32 + 31, rows - 1) / G;
@@ -524,13 +590,13 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
         const long long off = (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * h;
         if constexpr (HL) {
             const float *q = (const float *)a.q + off;
-            float4 x[NS][2];
+            float4 qx[NS][2];
             float mx = 0.f;
 #pragma unroll
             for (int i = 0; i < NS; i++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float4 v = x[i][j] = pg_ld4(q + 16 * i + 4 * j);
+                    const float4 v = qx[i][j] = pg_ld4(q + 16 * i + 4 * j);
                     mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
                 }
             const int sh = pg_row_shift(swap32_max(mx));
@@ -540,7 +606,7 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
             for (int i = 0; i < NS; i++)
 #pragma unroll
                 for (int j = 0; j < 2; j++) {
-                    const float v[4] = {x[i][j].x * f, x[i][j].y * f, x[i][j].z * f, x[i][j].w * f};
+                    const float v[4] = {qx[i][j].x * f, qx[i][j].y * f, qx[i][j].z * f, qx[i][j].w * f};
 #pragma unroll
                     for (int e = 0; e < 4; e++) {
                         qf[0][i][4 * j + e] = (TC)v[e];
@@ -565,21 +631,39 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
     }
     const uint32_t lk = lds_addr(st->k[0]), lv = lds_addr(st->v[0]);
     int pages = -1;   // lane i: the page of block i % 4 of tile i / 4 (of 16 tiles)
+    uint64_t nopage = 0;   // bit i: lane i has none
     auto look_up = [&](int n) {
         const int it = it0 + n + (lane >> 2);
         pages = it < it1 ? pg_block_page(a.pg, s, tiles.at(it) * PC_TS + 16 * (lane & 3), last) : -1;
+        nopage = __builtin_amdgcn_ballot_w64(pages < 0);
     };
+    const int pmask = (1 << a.pg.shift) - 1;
     const long long hbytes = (long long)(2 * D) << a.pg.shift;   // bytes of a kv head in a page
     auto copy = [&](int buf, int n) {
         const int k0 = tiles.at(it0 + n) * PC_TS;
+        auto at = [&](int b) {   // bytes before block b's rows
+            const int page = max(__builtin_amdgcn_readlane(pages, 4 * (n & 15) + b), 0);
+            return ((long long)page * a.pg.NKV + kvh) * hbytes + (long long)((k0 + 16 * b) & pmask) * (2 * D);
+        };
+        const uint32_t to = buf * (PC_TS * D * 2);
+        if (pmask >= PC_TS - 1) {   // the tile lies in one page (uniform)
+            const long long off = at(0);
+            const dma_rsrc_t kr = dma_rsrc((const uint8_t *)a.pg.k + off, PC_TS * 2 * D);
+            const dma_rsrc_t vr = dma_rsrc((const uint8_t *)a.pg.v + off, PC_TS * 2 * D);
 #pragma unroll
-        for (int i = 0; i < CPW; i++) {
-            const int c = wave + PC_WAVES * i, blk = c * RPC / 16;
-            const int page = max(__builtin_amdgcn_readlane(pages, 4 * (n & 15) + blk), 0);
-            const int in = (k0 + 16 * blk) & ((1 << a.pg.shift) - 1);
-            const long long off = ((long long)page * a.pg.NKV + kvh) * hbytes + (long long)in * (2 * D);
-            dma16(lk + buf * (PC_TS * D * 2) + c * 1024, ko[i], dma_rsrc((const uint8_t *)a.pg.k + off, 32 * D), 0);
-            dma16(lv + buf * (PC_TS * D * 2) + c * 1024, vo[i], dma_rsrc((const uint8_t *)a.pg.v + off, 32 * D), 0);
+            for (int i = 0; i < CPW; i++) {
+                const int c = wave + PC_WAVES * i, blk = c * RPC / 16;
+                dma16(lk + to + c * 1024, ko[i], kr, blk * 32 * D);
+                dma16(lv + to + c * 1024, vo[i], vr, blk * 32 * D);
+            }
+        } else {
+#pragma unroll
+            for (int i = 0; i < CPW; i++) {
+                const int c = wave + PC_WAVES * i;
+                const long long off = at(c * RPC / 16);
+                dma16(lk + to + c * 1024, ko[i], dma_rsrc((const uint8_t *)a.pg.k + off, 32 * D), 0);
+                dma16(lv + to + c * 1024, vo[i], dma_rsrc((const uint8_t *)a.pg.v + off, 32 * D), 0);
+            }
         }
     };
     // V's transposing reads: lane l of 16 addresses position kk = l / 4 of 4, dims 4 (l % 4) .. + 4
@@ -609,28 +693,32 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
         dma_wait_barrier();
         for (int n = 0, buf = 0; n < nt; n++, buf ^= 1) {
             const int k0 = tiles.at(it0 + n) * PC_TS;
-            uint64_t has = 0;   // positions of the tile that have a page
-#pragma unroll
-            for (int b = 0; b < 4; b++)
-                has |= __builtin_amdgcn_readlane(pages, 4 * (n & 15) + b) >= 0 ? 0xFFFFull << (16 * b) : 0ull;
+            const int none = (int)(nopage >> (4 * (n & 15))) & 15;   // its blocks without a page
             if (n + 1 < nt) {
                 if (((n + 1) & 15) == 0) look_up(n + 1);
                 copy(buf ^ 1, n + 1);
             }
-            // values that no row of the block sees are made zero
-            const uint64_t dead = ~(pg_seen(k0, plo - back, last, a.sinks) & has);
-            if (dead) {   // uniform
+            // every row of the block sees all of the tile
+            const bool inner = none == 0 && k0 + PC_TS - 1 <= min(plo, last) && (k0 > phi - back || k0 + PC_TS <= a.sinks);
+            uint64_t has = ~0ull;   // positions of the tile that have a page
+            if (!inner) {
 #pragma unroll
-                for (int i = 0; i < PC_TS * SEG / (64 * PC_WAVES); i++) {
-                    const int f = threadIdx.x + 64 * PC_WAVES * i;
-                    if ((dead >> (f / SEG)) & 1) *reinterpret_cast<pg_u4 *>(st->v[buf] + 16 * f) = pg_u4{};
+                for (int b = 0; b < 4; b++) has &= (none >> b) & 1 ? ~(0xFFFFull << (16 * b)) : ~0ull;
+                // values that no row of the block sees are made zero
+                const uint64_t dead = ~(pg_seen(k0, plo - back, last, a.sinks) & has);
+                if (dead) {   // uniform
+#pragma unroll
+                    for (int i = 0; i < PC_TS * SEG / (64 * PC_WAVES); i++) {
+                        const int f = threadIdx.x + 64 * PC_WAVES * i;
+                        if ((dead >> (f / SEG)) & 1) *reinterpret_cast<pg_u4 *>(st->v[buf] + 16 * f) = pg_u4{};
+                    }
+                    __syncthreads();
                 }
-                __syncthreads();
             }
             const int wlo = base + w0, whi = base + w1;
-            if (k0 <= whi && (k0 + PC_TS > wlo - back || k0 < a.sinks)) {   // the wave's rows see some of it
-                const bool whole = has == ~0ull && k0 + PC_TS - 1 <= min(wlo, a.pg.max_kv - 1) &&
-                                   (k0 > whi - back || k0 + PC_TS <= a.sinks);
+            if (inner || (k0 <= whi && (k0 + PC_TS > wlo - back || k0 < a.sinks))) {   // the wave's rows see some of it
+                const bool whole = inner || (has == ~0ull && k0 + PC_TS - 1 <= min(wlo, last) &&
+                                             (k0 > whi - back || k0 + PC_TS <= a.sinks));
                 // the positions that tokens at lo .. hi see, from the lane's 4 h on
                 auto seen = [&](int lo, int hi) {
                     return (pg_seen(k0, lo - back, min(hi, last), a.sinks) & has) >> (4 * h);
@@ -656,7 +744,7 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
 #pragma unroll
                 for (int e = 1; e < 32; e++) mx = fmaxf(mx, sc[e / 16][e % 16]);
                 mx = swap32_max(mx) * cs;
-                if (__builtin_amdgcn_ballot_w64(mx > m)) {
+                if (__builtin_amdgcn_ballot_w64(mx > m + LAG)) {
                     const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
                     m = mn;
                     l *= corr;
@@ -707,7 +795,7 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
         pg_slow_row<TA, TC, D>(a.pg, (const TA *)a.q + (long long)(q0 + t) * a.qs + (long long)(kvh * G + r % G) * D, a.scale,
                                s, kvh, base + t, back, a.sinks, tiles, it0, it1, so, &sm, &sl);
         const long long to = (long long)(q0 + t) * a.NQ + kvh * G + r % G;
-        float *rec = part + (to * nsplit + blockIdx.y) * pg_rec(D);
+        float *rec = part + (to * nsplit + z) * pg_rec(D);
 #pragma unroll
         for (int i = 0; i < D / 64; i++) {
             if (nz <= 1) ((TA *)a.out)[to * D + lane + 64 * i] = (TA)(sl == 0.f ? 0.f : so[i] / sl);
@@ -734,7 +822,7 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
             }
         return;
     }
-    float *rec = part + (at * nsplit + blockIdx.y) * pg_rec(D);
+    float *rec = part + (at * nsplit + z) * pg_rec(D);
 #pragma unroll
     for (int j = 0; j < NT; j++)
 #pragma unroll
@@ -747,74 +835,134 @@ __global__ __launch_bounds__(64 * PC_WAVES) __attribute__((amdgpu_waves_per_eu(2
     }
 }
 
-// Joins the splits of the many-row sequences' rows.  grid = NQ * n_tokens, D threads.
+// Sequences of many rows and, in the first workgroups, of few.  One launch: the
+// few rows' reads run beside the many rows' products.
 template <typename TC, int D, bool HL>
-__global__ __launch_bounds__(D) void k_pg_join_chunk(const PgAttn a, int nsplit, const float *__restrict__ part) {
-    const int hd = blockIdx.x % a.NQ, t = blockIdx.x / a.NQ, d = threadIdx.x, G = a.NQ / a.pg.NKV;
+__global__ __launch_bounds__(64 * PC_WAVES)
+    __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void k_pg_attn_chunk(
+        const PgAttn a, int nrb, int tps, int row_splits, float *__restrict__ row_part, int nsplit,
+        float *__restrict__ part) {
+    extern __shared__ __attribute__((aligned(1024))) unsigned char pc_lds[];
+    const int nrows = a.pg.NKV * nrb, rows = nrows * row_splits * a.pg.n_seqs, x = blockIdx.x;
+    if (x < rows) {
+        const int y = x / nrows;
+        pg_rows<TC, D, HL, false>(a, nrb, tps, row_splits, row_part, x % nrows, y % row_splits, y / row_splits,
+                           reinterpret_cast<PrLds<D> *>(pc_lds));
+    } else {
+        const int y = (x - rows) / a.pg.NKV;
+        pg_chunk<TC, D, HL>(a, nsplit, part, (x - rows) % a.pg.NKV + a.pg.NKV * (y / nsplit), y % nsplit,
+                            reinterpret_cast<PcLds<D> *>(pc_lds));
+    }
+}
+
+// Joins the splits of token t's rows in a sequence of many rows: D / 4 lanes have
+// a head, its at most PC_SPLITS records are loaded at once.
+constexpr int PC_SPLITS = 8;
+template <typename TC, int D, bool HL>
+__device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const float *__restrict__ part, int t) {
+    constexpr int REC = pg_rec(D);
+    const int G = a.NQ / a.pg.NKV;
     const int s = pg_seq_of(a.pg.q_start, a.pg.n_seqs, t);
     if (s >= a.pg.n_seqs || t < a.pg.q_start[s]) return;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
     if (q0 < 0 || qn > a.pg.n_tokens - q0 || (long long)qn * G <= PR_MAX) return;
-    const int rows = qn * G, base = a.pg.kv_len[s] - qn, r0 = ((t - q0) * G + hd % G) / PC_ROWS * PC_ROWS;
-    const int n = pg_tiles<PC_TS>(base + r0 / G, base + (min(r0 + PC_ROWS, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n;
-    const int tps = max((n + nsplit - 1) / nsplit, 1), nz = (n + tps - 1) / tps;
-    if (nz <= 1) return;
-    const long long at = (long long)t * a.NQ + hd;
-    const float *rec = part + at * nsplit * pg_rec(D);
-    float M = PG_LOW;
-    for (int i = 0; i < nz; i++) M = fmaxf(M, rec[i * pg_rec(D) + D]);
-    float num = 0.f, den = 0.f;
-#pragma unroll 4
-    for (int i = 0; i < nz; i++) {
-        const float f = __builtin_amdgcn_exp2f(rec[i * pg_rec(D) + D] - M);
-        num = fmaf(f, rec[i * pg_rec(D) + d], num);
-        den = fmaf(f, rec[i * pg_rec(D) + D + 1], den);
+    const int rows = qn * G, base = a.pg.kv_len[s] - qn;
+    for (int i = threadIdx.x; i < a.NQ * (D / 4); i += PJ_THREADS) {
+        const int hd = i / (D / 4), d = i % (D / 4) * 4;
+        const int r0 = ((t - q0) * G + hd % G) / PC_ROWS * PC_ROWS;
+        const int n = pg_tiles<PC_TS>(base + r0 / G, base + (min(r0 + PC_ROWS, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n;
+        const int tps = max((n + nsplit - 1) / nsplit, 1), nz = (n + tps - 1) / tps;
+        if (nz <= 1) continue;
+        const long long at = (long long)t * a.NQ + hd;
+        const float *rec = part + at * nsplit * REC;
+        float2 ml[PC_SPLITS];
+        float4 y[PC_SPLITS];
+        float M = PG_LOW;
+#pragma unroll
+        for (int z = 0; z < PC_SPLITS; z++) {   // past the last: the last again, not added
+            ml[z] = *reinterpret_cast<const float2 *>(rec + min(z, nz - 1) * REC + D);
+            y[z] = *reinterpret_cast<const float4 *>(rec + min(z, nz - 1) * REC + d);
+            M = fmaxf(M, ml[z].x);
+        }
+        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+        float den = 0.f;
+#pragma unroll
+        for (int z = 0; z < PC_SPLITS; z++) {
+            if (z >= nz) continue;
+            const float f = __builtin_amdgcn_exp2f(ml[z].x - M);
+            x = make_float4(fmaf(f, y[z].x, x.x), fmaf(f, y[z].y, x.y), fmaf(f, y[z].z, x.z), fmaf(f, y[z].w, x.w));
+            den = fmaf(f, ml[z].y, den);
+        }
+        const float inv = den == 0.f ? 0.f : 1.0f / den;
+        x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
+        if constexpr (HL) pg_st4((float *)a.out + at * D + d, x);
+        else pg_st4((TC *)a.out + at * D + d, x);
     }
-    const float x = den == 0.f ? 0.f : num / den;
-    if constexpr (HL) ((float *)a.out)[at * D + d] = x;
-    else ((TC *)a.out)[at * D + d] = (TC)x;
+}
+
+// grid: row_wgs = NKV * (most rows of a few-row sequence) * n_seqs workgroups for
+// few rows (0: they were not split), then one a token (none if the many rows were
+// not split).
+template <typename TC, int D, bool HL>
+__global__ __launch_bounds__(PJ_THREADS) void k_pg_join(const PgAttn a, int nrb, int tps, int row_splits,
+                                                        const float *__restrict__ row_part, int row_wgs, int most,
+                                                        int nsplit, const float *__restrict__ part) {
+    const int x = blockIdx.x, n = a.pg.NKV * most;
+    if (x < row_wgs) pg_join_rows<TC, D, HL>(a, nrb, tps, row_splits, row_part, x % n, x / n);
+    else pg_join_chunk<TC, D, HL>(a, nsplit, part, x - row_wgs);
 }
 
 // ---------------------------------------------------------------------------
 // Host side: the splits, by what the host knows (max_q, max_kv, n_tokens).
 // ---------------------------------------------------------------------------
 struct PgPlan {
-    int nrb, row_tps, row_splits;   // few rows: row blocks, tiles of a split, splits
-    bool chunks;                    // whether a sequence can have many rows
+    int most, nrb, row_tps, row_splits;   // few rows: most rows, row blocks, tiles of a split, splits
+    bool chunks;                          // whether a sequence can have many rows
     int blocks, chunk_splits;
-    size_t rows_bytes, bytes;       // workspace: the few rows' records, then the others'
+    size_t rows_bytes, bytes;             // workspace: the few rows' records, then the others'
 };
 
 static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32) {
     PgPlan p{};
     const int G = NQ / a.NKV, RB = f32 ? 8 : 16, cu = 256;
-    const long long most = std::min((long long)a.max_q * G, (long long)PR_MAX);
-    p.nrb = (int)((most + RB - 1) / RB);
+    p.most = (int)std::min((long long)a.max_q * G, (long long)PR_MAX);
+    p.nrb = (p.most + RB - 1) / RB;
     // positions that one block can see
     long long seen = a.max_kv;
     if (window > 0) seen = std::min(seen, (long long)window + sinks + 2 * PC_TS + std::min(a.max_q, PC_ROWS));
     const long long tiles = (seen + PR_TS - 1) / PR_TS + 1;
-    const long long wgs = (long long)a.NKV * p.nrb * a.n_seqs;
-    long long want = std::max(1ll, (4 * cu + wgs - 1) / wgs);
-    long long tps = (tiles + want - 1) / want;
-    tps = std::max(4ll, (tps + 3) / 4 * 4);
+    // Two workgroups a CU run at once, so at least as many splits as fill them.  Longer ranges than
+    // PR_LONG make the last workgroups of a ragged batch late (64 sequences of up to 8192 in ranges of
+    // 512 / 2048 / 4096 / 8192 positions: 212 / 210 / 218 / 295 us), shorter ones add to the join
+    // (one token over 131072: 58 us with 128 ranges, 66 with 256).
+    const long long wgs = (long long)a.NKV * p.nrb * a.n_seqs, want = (2 * cu + wgs - 1) / wgs;
+    auto splits = [&](long long tps) { return (tiles + tps - 1) / tps; };
+    long long tps = std::max((long long)PR_MIN, std::min((long long)PR_LONG, ((tiles + want - 1) / want + 3) / 4 * 4));
+    if (splits(tps) > PJ_MAX) tps = (tiles + PJ_MAX - 1) / PJ_MAX;
     p.row_tps = (int)tps;
-    p.row_splits = (int)((tiles + tps - 1) / tps);
-    if (p.row_splits > 1) p.rows_bytes = (size_t)a.n_seqs * a.NKV * p.nrb * RB * p.row_splits * pg_rec(D) * 4;
+    p.row_splits = (int)splits(tps);
+    // room for the most splits that any window can lead to
+    const long long all = ((long long)a.max_kv + PR_TS - 1) / PR_TS + 1;
+    const long long room = std::min((long long)PJ_MAX, std::max(std::min(want, (all + PR_MIN - 1) / PR_MIN),
+                                                                (all + PR_LONG - 1) / PR_LONG));
+    if (room > 1) p.rows_bytes = (size_t)a.n_seqs * a.NKV * p.nrb * RB * room * pg_rec(D) * 4;
     p.chunks = (long long)a.max_q * G > PR_MAX;
     p.bytes = p.rows_bytes;
+    p.chunk_splits = 1;
     if (p.chunks) {
-        p.blocks = (int)(((long long)a.n_tokens * G + PC_ROWS - 1) / PC_ROWS) + a.n_seqs;
-        const long long w = (long long)a.NKV * (((long long)a.n_tokens * G + PC_ROWS - 1) / PC_ROWS);
+        const long long full = ((long long)a.n_tokens * G + PC_ROWS - 1) / PC_ROWS, w = a.NKV * full;
+        p.blocks = (int)full + a.n_seqs;
+        // two workgroups a CU, each with 8 tiles at least: a workgroup's start and its share of the
+        // join cost as much as about 4 (1 / 4 prompts of 512 / 100 tokens after 3584 / 1000)
         const long long t = (seen + PC_TS - 1) / PC_TS;
-        p.chunk_splits = (int)std::max(1ll, std::min(std::min(8ll, (2 * cu + w - 1) / w), t / 2));
+        p.chunk_splits = (int)std::max(1ll, std::min(std::min((long long)PC_SPLITS, 2 * cu / w), t / 8));
         if (p.chunk_splits > 1) p.bytes += (size_t)a.n_tokens * NQ * p.chunk_splits * pg_rec(D) * 4;
     }
     return p;
 }
 
-// Without the window: a plan with one sees no more positions, so it has no more
-// tiles, but may split them less; its records fit.
+// What a call with any window needs: the rows' room does not depend on it, and
+// the chunks' splits only fall with it.
 size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32) {
     if (a.n_seqs == 0 || a.n_tokens == 0) return 0;
     return pg_plan(a, D, NQ, 0, 0, f32).bytes;
@@ -823,22 +971,31 @@ size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32) {
 template <typename TC, int D, bool HL>
 static hipError_t pg_attn(const PgAttn &a, float *ws, hipStream_t st) {
     const PgPlan p = pg_plan(a.pg, D, a.NQ, a.window, a.sinks, HL);
-    constexpr int RB = HL ? 8 : 16;
-    hipLaunchKernelGGL((k_pg_attn_rows<TC, D, HL>), dim3(a.pg.NKV * p.nrb, p.row_splits, a.pg.n_seqs), dim3(64 * PR_WAVES),
-                       0, st, a, p.nrb, p.row_tps, p.row_splits, ws);
-    if (p.row_splits > 1)
-        hipLaunchKernelGGL((k_pg_join_rows<TC, D, HL>), dim3(a.pg.NKV * std::min(p.nrb * RB, PR_MAX), a.pg.n_seqs), dim3(D), 0,
-                           st, a, p.nrb, p.row_tps, p.row_splits, ws);
-    if (p.chunks) {
+    float *part = ws + p.rows_bytes / 4;
+    if (!p.chunks) {
+        const dim3 grid(a.pg.NKV * p.nrb, p.row_splits, a.pg.n_seqs);
+        if (p.nrb == 1)
+            hipLaunchKernelGGL((k_pg_attn_rows<TC, D, HL, true>), grid, dim3(64 * PR_WAVES), 0, st, a, p.nrb, p.row_tps,
+                               p.row_splits, ws);
+        else
+            hipLaunchKernelGGL((k_pg_attn_rows<TC, D, HL, false>), grid, dim3(64 * PR_WAVES), 0, st, a, p.nrb, p.row_tps,
+                               p.row_splits, ws);
+    } else {
+        constexpr int lds = std::max(sizeof(PcLds<D>), sizeof(PrLds<D>));
         static const hipError_t e = hipFuncSetAttribute((const void *)k_pg_attn_chunk<TC, D, HL>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PcLds<D>));
+                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
         if (e != hipSuccess) return e;
-        float *part = ws + p.rows_bytes / 4;
-        hipLaunchKernelGGL((k_pg_attn_chunk<TC, D, HL>), dim3(a.pg.NKV * p.blocks, p.chunk_splits), dim3(64 * PC_WAVES),
-                           sizeof(PcLds<D>), st, a, p.chunk_splits, part);
-        if (p.chunk_splits > 1)
-            hipLaunchKernelGGL((k_pg_join_chunk<TC, D, HL>), dim3(a.NQ * a.pg.n_tokens), dim3(D), 0, st, a, p.chunk_splits, part);
+        const long long wgs = (long long)a.pg.NKV * ((long long)p.nrb * p.row_splits * a.pg.n_seqs +
+                                                     (long long)p.blocks * p.chunk_splits);
+        if (wgs > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+        hipLaunchKernelGGL((k_pg_attn_chunk<TC, D, HL>), dim3((unsigned)wgs), dim3(64 * PC_WAVES), lds, st, a, p.nrb,
+                           p.row_tps, p.row_splits, ws, p.chunk_splits, part);
     }
+    const int row_wgs = p.row_splits > 1 ? a.pg.NKV * p.most * a.pg.n_seqs : 0;
+    const int wgs = row_wgs + (p.chunk_splits > 1 ? a.pg.n_tokens : 0);
+    if (wgs > 0)
+        hipLaunchKernelGGL((k_pg_join<TC, D, HL>), dim3(wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps, p.row_splits, ws,
+                           row_wgs, p.most, p.chunk_splits, part);
     return hipGetLastError();
 }
 
