@@ -2,7 +2,8 @@
  * tbq_kv.h -- a paged key/value cache for many sequences, and the operators
  * that work on it: rotary positions with the append of new keys and values,
  * causal attention of new tokens over the pages (whole, or a sliding window
- * with sinks), page copies, row compaction, and a host-side page pool.  No counterpart in the reference,
+ * with sinks), page copies, row compaction, a host-side page pool, and the
+ * dense model's forward over such a cache.  No counterpart in the reference,
  * whose cache is one contiguous fp32 buffer of one sequence
  * (layer1/tb_tensor.c:229-291).
  *
@@ -170,6 +171,29 @@ int tbq_kv_pool_fork(tbq_kv_pool *p, int positions, int page_size, const int *pa
  * caller replaces src[i] by dst[i] in every page table.  Returns their
  * number (-1: error). */
 int tbq_kv_pool_defrag(tbq_kv_pool *p, int max, int *src, int *dst);
+
+/* ---- dense model over a paged cache ------------------------------------------- */
+/* The forward of tbq_dense_decode / tbq_dense_prefill (same model struct; its
+ * max_ctx, k_cache and v_cache are not used) for n_seqs sequences at once:
+ * sequence s's n_new[s] >= 1 tokens follow each other in tokens, kv_len[s]
+ * counts its positions with them, and page_table is [n_seqs][max_pages].
+ * n_new, kv_len, page_table and tokens are host arrays, read before
+ * the call returns.  Writes every
+ * layer's K and V rows and logits[s][vocab] of each sequence's last token.
+ * The cache is F16 and has the model's layers, kv heads and head_dim.  rope
+ * NULL: the model's theta on the whole head in halves.  window, sinks: as
+ * tbq_attn_paged, in every layer.  One token of one sequence runs on the
+ * decode step's matvecs (logits as exact as the fp16 cache lets them be),
+ * more on the batched prefill's fp16 products (within 1e-2 relative L2), for
+ * models whose rows those hold (tbq_dense_prefill_batched); others run one
+ * token after the other.  The workspace size covers every call with at most
+ * that many sequences, tokens and pages; n_tokens at most 65536, n_seqs at
+ * most 1024. */
+size_t tbq_dense_step_workspace_size(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int n_tokens,
+                                     int max_pages);
+int tbq_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new, const int *kv_len,
+                   const int *page_table, int max_pages, const int *tokens, const tbq_rope *rope, int window,
+                   int sinks, float *logits, void *workspace, size_t workspace_bytes, void *stream);
 
 #ifdef __cplusplus
 }

@@ -1,0 +1,292 @@
+"""GPU parity of tbq_dense_step (the dense model's forward over a paged
+cache for several sequences, include/tbq_kv.h) against the float64 oracle of
+oracle/dense.py with a cache of its own per sequence: prompts, chunks and
+single tokens in one call, forks, compaction, defragmentation, windows and
+rotations, as a server would use them together.
+
+Tolerances.  STEP_TOL: the matvecs' path with keys and values rounded to fp16
+(half a step is 2^-11): values change the attention's output by at most
+2^-11 of their size, keys the scores by 2^-11 |s|, |s| of 1 to 3 here, so a
+layer's output by below 4 * 2^-11 = 2e-3 of the attention's share, two layers
+4e-3.  BATCH_TOL: the fp16 products of the batched prefill (the same 1e-2 as
+tbq_dense_prefill's)."""
+import numpy as np
+import pytest
+
+import trailblaze_amd as tb
+from conftest import rel_l2
+from gpu_util import host
+from trailblaze_amd import formats as fm
+from trailblaze_amd import paged
+
+pytestmark = pytest.mark.gpu
+STEP_TOL, BATCH_TOL = 5e-3, 1e-2
+
+
+@pytest.fixture(scope="module", autouse=True)
+def _init():
+    print("device:", tb.init(), flush=True)
+
+
+def _model(oracle, seed=1, **kw):
+    from oracle.dense import DenseOracle
+    from trailblaze_amd.dense import DenseConfig, SyntheticDense
+    base = dict(n_layers=2, hidden=256, n_heads=4, n_kv_heads=2, head_dim=64, ffn=512, vocab=512, max_ctx=512)
+    base.update(kw)
+    cfg = DenseConfig(**base)
+    m = SyntheticDense(cfg, seed, keep_host=True)
+    return m, Model(DenseOracle(oracle, cfg, m.host))
+
+
+class Model:
+    """DenseOracle's forward over a cache handed to it, with a rotation and a window."""
+
+    def __init__(self, ref):
+        self.ref, self.cfg = ref, ref.cfg
+        self.freq, self.mscale, self.interleaved = None, 1.0, False
+        self.window = self.sinks = 0
+
+    def rope(self, x, pos):
+        D = x.shape[-1]
+        f = self.cfg.rope_theta ** (-2.0 * np.arange(D // 2) / D) if self.freq is None else self.freq
+        j, n = np.arange(len(f)), len(f)
+        u, w = (2 * j, 2 * j + 1) if self.interleaved else (j, j + n)
+        c, s = np.cos(pos * f) * self.mscale, np.sin(pos * f) * self.mscale
+        y = x.copy()
+        y[..., u], y[..., w] = x[..., u] * c - x[..., w] * s, x[..., u] * s + x[..., w] * c
+        return y
+
+    def decode(self, cache, token, rng=None):
+        """Appends the token to cache = [K, V], each [layers][positions] of [kv heads][D].  rng: every
+        operand that the batched path holds in fp16 is off by half a step, 2^-11, up or down at
+        random: weights by that of the largest of their 32 (the GEMM's Q4_K form of them), others by
+        that of themselves."""
+        off = lambda x: x if rng is None else x * (1 + 2.0 ** -11 * rng.choice([-1.0, 1.0], x.shape))   # noqa: E731
+
+        def mul(W, h):
+            if rng is not None:
+                big = np.abs(W).reshape(len(W), -1, 32).max(-1, keepdims=True)
+                W = W + (2.0 ** -11 * big * rng.choice([-1.0, 1.0], (len(W), W.shape[1] // 32, 32))).reshape(W.shape)
+            return W @ off(h)
+        from oracle.dense import attention, rmsnorm, silu_mul
+        c, r = self.cfg, self.ref
+        D, NQ, NKV = c.head_dim, c.n_heads, c.n_kv_heads
+        x, pos = r.lm[token].copy(), len(cache[0][0])
+        seen = [p for p in range(pos + 1) if not self.window or p > pos - self.window or p < self.sinks]
+        for l, L in enumerate(r.layers):
+            qkv = mul(L["wqkv"], rmsnorm(x, L["attn_norm"], c.norm_eps)).reshape(NQ + 2 * NKV, D)
+            q = off(self.rope(np.stack([rmsnorm(v, L["q_norm"], c.norm_eps) for v in qkv[:NQ]]), pos))
+            k = off(self.rope(np.stack([rmsnorm(v, L["k_norm"], c.norm_eps) for v in qkv[NQ:NQ + NKV]]), pos))
+            cache[0][l].append(k)
+            cache[1][l].append(off(qkv[NQ + NKV:].copy()))
+            K, V = (np.stack([t[l][p] for p in seen], 1) for t in cache)
+            x = x + mul(L["wo"], attention(q, K, V, len(seen)).reshape(-1))
+            gu = mul(L["wgu"], rmsnorm(x, L["ffn_norm"], c.norm_eps))
+            x = x + mul(L["wdown"], silu_mul(gu[:c.ffn], gu[c.ffn:]))
+        return r.lm @ rmsnorm(x, r.output_norm, c.norm_eps)
+
+    def magnified(self, tokens, want):
+        """How far half a step in every fp16 operand takes this prompt's logits: the largest of 8 random
+        ways.  Roundings are half a step at most and 0.58 of one on average, so theirs is below twice
+        that."""
+        err = 0.0
+        for i in range(8):
+            cache, rng = self.empty(), np.random.default_rng(i)
+            for t in tokens:
+                got = self.decode(cache, t, rng)
+            err = max(err, rel_l2(got, want))
+        return 2 * err
+
+    def empty(self):
+        return [[[] for _ in range(self.cfg.n_layers)] for _ in range(2)]
+
+
+class Server:
+    """Sequences over one paged cache and the oracle's caches beside them."""
+
+    def __init__(self, m, model, n_pages=40, page=16):
+        self.m, self.model, self.page = m, model, page
+        self.cache, self.pool = m.paged_cache(n_pages, page), paged.PagePool(n_pages)
+        for t in self.cache._keep:
+            t.fill_(float("nan"))   # what nobody has written must not show
+        self.pages, self.len, self.ref = [], [], []
+
+    def add(self):
+        self.pages.append([])
+        self.len.append(0)
+        self.ref.append(self.model.empty())
+        return len(self.len) - 1
+
+    def table(self, seqs, width=None):
+        width = width or max(len(self.pages[s]) for s in seqs)
+        return [self.pages[s] + [-1] * (width - len(self.pages[s])) for s in seqs]
+
+    def step(self, work, tol, **kw):
+        """work: {sequence: its new tokens}."""
+        import torch
+        seqs = list(work)
+        for s in seqs:
+            self.len[s] += len(work[s])
+            need = -(-self.len[s] // self.page) - len(self.pages[s])
+            if need > 0:
+                self.pages[s] += self.pool.alloc(need)
+        logits = torch.full((len(seqs), self.m.cfg.vocab), float("nan"), device="cuda")
+        print("step", {s: (len(work[s]), self.len[s]) for s in seqs}, flush=True)
+        self.m.step(self.cache, [len(work[s]) for s in seqs], [self.len[s] for s in seqs], self.table(seqs),
+                    [t for s in seqs for t in work[s]], logits, **kw)
+        got = host(logits)
+        for i, s in enumerate(seqs):
+            for t in work[s]:
+                want = self.model.decode(self.ref[s], t)
+            err = rel_l2(got[i], want)
+            assert err <= tol, (s, err)
+        self.check_rows(seqs, tol)
+
+    def check_rows(self, seqs, tol):
+        k, v = (host(t) for t in self.cache._keep)
+        for s in seqs:
+            for t, r in ((k, 0), (v, 1)):
+                rows = [p for p in range(self.len[s]) if self.pages[s][p // self.page] >= 0]
+                got = np.stack([t[:, self.pages[s][p // self.page], :, p % self.page] for p in rows])
+                want = np.stack([np.stack([self.ref[s][r][l][p] for l in range(self.m.cfg.n_layers)]) for p in rows])
+                assert rel_l2(got, want) <= tol
+
+
+def _tokens(rng, n):
+    return [int(t) for t in rng.integers(0, 512, n)]
+
+
+def test_single_sequence_decode(oracle):
+    m, model = _model(oracle)
+    s, rng = Server(m, model), np.random.default_rng(1)
+    a = s.add()
+    for t in _tokens(rng, 20):
+        s.step({a: [t]}, STEP_TOL)
+
+
+@pytest.mark.parametrize("kw", [dict(head_dim=128, n_heads=8, n_kv_heads=2, hidden=512), dict(qtype_layers=fm.Q6_K),
+                                dict(n_heads=8, n_kv_heads=1, qtype_layers=fm.GGML | fm.Q4_K)])
+def test_prompts_and_tokens_in_one_call(oracle, kw):
+    m, model = _model(oracle, seed=3, **kw)
+    s, rng = Server(m, model), np.random.default_rng(2)
+    a, b, c = s.add(), s.add(), s.add()
+    s.step({a: _tokens(rng, 40), b: _tokens(rng, 1)}, BATCH_TOL)
+    s.step({b: _tokens(rng, 17), c: _tokens(rng, 100), a: _tokens(rng, 1)}, BATCH_TOL)
+    s.step({a: _tokens(rng, 1), b: _tokens(rng, 1), c: _tokens(rng, 1)}, BATCH_TOL)
+    s.step({c: _tokens(rng, 1)}, BATCH_TOL)   # earlier rows came from the fp16 products
+
+
+def test_fork_compact_and_defragment(oracle):
+    """A served run: two prompts, a fork with its copied page, drafted tokens
+    of which one branch stays, a sequence that ends, pages moved together."""
+    import torch
+    m, model = _model(oracle, seed=4)
+    s, rng = Server(m, model), np.random.default_rng(3)
+    a, b = s.add(), s.add()
+    s.step({a: _tokens(rng, 37), b: _tokens(rng, 20)}, BATCH_TOL)
+    c = s.add()
+    s.pages[c], copy = s.pool.fork(s.len[a], s.page, s.pages[a])
+    assert copy is not None
+    paged.kv_copy_pages(s.cache, [copy[0]], [copy[1]])
+    s.len[c], s.ref[c] = s.len[a], [[list(rows) for rows in t] for t in s.ref[a]]
+    s.step({a: _tokens(rng, 1), b: _tokens(rng, 1), c: _tokens(rng, 1)}, BATCH_TOL)
+    s.step({a: _tokens(rng, 6), c: _tokens(rng, 4)}, BATCH_TOL)          # drafts
+    keep = [list(range(39)) + [40, 43], list(range(38)) + [41]]
+    ints = lambda v: torch.tensor(v, dtype=torch.int32, device="cuda")   # noqa: E731
+    paged.kv_compact(s.cache, ints(s.table([a, c])), ints([0, 41, 80]), ints(keep[0] + keep[1]))
+    for q, rows in zip((a, c), keep):
+        s.len[q] = len(rows)
+        s.ref[q] = [[[t[p] for p in rows] for t in side] for side in s.ref[q]]
+        n = -(-s.len[q] // s.page)
+        s.pool.release(s.pages[q][n:])
+        s.pages[q] = s.pages[q][:n]
+    s.check_rows([a, c], BATCH_TOL)
+    s.pool.release(s.pages[b])
+    moves = s.pool.defrag(40)
+    assert moves
+    paged.kv_copy_pages(s.cache, [x for x, _ in moves], [y for _, y in moves])
+    to = dict(moves)
+    for q in (a, c):
+        s.pages[q] = [to.get(p, p) for p in s.pages[q]]
+    s.step({c: _tokens(rng, 3), a: _tokens(rng, 2)}, BATCH_TOL)
+    s.step({a: _tokens(rng, 1), c: _tokens(rng, 1)}, BATCH_TOL)
+
+
+def test_window_with_freed_pages(oracle):
+    m, model = _model(oracle, seed=5)
+    model.window, model.sinks = 20, 3
+    s, rng = Server(m, model), np.random.default_rng(4)
+    a, b = s.add(), s.add()
+    s.step({a: _tokens(rng, 70), b: _tokens(rng, 9)}, BATCH_TOL, window=20, sinks=3)
+    s.pages[a][1] = s.pages[a][2] = -1    # positions 16..47: behind the window of 71 and on
+    s.step({a: _tokens(rng, 1), b: _tokens(rng, 30)}, BATCH_TOL, window=20, sinks=3)
+    s.step({a: _tokens(rng, 1)}, BATCH_TOL, window=20, sinks=3)
+    with pytest.raises(tb.TbqError, match="page -1"):
+        s.step({a: _tokens(rng, 1)}, BATCH_TOL)   # without a window it would see them
+
+
+@pytest.mark.parametrize("layout,rot,scaling", [("interleaved", 64, "none"), ("half", 32, "yarn")])
+def test_rotations(oracle, layout, rot, scaling):
+    from paged_ref import frequencies
+    m, model = _model(oracle, seed=6)
+    kw = dict(factor=4.0, orig_ctx=64) if scaling == "yarn" else {}
+    f, model.mscale = frequencies(rot, 1e4, scaling, **kw)
+    model.freq, model.interleaved = f.numpy(), layout == "interleaved"
+    s, rng = Server(m, model), np.random.default_rng(5)
+    a, b = s.add(), s.add()
+    rope = paged.rope(rot, 1e4, layout=layout, scaling=scaling, **kw)
+    for t in _tokens(rng, 4):
+        s.step({a: [t]}, STEP_TOL, rope=rope)
+    s.step({a: _tokens(rng, 5), b: _tokens(rng, 33)}, BATCH_TOL, rope=rope)
+
+
+def test_models_beyond_the_batched_rows(oracle):
+    """hidden 8448: one token after the other on the decode step's matvecs."""
+    m, model = _model(oracle, seed=7, n_layers=1, hidden=8448, ffn=256, vocab=512)
+    assert not m.prefill_batched()
+    s, rng = Server(m, model), np.random.default_rng(6)
+    a, b = s.add(), s.add()
+    s.step({a: _tokens(rng, 18), b: _tokens(rng, 2)}, STEP_TOL)
+    s.step({a: _tokens(rng, 1), b: _tokens(rng, 1)}, STEP_TOL)
+
+
+def test_many_sequences(oracle):
+    """More sequences than the 256 whose starts travel in one launch."""
+    m, model = _model(oracle, seed=8, n_layers=1)
+    import torch
+    n = 300
+    cache = m.paged_cache(n)
+    rng = np.random.default_rng(7)
+    n_new = [1 + i % 3 for i in range(n)]
+    toks = _tokens(rng, sum(n_new))
+    logits = torch.empty(n, 512, device="cuda")
+    m.step(cache, n_new, n_new, [[i] for i in range(n)], toks, logits)
+    got, at = host(logits), 0
+    for i in range(n):
+        ref = model.empty()
+        mine = toks[at:at + n_new[i]]
+        for t in mine:
+            want = model.decode(ref, t)
+        at += n_new[i]
+        err = rel_l2(got[i], want)
+        # a few of these prompts of two or three tokens magnify the roundings of their products
+        # (synthetic weights whose rows have a mean: sums that nearly cancel)
+        assert err <= BATCH_TOL or err <= model.magnified(mine, want), (i, err)
+
+
+def test_step_is_reproducible_and_takes_other_streams(oracle):
+    import torch
+    m, _ = _model(oracle, seed=9)
+    rng = np.random.default_rng(8)
+    toks = _tokens(rng, 50)
+    out = []
+    for i in range(3):
+        cache = m.paged_cache(8, 16)
+        logits = torch.empty(2, 512, device="cuda")
+        st = torch.cuda.Stream() if i == 2 else torch.cuda.current_stream()
+        st.wait_stream(torch.cuda.current_stream())
+        m.step(cache, [45, 5], [45, 5], [[4, 1, 7], [2, -1, -1]], toks, logits, stream=st)
+        st.synchronize()
+        out.append((host(logits), host(cache._keep[0]), host(cache._keep[1])))
+    for o in out[1:]:
+        assert all(np.array_equal(x, y) for x, y in zip(out[0], o))

@@ -226,3 +226,67 @@ def test_nothing_to_do_is_done():
         assert append(c, b) == 1 and attn(c, b) == 1
     assert tb.lib().tbq_kv_copy_pages(C.byref(c), None, None, 0, None) == 1
     assert tb.lib().tbq_kv_compact(C.byref(c), 0, None, 4, None, None, None) == 1
+
+
+# ---- the dense step ----------------------------------------------------------------
+def _dense():
+    from trailblaze_amd import formats as fm
+    from trailblaze_amd.dense import DenseLayer, DenseModel
+    layers = (DenseLayer * 2)()
+    for L in layers:
+        for name in ("attn_norm", "q_norm", "k_norm", "ffn_norm", "wqkv", "wo", "wgu", "wdown"):
+            setattr(L, name, FAKE)
+    m = DenseModel(2, 512, 8, 2, 128, 512, 1000, 0, 1e-6, 1e6, fm.Q4_K, fm.Q6_K, FAKE, FAKE, FAKE, layers, None, None)
+    m._layers = layers
+    return m
+
+
+def step(m, c, n_new=(3, 1), kv_len=(20, 1), table=((0, 1), (2, -1)), tokens=(1, 2, 3, 4), rope=None, window=0, sinks=0,
+         logits=FAKE, ws=FAKE, wsb=1 << 40, n=None):
+    a = lambda v: (C.c_int * len(v))(*v)   # noqa: E731
+    return tb.lib().tbq_dense_step(C.byref(m), C.byref(c), len(n_new) if n is None else n, a(n_new), a(kv_len),
+                                   a([p for r in table for p in r]), len(table[0]), a(tokens),
+                                   None if rope is None else C.byref(rope), window, sinks, logits, ws, wsb, None)
+
+
+@pytest.mark.parametrize("kw,words", [
+    (dict(n=0), "sequences"), (dict(n=1025), "sequences"), (dict(n_new=(0, 1)), "new tokens"), (dict(kv_len=(2, 1)), "new tokens"),
+    (dict(kv_len=(33, 1)), "new tokens"), (dict(table=((0, 8), (2, -1))), "page 8"), (dict(table=((-1, 1), (2, -1))), "page -1"),
+    (dict(table=((-1, 1), (2, -1)), window=4, sinks=1), "page -1"), (dict(tokens=(1, 2, 3, 1000)), "token 1000"),
+    (dict(tokens=(-1, 2, 3, 4)), "token -1"), (dict(window=-1), "window"), (dict(sinks=-2), "sinks"), (dict(logits=None), "null"),
+    (dict(ws=FAKE + 8), "misaligned"), (dict(wsb=100), "workspace"), (dict(rope=paged.Rope(4, 0, 1.0)), "rope")])
+def test_dense_step_refusals(kw, words):
+    refused(step(_dense(), cache(), **kw), words)
+
+
+@pytest.mark.parametrize("kw,words", [(dict(type=30), "cache type"), (dict(n_layers=3), "a cache of"), (dict(n_kv_heads=4), "a cache of"),
+                                      (dict(head_dim=64), "a cache of"), (dict(page_size=48), "page_size")])
+def test_dense_step_cache_refusals(kw, words):
+    refused(step(_dense(), cache(**kw)), words)
+
+
+def test_dense_step_workspace_serves_every_smaller_call():
+    m, c = _dense(), cache(page_size=64)
+    size = lambda *a: tb.lib().tbq_dense_step_workspace_size(C.byref(m), C.byref(c), *a)   # noqa: E731
+    assert size(2, 1, 4) == 0 and size(1, 65537, 4) == 0 and size(1025, 2000, 4) == 0 and size(1, 1, 0) == 0
+    rng = random.Random(3)
+    for _ in range(2000):
+        n = rng.randrange(1, 200)
+        a = (n, rng.randrange(n, 3000), rng.randrange(1, 300))
+        s = rng.randrange(1, a[0] + 1)
+        b = (s, rng.randrange(s, a[1] + 1), rng.randrange(1, a[2] + 1))
+        assert 0 < size(*b) <= size(*a), (a, b)
+
+
+def test_attention_workspace_is_within_the_steps():
+    """What tbq_attn_paged asks for a batch never exceeds the room that the step sets aside
+    for one of that size: the step's size less that of the same step with hardly any room."""
+    m = _dense()
+    rng = random.Random(5)
+    for _ in range(500):
+        page, pages, n = 64, rng.randrange(1, 400), rng.randrange(1, 300)
+        T = n if rng.random() < 0.5 else rng.randrange(n, 5000)
+        c = cache(page_size=page)
+        b = batch(n_seqs=n, n_tokens=T, max_pages=pages, max_q=0 if T > n else 1)
+        need = tb.lib().tbq_attn_paged_workspace_size(C.byref(c), C.byref(b), 8, 1)
+        assert need <= tb.lib().tbq_dense_step_workspace_size(C.byref(m), C.byref(c), n, max(T, 2), pages)

@@ -68,6 +68,8 @@ SYMBOLS = {
     "tbq_attn_paged": (_i, [_vp, _i, _vp, _i, _i, _vp, _ll, _vp, _i, _i, _f, _vp, _sz, _vp]),
     "tbq_kv_copy_pages": (_i, [_vp, _vp, _vp, _i, _vp]),
     "tbq_kv_compact": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp]),
+    "tbq_dense_step_workspace_size": (_sz, [_vp, _vp, _i, _i, _i]),
+    "tbq_dense_step": (_i, [_vp, _vp, _i, _vp, _vp, _vp, _i, _vp, _vp, _i, _i, _vp, _vp, _sz, _vp]),
     "tbq_kv_pool_create": (_vp, [_i]),
     "tbq_kv_pool_destroy": (None, [_vp]),
     "tbq_kv_pool_free_pages": (_i, [_vp]),

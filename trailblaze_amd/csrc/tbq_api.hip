@@ -10,8 +10,10 @@
 #include <string.h>
 
 #include "../../include/tbq.h"
+#include "../../include/tbq_kv.h"
 #include "tbq_device.hpp"
 #include "tbq_kernels.h"
+#include "tbq_paged.hpp"
 
 using namespace tbq;
 
@@ -387,16 +389,17 @@ int tbq_moe_forward(const tbq_moe_layer *L, int T, const float *xn, const float 
     return hip_ok(launch_moe_fp32(a, S(s)), "moe launch");
 }
 
-static int check_dense(const tbq_dense_model *m) {
+// paged: the model's own cache (max_ctx, k_cache, v_cache) is not used.
+static int check_dense(const tbq_dense_model *m, bool paged = false) {
     if (!m || !m->layers) return fail("tbq_dense: null model");
     if (m->n_layers <= 0 || m->hidden <= 0 || m->n_heads <= 0 || m->n_kv_heads <= 0 || m->ffn <= 0 || m->vocab <= 0 ||
-        m->max_ctx <= 0)
+        (!paged && m->max_ctx <= 0))
         return fail("tbq_dense: non-positive size");
     if (m->head_dim != 64 && m->head_dim != 128) return fail("tbq_dense: head_dim must be 64 or 128");
     const int G = m->n_heads / m->n_kv_heads;
     if (m->n_heads % m->n_kv_heads || (G != 1 && G != 2 && G != 4 && G != 8))
         return fail("tbq_dense: n_heads / n_kv_heads must be 1, 2, 4 or 8");
-    if (m->max_ctx > 131072) return fail("tbq_dense: max_ctx above 131072");
+    if (!paged && m->max_ctx > 131072) return fail("tbq_dense: max_ctx above 131072");
     if (m->hidden % 256 || m->ffn % 256 || (m->n_heads * m->head_dim) % 256)
         return fail("tbq_dense: hidden, ffn and n_heads*head_dim must be multiples of 256");
     if (m->hidden > TBQ_MAX_K || m->ffn > TBQ_MAX_K || m->n_heads * m->head_dim > TBQ_MAX_K)
@@ -404,7 +407,7 @@ static int check_dense(const tbq_dense_model *m) {
                     TBQ_MAX_K);
     if (!tbq_qtype_supported(m->qtype_layers) || !tbq_qtype_supported(m->qtype_embd))
         return fail("tbq_dense: unsupported qtype");
-    if (!m->tok_embd || !m->lm_head || !m->output_norm || !m->k_cache || !m->v_cache)
+    if (!m->tok_embd || !m->lm_head || !m->output_norm || (!paged && (!m->k_cache || !m->v_cache)))
         return fail("tbq_dense: null tensor");
     auto qt_ok = [m](int q) { return tbq_qtype_supported(q ? q : m->qtype_layers); };
     auto w_ok = [](const void *p) { return p && aligned16(p); };
@@ -458,6 +461,82 @@ int tbq_dense_prefill(const tbq_dense_model *m, const int *tokens_host, int T, i
     if (ws_bytes < dense_prefill_workspace_min(m, T)) return fail("tbq_dense_prefill: workspace too small");
     return hip_ok(launch_dense_prefill(m, tokens_host, T, pos0, logits, workspace, ws_bytes, S(s)),
                   "dense prefill launch");
+}
+
+// tbq_kv_api.hip (hidden)
+int tbq_kv_check_cache(const char *who, const tbq_kv_cache *c);
+
+static int check_step(const char *who, const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int max_pages) {
+    if (!check_dense(m, true) || !tbq_kv_check_cache(who, c)) return 0;
+    if (c->type != TBQ_KV_F16) return fail("%s: cache type %d (F16)", who, c->type);
+    if (c->n_layers != m->n_layers || c->n_kv_heads != m->n_kv_heads || c->head_dim != m->head_dim)
+        return fail("%s: a cache of %d layers, %d kv heads of %d for a model of %d, %d of %d", who, c->n_layers,
+                    c->n_kv_heads, c->head_dim, m->n_layers, m->n_kv_heads, m->head_dim);
+    if (n_seqs < 1 || n_seqs > 1024) return fail("%s: %d sequences (1..1024)", who, n_seqs);
+    if (max_pages < 1 || max_pages > 0x7FFFFFFF / 2048 || (long long)max_pages * c->page_size > 0x7FFFFFFF)
+        return fail("%s: max_pages %d", who, max_pages);
+    return 1;
+}
+
+// The model without its own cache, so that no workspace is sized by it.
+static tbq_dense_model uncached(const tbq_dense_model *m) {
+    tbq_dense_model p = *m;
+    p.max_ctx = 0;
+    p.k_cache = p.v_cache = nullptr;
+    return p;
+}
+
+size_t tbq_dense_step_workspace_size(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int n_tokens,
+                                     int max_pages) {
+    if (!check_step("tbq_dense_step_workspace_size", m, c, n_seqs, max_pages)) return 0;
+    if (n_tokens < n_seqs || n_tokens > 65536)
+        return fail("tbq_dense_step_workspace_size: %d tokens of %d sequences", n_tokens, n_seqs);
+    const tbq_dense_model p = uncached(m);
+    return dense_step_workspace_bytes(&p, c, n_seqs, n_tokens, max_pages);
+}
+
+int tbq_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new, const int *kv_len,
+                   const int *page_table, int max_pages, const int *tokens, const tbq_rope *rope, int window, int sinks,
+                   float *logits, void *ws, size_t ws_bytes, void *s) {
+    const char *who = "tbq_dense_step";
+    if (!check_step(who, m, c, n_seqs, max_pages)) return 0;
+    if (!n_new || !kv_len || !page_table || !tokens || !logits || !ws || !aligned16(ws))
+        return fail("%s: null pointer or misaligned workspace", who);
+    if (window < 0 || sinks < 0) return fail("%s: window %d, sinks %d", who, window, sinks);
+    if (rope && (rope->rot_dim < 8 || rope->rot_dim > m->head_dim || rope->rot_dim % 8 ||
+                 (rope->layout != TBQ_ROPE_HALF && rope->layout != TBQ_ROPE_INTERLEAVED)))
+        return fail("%s: rope of %d elements, layout %d", who, rope->rot_dim, rope->layout);
+    long long T = 0;
+    for (int q = 0; q < n_seqs; q++) {
+        const long long room = (long long)max_pages * c->page_size;
+        if (n_new[q] < 1 || kv_len[q] < n_new[q] || kv_len[q] > room)
+            return fail("%s: sequence %d: %d new tokens of %d positions, room for %lld", who, q, n_new[q], kv_len[q], room);
+        T += n_new[q];
+        // the pages that the sequence's tokens see some of, or are written to
+        const int first = kv_len[q] - n_new[q], back = pg_window(window);
+        const int lo = window > 0 && first - back + 1 > 0 ? first - back + 1 : 0;
+        for (int e = 0; e <= (kv_len[q] - 1) / c->page_size; e++) {
+            const int page = page_table[(long long)q * max_pages + e];
+            const long long at = (long long)e * c->page_size;
+            if ((at + c->page_size > lo || at < sinks) && (page < 0 || page >= c->n_pages))
+                return fail("%s: sequence %d: page %d of %d at %d", who, q, page, c->n_pages, e);
+        }
+    }
+    if (T > 65536) return fail("%s: %lld tokens above 65536", who, T);
+    for (int t = 0; t < T; t++)
+        if (tokens[t] < 0 || tokens[t] >= m->vocab) return fail("%s: token %d at %d out of range", who, tokens[t], t);
+    tbq_rope own;
+    if (!rope) {
+        if (!tbq_rope_init(&own, m->head_dim, TBQ_ROPE_HALF, m->rope_theta, TBQ_ROPE_NO_SCALING, 1, 0, 0, 0, nullptr)) return 0;
+        rope = &own;
+    }
+    const tbq_dense_model p = uncached(m);
+    const size_t need = dense_step_workspace_bytes(&p, c, n_seqs, (int)T, max_pages);
+    if (ws_bytes < need) return fail("%s: workspace %zu < %zu bytes", who, ws_bytes, need);
+    if (!ensure_init()) return 0;
+    return hip_ok(launch_dense_step(&p, c, n_seqs, n_new, kv_len, page_table, max_pages, tokens, *rope, pg_window(window),
+                                    window > 0 ? pg_window(sinks) : 0, logits, ws, ws_bytes, S(s)),
+                  "dense step launch");
 }
 
 int tbq_quantize_q8k(const float *x, long long n, void *blocks, void *s) {

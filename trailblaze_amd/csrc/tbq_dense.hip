@@ -31,6 +31,7 @@
 // head, and k_attn_combine merges the chunks.
 #include "tbq_kernels.h"
 #include "tbq_device.hpp"
+#include "tbq_paged.hpp"
 #include "../../include/tbq.h"
 
 namespace tbq {
@@ -515,17 +516,17 @@ static hipError_t dense_mv(int qt, const void *W, int M, int K, const float *x, 
 // each RMSNorm is the next matvec's PRO_NORMD (x * w staged, the scale
 // applied to the dot products, the sum of squares taken over the staged x
 // at the staging barrier), so no launch waits on a reduction of its own.
-hipError_t launch_dense_decode(const tbq_dense_model *m, int token, int pos, float *logits, void *ws,
+// attn(l, L) forms w.att from w.qkv and layer l's cache, and appends to it.
+template <typename Attn>
+static hipError_t dense_decode(const tbq_dense_model *m, int token, const DenseWs &w, float *logits, Attn attn,
                                hipStream_t st) {
-    const int H = m->hidden, D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads, G = NQ / NKV, F = m->ffn;
+    const int H = m->hidden, D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads, F = m->ffn;
     const int QKVR = (NQ + 2 * NKV) * D;
     auto qt_of = [m](int q) { return canon_qt(q ? q : m->qtype_layers); };
-    const DenseWs w = dense_ws(m, ws, nullptr);
     const size_t erb = tbq_row_bytes(m->qtype_embd, H);
     float *res = w.x;
     hipError_t err = launch_dequant(canon_qt(m->qtype_embd), (const uint8_t *)m->tok_embd + (size_t)token * erb, H, res, st);
     if (err != hipSuccess) return err;
-    hipLaunchKernelGGL(k_rope_table, dim3(1), dim3(64), 0, st, pos, m->rope_theta, D, w.rope);
     // rmsnorm(res) * wn as the next matvec's prologue
     auto norm_pro = [&](const float *wn, int *mode) {
         *mode = PRO_NORMD;
@@ -534,7 +535,6 @@ hipError_t launch_dense_decode(const tbq_dense_model *m, int token, int pos, flo
     const MvPro pres{};
     for (int l = 0; l < m->n_layers; l++) {
         const tbq_dense_layer &L = m->layers[l];
-        const size_t kvoff = (size_t)l * NKV * m->max_ctx * D;
         // qkv = Wqkv rmsnorm(res)
         int pm;
         const MvPro pa = norm_pro(L.attn_norm, &pm);
@@ -549,11 +549,7 @@ hipError_t launch_dense_decode(const tbq_dense_model *m, int token, int pos, flo
                                st);
         }
         if (err != hipSuccess) return err;
-        err = D == 128 ? launch_attn_d<128>(G, w.qkv, L.q_norm, L.k_norm, NQ, NKV, pos, w.rope, m->norm_eps,
-                                            m->k_cache + kvoff, m->v_cache + kvoff, m->max_ctx, w.part, w.att, st)
-                       : launch_attn_d<64>(G, w.qkv, L.q_norm, L.k_norm, NQ, NKV, pos, w.rope, m->norm_eps,
-                                           m->k_cache + kvoff, m->v_cache + kvoff, m->max_ctx, w.part, w.att, st);
-        if (err != hipSuccess) return err;
+        if ((err = attn(l, L)) != hipSuccess) return err;
         // res += Wo att
         if ((err = dense_mv(qt_of(L.qt_o), L.wo, H, NQ * D, w.att, res, PRO_RES, pres, nullptr, w.y, st)) !=
             hipSuccess)
@@ -582,6 +578,56 @@ hipError_t launch_dense_decode(const tbq_dense_model *m, int token, int pos, flo
         hipSuccess)
         return err;
     return hipGetLastError();
+}
+
+hipError_t launch_dense_decode(const tbq_dense_model *m, int token, int pos, float *logits, void *ws,
+                               hipStream_t st) {
+    const int D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads, G = NQ / NKV;
+    const DenseWs w = dense_ws(m, ws, nullptr);
+    hipLaunchKernelGGL(k_rope_table, dim3(1), dim3(64), 0, st, pos, m->rope_theta, D, w.rope);
+    return dense_decode(m, token, w, logits, [&](int l, const tbq_dense_layer &L) {
+        const size_t kvoff = (size_t)l * NKV * m->max_ctx * D;
+        return D == 128 ? launch_attn_d<128>(G, w.qkv, L.q_norm, L.k_norm, NQ, NKV, pos, w.rope, m->norm_eps,
+                                             m->k_cache + kvoff, m->v_cache + kvoff, m->max_ctx, w.part, w.att, st)
+                        : launch_attn_d<64>(G, w.qkv, L.q_norm, L.k_norm, NQ, NKV, pos, w.rope, m->norm_eps,
+                                            m->k_cache + kvoff, m->v_cache + kvoff, m->max_ctx, w.part, w.att, st);
+    }, st);
+}
+
+// The same step over a paged cache: pg is a batch of one sequence with one token
+// (layer 0's pages), layer_bytes lies between two layers of K (of V).
+hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const PgArgs &pg, size_t layer_bytes,
+                                     const PgRope &rope, int window, int sinks, float *logits, void *ws, void *attn_ws,
+                                     hipStream_t st) {
+    const int D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads;
+    const DenseWs w = dense_ws(m, ws, nullptr);
+    PgAppend ap{};
+    ap.pg = pg;
+    ap.q = ap.qo = w.qkv;   // rotated in place
+    ap.k = w.qkv + NQ * D;
+    ap.v = w.qkv + (NQ + NKV) * D;
+    ap.qs = ap.ks = ap.vs = (long long)(NQ + 2 * NKV) * D;
+    ap.eps = m->norm_eps;
+    ap.NQ = NQ;
+    ap.nsl = 1;
+    ap.rope = rope;
+    PgAttn at{};
+    at.q = w.qkv;
+    at.qs = ap.qs;
+    at.out = w.att;
+    at.NQ = NQ;
+    at.window = window;
+    at.sinks = sinks;
+    at.scale = pg_scale(0.f, D);
+    return dense_decode(m, token, w, logits, [&](int l, const tbq_dense_layer &L) {
+        ap.pg.k = (char *)pg.k + l * layer_bytes;
+        ap.pg.v = (char *)pg.v + l * layer_bytes;
+        ap.qn = L.q_norm;
+        ap.kn = L.k_norm;
+        at.pg = ap.pg;
+        const hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F32, TBQ_KV_F16, st);
+        return e != hipSuccess ? e : launch_pg_attn(at, D, TBQ_KV_F32, TBQ_KV_F16, attn_ws, st);
+    }, st);
 }
 
 // logits = Wlm rmsnorm(x + y) * output_norm for one residual row x and the

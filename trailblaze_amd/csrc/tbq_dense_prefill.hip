@@ -38,6 +38,7 @@
 #include "tbq_dma.hpp"
 #include "tbq_kernels.h"
 #include "tbq_device.hpp"
+#include "tbq_paged.hpp"
 #include "../../include/tbq.h"
 
 namespace tbq {
@@ -710,7 +711,8 @@ struct PfWs {
 };
 
 // *total: the bytes used, without gpart's, which is what the caller's ws_bytes leave.
-static PfWs pf_ws(const tbq_dense_model *m, int T, void *ws, size_t ws_bytes, size_t *total) {
+// paged: for tbq_dense_step, whose attention has a workspace of its own.
+static PfWs pf_ws(const tbq_dense_model *m, int T, void *ws, size_t ws_bytes, size_t *total, bool paged = false) {
     const size_t H = m->hidden, QD = (size_t)m->n_heads * m->head_dim, F = m->ffn;
     const size_t QKVR = (size_t)(m->n_heads + 2 * m->n_kv_heads) * m->head_dim;
     const size_t wide = std::max(std::max(H, QD), F);
@@ -730,21 +732,25 @@ static PfWs pf_ws(const tbq_dense_model *m, int T, void *ws, size_t ws_bytes, si
         w.y = (float *)take((size_t)T * H * 4);
         w.qkv = (float *)take((size_t)T * QKVR * 4);
         w.qb = (_Float16 *)take((size_t)T * QD * 2);
-        // fp16 K and V of one layer (a prefill reaches position kmax - 1 < max_ctx)
-        w.cp = (m->max_ctx + PC_KC - 1) / PC_KC * PC_KC;
-        w.k16 = (_Float16 *)take((size_t)m->n_kv_heads * w.cp * m->head_dim * 2);
-        w.vt = (_Float16 *)take((size_t)m->n_kv_heads * w.cp * m->head_dim * 2);
-        w.att = (float *)take((size_t)T * QD * 4);
+        if (!paged) {
+            // fp16 K and V of one layer (a prefill reaches position kmax - 1 < max_ctx)
+            w.cp = (m->max_ctx + PC_KC - 1) / PC_KC * PC_KC;
+            w.k16 = (_Float16 *)take((size_t)m->n_kv_heads * w.cp * m->head_dim * 2);
+            w.vt = (_Float16 *)take((size_t)m->n_kv_heads * w.cp * m->head_dim * 2);
+            w.att = (float *)take((size_t)T * QD * 4);
+        }
         w.gu = (float *)take((size_t)T * 2 * F * 4);
         w.h16 = (_Float16 *)take((size_t)T * wide * 2);
         w.sa = (float *)take((size_t)T * 4);
         w.sb = (float *)take((size_t)T * 4);
         w.wh = (_Float16 *)take(wmax * 2);
-        w.rope = (float *)take((size_t)T * m->head_dim * 4);
-        // attention split partials: a prefill reaching position kmax - 1 uses
-        // at most min(PA_MAX_SPLIT, ceil(kmax / PA_MIN_KS)) splits, and kmax <= max_ctx
-        const int ns = std::min(PA_MAX_SPLIT, (m->max_ctx + PA_MIN_KS - 1) / PA_MIN_KS);
-        w.part = ns > 1 ? (float *)take((size_t)T * m->n_heads * ns * pf_rec(m->head_dim) * 4) : nullptr;
+        if (!paged) {
+            w.rope = (float *)take((size_t)T * m->head_dim * 4);
+            // attention split partials: a prefill reaching position kmax - 1 uses
+            // at most min(PA_MAX_SPLIT, ceil(kmax / PA_MIN_KS)) splits, and kmax <= max_ctx
+            const int ns = std::min(PA_MAX_SPLIT, (m->max_ctx + PA_MIN_KS - 1) / PA_MIN_KS);
+            w.part = ns > 1 ? (float *)take((size_t)T * m->n_heads * ns * pf_rec(m->head_dim) * 4) : nullptr;
+        }
         // a product's split-K partials until their consumer has added them.  (A
         // region of their own: with the attention's records in the same memory a
         // prefill of 200 tokens took 250 us instead of 241)
@@ -761,11 +767,10 @@ size_t dense_prefill_workspace_min(const tbq_dense_model *m, int T) {
     return t;
 }
 
-// With room for the partial sums of the products that split K (a gate|up
-// matrix's does not) at any T up to this one: never less for a larger T.
-size_t dense_prefill_workspace_bytes(const tbq_dense_model *m, int T) {
-    const size_t base = dense_prefill_workspace_min(m, T);
-    if (!dense_prefill_batched(m) || T < 2) return base;
+// Room for the partial sums of the products that split K (a gate|up matrix's
+// does not) at any T up to this one: never less for a larger T.
+static size_t pf_partials(const tbq_dense_model *m, int T) {
+    if (!dense_prefill_batched(m) || T < 2) return 0;
     const int H = m->hidden, QD = m->n_heads * m->head_dim, KD = m->n_kv_heads * m->head_dim, F = m->ffn, cu = hgemm_cus();
     bool qkv = false, q_k_v = false, gate_up = false;
     for (int l = 0; l < m->n_layers; l++) {
@@ -776,13 +781,22 @@ size_t dense_prefill_workspace_bytes(const tbq_dense_model *m, int T) {
     if (qkv) gp = std::max(gp, hgemm_partial_upto(T, QD + 2 * KD, H, cu));
     if (q_k_v) gp = std::max(gp, std::max(hgemm_partial_upto(T, QD, H, cu), hgemm_partial_upto(T, KD, H, cu)));
     if (gate_up) gp = std::max(gp, hgemm_partial_upto(T, F, H, cu));
-    return base + gp;
+    return gp;
 }
 
-// tokens: T device ints (in range); T >= 2.
-static hipError_t pf_batched(const tbq_dense_model *m, const PfWs &w, int T, int pos0, float *logits,
-                             hipStream_t st) {
-    const int H = m->hidden, D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads, G = NQ / NKV, F = m->ffn;
+size_t dense_prefill_workspace_bytes(const tbq_dense_model *m, int T) {
+    return dense_prefill_workspace_min(m, T) + pf_partials(m, T);
+}
+
+// The layers over T >= 2 tokens (w.tok: T device ints, in range).  attn(l, L, qsrc,
+// qns) takes layer l's q | k | v rows (qns split-K slices T * QKVR apart, scaled by
+// 1 / w.sa), appends to the cache and writes the o GEMM's operand to w.h16, with
+// the inverse row scales at the pointer it sets.  *last, *lns: the last layer's
+// output (slices T * H apart, scaled by 1 / w.sb), not yet added to w.x.
+template <typename Attn>
+static hipError_t pf_layers(const tbq_dense_model *m, const PfWs &w, int T, Attn attn, const float **last, int *lns,
+                            hipStream_t st) {
+    const int H = m->hidden, D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads, F = m->ffn;
     const int QD = NQ * D, KD = NKV * D, QKVR = QD + 2 * KD;
     auto qt_of = [m](int q) { return canon_qt(q ? q : m->qtype_layers); };
     const int cu = hgemm_cus();
@@ -798,12 +812,9 @@ static hipError_t pf_batched(const tbq_dense_model *m, const PfWs &w, int T, int
     };
     const float *ysrc = w.y;   // the previous sublayer's output, as yns slices
     int yns = 1;
-    hipLaunchKernelGGL(k_pf_rope, dim3(T), dim3(64), 0, st, pos0, m->rope_theta, D, w.rope);
     hipError_t err = launch_dequant_rows(canon_qt(m->qtype_embd), m->tok_embd, w.tok, T, H, w.x, st);
     for (int l = 0; l < m->n_layers && err == hipSuccess; l++) {
         const tbq_dense_layer &L = m->layers[l];
-        const size_t kvoff = (size_t)l * NKV * m->max_ctx * D;
-        float *kc = m->k_cache + kvoff, *vc = m->v_cache + kvoff;
         err = launch_pf_norm(T, w.x, l ? ysrc : nullptr, yns, (long long)T * H, l ? w.sb : nullptr, L.attn_norm, H,
                              m->norm_eps, w.h16, w.sa, st);
         if (err != hipSuccess) break;
@@ -816,24 +827,11 @@ static hipError_t pf_batched(const tbq_dense_model *m, const PfWs &w, int T, int
             if (err == hipSuccess) err = gemm(qt_of(L.qt_v), L.wv, KD, H, w.qkv + QD + KD, QKVR);
         }
         if (err != hipSuccess) break;
-        const float *qsrc = qns > 1 ? w.gpart : w.qkv;
-        if (D == 128) {
-            hipLaunchKernelGGL(k_pf_qk<128>, dim3(T, (NQ + NKV + 7) / 8), dim3(PQ_THREADS), 0, st, qsrc, qns,
-                               (long long)T * QKVR, w.sa, L.q_norm, L.k_norm, NQ, NKV, pos0, w.rope, m->norm_eps, kc,
-                               vc, m->max_ctx, w.qb);
-            err = launch_pf_attn<128>(G, w.qb, kc, vc, T, pos0, NQ, NKV, m->max_ctx, w.k16, w.vt, w.cp, w.part, w.att,
-                                     w.h16, w.sb, cu, st);
-        } else {
-            hipLaunchKernelGGL(k_pf_qk<64>, dim3(T, (NQ + NKV + 15) / 16), dim3(PQ_THREADS), 0, st, qsrc, qns,
-                               (long long)T * QKVR, w.sa, L.q_norm, L.k_norm, NQ, NKV, pos0, w.rope, m->norm_eps, kc,
-                               vc, m->max_ctx, w.qb);
-            err = launch_pf_attn<64>(G, w.qb, kc, vc, T, pos0, NQ, NKV, m->max_ctx, w.k16, w.vt, w.cp, w.part, w.att,
-                                     w.h16, w.sb, cu, st);
-        }
-        if (err != hipSuccess) break;
+        const float *osc = w.sb;   // inverse scales of the attention's rows
+        if ((err = attn(l, L, qns > 1 ? w.gpart : w.qkv, qns, &osc)) != hipSuccess) break;
         if ((err = gemm(qt_of(L.qt_o), L.wo, H, QD, w.y, H, &yns)) != hipSuccess) break;
         ysrc = yns > 1 ? w.gpart : w.y;
-        if ((err = launch_pf_norm(T, w.x, ysrc, yns, (long long)T * H, w.sb, L.ffn_norm, H, m->norm_eps, w.h16,
+        if ((err = launch_pf_norm(T, w.x, ysrc, yns, (long long)T * H, osc, L.ffn_norm, H, m->norm_eps, w.h16,
                                   w.sa, st)) != hipSuccess)
             break;
         // a fused gate|up matrix: SwiGLU in the GEMM's epilogue, then the
@@ -857,12 +855,50 @@ static hipError_t pf_batched(const tbq_dense_model *m, const PfWs &w, int T, int
         err = gemm(qt_of(L.qt_down), L.wdown, H, F, w.y, H, &yns);
         ysrc = yns > 1 ? w.gpart : w.y;
     }
+    *last = ysrc;
+    *lns = yns;
+    return err;
+}
+
+// Token t's logits: its residual row and its row of the last layer's output.
+static hipError_t pf_logits(const tbq_dense_model *m, const PfWs &w, int T, int t, const float *ysrc, int yns, float *logits,
+                            hipStream_t st) {
+    const int H = m->hidden;
+    float *ylast = w.y + (size_t)t * H;
+    hipLaunchKernelGGL(k_pf_scale_row, dim3((H + 63) / 64), dim3(64), 0, st, ysrc + (size_t)t * H, yns, (long long)T * H,
+                       w.sb + t, H, ylast);
+    const hipError_t err = hipGetLastError();
     if (err != hipSuccess) return err;
-    float *ylast = w.y + (size_t)(T - 1) * H;
-    hipLaunchKernelGGL(k_pf_scale_row, dim3((H + 63) / 64), dim3(64), 0, st, ysrc + (size_t)(T - 1) * H, yns, (long long)T * H,
-                       w.sb + (T - 1), H, ylast);
-    if ((err = hipGetLastError()) != hipSuccess) return err;
-    return dense_final_logits(m, w.x + (size_t)(T - 1) * H, ylast, logits, w.dec, st);
+    return dense_final_logits(m, w.x + (size_t)t * H, ylast, logits, w.dec, st);
+}
+
+// tokens: T device ints (in range); T >= 2.
+static hipError_t pf_batched(const tbq_dense_model *m, const PfWs &w, int T, int pos0, float *logits,
+                             hipStream_t st) {
+    const int D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads, G = NQ / NKV, QKVR = (NQ + 2 * NKV) * D;
+    const int cu = hgemm_cus();
+    hipLaunchKernelGGL(k_pf_rope, dim3(T), dim3(64), 0, st, pos0, m->rope_theta, D, w.rope);
+    const float *ysrc = nullptr;
+    int yns = 1;
+    const hipError_t err = pf_layers(m, w, T, [&](int l, const tbq_dense_layer &L, const float *qsrc, int qns,
+                                                  const float **) {
+        const size_t kvoff = (size_t)l * NKV * m->max_ctx * D;
+        float *kc = m->k_cache + kvoff, *vc = m->v_cache + kvoff;
+        if (D == 128) {
+            hipLaunchKernelGGL(k_pf_qk<128>, dim3(T, (NQ + NKV + 7) / 8), dim3(PQ_THREADS), 0, st, qsrc, qns,
+                               (long long)T * QKVR, w.sa, L.q_norm, L.k_norm, NQ, NKV, pos0, w.rope, m->norm_eps, kc,
+                               vc, m->max_ctx, w.qb);
+            return launch_pf_attn<128>(G, w.qb, kc, vc, T, pos0, NQ, NKV, m->max_ctx, w.k16, w.vt, w.cp, w.part, w.att,
+                                       w.h16, w.sb, cu, st);
+        }
+        hipLaunchKernelGGL(k_pf_qk<64>, dim3(T, (NQ + NKV + 15) / 16), dim3(PQ_THREADS), 0, st, qsrc, qns,
+                           (long long)T * QKVR, w.sa, L.q_norm, L.k_norm, NQ, NKV, pos0, w.rope, m->norm_eps, kc,
+                           vc, m->max_ctx, w.qb);
+        return launch_pf_attn<64>(G, w.qb, kc, vc, T, pos0, NQ, NKV, m->max_ctx, w.k16, w.vt, w.cp, w.part, w.att,
+                                  w.h16, w.sb, cu, st);
+    }, &ysrc, &yns, st);
+    if (err != hipSuccess) return err;
+    return pf_logits(m, w, T, T - 1, ysrc, yns, logits, st);
 }
 
 hipError_t launch_dense_prefill(const tbq_dense_model *m, const int *tokens_host, int T, int pos0, float *logits,
@@ -879,6 +915,155 @@ hipError_t launch_dense_prefill(const tbq_dense_model *m, const int *tokens_host
     const hipError_t err = hipMemcpyAsync(w.tok, tokens_host, (size_t)T * 4, hipMemcpyHostToDevice, st);
     if (err != hipSuccess) return err;
     return pf_batched(m, w, T, pos0, logits, st);
+}
+
+// ---------------------------------------------------------------------------
+// The forward over a paged cache (tbq_dense_step).
+// ---------------------------------------------------------------------------
+__global__ __launch_bounds__(256) void k_pf_ones(float *__restrict__ p, int n) {
+    const int i = blockIdx.x * 256 + threadIdx.x;
+    if (i < n) p[i] = 1.f;
+}
+
+// Behind the prefill's regions: the batch's ints, ones for the attention's row
+// scales, and the attention's workspace.
+struct StepWs {
+    PfWs pf;
+    int *ints;
+    float *ones;
+    void *attn;
+};
+static StepWs step_ws(const tbq_dense_model *m, int n_seqs, int T, int max_pages, void *ws, size_t ws_bytes,
+                      size_t *total) {
+    StepWs w{};
+    size_t off = 0;
+    // (the prefill's first, without their split-K partials, which are what is left at the end)
+    pf_ws(m, T, ws, 0, &off, true);
+    auto take = [&](size_t bytes) {
+        void *r = (char *)ws + off;
+        off += pf_up(bytes);
+        return r;
+    };
+    w.ints = (int *)take(((size_t)n_seqs * (max_pages + 2) + 1) * 4);
+    w.ones = (float *)take((size_t)T * 4);
+    return *total = off, w;
+}
+
+static size_t step_attn_bytes(const tbq_dense_model *m, int n_seqs, int T, long long max_kv) {
+    const int kv = (int)std::min(max_kv, 0x7FFFFFFFll), NKV = m->n_kv_heads, D = m->head_dim, NQ = m->n_heads;
+    return std::max(pg_attn_workspace_upto(n_seqs, T, kv, NKV, D, NQ, false), pg_attn_workspace_upto(1, 1, kv, NKV, D, NQ, true));
+}
+
+size_t dense_step_workspace_bytes(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int T, int max_pages) {
+    size_t t = 0;
+    step_ws(m, n_seqs, T, max_pages, nullptr, 0, &t);
+    return t + pf_up(step_attn_bytes(m, n_seqs, T, (long long)max_pages * c->page_size)) + pf_partials(m, T);
+}
+
+hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new,
+                             const int *kv_len, const int *page_table, int max_pages, const int *tokens,
+                             const tbq_rope &rope, int window, int sinks, float *logits, void *ws, size_t ws_bytes,
+                             hipStream_t st) {
+    int T = 0, max_q = 0, max_kv = 0;
+    for (int s = 0; s < n_seqs; s++) {
+        T += n_new[s];
+        max_q = std::max(max_q, n_new[s]);
+        max_kv = std::max(max_kv, kv_len[s]);
+    }
+    size_t off = 0;
+    StepWs w = step_ws(m, n_seqs, T, max_pages, ws, ws_bytes, &off);
+    w.attn = (char *)ws + off;
+    off += pf_up(step_attn_bytes(m, n_seqs, T, (long long)max_pages * c->page_size));
+    w.pf = pf_ws(m, T, ws, ws_bytes, nullptr, true);
+    w.pf.gpart_bytes = ws_bytes > off ? ws_bytes - off : 0;
+    w.pf.gpart = w.pf.gpart_bytes ? (float *)((char *)ws + off) : nullptr;
+    const size_t layer_bytes = (size_t)c->n_pages * c->n_kv_heads * c->page_size * c->head_dim * 2;
+    PgArgs pg = pg_layer(c, 0);
+    PgRope rp{};
+    pg_rope(rope, rp);
+    int *q_start = w.ints, *len = q_start + n_seqs + 1, *table = len + n_seqs;
+    pg.q_start = q_start;
+    pg.kv_len = len;
+    pg.max_pages = max_pages;
+    hipError_t err = launch_put_ints(table, page_table, (long long)n_seqs * max_pages, st);
+    if (err != hipSuccess) return err;
+    if (!dense_prefill_batched(m) || T < 2) {
+        // the decode step per token
+        pg.n_seqs = pg.n_tokens = pg.max_q = 1;
+        for (int s = 0, t = 0; s < n_seqs; s++) {
+            pg.table = table + (long long)s * max_pages;
+            for (int i = 0; i < n_new[s]; i++, t++) {
+                const int one[2] = {0, 1};
+                pg.max_kv = kv_len[s] - n_new[s] + i + 1;
+                pg.kv_len = q_start + 2;   // q_start and its length side by side
+                const int three[3] = {one[0], one[1], pg.max_kv};
+                if ((err = launch_put_ints(q_start, three, 3, st)) != hipSuccess) return err;
+                if ((err = launch_dense_decode_paged(m, tokens[t], pg, layer_bytes, rp, window, sinks,
+                                                     logits + (size_t)s * m->vocab, w.pf.dec, w.attn, st)) != hipSuccess)
+                    return err;
+            }
+        }
+        return hipSuccess;
+    }
+    pg.n_seqs = n_seqs;
+    pg.n_tokens = T;
+    pg.max_q = max_q;
+    pg.max_kv = max_kv;
+    pg.table = table;
+    if ((err = launch_put_ints(w.pf.tok, tokens, T, st)) != hipSuccess) return err;
+    {
+        int at = 0, host[257];   // q_start, 256 at a time
+        for (int s = 0; s <= n_seqs; s += 256) {
+            int n = 0;
+            for (; n < 256 && s + n <= n_seqs; n++) {
+                host[n] = at;
+                if (s + n < n_seqs) at += n_new[s + n];
+            }
+            if ((err = launch_put_ints(q_start + s, host, n, st)) != hipSuccess) return err;
+        }
+    }
+    if ((err = launch_put_ints(len, kv_len, n_seqs, st)) != hipSuccess) return err;
+    hipLaunchKernelGGL(k_pf_ones, dim3((T + 255) / 256), dim3(256), 0, st, w.ones, T);
+    const int D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads, QKVR = (NQ + 2 * NKV) * D;
+    PgAppend ap{};
+    ap.pg = pg;
+    ap.qs = ap.ks = ap.vs = QKVR;
+    ap.qo = w.pf.qb;
+    ap.eps = m->norm_eps;
+    ap.NQ = NQ;
+    ap.rs = w.pf.sa;
+    ap.slstride = (long long)T * QKVR;
+    ap.rope = rp;
+    // the attention's fp16 rows are averages of fp16 values: the o GEMM takes them as they are
+    PgAttn at{};
+    at.q = w.pf.qb;
+    at.qs = NQ * D;
+    at.out = w.pf.h16;
+    at.NQ = NQ;
+    at.window = window;
+    at.sinks = sinks;
+    at.scale = pg_scale(0.f, D);
+    const float *ysrc = nullptr;
+    int yns = 1;
+    err = pf_layers(m, w.pf, T, [&](int l, const tbq_dense_layer &L, const float *qsrc, int qns, const float **osc) {
+        ap.pg.k = (char *)pg.k + l * layer_bytes;
+        ap.pg.v = (char *)pg.v + l * layer_bytes;
+        ap.q = qsrc;
+        ap.k = qsrc + NQ * D;
+        ap.v = qsrc + (NQ + NKV) * D;
+        ap.nsl = qns;
+        ap.qn = L.q_norm;
+        ap.kn = L.k_norm;
+        at.pg = ap.pg;
+        *osc = w.ones;
+        const hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F16, TBQ_KV_F16, st);
+        return e != hipSuccess ? e : launch_pg_attn(at, D, TBQ_KV_F16, TBQ_KV_F16, w.attn, st);
+    }, &ysrc, &yns, st);
+    for (int s = 0, t = -1; s < n_seqs && err == hipSuccess; s++) {
+        t += n_new[s];
+        err = pf_logits(m, w.pf, T, t, ysrc, yns, logits + (size_t)s * m->vocab, st);
+    }
+    return err;
 }
 
 }  // namespace tbq

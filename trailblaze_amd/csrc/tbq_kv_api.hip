@@ -35,12 +35,6 @@ bool aligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; 
 
 hipStream_t S(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
-int log2i(int n) {
-    int s = 0;
-    while ((1 << s) < n) s++;
-    return s;
-}
-
 int check_cache(const char *who, const tbq_kv_cache *c) {
     if (!c) return fail("%s: null cache", who);
     if (c->type != TBQ_KV_F16 && c->type != TBQ_KV_BF16) return fail("%s: cache type %d (F16 or BF16)", who, c->type);
@@ -71,13 +65,7 @@ int check_batch(const char *who, const tbq_kv_batch *b) {
 long long page_elems(const tbq_kv_cache *c) { return (long long)c->n_kv_heads * c->page_size * c->head_dim; }
 
 PgArgs pg_args(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b) {
-    PgArgs a{};
-    const long long off = (long long)layer * c->n_pages * page_elems(c);
-    a.k = (uint16_t *)c->k + off;
-    a.v = (uint16_t *)c->v + off;
-    a.n_pages = c->n_pages;
-    a.NKV = c->n_kv_heads;
-    a.shift = log2i(c->page_size);
+    PgArgs a = pg_layer(c, layer);
     a.n_seqs = b->n_seqs;
     a.n_tokens = b->n_tokens;
     a.max_pages = b->max_pages;
@@ -94,6 +82,11 @@ PgArgs pg_args(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b) {
 }  // namespace
 
 extern "C" {
+
+// For tbq_api.hip (hidden): the checks of a cache.
+__attribute__((visibility("hidden"))) int tbq_kv_check_cache(const char *who, const tbq_kv_cache *c) {
+    return check_cache(who, c);
+}
 
 int tbq_rope_init(tbq_rope *r, int rot_dim, int layout, double theta, int scaling, double factor, int orig_ctx,
                   double beta_fast, double beta_slow, const float *factors) {
@@ -216,9 +209,9 @@ int tbq_attn_paged(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int 
     a.qs = qs;
     a.out = out;
     a.NQ = n_heads;
-    a.window = window < (1 << 30) ? window : 1 << 30;   // differences of positions stay in 32 bits
-    a.sinks = window > 0 ? (sinks < (1 << 30) ? sinks : 1 << 30) : 0;
-    a.scale = (scale > 0 ? scale : 1.0f / sqrtf((float)c->head_dim)) * 1.4426950408889634f;
+    a.window = pg_window(window);
+    a.sinks = window > 0 ? pg_window(sinks) : 0;
+    a.scale = pg_scale(scale, c->head_dim);
     return hip_ok(launch_pg_attn(a, c->head_dim, q_type, c->type, ws, S(stream)), "paged attention launch");
 }
 

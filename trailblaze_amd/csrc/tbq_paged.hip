@@ -2,6 +2,8 @@
 // (include/tbq_kv.h) on gfx950: rotary positions with the append of new rows,
 // page copies, and compaction of a sequence's kept rows.  Attention over the
 // pages is in tbq_paged_attn.hip.
+#include <string.h>
+
 #include "tbq_kernels.h"
 #include "tbq_paged.hpp"
 
@@ -237,6 +239,25 @@ hipError_t launch_pg_compact(void *k, void *v, int n_layers, long long lelems, i
     else
         hipLaunchKernelGGL(k_pg_compact<64>, grid, dim3(CO_THREADS), 0, st, (uint16_t *)k, (uint16_t *)v, lelems, a,
                            keep_start, keep, hpw);
+    return hipGetLastError();
+}
+
+// Host ints to the device in the kernel's arguments.
+constexpr int PUT_INTS = 960;
+struct PgInts {
+    int v[PUT_INTS];
+};
+__global__ __launch_bounds__(PUT_INTS) void k_pg_put(int *dst, const PgInts src, int n) {
+    if ((int)threadIdx.x < n) dst[threadIdx.x] = src.v[threadIdx.x];
+}
+
+hipError_t launch_put_ints(int *dst, const int *src, long long n, hipStream_t st) {
+    for (long long i = 0; i < n; i += PUT_INTS) {
+        PgInts v;
+        const int m = (int)(n - i < PUT_INTS ? n - i : PUT_INTS);
+        memcpy(v.v, src + i, m * sizeof(int));
+        hipLaunchKernelGGL(k_pg_put, dim3(1), dim3(PUT_INTS), 0, st, dst + i, v, m);
+    }
     return hipGetLastError();
 }
 

@@ -3,6 +3,8 @@
 // lookups of a token's sequence and of a position's row.
 #pragma once
 
+#include <math.h>
+
 #include "tbq_device.hpp"
 #include "../../include/tbq_kv.h"
 
@@ -54,6 +56,30 @@ struct PgAttn {
     int NQ, window, sinks;
     float scale;           // of q . k, times log2(e): the softmax is in powers of two
 };
+
+// The scale of q . k times log2(e); 0 stands for 1 / sqrt(D).
+inline float pg_scale(float scale, int D) { return (scale > 0 ? scale : 1.0f / sqrtf((float)D)) * 1.4426950408889634f; }
+
+// Differences of positions and windows stay in 32 bits.
+inline int pg_window(int n) { return n < (1 << 30) ? n : 1 << 30; }
+
+inline int pg_log2(int n) {
+    int s = 0;
+    while ((1 << s) < n) s++;
+    return s;
+}
+
+// Layer `layer` of a cache.
+inline PgArgs pg_layer(const tbq_kv_cache *c, int layer) {
+    PgArgs a{};
+    const long long off = (long long)layer * c->n_pages * c->n_kv_heads * c->page_size * c->head_dim;
+    a.k = (uint16_t *)c->k + off;
+    a.v = (uint16_t *)c->v + off;
+    a.n_pages = c->n_pages;
+    a.NKV = c->n_kv_heads;
+    a.shift = pg_log2(c->page_size);
+    return a;
+}
 
 constexpr int PG_PAIRS = 128;   // page copies per launch, 1 KiB of kernel arguments
 struct PgPairs {
@@ -110,6 +136,19 @@ hipError_t launch_pg_copy(void *k, void *v, int n_layers, long long pbytes, long
 hipError_t launch_pg_compact(void *k, void *v, int n_layers, long long lelems, int D, const PgArgs &a, const int *keep_start,
                              const int *keep, hipStream_t st);
 size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32);
+// at least that of every batch of up to n_seqs sequences, n_tokens tokens and max_kv positions
+size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int D, int NQ, bool f32);
+// One token of one sequence (tbq_dense.hip), a batch of sequences (tbq_dense_prefill.hip).
+hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const PgArgs &pg, size_t layer_bytes,
+                                     const PgRope &rope, int window, int sinks, float *logits, void *ws, void *attn_ws,
+                                     hipStream_t st);
+size_t dense_step_workspace_bytes(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int T, int max_pages);
+hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new,
+                             const int *kv_len, const int *page_table, int max_pages, const int *tokens,
+                             const tbq_rope &rope, int window, int sinks, float *logits, void *ws, size_t ws_bytes,
+                             hipStream_t st);
+// *dst = n host ints, through kernel arguments (the host array is free at once)
+hipError_t launch_put_ints(int *dst, const int *src, long long n, hipStream_t st);
 hipError_t launch_pg_attn(const PgAttn &a, int D, int q_type, int c_type, void *ws, hipStream_t st);
 
 }  // namespace tbq

@@ -173,6 +173,7 @@ constexpr int PR_WAVES = 4, PR_TS = 32;
 // of 8 sequences after 2000 40.0 us as four, 33.4 as many.
 constexpr int PR_MAX = 32;
 constexpr int PR_MIN = 4, PR_LONG = 64;   // tiles of a split: one a wave at least, 2048 positions at most
+constexpr int PR_MANY = 1024;              // (in batches of up to twice so many workgroups)
 
 template <int D>
 struct PrLds {
@@ -936,15 +937,17 @@ static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, boo
     // 512 / 2048 / 4096 / 8192 positions: 212 / 210 / 218 / 295 us), shorter ones add to the join
     // (one token over 131072: 58 us with 128 ranges, 66 with 256).
     const long long wgs = (long long)a.NKV * p.nrb * a.n_seqs, want = (2 * cu + wgs - 1) / wgs;
+    // (a batch of thousands of workgroups evens out by itself, so its ranges, and records, stay few)
+    const long long longest = PR_LONG * std::max(1ll, wgs / PR_MANY);
     auto splits = [&](long long tps) { return (tiles + tps - 1) / tps; };
-    long long tps = std::max((long long)PR_MIN, std::min((long long)PR_LONG, ((tiles + want - 1) / want + 3) / 4 * 4));
+    long long tps = std::max((long long)PR_MIN, std::min(longest, ((tiles + want - 1) / want + 3) / 4 * 4));
     if (splits(tps) > PJ_MAX) tps = (tiles + PJ_MAX - 1) / PJ_MAX;
     p.row_tps = (int)tps;
     p.row_splits = (int)splits(tps);
     // room for the most splits that any window can lead to
     const long long all = ((long long)a.max_kv + PR_TS - 1) / PR_TS + 1;
     const long long room = std::min((long long)PJ_MAX, std::max(std::min(want, (all + PR_MIN - 1) / PR_MIN),
-                                                                (all + PR_LONG - 1) / PR_LONG));
+                                                                (all + longest - 1) / longest));
     if (room > 1) p.rows_bytes = (size_t)a.n_seqs * a.NKV * p.nrb * RB * room * pg_rec(D) * 4;
     p.chunks = (long long)a.max_q * G > PR_MAX;
     p.bytes = p.rows_bytes;
@@ -966,6 +969,18 @@ static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, boo
 size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32) {
     if (a.n_seqs == 0 || a.n_tokens == 0) return 0;
     return pg_plan(a, D, NQ, 0, 0, f32).bytes;
+}
+
+// Rows: a batch of w workgroups a split has at most 512 / w + 1 splits to fill the
+// chip, or one for each `longest` tiles, where w / longest <= 2 PR_MANY / PR_LONG;
+// chunks: more than one split only while all of them fill two workgroups a CU.
+size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int D, int NQ, bool f32) {
+    const long long RB = f32 ? 8 : 16, w = (long long)NKV * (PR_MAX / RB) * n_seqs;
+    const long long all = ((long long)max_kv + PR_TS - 1) / PR_TS + 1;
+    const long long rows = std::max(512 + w, std::max(std::min(w, 2ll * PR_MANY) * ((all + PR_LONG - 1) / PR_LONG),
+                                                      2ll * PR_MANY * all / PR_LONG + w));
+    const long long chunk = std::min((long long)n_tokens * NQ * PC_SPLITS, 512ll * PC_ROWS);
+    return (size_t)(rows * RB + chunk) * pg_rec(D) * 4;
 }
 
 template <typename TC, int D, bool HL>

@@ -127,6 +127,42 @@ class SyntheticDense:
     def prefill_batched(self) -> bool:
         return bool(lib().tbq_dense_prefill_batched(C.byref(self.model)))
 
+    def paged_cache(self, n_pages: int, page_size: int = 64):
+        """An F16 ``paged.KvCache`` of this model's shape, for ``step``."""
+        import torch
+        from . import paged
+        c = self.cfg
+        shape = (c.n_layers, n_pages, c.n_kv_heads, page_size, c.head_dim)
+        return paged.kv_cache(*(torch.zeros(shape, dtype=torch.float16, device="cuda") for _ in range(2)))
+
+    def step(self, cache, n_new, kv_len, page_table, tokens, logits, rope=None, window: int = 0, sinks: int = 0,
+             stream=None):
+        """tbq_dense_step: n_new[s] tokens of every sequence s (side by side in
+        `tokens`), kv_len[s] its positions with them, page_table
+        [sequences][pages] (host ints); logits [sequences][vocab] (device fp32)
+        of each one's last token."""
+        import torch
+        ints = lambda v: np.ascontiguousarray(v, dtype=np.int32)   # noqa: E731
+        n_new, kv_len, page_table, toks = ints(n_new), ints(kv_len), ints(page_table), ints(tokens)
+        n = len(n_new)
+        if page_table.ndim != 2 or kv_len.shape != (n,) or len(page_table) != n or len(toks) != n_new.sum():
+            raise ValueError("n_new, kv_len and page_table: one row a sequence; tokens: the sum of n_new")
+        if logits.numel() != n * self.cfg.vocab or logits.dtype != torch.float32 or not logits.is_contiguous():
+            raise ValueError("logits: contiguous float32 [sequences][vocab]")
+        need = int(lib().tbq_dense_step_workspace_size(C.byref(self.model), C.byref(cache), n, len(toks),
+                                                       page_table.shape[1]))
+        ws = getattr(self, "_step_ws", None)
+        if need > (0 if ws is None else ws.numel()):
+            ws = self._step_ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+        if ws is not None:   # used on this stream, whichever it was made on
+            ws.record_stream(torch.cuda.current_stream() if stream is None else stream)
+        # (need == 0: bad arguments, which the call itself reports)
+        _check(lib().tbq_dense_step(C.byref(self.model), C.byref(cache), n, n_new.ctypes.data, kv_len.ctypes.data,
+                                    page_table.ctypes.data, page_table.shape[1], toks.ctypes.data,
+                                    None if rope is None else C.byref(rope), window, sinks, _ptr(logits), _ptr(ws),
+                                    0 if ws is None else ws.numel(), _stream(stream)), "tbq_dense_step")
+        return logits
+
     def matvec_shapes(self):
         """(qtype, M, K, weight tensor) of every matvec one decode step runs."""
         c = self.cfg
