@@ -475,6 +475,10 @@ def test_python_refusals():
     x, c, b = s["x"], s["c"], s["b"]
     with pytest.raises(ValueError, match="cpu"):
         paged.attn_paged(c, 0, b, s["q"].cpu(), s["out"])
+    with pytest.raises(ValueError, match="device"):
+        paged.kv_cache(s["K"].cpu(), s["V"].cpu())
+    with pytest.raises(ValueError, match="device"):
+        paged.kv_batch(b._keep[0].cpu(), b._keep[1], b._keep[2], 2)
     with pytest.raises(ValueError, match="out"):
         paged.attn_paged(c, 0, b, s["q"], s["out"].half())
     with pytest.raises(ValueError, match="side by side"):

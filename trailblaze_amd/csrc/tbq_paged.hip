@@ -4,6 +4,8 @@
 // pages is in tbq_paged_attn.hip.
 #include <string.h>
 
+#include <algorithm>
+
 #include "tbq_kernels.h"
 #include "tbq_paged.hpp"
 
@@ -120,7 +122,14 @@ template <typename TI, typename TQ, typename TC, int D>
 static hipError_t append_d(const PgAppend &a, hipStream_t st) {
     constexpr int SL = AP_THREADS / (D / 8);
     const int nb = (a.NQ + 2 * a.pg.NKV + SL - 1) / SL;
-    hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 1>), dim3(a.pg.n_tokens, nb), dim3(AP_THREADS), 0, st, a);
+    // Long prompts share the angles between up to three heads a lane: 8192 tokens, 48 heads of 128,
+    // fp32 71 -> 61 us, bf16 67 -> 49; below about eight workgroups a CU one head a lane is as fast
+    // (512 tokens) or faster (64 tokens 3.8 us, 4.8 with three).
+    const int hpt = (long long)a.pg.n_tokens * nb >= 2048 ? std::min(nb, 3) : 1;
+    const dim3 grid(a.pg.n_tokens, (nb + hpt - 1) / hpt);
+    if (hpt == 3) hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 3>), grid, dim3(AP_THREADS), 0, st, a);
+    else if (hpt == 2) hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 2>), grid, dim3(AP_THREADS), 0, st, a);
+    else hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 1>), grid, dim3(AP_THREADS), 0, st, a);
     return hipGetLastError();
 }
 
@@ -154,10 +163,10 @@ __global__ __launch_bounds__(CP_THREADS) void k_pg_copy(uint8_t *k, uint8_t *v, 
     pg_u4 r[CP_V];
 #pragma unroll
     for (int i = 0; i < CP_V; i++)   // clamped: loads stay unconditional
-        r[i] = *reinterpret_cast<const pg_u4 *>(src + min(at + i * CP_THREADS * 16, pbytes - 16));
+        r[i] = __builtin_nontemporal_load(reinterpret_cast<const pg_u4 *>(src + min(at + i * CP_THREADS * 16, pbytes - 16)));
 #pragma unroll
     for (int i = 0; i < CP_V; i++)
-        if (at + i * CP_THREADS * 16 < pbytes) *reinterpret_cast<pg_u4 *>(dst + at + i * CP_THREADS * 16) = r[i];
+        if (at + i * CP_THREADS * 16 < pbytes) __builtin_nontemporal_store(r[i], reinterpret_cast<pg_u4 *>(dst + at + i * CP_THREADS * 16));
 }
 
 hipError_t launch_pg_copy(void *k, void *v, int n_layers, long long pbytes, long long lbytes, const PgPairs &pairs, int n,
@@ -169,70 +178,87 @@ hipError_t launch_pg_copy(void *k, void *v, int n_layers, long long pbytes, long
 
 // ---------------------------------------------------------------------------
 // Compaction, in place: row j of a sequence becomes its row keep[j] >= j, keep
-// ascending.  A workgroup has one sequence, layer, K or V, hpw kv heads and a
-// 128-byte column of their rows (no other workgroup touches it) and goes through
-// the kept rows a step at a time: all of a step's rows have arrived in every
-// wave before any is stored, and a step's stores reach no row that a later step
-// loads (keep[j'] >= j' > j), so the next step's rows are loaded before this
-// one's are stored, and its page lookups before those.
+// ascending.  Rows are moved as columns of 128 bytes.  A workgroup has one
+// sequence, layer, K or V, and hpw of the NKV * D / 64 columns (no other
+// workgroup touches them) and goes through the kept rows a step of CO_UNITS / hpw
+// at a time: all of a step's rows have arrived in every wave before any is
+// stored, and a step's stores reach no row that a later step loads (keep[j'] >=
+// j' > j), so the next step's rows are loaded before this one's are stored.
+// Pages are looked up for CO_LIST rows at a time, into LDS: memory operations
+// complete in order, so a lookup per step would have waited for all of the
+// step's rows first.
 // ---------------------------------------------------------------------------
-constexpr int CO_THREADS = 256, CO_V = 8, CO_UNITS = CO_THREADS / 8 * CO_V;   // rows of one head in a step
+constexpr int CO_THREADS = 256, CO_V = 4, CO_UNITS = CO_THREADS / 8 * CO_V, CO_LIST = 1024;
 template <int D>
 __global__ __launch_bounds__(CO_THREADS) void k_pg_compact(uint16_t *k, uint16_t *v, long long lelems, const PgArgs a,
                                                            const int *__restrict__ keep_start,
                                                            const int *__restrict__ keep, int hpw) {
-    constexpr int SL = D / 64;   // 128-byte columns of a row
-    const int s = blockIdx.z, l = threadIdx.x % 8, u0 = threadIdx.x / 8;
-    const int col = blockIdx.x % SL, h0 = blockIdx.x / SL * hpw, jr = CO_UNITS / hpw;   // rows of a step
-    uint16_t *base = (blockIdx.y & 1 ? v : k) + (blockIdx.y >> 1) * lelems + 64 * col + 8 * l;
+    constexpr int SL = D / 64;   // columns of a row
+    __shared__ int src[2][CO_LIST], dst[2][CO_LIST];   // rows of head 0, dst -1: nothing to store
+    const int s = blockIdx.z, l = threadIdx.x % 8, u0 = threadIdx.x / 8, c0 = blockIdx.x * hpw;
+    const int jr = CO_UNITS / hpw, lr = CO_LIST / jr * jr;   // rows of a step, of a list
+    uint16_t *base = (blockIdx.y & 1 ? v : k) + (blockIdx.y >> 1) * lelems + 8 * l;
     const int at = keep_start[s], n = keep_start[s + 1] - at;
-    int src[2][CO_V], dst[2][CO_V];   // rows from `base` on, dst -1: nothing to store
-    pg_u4 r[2][CO_V];
-    auto find = [&](int b, int j0) {
+    if (n <= 0) return;
+    auto look_up = [&](int j0) {
+        const int b = j0 / lr & 1;
 #pragma unroll
-        for (int i = 0; i < CO_V; i++) {
-            const int u = i * (CO_THREADS / 8) + u0, h = u / jr;
-            const int j = j0 + u % jr, jc = min(j, n - 1), from = keep[at + jc], p = max(from, 0);
-            const int ps = pg_page(a, s, p), pd = pg_page(a, s, jc);
-            const bool moves = j < n && h < hpw && from >= 0 && p != j && ps >= 0 && pd >= 0;
+        for (int i = 0; i < CO_LIST / CO_THREADS; i++) {
+            const int e = threadIdx.x + CO_THREADS * i, j = j0 + e, jc = min(j, n - 1);
+            const int from = keep[at + jc], p = max(from, 0), ps = pg_page(a, s, p), pd = pg_page(a, s, jc);
+            const bool moves = j < n && from >= 0 && p != j && ps >= 0 && pd >= 0;
             // a row that does not move is loaded from where it is (or page 0) and not stored
-            src[b][i] = (int)(pg_row<D>(a, max(ps, 0), h0 + min(h, hpw - 1), p) / D);
-            dst[b][i] = moves ? (int)(pg_row<D>(a, pd, h0 + h, jc) / D) : -1;
+            src[b][e] = (int)(pg_row<1>(a, max(ps, 0), 0, p));
+            dst[b][e] = moves ? (int)(pg_row<1>(a, pd, 0, jc)) : -1;
         }
     };
-    auto load = [&](int b) {
+    // unit u of a step: row u % jr, column c0 + u / jr
+    int uj[CO_V];
+    long long uc[CO_V];   // elements between row 0 of head 0 and of the column; -1: no unit
 #pragma unroll
-        for (int i = 0; i < CO_V; i++) r[b][i] = *reinterpret_cast<const pg_u4 *>(base + (long long)src[b][i] * D);
-    };
-    auto store = [&](int b) {
+    for (int i = 0; i < CO_V; i++) {
+        const int u = i * (CO_THREADS / 8) + u0, c = u / jr, cc = c0 + min(c, hpw - 1);
+        uj[i] = u % jr;
+        uc[i] = (((long long)(cc / SL) << a.shift) * D + 64 * (cc % SL)) | (c < hpw ? 0 : 1);
+    }
+    pg_u4 r[2][CO_V];
+    auto load = [&](int b, int j0) {
 #pragma unroll
         for (int i = 0; i < CO_V; i++)
-            if (dst[b][i] >= 0) *reinterpret_cast<pg_u4 *>(base + (long long)dst[b][i] * D) = r[b][i];
+            r[b][i] = *reinterpret_cast<const pg_u4 *>(base + (uc[i] & ~1ll) + (long long)src[j0 / lr & 1][j0 % lr + uj[i]] * D);
     };
-    if (n <= 0) return;
+    auto store = [&](int b, int j0) {
+#pragma unroll
+        for (int i = 0; i < CO_V; i++) {
+            const int to = uc[i] & 1 ? -1 : dst[j0 / lr & 1][j0 % lr + uj[i]];
+            if (to >= 0) *reinterpret_cast<pg_u4 *>(base + uc[i] + (long long)to * D) = r[b][i];
+        }
+    };
     auto step = [&](int b, int j0) {
-        if (j0 + jr < n) find(b ^ 1, j0 + jr);
-        // every wave's rows have arrived
+        // every wave's rows have arrived, and it is done with the list before this one
         asm volatile("s_waitcnt vmcnt(0) lgkmcnt(0)\n\ts_barrier" ::: "memory");
-        if (j0 + jr < n) load(b ^ 1);
-        store(b);
+        if (j0 + jr < n) load(b ^ 1, j0 + jr);
+        store(b, j0);
+        if (j0 % lr == 0 && j0 + lr < n) look_up(j0 + lr);   // a list (of two steps or more) ahead
     };
-    find(0, 0);
-    load(0);
+    look_up(0);
+    __syncthreads();
+    load(0, 0);
     for (int j0 = 0; j0 < n; j0 += 2 * jr) {   // uniform
         step(0, j0);
         if (j0 + jr < n) step(1, j0 + jr);
     }
 }
 
-// Heads of a workgroup: all, or as many as leave about four workgroups a CU
-// (many short sequences: one step does it all, and the page lookups are shared).
+// Columns of a workgroup: all, or as many as leave about four workgroups a CU
+// (many short sequences: one step does it all, and the lookups are shared).
 hipError_t launch_pg_compact(void *k, void *v, int n_layers, long long lelems, int D, const PgArgs &a, const int *keep_start,
                              const int *keep, hipStream_t st) {
+    const int cols = a.NKV * (D / 64);
     int hpw = 1;
-    for (int h = 2; h <= a.NKV && h <= 32; h++)
-        if (a.NKV % h == 0 && (long long)a.n_seqs * 2 * n_layers * (a.NKV / h) * (D / 64) >= 1024) hpw = h;
-    const dim3 grid(a.NKV / hpw * (D / 64), 2 * n_layers, a.n_seqs);
+    for (int h = 2; h <= cols && h <= 64; h++)
+        if (cols % h == 0 && (long long)a.n_seqs * 2 * n_layers * (cols / h) >= 1024) hpw = h;
+    const dim3 grid(cols / hpw, 2 * n_layers, a.n_seqs);
     if (D == 128)
         hipLaunchKernelGGL(k_pg_compact<128>, grid, dim3(CO_THREADS), 0, st, (uint16_t *)k, (uint16_t *)v, lelems, a,
                            keep_start, keep, hpw);

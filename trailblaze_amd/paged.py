@@ -37,58 +37,74 @@ class Rope(C.Structure):
     _fields_ = [("rot_dim", C.c_int), ("layout", C.c_int), ("mscale", C.c_double), ("freq", C.c_double * 64)]
 
 
+_torch, _ids = None, {}
+
+
+def _init_torch():
+    """torch, imported at the first use as everywhere in this package."""
+    global _torch
+    if _torch is None:
+        import torch
+        _torch = torch
+        _ids.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
+    return _torch
+
+
 def _type_id(dtype):
-    import torch
-    ids = {torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16}
-    if dtype not in ids:
+    _init_torch()
+    if dtype not in _ids:
         raise ValueError(f"{dtype}: float32, float16 or bfloat16")
-    return ids[dtype]
+    return _ids[dtype]
 
 
-def _here(*tensors):
-    """All on the current device (whose stream the call takes)."""
-    import torch
-    cur = torch.cuda.current_device()
-    for t in tensors:
-        if t is not None and (t.device.type != "cuda" or t.device.index != cur):
-            raise ValueError(f"tensor on {t.device}, current device is cuda:{cur}")
+def _here(*owners):
+    """The current device, whose stream the call takes: that of the cache and the batch."""
+    cur = _init_torch().cuda.current_device()
+    for o in owners:
+        if o._dev != cur:
+            raise ValueError(f"tensors on device {o._dev}, current device is cuda:{cur}")
+    return cur
+
+
+def _on(name, t, dev):
+    if t.get_device() != dev:
+        raise ValueError(f"{name}: tensor on {t.device}, current device is cuda:{dev}")
 
 
 def _ints(name, t, shape):
-    import torch
-    if t.dtype != torch.int32 or tuple(t.shape) != shape or not t.is_contiguous():
-        raise ValueError(f"{name}: contiguous int32 {shape} expected, got {t.dtype} {tuple(t.shape)}")
+    if t.dtype != _init_torch().int32 or t.shape != shape or not t.is_contiguous():
+        raise ValueError(f"{name}: contiguous int32 {tuple(shape)} expected, got {t.dtype} {tuple(t.shape)}")
 
 
-def _heads(name, t, rows, n_heads, D):
+def _heads(name, t, rows, n_heads, D, dev):
     """Elements between the rows of [rows][heads][D], whose heads lie side by side."""
-    if t.dim() != 3 or tuple(t.shape) != (rows, n_heads, D):
+    if t.shape != (rows, n_heads, D):
         raise ValueError(f"{name}: {(rows, n_heads, D)} expected, got {tuple(t.shape)}")
-    if t.stride(2) != 1 or (n_heads > 1 and t.stride(1) != D):
+    _on(name, t, dev)
+    st = t.stride()
+    if st[2] != 1 or (n_heads > 1 and st[1] != D):
         raise ValueError(f"{name}: the heads of a row must lie side by side")
-    return t.stride(0) if rows > 1 else n_heads * D
+    return st[0] if rows > 1 else n_heads * D
 
 
-def _flat(name, t, shape, dtype):
-    if tuple(t.shape) != shape or t.dtype != dtype or not t.is_contiguous():
+def _flat(name, t, shape, dtype, dev):
+    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
         raise ValueError(f"{name}: contiguous {dtype} {shape} expected, got {t.dtype} {tuple(t.shape)}")
+    _on(name, t, dev)
 
 
 def kv_cache(k, v) -> KvCache:
     """A ``tbq_kv_cache`` over two device tensors."""
     if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous():
         raise ValueError("k and v: contiguous [layers][pages][kv heads][page size][head dim], alike")
-    if k.dtype == _torch().float32:
+    if _type_id(k.dtype) == F32:
         raise ValueError("k and v: float16 or bfloat16")
+    if k.get_device() < 0 or k.get_device() != v.get_device():
+        raise ValueError(f"k and v: on one device, got {k.device} and {v.device}")
     L, P, H, S, D = k.shape
     c = KvCache(L, P, H, S, D, _type_id(k.dtype), k.data_ptr(), v.data_ptr())
-    c._keep = (k, v)
+    c._keep, c._dev = (k, v), k.get_device()
     return c
-
-
-def _torch():
-    import torch
-    return torch
 
 
 def kv_batch(q_start, kv_len, page_table, n_tokens: int, max_q: int = 0, max_kv: int = 0) -> KvBatch:
@@ -100,9 +116,12 @@ def kv_batch(q_start, kv_len, page_table, n_tokens: int, max_q: int = 0, max_kv:
     if page_table.dim() != 2:
         raise ValueError("page_table: [sequences][pages]")
     _ints("page_table", page_table, (n, page_table.shape[1]))
+    dev = kv_len.get_device()
+    if dev < 0 or q_start.get_device() != dev or page_table.get_device() != dev:
+        raise ValueError("q_start, kv_len and page_table: on one device")
     b = KvBatch(n, n_tokens, page_table.shape[1], max_q, max_kv, q_start.data_ptr(), kv_len.data_ptr(),
                 page_table.data_ptr())
-    b._keep = (q_start, kv_len, page_table)
+    b._keep, b._dev = (q_start, kv_len, page_table), dev
     return b
 
 
@@ -127,29 +146,31 @@ def kv_append(cache: KvCache, layer: int, batch: KvBatch, q, k, v, q_out, rope: 
               eps: float = 1e-6, positions=None, stream=None):
     """Rotate and append the batch's new rows: q [tokens][heads][D] to q_out
     (both may be None), k and v [tokens][kv heads][D] to their pages."""
-    T, D = batch.n_tokens, cache.head_dim
-    torch = _torch()
-    _here(q, k, v, q_out, q_norm, k_norm, positions, *cache._keep, *batch._keep)
+    dev = _here(cache, batch)
+    T, D, nkv = batch.n_tokens, cache.head_dim, cache.n_kv_heads
     in_type = _type_id(k.dtype)
     if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
         raise ValueError("q, k and v: one type")
-    ks, vs = _heads("k", k, T, cache.n_kv_heads, D), _heads("v", v, T, cache.n_kv_heads, D)
-    nq, qs, q_type = 0, 0, cache.type
+    ks, vs = _heads("k", k, T, nkv, D, dev), _heads("v", v, T, nkv, D, dev)
+    nq, qs, q_type, qp, qo = 0, 0, cache.type, None, None
     if (q is None) != (q_out is None):
         raise ValueError("q and q_out go together")
     if q is not None:
         nq = q.shape[1]
-        qs = _heads("q", q, T, nq, D)
+        qs = _heads("q", q, T, nq, D, dev)
         q_type = _type_id(q_out.dtype)
-        _flat("q_out", q_out, (T, nq, D), q_out.dtype)
-    for name, w in (("q_norm", q_norm), ("k_norm", k_norm)):
-        if w is not None:
-            _flat(name, w, (D,), torch.float32)
+        _flat("q_out", q_out, (T, nq, D), q_out.dtype, dev)
+        qp, qo = q.data_ptr(), q_out.data_ptr()
+    if q_norm is not None:
+        _flat("q_norm", q_norm, (D,), _torch.float32, dev)
+    if k_norm is not None:
+        _flat("k_norm", k_norm, (D,), _torch.float32, dev)
     if positions is not None:
         _ints("positions", positions, (T,))
+        _on("positions", positions, dev)
     _check(lib().tbq_kv_append(C.byref(cache), layer, C.byref(batch), nq, None if rope is None else C.byref(rope),
-                               _ptr(q_norm), _ptr(k_norm), eps, _ptr(positions), in_type, _ptr(q), qs, _ptr(k), ks,
-                               _ptr(v), vs, q_type, _ptr(q_out), _stream(stream)), "tbq_kv_append")
+                               _ptr(q_norm), _ptr(k_norm), eps, _ptr(positions), in_type, qp, qs, k.data_ptr(), ks,
+                               v.data_ptr(), vs, q_type, qo, _stream(stream)), "tbq_kv_append")
     return q_out
 
 
@@ -160,24 +181,26 @@ def attn_workspace_size(cache: KvCache, batch: KvBatch, n_heads: int, dtype) -> 
 def attn_paged(cache: KvCache, layer: int, batch: KvBatch, q, out, window: int = 0, sinks: int = 0,
                scale: float = 0.0, workspace=None, stream=None):
     """out[token][head] = attention of q over the pages the token sees."""
-    torch = _torch()
-    _here(q, out, workspace, *cache._keep, *batch._keep)
+    dev = _here(cache, batch)
     T, D = batch.n_tokens, cache.head_dim
     if q.dim() != 3:
         raise ValueError("q: [tokens][heads][head dim]")
     nq = q.shape[1]
-    qs = _heads("q", q, T, nq, D)
-    _flat("out", out, (T, nq, D), q.dtype)
+    qs = _heads("q", q, T, nq, D, dev)
+    _flat("out", out, (T, nq, D), q.dtype, dev)
     if workspace is None:
         n = attn_workspace_size(cache, batch, nq, q.dtype)
-        workspace = torch.empty(n, dtype=torch.uint8, device=q.device) if n else None
-        if workspace is not None and stream is not None:
-            workspace.record_stream(stream)
-    elif not workspace.is_contiguous():
-        raise ValueError("workspace: contiguous")
-    ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
-    _check(lib().tbq_attn_paged(C.byref(cache), layer, C.byref(batch), nq, _type_id(q.dtype), _ptr(q), qs, _ptr(out),
-                                window, sinks, scale, _ptr(workspace), ws_bytes, _stream(stream)), "tbq_attn_paged")
+        if n:
+            workspace = _torch.empty(n, dtype=_torch.uint8, device=q.device)
+            if stream is not None:
+                workspace.record_stream(stream)
+    else:
+        _on("workspace", workspace, dev)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace: contiguous")
+    wp, wb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    _check(lib().tbq_attn_paged(C.byref(cache), layer, C.byref(batch), nq, _type_id(q.dtype), q.data_ptr(), qs,
+                                out.data_ptr(), window, sinks, scale, wp, wb, _stream(stream)), "tbq_attn_paged")
     return out
 
 
@@ -186,23 +209,25 @@ def kv_copy_pages(cache: KvCache, src, dst, stream=None):
     n = len(src)
     if len(dst) != n:
         raise ValueError(f"{n} sources, {len(dst)} destinations")
-    _here(*cache._keep)
-    _check(lib().tbq_kv_copy_pages(C.byref(cache), (C.c_int * n)(*src), (C.c_int * n)(*dst), n, _stream(stream)),
-           "tbq_kv_copy_pages")
+    _here(cache)
+    arr = C.c_int * n
+    _check(lib().tbq_kv_copy_pages(C.byref(cache), arr(*src), arr(*dst), n, _stream(stream)), "tbq_kv_copy_pages")
 
 
 def kv_compact(cache: KvCache, page_table, keep_start, keep, stream=None):
     """Row j of sequence s becomes its row keep[keep_start[s] + j] (int32
     device tensors: page_table [sequences][pages], keep_start [sequences + 1])."""
-    _here(page_table, keep_start, keep, *cache._keep)
+    dev = _here(cache)
     if page_table.dim() != 2:
         raise ValueError("page_table: [sequences][pages]")
     n = page_table.shape[0]
-    _ints("page_table", page_table, tuple(page_table.shape))
+    _ints("page_table", page_table, page_table.shape)
     _ints("keep_start", keep_start, (n + 1,))
     _ints("keep", keep, (keep.numel(),))
-    _check(lib().tbq_kv_compact(C.byref(cache), n, _ptr(page_table), page_table.shape[1], _ptr(keep_start), _ptr(keep),
-                                _stream(stream)), "tbq_kv_compact")
+    for name, t in (("page_table", page_table), ("keep_start", keep_start), ("keep", keep)):
+        _on(name, t, dev)
+    _check(lib().tbq_kv_compact(C.byref(cache), n, page_table.data_ptr(), page_table.shape[1], keep_start.data_ptr(),
+                                keep.data_ptr(), _stream(stream)), "tbq_kv_compact")
 
 
 class PagePool:
