@@ -303,6 +303,22 @@ def test_attention_unseen_values_have_no_influence(bad, which):
                           spoil_pool=spoil_pool)
 
 
+def test_attention_unseen_values_in_one_of_several_splits():
+    """A chunk over a context long enough to be split: the last split holds a NaN that only the
+    last token sees, the first one what a window has passed; the other rows join as if they were
+    not there."""
+    def last(K, V, table, kv):
+        for t in (K, V):
+            t[:, table[0][(kv[0] - 1) // 64], :, (kv[0] - 1) % 64] = float("nan")
+    for act, cache in ATTN_TYPES:
+        run_attention(act, cache, 64, 4, 1, 64, [40], [2500], spoil_pool=last)
+
+    def early(K, V, table, kv):
+        V[:, table[0][20], :, 40:] = float("inf")   # positions 1320..1343 of a window of 1200
+    for act, cache in ATTN_TYPES:
+        run_attention(act, cache, 64, 4, 1, 64, [40], [2510], window=1200, sinks=70, spoil_pool=early)
+
+
 @pytest.mark.parametrize("peak", [0.0, 30.0])
 def test_attention_score_sizes(peak):
     """All scores alike, and one position that takes nearly all of a row."""

@@ -117,11 +117,12 @@ __device__ __forceinline__ V pg_keep(V v, uint32_t ones) {
 
 // One row by one wave, 64 positions at a time, from what the row sees only: lane
 // i scores position i of the tile, then the wave adds p V for the seen positions
-// in turn, lane l the dims l and l + 64.  *m, *l: maximum and sum.
+// in turn, lane l the dims l and l + 64.  *m, *l: maximum and sum; probabilities,
+// sum and output are scaled by 2^shift, as the other splits of the row have them.
 template <typename TA, typename TC, int D>
 __device__ __forceinline__ void pg_slow_row(const PgArgs &pg, const TA *q, float cs, int s, int kvh, int pos, int back,
-                                         int sinks, PgTiles tiles, int it0, int it1, float (&o)[D / 64], float *m,
-                                         float *l) {
+                                         int sinks, PgTiles tiles, int it0, int it1, float shift,
+                                         float (&o)[D / 64], float *m, float *l) {
     const int lane = threadIdx.x & 63, last = min(pos, pg.max_kv - 1);
 #pragma unroll
     for (int i = 0; i < D / 64; i++) o[i] = 0.f;
@@ -139,7 +140,7 @@ __device__ __forceinline__ void pg_slow_row(const PgArgs &pg, const TA *q, float
         }
         dot = sees ? dot * cs : -__builtin_huge_valf();
         const float mn = fmaxf(*m, wave_max(dot)), corr = __builtin_amdgcn_exp2f(*m - mn);
-        const float p = __builtin_amdgcn_exp2f(dot - mn);
+        const float p = __builtin_amdgcn_exp2f(dot - mn + shift);
         *m = mn;
         *l = *l * corr + group_sum<64>(p);
 #pragma unroll
@@ -531,12 +532,16 @@ __device__ __forceinline__ pg_s4 pg_read_tr(uint32_t addr) {
     return __builtin_amdgcn_ds_read_tr16_b64_v4i16((__attribute__((address_space(3))) pg_s4 *)(uintptr_t)addr);
 }
 
-// Block y of the batch: its sequence (-1: there is none) and its number in it.
-__device__ __forceinline__ int pg_chunk_block(const PgArgs &a, int G, int y, int *yb) {
+// Block y of the batch: its sequence s (-1: there is none) with its first token row,
+// its tokens and positions, and the block's number in it.  One round of loads.
+struct PcBlock {
+    int s, q0, qn, len, yb;
+};
+__device__ __forceinline__ PcBlock pg_chunk_block(const PgArgs &a, int G, int y) {
     const int lane = threadIdx.x & 63;
     for (int i = 0; i < a.n_seqs; i += 64) {
-        long long rows = 0;
-        if (i + lane < a.n_seqs) rows = (long long)(a.q_start[i + lane + 1] - a.q_start[i + lane]) * G;
+        const int s = min(i + lane, a.n_seqs - 1), q0 = a.q_start[s], qn = a.q_start[s + 1] - q0, len = a.kv_len[s];
+        const long long rows = i + lane < a.n_seqs ? (long long)qn * G : 0;
         const int nb = rows > PR_MAX ? (int)((rows + PC_ROWS - 1) / PC_ROWS) : 0;
         int sum = nb;   // inclusive over the lanes
 #pragma unroll
@@ -547,13 +552,12 @@ __device__ __forceinline__ int pg_chunk_block(const PgArgs &a, int G, int y, int
         const unsigned long long past = __builtin_amdgcn_ballot_w64(sum > y);
         if (past) {
             const int f = __builtin_ctzll(past);
-            const int end = __builtin_amdgcn_readlane(sum, f);
-            *yb = end - 1 - y;   // the last block first
-            return i + f;
+            return {i + f, __builtin_amdgcn_readlane(q0, f), __builtin_amdgcn_readlane(qn, f),
+                    __builtin_amdgcn_readlane(len, f), __builtin_amdgcn_readlane(sum, f) - 1 - y};   // the last block first
         }
         y -= __builtin_amdgcn_readlane(sum, 63);
     }
-    return -1;
+    return {-1, 0, 0, 0, 0};
 }
 
 // x: kv head + NKV * block; z: split.
@@ -568,13 +572,11 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
     constexpr float LAG = 8.f, SH = PgVec<TC>::SHIFT - (PgVec<TC>::SHIFT > 0.f ? 7.f : 0.f);
     const int kvh = x % a.pg.NKV, G = a.NQ / a.pg.NKV;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, h = lane >> 5;
-    int yb = 0;
-    const int s = pg_chunk_block(a.pg, G, x / a.pg.NKV, &yb);
-    if (s < 0) return;
-    const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
-    if (q0 < 0 || qn > a.pg.n_tokens - q0) return;
-    const int rows = qn * G, base = a.pg.kv_len[s] - qn;
-    const int r0 = yb * PC_ROWS, r1 = min(r0 + PC_ROWS, rows) - 1;
+    const PcBlock blk = pg_chunk_block(a.pg, G, x / a.pg.NKV);
+    const int s = blk.s, q0 = blk.q0, qn = blk.qn;
+    if (s < 0 || q0 < 0 || qn > a.pg.n_tokens - q0) return;
+    const int rows = qn * G, base = blk.len - qn;
+    const int r0 = blk.yb * PC_ROWS, r1 = min(r0 + PC_ROWS, rows) - 1;
     const int plo = base + r0 / G, phi = base + r1 / G, last = min(phi, a.pg.max_kv - 1);
     const int back = a.window > 0 ? a.window : 0x40000000;   // a token at p sees the positions > p - back
     const PgTiles tiles = pg_tiles<PC_TS>(plo, phi, a.window, a.sinks, a.pg.max_kv);
@@ -794,7 +796,7 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
         const int c = __builtin_ctzll(left), r = r0 + wave * 32 + c, t = r / G;
         float so[D / 64], sm, sl;
         pg_slow_row<TA, TC, D>(a.pg, (const TA *)a.q + (long long)(q0 + t) * a.qs + (long long)(kvh * G + r % G) * D, a.scale,
-                               s, kvh, base + t, back, a.sinks, tiles, it0, it1, so, &sm, &sl);
+                               s, kvh, base + t, back, a.sinks, tiles, it0, it1, SH, so, &sm, &sl);
         const long long to = (long long)(q0 + t) * a.NQ + kvh * G + r % G;
         float *rec = part + (to * nsplit + z) * pg_rec(D);
 #pragma unroll
@@ -836,22 +838,23 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
     }
 }
 
-// Sequences of many rows and, in the first workgroups, of few.  One launch: the
-// few rows' reads run beside the many rows' products.
+// Sequences of many rows and, in the last workgroups, of few.  One launch: the few
+// rows' reads run beside the last of the many rows' products (9 mixed sequences
+// 39.8 us, 45.5 as two launches, 41.7 with the few rows first).
 template <typename TC, int D, bool HL>
 __global__ __launch_bounds__(64 * PC_WAVES)
     __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void k_pg_attn_chunk(
         const PgAttn a, int nrb, int tps, int row_splits, float *__restrict__ row_part, int nsplit,
         float *__restrict__ part) {
     extern __shared__ __attribute__((aligned(1024))) unsigned char pc_lds[];
-    const int nrows = a.pg.NKV * nrb, rows = nrows * row_splits * a.pg.n_seqs, x = blockIdx.x;
-    if (x < rows) {
-        const int y = x / nrows;
-        pg_rows<TC, D, HL, false>(a, nrb, tps, row_splits, row_part, x % nrows, y % row_splits, y / row_splits,
-                           reinterpret_cast<PrLds<D> *>(pc_lds));
+    const int nrows = a.pg.NKV * nrb, chunks = (int)gridDim.x - nrows * row_splits * a.pg.n_seqs, x = blockIdx.x;
+    if (x >= chunks) {
+        const int y = (x - chunks) / nrows;
+        pg_rows<TC, D, HL, false>(a, nrb, tps, row_splits, row_part, (x - chunks) % nrows, y % row_splits, y / row_splits,
+                                  reinterpret_cast<PrLds<D> *>(pc_lds));
     } else {
-        const int y = (x - rows) / a.pg.NKV;
-        pg_chunk<TC, D, HL>(a, nsplit, part, (x - rows) % a.pg.NKV + a.pg.NKV * (y / nsplit), y % nsplit,
+        const int y = x / a.pg.NKV;
+        pg_chunk<TC, D, HL>(a, nsplit, part, x % a.pg.NKV + a.pg.NKV * (y / nsplit), y % nsplit,
                             reinterpret_cast<PcLds<D> *>(pc_lds));
     }
 }
