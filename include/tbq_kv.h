@@ -47,8 +47,8 @@ typedef struct {
  * n_tokens: rows of q, k, v and the outputs.  max_q, max_kv: what no
  * sequence's number of new tokens and of positions exceeds; launches are sized
  * by them, and 0 stands for n_tokens and max_pages * page_size.  Lengths
- * above them are an error that the device does not report: what lies beyond is
- * left out.  A page number outside the cache is never followed: keys there are
+ * above them (or above 2^30 positions) are an error that the device does not
+ * report: what lies beyond is left out.  A page number outside the cache is never followed: keys there are
  * not written and not visible. */
 typedef struct {
     int n_seqs, n_tokens, max_pages, max_q, max_kv;
@@ -116,8 +116,8 @@ int tbq_kv_append(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n
  * sees one is not finite where the formula is not), and pages that no token of the call sees any part of may be free: the kernel reads
  * nothing of theirs that enters a result.
  * q [n_tokens][n_heads][head_dim] with q_stride elements between tokens (a
- * multiple of 8), out contiguous, both of type q_type: the cache's type, or
- * F32 with an F16 cache.  Scores, softmax and sums are fp32.  16-bit products
+ * multiple of 8), out contiguous, not overlapping q, both of type q_type: the
+ * cache's type, or F32 with an F16 cache.  Scores, softmax and sums are fp32.  16-bit products
  * round the probabilities to the cache's type; F32 takes q and the
  * probabilities as pairs of halves (~22 bits, relative to a row's largest
  * element), so its rows are exact to about 1e-6.

@@ -250,16 +250,18 @@ def test_models_beyond_the_batched_rows(oracle):
     s.step({a: _tokens(rng, 1), b: _tokens(rng, 1)}, STEP_TOL)
 
 
-def test_many_sequences(oracle):
-    """More sequences than the 256 whose starts travel in one launch."""
-    m, model = _model(oracle, seed=8, n_layers=1)
+@pytest.mark.parametrize("n,vocab", [(300, 512), (9, 2064), (9, 514)])
+def test_many_sequences(oracle, n, vocab):
+    """More sequences than the 256 whose starts travel in one launch; an lm_head of several of the
+    weight buffer's 1024 rows, the last part of 16; one that the product does not take (rows not a
+    multiple of 4)."""
+    m, model = _model(oracle, seed=8, n_layers=1, vocab=vocab)
     import torch
-    n = 300
     cache = m.paged_cache(n)
     rng = np.random.default_rng(7)
     n_new = [1 + i % 3 for i in range(n)]
     toks = _tokens(rng, sum(n_new))
-    logits = torch.empty(n, 512, device="cuda")
+    logits = torch.empty(n, vocab, device="cuda")
     m.step(cache, n_new, n_new, [[i] for i in range(n)], toks, logits)
     got, at = host(logits), 0
     for i in range(n):

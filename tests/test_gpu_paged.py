@@ -269,6 +269,25 @@ def test_attention_long_context(act, cache):
     run_attention(act, cache, 64, 4, 1, 64, [33], [3000])
 
 
+def test_attention_bounds_leave_out_what_lies_beyond():
+    """Lengths above max_q and max_kv: the rows within them are as ever where nothing of theirs is
+    left out, nothing else is written or read."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(2)
+    q_lens, kv = [1, 60, 2], [90, 70, 200]
+    table, P = make_table(kv, 16, g)
+    K, V = fill_seen((1, P, 2, 16, 64), table, kv, 16, torch.float16, g)
+    Q = torch.randn(63, 4, 64, generator=g).half()
+    c, out = paged.kv_cache(K.cuda(), V.cuda()), torch.full((63, 4, 64), 7.0, dtype=torch.float16, device="cuda")
+    b = make_batch(q_lens, kv, table, max_q=2, max_kv=100)
+    paged.attn_paged(c, 0, b, Q.cuda(), out)
+    ref = attention(K, V, 0, starts(q_lens), kv, table, Q)
+    o, spread, size = ref[0]
+    assert bool(((out[0].cpu().double() - o).abs() <= attention_tolerance(o, spread, size, torch.float16, torch.float16)).all())
+    assert bool((out[1:61] == 7.0).all())          # more tokens than max_q
+    assert bool(torch.isfinite(out[61:]).all())    # positions from 100 on left out
+
+
 def test_attention_bad_pages_are_not_seen():
     def spoil(table, P):
         table[0][1] = -1                 # a hole
@@ -324,6 +343,14 @@ def test_attention_score_sizes(peak):
     """All scores alike, and one position that takes nearly all of a row."""
     for act, cache in ATTN_TYPES:
         run_attention(act, cache, 128, 4, 2, 16, [1, 50], [200, 10], peak=peak)
+
+
+@pytest.mark.parametrize("peak,scale", [(1e-37, 0.0), (1e-37, 1e-37), (1.0, 1e-38), (1e30, 1e-32), (6e4, 1e-6)])
+def test_attention_sizes_at_the_ends_of_the_types(peak, scale):
+    """Rows and scales whose product leaves fp32's normal numbers, or whose scores come near its end."""
+    for act, cache in ATTN_TYPES:
+        p = min(peak, 1e4) if act == "f16" else peak
+        run_attention(act, cache, 64, 4, 2, 16, [1, 50], [200, 10], peak=p, scale=scale if p == peak else 1e-6)
 
 
 def test_attention_scale_strides_and_bounds():

@@ -290,3 +290,24 @@ def test_attention_workspace_is_within_the_steps():
         b = batch(n_seqs=n, n_tokens=T, max_pages=pages, max_q=0 if T > n else 1)
         need = tb.lib().tbq_attn_paged_workspace_size(C.byref(c), C.byref(b), 8, 1)
         assert need <= tb.lib().tbq_dense_step_workspace_size(C.byref(m), C.byref(c), n, max(T, 2), pages)
+
+
+# ---- the built code ------------------------------------------------------------------
+def test_built_copies_wait_for_lds_reads(tmp_path):
+    """The chunk kernel's direct copies are issued with no LDS read outstanding (the walk of
+    test_lds_copies.py over this kernel)."""
+    import os
+    import shutil
+    import subprocess
+    from test_lds_copies import OBJDUMP, _copies
+    if not os.path.exists(OBJDUMP):
+        pytest.skip("no llvm-objdump")
+    lib = shutil.copy(tb.LIB_PATH, tmp_path / "lib.so")
+    subprocess.run([OBJDUMP, "--offloading", lib], cwd=tmp_path, check=True, capture_output=True)
+    seen = {}
+    for f in sorted(os.listdir(tmp_path)):
+        if "amdgcn" in f and b"k_pg_attn_chunk" in (tmp_path / f).read_bytes():
+            r = subprocess.run([OBJDUMP, "-d", "--no-show-raw-insn", f], cwd=tmp_path, check=True, capture_output=True, text=True)
+            seen.update(_copies(r.stdout.splitlines()))
+    assert any("k_pg_attn_chunk" in k for k in seen)
+    assert {k: c for k, c in seen.items() if c[1]} == {}

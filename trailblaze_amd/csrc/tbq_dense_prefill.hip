@@ -705,6 +705,7 @@ struct PfWs {
     float *x, *y, *qkv, *att, *gu, *sa, *sb, *part, *rope, *gpart;
     _Float16 *h16, *wh, *qb, *k16, *vt;
     size_t gpart_bytes;
+    size_t wh_halves;
     int cp;   // positions per head of k16 and vt
     int *tok;
     void *dec;
@@ -744,6 +745,7 @@ static PfWs pf_ws(const tbq_dense_model *m, int T, void *ws, size_t ws_bytes, si
         w.sa = (float *)take((size_t)T * 4);
         w.sb = (float *)take((size_t)T * 4);
         w.wh = (_Float16 *)take(wmax * 2);
+        w.wh_halves = wmax;
         if (!paged) {
             w.rope = (float *)take((size_t)T * m->head_dim * 4);
             // attention split partials: a prefill reaching position kmax - 1 uses
@@ -925,14 +927,62 @@ __global__ __launch_bounds__(256) void k_pf_ones(float *__restrict__ p, int n) {
     if (i < n) p[i] = 1.f;
 }
 
+// Row s of xg and yg: the residual and the last layer's output (its ny slices added
+// in slice order, scaled) of sequence s's last token.  grid = (ceil(H / 256), n_seqs).
+__global__ __launch_bounds__(256) void k_pf_last_rows(const float *__restrict__ x, const float *__restrict__ y, int ny,
+                                                      long long ystride, const float *__restrict__ ys,
+                                                      const int *__restrict__ q_start, int H, float *__restrict__ xg,
+                                                      float *__restrict__ yg) {
+    const int j = blockIdx.x * 256 + threadIdx.x, s = blockIdx.y, t = q_start[s + 1] - 1;
+    if (j >= H) return;
+    const long long at = (long long)t * H + j;
+    float a = y[at];
+    for (int z = 1; z < ny; z++) a = a + y[at + z * ystride];
+    xg[(long long)s * H + j] = x[at];
+    yg[(long long)s * H + j] = a * ys[t];
+}
+
+// Row s of n floats times sc[s].  grid = (ceil(n / 1024), rows).
+__global__ __launch_bounds__(256) void k_pf_scale_rows(float *__restrict__ p, int n, const float *__restrict__ sc) {
+    const float f = sc[blockIdx.y];
+    float *row = p + (long long)blockIdx.y * n;
+    for (int j = blockIdx.x * 1024 + threadIdx.x; j < min(n, (int)(blockIdx.x + 1) * 1024); j += 256) row[j] *= f;
+}
+
 // Behind the prefill's regions: the batch's ints, ones for the attention's row
-// scales, and the attention's workspace.
+// scales, the last tokens' rows, and the attention's workspace.
 struct StepWs {
     PfWs pf;
     int *ints;
-    float *ones;
+    float *ones, *xg, *yg;
     void *attn;
 };
+
+// Sequences from which the logits are one fp16 product with the lm_head, dequantised
+// as many rows at a time as the weights' buffer holds, instead of a matvec each.
+constexpr int STEP_LM_GEMM = 8;
+static hipError_t step_logits(const tbq_dense_model *m, const StepWs &w, int n_seqs, int T, const int *q_start,
+                              const float *ysrc, int yns, float *logits, hipStream_t st) {
+    const int H = m->hidden, V = m->vocab, qt = canon_qt(m->qtype_embd), cu = hgemm_cus();
+    hipLaunchKernelGGL(k_pf_last_rows, dim3((H + 255) / 256, n_seqs), dim3(256), 0, st, w.pf.x, ysrc, yns, (long long)T * H,
+                       w.pf.sb, q_start, H, w.xg, w.yg);
+    hipError_t err = launch_pf_norm(n_seqs, w.xg, w.yg, 1, 0, nullptr, m->output_norm, H, m->norm_eps, w.pf.h16, w.pf.sa, st);
+    const int most = (int)std::min<size_t>(w.pf.wh_halves / H, 1u << 20) / 16 * 16;
+    const size_t rb = tbq_row_bytes(qt, H);
+    for (int r = 0; r < V && err == hipSuccess; r += most) {
+        const int n = std::min(most, V - r);
+        const void *W = (const uint8_t *)m->lm_head + r * rb;
+        if (qt != QT_Q4_K) {
+            if ((err = launch_dequant_f16(qt, W, (long long)n * H, w.pf.wh, st)) != hipSuccess) break;
+            W = w.pf.wh;
+        }
+        err = launch_hgemm(qt == QT_Q4_K ? QT_Q4_K : QT_F16, W, w.pf.h16, n_seqs, n, H, logits + r, V, w.pf.gpart,
+                           w.pf.gpart_bytes, cu, st);
+    }
+    if (err != hipSuccess) return err;
+    hipLaunchKernelGGL(k_pf_scale_rows, dim3((V + 1023) / 1024, n_seqs), dim3(256), 0, st, logits, V, w.pf.sa);
+    return hipGetLastError();
+}
 static StepWs step_ws(const tbq_dense_model *m, int n_seqs, int T, int max_pages, void *ws, size_t ws_bytes,
                       size_t *total) {
     StepWs w{};
@@ -946,7 +996,10 @@ static StepWs step_ws(const tbq_dense_model *m, int n_seqs, int T, int max_pages
     };
     w.ints = (int *)take(((size_t)n_seqs * (max_pages + 2) + 1) * 4);
     w.ones = (float *)take((size_t)T * 4);
-    return *total = off, w;
+    w.xg = (float *)take((size_t)n_seqs * m->hidden * 4);
+    w.yg = (float *)take((size_t)n_seqs * m->hidden * 4);
+    *total = off;
+    return w;
 }
 
 static size_t step_attn_bytes(const tbq_dense_model *m, int n_seqs, int T, long long max_kv) {
@@ -1059,6 +1112,9 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
         const hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F16, TBQ_KV_F16, st);
         return e != hipSuccess ? e : launch_pg_attn(at, D, TBQ_KV_F16, TBQ_KV_F16, w.attn, st);
     }, &ysrc, &yns, st);
+    if (err != hipSuccess) return err;
+    if (n_seqs >= STEP_LM_GEMM && m->vocab % 4 == 0 && ((uintptr_t)logits & 15) == 0)
+        return step_logits(m, w, n_seqs, T, q_start, ysrc, yns, logits, st);
     for (int s = 0, t = -1; s < n_seqs && err == hipSuccess; s++) {
         t += n_new[s];
         err = pf_logits(m, w.pf, T, t, ysrc, yns, logits + (size_t)s * m->vocab, st);

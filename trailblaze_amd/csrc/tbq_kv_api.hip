@@ -71,7 +71,7 @@ PgArgs pg_args(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b) {
     a.max_pages = b->max_pages;
     a.max_q = b->max_q > 0 && b->max_q < b->n_tokens ? b->max_q : b->n_tokens;
     const long long room = (long long)b->max_pages * c->page_size;
-    const int most = room > 0x7FFFFFFF ? 0x7FFFFFFF : (int)room;
+    const int most = room > (1 << 30) ? 1 << 30 : (int)room;   // position arithmetic stays in 32 bits
     a.max_kv = b->max_kv > 0 && b->max_kv < most ? b->max_kv : most;
     a.q_start = b->q_start;
     a.kv_len = b->kv_len;

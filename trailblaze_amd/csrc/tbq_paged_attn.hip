@@ -34,6 +34,7 @@
 namespace tbq {
 
 constexpr float PG_LOW = -3.402823466e38f;   // the running maximum before any score
+constexpr float PG_TINY = 1.17549435e-38f;   // least scale: a hidden score, -infinity, times it stays one
 
 template <typename T>
 struct PgVec;
@@ -207,7 +208,7 @@ __device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int n
     const int row = r0 + (HL ? li & 7 : li), rc = min(row, rows - 1), tok = rc / G, pos = base + tok;
     // Q^T's columns
     h8 qf[NS];
-    float cs = a.scale;
+    float cs = fmaxf(a.scale, PG_TINY);
     {
         const long long off = (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * h;
         if constexpr (HL) {
@@ -224,7 +225,7 @@ __device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int n
             mx = swap32_max(swap16_max(mx));
             const int sh = pg_row_shift(mx);
             const float f = ldexpf(1.f, sh);
-            cs *= ldexpf(1.f, -sh);
+            cs = fmaxf(cs * ldexpf(1.f, -sh), PG_TINY);
 #pragma unroll
             for (int i = 0; i < NS; i++)
 #pragma unroll
@@ -588,7 +589,7 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
     const int w0 = min(r0 + wave * 32, rows - 1) / G, w1 = min(r0 + wave * 32 + 31, rows - 1) / G;
     // Q^T's columns: dim step i, lane half h has dims 16 i + 8 h .. + 8
     h8 qf[NP][NS];
-    float cs = a.scale;
+    float cs = fmaxf(a.scale, PG_TINY);
     {
         const long long off = (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * h;
         if constexpr (HL) {
@@ -604,7 +605,7 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
                 }
             const int sh = pg_row_shift(swap32_max(mx));
             const float f = ldexpf(1.f, sh);
-            cs *= ldexpf(1.f, -sh);
+            cs = fmaxf(cs * ldexpf(1.f, -sh), PG_TINY);
 #pragma unroll
             for (int i = 0; i < NS; i++)
 #pragma unroll
