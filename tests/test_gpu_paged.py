@@ -269,6 +269,13 @@ def test_attention_long_context(act, cache):
     run_attention(act, cache, 64, 4, 1, 64, [33], [3000])
 
 
+@pytest.mark.parametrize("act,cache", ATTN_TYPES)
+@pytest.mark.parametrize("q,heads,kv,past", [(9, 4, 1, 700), (17, 8, 4, 2300), (40, 4, 1, 5000), (33, 6, 2, 1100)])
+def test_attention_chunks_split_over_the_positions(act, cache, q, heads, kv, past):
+    """A few tokens over a long context, in one to dozens of splits, beside a single token."""
+    run_attention(act, cache, 64, heads, kv, 64, [q, 1], [past, 900])
+
+
 def test_attention_bounds_leave_out_what_lies_beyond():
     """Lengths above max_q and max_kv: the rows within them are as ever where nothing of theirs is
     left out, nothing else is written or read."""

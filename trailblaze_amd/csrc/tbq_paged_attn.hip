@@ -14,9 +14,8 @@
 // F32 rows (HL): q, scaled by the power of two that puts its largest element in
 // [2^13, 2^14), and the probabilities are each taken as two halves, x = hi + lo,
 // which keeps ~22 bits; the keys and values are halves already.  16-bit rows
-// round the probabilities to the cache's type.  Half probabilities are scaled up
-// (by 2^14, or 2^7 where the running maximum may lag 2^8 behind), so those that
-// a half cannot hold are below 2^-31 of the largest.
+// round the probabilities to the cache's type.  Half probabilities are scaled by
+// 2^14, so those that a half cannot hold are below 2^-38 of the largest.
 //
 // What a row does not see must not reach it, NaN and infinities included.
 // Scores are replaced before the maximum.  In the product with V an unseen
@@ -168,6 +167,11 @@ constexpr int pg_rec(int D) { return D + 4; }   // floats of a split's record: D
 // whose probabilities it computed, and the 8 x 8 halves, transposed in
 // registers, are the A operands of D / 16 products, product j giving the dims
 // congruent to j.  A tile's loads are issued a tile ahead.
+//
+// Bound by HBM: 64 ragged sequences of up to 8192 positions, 32 / 8 heads of 128,
+// read their 1.19 GB of keys and values once in 193 to 202 us (5.9 to 6.2 TB/s);
+// one token over 131072 positions, 268 MB, 45 to 48 us; one over 4096, 16.8 MB,
+// 6.8 us, which is the chain of lengths, page, rows and merge.
 // ---------------------------------------------------------------------------
 constexpr int PR_WAVES = 4, PR_TS = 32;
 // Rows up to which a sequence is one of few rows: 8 tokens of 4 heads a kv head
@@ -428,30 +432,19 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2
     pg_rows<TC, D, HL, ONCE>(a, nrb, tps, nsplit, part, blockIdx.x, blockIdx.y, blockIdx.z, &lds);
 }
 
-// Joins the splits of a row: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.
-// One workgroup a row.  GROUPS groups of D / 4
-// lanes each add every GROUPS-th split, then the groups are added in order:
-// a row's records (hundreds for one token over a long context) are read by as
-// many lanes as there are, 8 in flight each.
+// Joins the nz splits of a row: out = sum_z 2^(m_z - M) o_z / sum_z 2^(m_z - M) l_z.
+// One workgroup a row.  GROUPS groups of D / 4 lanes each add every GROUPS-th
+// split, then the groups are added in order: a row's records (hundreds for one
+// token over a long context) are read by as many lanes as there are, 8 in flight
+// each.
 constexpr int PJ_THREADS = 256, PJ_MAX = 1024;   // most splits (pg_plan)
-// x: kv head + NKV * row; s: sequence.
-template <typename TC, int D, bool HL>
-__device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, int nsplit, const float *__restrict__ part,
-                                             int xx, int s) {
-    constexpr int RB = HL ? 8 : 16, GROUPS = PJ_THREADS / (D / 4), REC = pg_rec(D);
+template <typename TO, int D>
+__device__ __forceinline__ void pg_join_row(const float *__restrict__ rec, int nz, TO *out) {
+    constexpr int GROUPS = PJ_THREADS / (D / 4), REC = pg_rec(D);
     __shared__ float fs[PJ_MAX];
     __shared__ float red[2][PJ_THREADS / 64];
     __shared__ __attribute__((aligned(16))) float os[GROUPS][D];
-    const int kvh = xx % a.pg.NKV, r = xx / a.pg.NKV, G = a.NQ / a.pg.NKV, tid = threadIdx.x;
-    const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
-    if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
-    const int rows = qn * G;
-    if (rows > PR_MAX || r >= rows) return;
-    const int base = a.pg.kv_len[s] - qn, r0 = r / RB * RB;
-    const int nz = (pg_tiles<PR_TS>(base + r0 / G, base + (min(r0 + RB, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n +
-                    tps - 1) / tps;
-    if (nz <= 1) return;
-    const float *rec = part + (((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit * REC;
+    const int tid = threadIdx.x;
     float mz[PJ_MAX / PJ_THREADS], lz[PJ_MAX / PJ_THREADS], M = PG_LOW;
 #pragma unroll
     for (int i = 0; i < PJ_MAX / PJ_THREADS; i++) {
@@ -499,10 +492,25 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
     float num = os[0][tid];
 #pragma unroll
     for (int i = 1; i < GROUPS; i++) num += os[i][tid];
-    const float out = den == 0.f ? 0.f : num / den;
-    const long long at = ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D + tid;
-    if constexpr (HL) ((float *)a.out)[at] = out;
-    else ((TC *)a.out)[at] = (TC)out;
+    out[tid] = (TO)(den == 0.f ? 0.f : num / den);
+}
+
+// A row of a sequence of few rows.  x: kv head + NKV * row; s: sequence.
+template <typename TO, int D, bool HL>
+__device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, int nsplit, const float *__restrict__ part,
+                                             int x, int s) {
+    constexpr int RB = HL ? 8 : 16;
+    const int kvh = x % a.pg.NKV, r = x / a.pg.NKV, G = a.NQ / a.pg.NKV;
+    const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
+    if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
+    const int rows = qn * G;
+    if (rows > PR_MAX || r >= rows) return;
+    const int base = a.pg.kv_len[s] - qn, r0 = r / RB * RB;
+    const int nz = (pg_tiles<PR_TS>(base + r0 / G, base + (min(r0 + RB, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n +
+                    tps - 1) / tps;
+    if (nz > 1)
+        pg_join_row<TO, D>(part + (((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit * pg_rec(D), nz,
+                           (TO *)a.out + ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D);
 }
 
 // ---------------------------------------------------------------------------
@@ -518,7 +526,7 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
 // transposing read lie in different banks.
 //
 // Blocks are numbered over the batch (a sequence's last one first, its rows see
-// most); blockIdx.y takes a share of the block's tiles where there are few
+// most); several workgroups share a block's tiles where there are few
 // blocks.
 // ---------------------------------------------------------------------------
 constexpr int PC_WAVES = 4, PC_TS = 64, PC_ROWS = 32 * PC_WAVES;
@@ -568,9 +576,10 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
     typedef typename PgVec<TC>::h8 h8;
     constexpr int NT = D / 32, NS = D / 16, SEG = D / 8, NP = HL ? 2 : 1, RPC = 64 / SEG;   // rows per copy
     constexpr int CPW = PC_TS / RPC / PC_WAVES;                                                 // copies per wave
-    // a running maximum that lags by up to LAG spares most of the rescalings of o (a wave's 32 rows
-    // rarely all keep theirs): 350 -> 340 us for 2048 tokens after 8192, 32 / 8 heads of 128
-    constexpr float LAG = 8.f, SH = PgVec<TC>::SHIFT - (PgVec<TC>::SHIFT > 0.f ? 7.f : 0.f);
+    // (m is the exact maximum: the position that holds it then has a power of two for its weight and no
+    // rounding.  One that may lag 2^8 behind spares most rescalings of o, 350 -> 340 us for 2048 tokens
+    // after 8192, but the errors of 16-bit rows grow by 8 to 15%)
+    constexpr float SH = PgVec<TC>::SHIFT;
     const int kvh = x % a.pg.NKV, G = a.NQ / a.pg.NKV;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, h = lane >> 5;
     const PcBlock blk = pg_chunk_block(a.pg, G, x / a.pg.NKV);
@@ -748,7 +757,7 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
 #pragma unroll
                 for (int e = 1; e < 32; e++) mx = fmaxf(mx, sc[e / 16][e % 16]);
                 mx = swap32_max(mx) * cs;
-                if (__builtin_amdgcn_ballot_w64(mx > m + LAG)) {
+                if (__builtin_amdgcn_ballot_w64(mx > m)) {
                     const float mn = fmaxf(m, mx), corr = __builtin_amdgcn_exp2f(m - mn);
                     m = mn;
                     l *= corr;
@@ -860,31 +869,44 @@ __global__ __launch_bounds__(64 * PC_WAVES)
     }
 }
 
-// Joins the splits of token t's rows in a sequence of many rows: D / 4 lanes have
-// a head, its at most PC_SPLITS records are loaded at once.
-constexpr int PC_SPLITS = 8;
-template <typename TC, int D, bool HL>
-__device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const float *__restrict__ part, int t) {
+// The splits of head hd's row of token t in a sequence of many rows (0 or 1: no records).
+__device__ __forceinline__ int pg_chunk_splits(const PgAttn &a, int q0, int rows, int base, int t, int hd, int nsplit) {
+    const int G = a.NQ / a.pg.NKV, r0 = ((t - q0) * G + hd % G) / PC_ROWS * PC_ROWS;
+    const int n = pg_tiles<PC_TS>(base + r0 / G, base + (min(r0 + PC_ROWS, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n;
+    const int tps = max((n + nsplit - 1) / nsplit, 1);
+    return (n + tps - 1) / tps;
+}
+
+// Joins the rows of token t (heads hd0 .. hd1 - 1) in a sequence of many rows: up to
+// PC_FEW splits D / 4 lanes have a head and load its records at once, else a
+// workgroup has a head.
+constexpr int PC_FEW = 8, PC_SPLITS = 256, PC_LEAST = 4;   // ..., most splits, tiles of one at least
+template <typename TO, int D>
+__device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const float *__restrict__ part, int t, int hd0,
+                                              int hd1) {
     constexpr int REC = pg_rec(D);
-    const int G = a.NQ / a.pg.NKV;
     const int s = pg_seq_of(a.pg.q_start, a.pg.n_seqs, t);
     if (s >= a.pg.n_seqs || t < a.pg.q_start[s]) return;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
-    if (q0 < 0 || qn > a.pg.n_tokens - q0 || (long long)qn * G <= PR_MAX) return;
-    const int rows = qn * G, base = a.pg.kv_len[s] - qn;
-    for (int i = threadIdx.x; i < a.NQ * (D / 4); i += PJ_THREADS) {
+    if (q0 < 0 || qn > a.pg.n_tokens - q0 || (long long)qn * (a.NQ / a.pg.NKV) <= PR_MAX) return;
+    const int rows = qn * (a.NQ / a.pg.NKV), base = a.pg.kv_len[s] - qn;
+    if (nsplit > PC_FEW) {
+        const long long at = (long long)t * a.NQ + hd0;
+        const int nz = pg_chunk_splits(a, q0, rows, base, t, hd0, nsplit);
+        if (nz > 1) pg_join_row<TO, D>(part + at * nsplit * REC, nz, (TO *)a.out + at * D);
+        return;
+    }
+    for (int i = hd0 * (D / 4) + threadIdx.x; i < hd1 * (D / 4); i += PJ_THREADS) {
         const int hd = i / (D / 4), d = i % (D / 4) * 4;
-        const int r0 = ((t - q0) * G + hd % G) / PC_ROWS * PC_ROWS;
-        const int n = pg_tiles<PC_TS>(base + r0 / G, base + (min(r0 + PC_ROWS, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n;
-        const int tps = max((n + nsplit - 1) / nsplit, 1), nz = (n + tps - 1) / tps;
+        const int nz = pg_chunk_splits(a, q0, rows, base, t, hd, nsplit);
         if (nz <= 1) continue;
         const long long at = (long long)t * a.NQ + hd;
         const float *rec = part + at * nsplit * REC;
-        float2 ml[PC_SPLITS];
-        float4 y[PC_SPLITS];
+        float2 ml[PC_FEW];
+        float4 y[PC_FEW];
         float M = PG_LOW;
 #pragma unroll
-        for (int z = 0; z < PC_SPLITS; z++) {   // past the last: the last again, not added
+        for (int z = 0; z < PC_FEW; z++) {   // past the last: the last again, not added
             ml[z] = *reinterpret_cast<const float2 *>(rec + min(z, nz - 1) * REC + D);
             y[z] = *reinterpret_cast<const float4 *>(rec + min(z, nz - 1) * REC + d);
             M = fmaxf(M, ml[z].x);
@@ -892,29 +914,28 @@ __device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const
         float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
         float den = 0.f;
 #pragma unroll
-        for (int z = 0; z < PC_SPLITS; z++) {
+        for (int z = 0; z < PC_FEW; z++) {
             if (z >= nz) continue;
             const float f = __builtin_amdgcn_exp2f(ml[z].x - M);
             x = make_float4(fmaf(f, y[z].x, x.x), fmaf(f, y[z].y, x.y), fmaf(f, y[z].z, x.z), fmaf(f, y[z].w, x.w));
             den = fmaf(f, ml[z].y, den);
         }
         const float inv = den == 0.f ? 0.f : 1.0f / den;
-        x = make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv);
-        if constexpr (HL) pg_st4((float *)a.out + at * D + d, x);
-        else pg_st4((TC *)a.out + at * D + d, x);
+        pg_st4((TO *)a.out + at * D + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
     }
 }
 
 // grid: row_wgs = NKV * (most rows of a few-row sequence) * n_seqs workgroups for
-// few rows (0: they were not split), then one a token (none if the many rows were
-// not split).
-template <typename TC, int D, bool HL>
+// few rows (0: they were not split), then one a token, or a token's head (none if
+// the many rows were not split).
+template <typename TO, int D, bool HL>
 __global__ __launch_bounds__(PJ_THREADS) void k_pg_join(const PgAttn a, int nrb, int tps, int row_splits,
                                                         const float *__restrict__ row_part, int row_wgs, int most,
                                                         int nsplit, const float *__restrict__ part) {
-    const int x = blockIdx.x, n = a.pg.NKV * most;
-    if (x < row_wgs) pg_join_rows<TC, D, HL>(a, nrb, tps, row_splits, row_part, x % n, x / n);
-    else pg_join_chunk<TC, D, HL>(a, nsplit, part, x - row_wgs);
+    const int x = blockIdx.x, n = a.pg.NKV * most, y = x - row_wgs;
+    if (x < row_wgs) pg_join_rows<TO, D, HL>(a, nrb, tps, row_splits, row_part, x % n, x / n);
+    else if (nsplit > PC_FEW) pg_join_chunk<TO, D>(a, nsplit, part, y / a.NQ, y % a.NQ, y % a.NQ + 1);
+    else pg_join_chunk<TO, D>(a, nsplit, part, y, 0, a.NQ);
 }
 
 // ---------------------------------------------------------------------------
@@ -958,11 +979,13 @@ static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, boo
     p.chunk_splits = 1;
     if (p.chunks) {
         const long long full = ((long long)a.n_tokens * G + PC_ROWS - 1) / PC_ROWS, w = a.NKV * full;
-        p.blocks = (int)full + a.n_seqs;
-        // two workgroups a CU, each with 8 tiles at least: a workgroup's start and its share of the
-        // join cost as much as about 4 (1 / 4 prompts of 512 / 100 tokens after 3584 / 1000)
+        // a last block that is not full for each sequence that has more than PR_MAX rows
+        p.blocks = (int)(full + std::min((long long)a.n_seqs, (long long)a.n_tokens * G / (PR_MAX + 1)));
+        // two workgroups a CU, each with PC_LEAST tiles: 16 tokens of 32 / 8 heads after 100000 positions
+        // 351 us in 8 splits, 97 in 64; 40 tokens after 2500 27.2 us with 8 tiles at least, 21.7 with 4,
+        // 4 prompts of 100 after 1000 32.8 and 33.4
         const long long t = (seen + PC_TS - 1) / PC_TS;
-        p.chunk_splits = (int)std::max(1ll, std::min(std::min((long long)PC_SPLITS, 2 * cu / w), t / 8));
+        p.chunk_splits = (int)std::max(1ll, std::min(std::min((long long)PC_SPLITS, 2 * cu / w), t / PC_LEAST));
         if (p.chunk_splits > 1) p.bytes += (size_t)a.n_tokens * NQ * p.chunk_splits * pg_rec(D) * 4;
     }
     return p;
@@ -1011,9 +1034,10 @@ static hipError_t pg_attn(const PgAttn &a, float *ws, hipStream_t st) {
                            p.row_tps, p.row_splits, ws, p.chunk_splits, part);
     }
     const int row_wgs = p.row_splits > 1 ? a.pg.NKV * p.most * a.pg.n_seqs : 0;
-    const int wgs = row_wgs + (p.chunk_splits > 1 ? a.pg.n_tokens : 0);
+    const int wgs = row_wgs + (p.chunk_splits > PC_FEW ? a.pg.n_tokens * a.NQ : p.chunk_splits > 1 ? a.pg.n_tokens : 0);
+    typedef typename std::conditional<HL, float, TC>::type TO;
     if (wgs > 0)
-        hipLaunchKernelGGL((k_pg_join<TC, D, HL>), dim3(wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps, p.row_splits, ws,
+        hipLaunchKernelGGL((k_pg_join<TO, D, HL>), dim3(wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps, p.row_splits, ws,
                            row_wgs, p.most, p.chunk_splits, part);
     return hipGetLastError();
 }
