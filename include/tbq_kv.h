@@ -48,8 +48,8 @@ typedef struct {
  * sequence's number of new tokens and of positions exceeds; launches are sized
  * by them, and 0 stands for n_tokens and max_pages * page_size.  Lengths
  * above them (or above 2^30 positions) are an error that the device does not
- * report: what lies beyond is left out.  A page number outside the cache is never followed: keys there are
- * not written and not visible. */
+ * report: what lies beyond is left out.  A page number outside the cache is
+ * never followed: keys there are not written and not visible. */
 typedef struct {
     int n_seqs, n_tokens, max_pages, max_q, max_kv;
     const int *q_start;    /* [n_seqs + 1] */
@@ -111,15 +111,16 @@ int tbq_kv_append(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n
  * t's sequence, query head h on kv head h / (n_heads / n_kv_heads).  A token
  * at position p sees the positions <= p; with window > 0 only those > p -
  * window, and the first `sinks` ones.  scale 0 stands for 1 / sqrt(head_dim);
- * else it is positive.  A row that sees nothing is 0.  What a token does not
- * see has no influence on its row, infinities and NaN included (a row that
- * sees one is not finite where the formula is not), and pages that no token of the call sees any part of may be free: the kernel reads
- * nothing of theirs that enters a result.
+ * else it is positive.  A row that sees nothing, or whose scores are all
+ * -infinity, is 0.  What a token does not see has no influence on its row,
+ * infinities and NaN included (a row that sees one is not finite where the
+ * formula is not), and pages that no token of the call sees any part of may be
+ * free: the kernel reads nothing of theirs that enters a result.
  * q [n_tokens][n_heads][head_dim] with q_stride elements between tokens (a
  * multiple of 8), out contiguous, not overlapping q, both of type q_type: the
- * cache's type, or F32 with an F16 cache.  Scores, softmax and sums are fp32.  16-bit products
- * round the probabilities to the cache's type; F32 takes q and the
- * probabilities as pairs of halves (~22 bits, relative to a row's largest
+ * cache's type, or F32 with an F16 cache.  Scores, softmax and sums are fp32.
+ * 16-bit products round the probabilities to the cache's type; F32 takes q and
+ * the probabilities as pairs of halves (~22 bits, relative to a row's largest
  * element), so its rows are exact to about 1e-6.
  * workspace: tbq_attn_paged_workspace_size() bytes, 16-byte aligned, no
  * zero-fill needed; calls that share one must not overlap. */
@@ -179,7 +180,8 @@ int tbq_kv_pool_defrag(tbq_kv_pool *p, int max, int *src, int *dst);
  * counts its positions with them, and page_table is [n_seqs][max_pages].
  * n_new, kv_len, page_table and tokens are host arrays, read before
  * the call returns.  Writes every
- * layer's K and V rows and logits[s][vocab] of each sequence's last token.
+ * layer's K and V rows and logits[s][vocab] of each sequence's last token.  A
+ * row of a page that two new tokens would write is refused.
  * The cache is F16 and has the model's layers, kv heads and head_dim.  rope
  * NULL: the model's theta on the whole head in halves.  window, sinks: as
  * tbq_attn_paged, in every layer.  One token of one sequence runs on the

@@ -292,3 +292,26 @@ def test_step_is_reproducible_and_takes_other_streams(oracle):
         out.append((host(logits), host(cache._keep[0]), host(cache._keep[1])))
     for o in out[1:]:
         assert all(np.array_equal(x, y) for x, y in zip(out[0], o))
+
+
+def test_step_refusals(oracle):
+    """What the Python entry checks: logits on the cache's device, no capture (a replay would take the
+    tokens and lengths of the captured call)."""
+    import torch
+    m, _ = _model(oracle)
+    c = m.paged_cache(4, 16)
+    logits = torch.empty(1, m.cfg.vocab, device="cuda")
+    a = (c, [1], [1], [[0]], [3])
+    with pytest.raises(ValueError, match="cpu"):
+        m.step(*a, logits.cpu())
+    m.step(*a, logits)
+    torch.cuda.synchronize()
+    st = torch.cuda.Stream()
+    with torch.cuda.stream(st):
+        g = torch.cuda.CUDAGraph()
+        g.capture_begin()
+        try:
+            with pytest.raises(ValueError, match="capture"):
+                m.step(*a, logits)
+        finally:
+            g.capture_end()

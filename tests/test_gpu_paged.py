@@ -329,6 +329,32 @@ def test_attention_unseen_values_have_no_influence(bad, which):
                           spoil_pool=spoil_pool)
 
 
+@pytest.mark.parametrize("past", [40, 900])
+def test_attention_keys_of_minus_infinity_weigh_nothing(past):
+    """A key that a 16-bit cache holds as -infinity in one place, where every row of q is positive: the
+    formula gives it the weight 0 and a finite row, in few rows and in many, split or not."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(past)
+    q_lens, kv = [1, 3, 60], [1 + past, 3 + past, 60 + past]
+    for act, cache in ATTN_TYPES:
+        table, P = make_table(kv, 16, g)
+        K, V = fill_seen((1, P, 2, 16, 64), table, kv, 16, TYPES[cache], g)
+        K0 = K.clone()
+        for s in range(3):
+            for p in (5, 33, past - 1):
+                K[0, table[s][p // 16], :, p % 16, 7] = -float("inf")
+                K0[0, table[s][p // 16], :, p % 16, 7] = 0
+        Q = torch.randn(64, 8, 64, generator=g).to(TYPES[act])
+        Q[:, :, 7] = Q[:, :, 7].abs() + 0.1
+        out = torch.empty(64, 8, 64, dtype=TYPES[act], device="cuda")
+        paged.attn_paged(paged.kv_cache(K.cuda(), V.cuda()), 0, make_batch(q_lens, kv, table), Q.cuda(), out)
+        ref, sizes = (attention(k, V, 0, starts(q_lens), kv, table, Q) for k in (K, K0))
+        for t in ref:
+            o, spread, _ = ref[t]
+            tol = attention_tolerance(o, spread, sizes[t][2], TYPES[act], TYPES[cache])   # finite scores' sizes
+            assert bool(torch.isfinite(o).all()) and bool(((out[t].cpu().double() - o).abs() <= tol).all()), (act, t)
+
+
 def test_attention_unseen_values_in_one_of_several_splits():
     """A chunk over a context long enough to be split: the last split holds a NaN that only the
     last token sees, the first one what a window has passed; the other rows join as if they were
@@ -438,6 +464,15 @@ def test_compact(D, page, lens, kept):
             for j, p in enumerate(r):
                 t[:, table[s][j // page], :, j % page] = old[:, table[s][p // page], :, p % page]
         assert torch.equal(dev.cpu(), t)
+
+
+def test_compact_of_nothing():
+    """No row of any sequence kept: nothing to move, and keep is an empty tensor."""
+    torch = _torch()
+    k = torch.randn(1, 4, 1, 16, 64).half().cuda()
+    old = k.clone()
+    paged.kv_compact(paged.kv_cache(k, k.clone()), ints([[0, 1], [2, 3]]), ints([0, 0, 0]), ints([]))
+    assert torch.equal(k, old)
 
 
 def test_compact_skips_bad_pages():

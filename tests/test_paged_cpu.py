@@ -104,6 +104,12 @@ def test_pool_fork(positions, page):
     assert pool.free_pages() == 8
 
 
+@pytest.mark.parametrize("positions,page", [(-1, 16), (3, 0), (17, 16)])
+def test_pool_fork_sizes(positions, page):
+    with pytest.raises(ValueError):
+        paged.PagePool(4).fork(positions, page, [0])
+
+
 def test_pool_refusals():
     with pytest.raises(tb.TbqError):
         paged.PagePool(0)
@@ -257,6 +263,21 @@ def step(m, c, n_new=(3, 1), kv_len=(20, 1), table=((0, 1), (2, -1)), tokens=(1,
     (dict(ws=FAKE + 8), "misaligned"), (dict(wsb=100), "workspace"), (dict(rope=paged.Rope(4, 0, 1.0)), "rope")])
 def test_dense_step_refusals(kw, words):
     refused(step(_dense(), cache(), **kw), words)
+
+
+@pytest.mark.parametrize("kw", [
+    dict(table=((0, 1), (1, -1)), n_new=(17, 3), kv_len=(32, 3)),      # 15..31 and 0..2 of pages 0, 1 and 1
+    dict(table=((0, 0), (1, -1)), n_new=(18, 1), kv_len=(32, 1)),      # 14 of a page and 14 of it again
+    dict(table=((0, 1), (0, 1)), n_new=(1, 1), kv_len=(20, 20))])
+def test_dense_step_refuses_two_tokens_in_one_row(kw):
+    refused(step(_dense(), cache(page_size=16), tokens=(1,) * 20, **kw), "share row")
+
+
+@pytest.mark.parametrize("kw", [
+    dict(table=((0, 1), (0, 2)), n_new=(1, 1), kv_len=(20, 20)),       # a shared page that is read only
+    dict(table=((0, 1), (0, 1)), n_new=(2, 1), kv_len=(20, 21))])      # rows 2, 3 and 4 of one page
+def test_dense_step_takes_shared_pages(kw):
+    refused(step(_dense(), cache(page_size=16), wsb=100, **kw), "workspace")   # what is checked last
 
 
 @pytest.mark.parametrize("kw,words", [(dict(type=30), "cache type"), (dict(n_layers=3), "a cache of"), (dict(n_kv_heads=4), "a cache of"),

@@ -523,6 +523,19 @@ int tbq_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, 
         }
     }
     if (T > 65536) return fail("%s: %lld tokens above 65536", who, T);
+    // a bit a row of the pages that new tokens are written to
+    unsigned char *written = (unsigned char *)calloc(((size_t)c->n_pages * c->page_size + 7) / 8, 1);
+    if (!written) return fail("%s: out of host memory", who);
+    long long twice = -1;
+    for (int q = 0; q < n_seqs; q++)
+        for (int p = kv_len[q] - n_new[q]; p < kv_len[q]; p++) {
+            const long long row = (long long)page_table[(long long)q * max_pages + p / c->page_size] * c->page_size + p % c->page_size;
+            if (written[row >> 3] >> (row & 7) & 1) twice = row;
+            written[row >> 3] |= 1 << (row & 7);
+        }
+    free(written);
+    if (twice >= 0)
+        return fail("%s: two new tokens share row %lld of page %lld", who, twice % c->page_size, twice / c->page_size);
     for (int t = 0; t < T; t++)
         if (tokens[t] < 0 || tokens[t] >= m->vocab) return fail("%s: token %d at %d out of range", who, tokens[t], t);
     tbq_rope own;

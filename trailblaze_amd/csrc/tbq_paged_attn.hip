@@ -298,7 +298,11 @@ __device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int n
 #pragma unroll
             for (int b = 0; b < 2; b++)
 #pragma unroll
-                for (int r = 0; r < 4; r++) sc[b][r] += dpp_f32<0x128>(sc[b][r]);   // row_ror:8
+                for (int r = 0; r < 4; r++) {
+                    const float x = sc[b][r], y = dpp_f32<0x128>(x), hi = li < 8 ? x : y;   // row_ror:8
+                    // (q's lo half times an infinite key may be the other infinity, or 0 times it)
+                    sc[b][r] = safe && !(fabsf(hi) < __builtin_huge_valf()) ? hi : x + y;
+                }
         }
         auto bit = [](int e) { return 16 * (e / 4) + e % 4; };
         if (!whole) {
@@ -1016,6 +1020,8 @@ size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int
     return (size_t)(rows * RB + chunk) * pg_rec(D) * 4;
 }
 
+constexpr long long PG_WGS = (1ll << 32) / 256 - 1;   // a launch's threads along x stay below 2^32
+
 template <typename TC, int D, bool HL>
 static hipError_t pg_attn(const PgAttn &a, float *ws, hipStream_t st) {
     const PgPlan p = pg_plan(a.pg, D, a.NQ, a.window, a.sinks, HL);
@@ -1035,16 +1041,19 @@ static hipError_t pg_attn(const PgAttn &a, float *ws, hipStream_t st) {
         if (e != hipSuccess) return e;
         const long long wgs = (long long)a.pg.NKV * ((long long)p.nrb * p.row_splits * a.pg.n_seqs +
                                                      (long long)p.blocks * p.chunk_splits);
-        if (wgs > 0x7FFFFFFF) return hipErrorInvalidConfiguration;
+        if (wgs > PG_WGS) return hipErrorInvalidConfiguration;
         hipLaunchKernelGGL((k_pg_attn_chunk<TC, D, HL>), dim3((unsigned)wgs), dim3(64 * PC_WAVES), lds, st, a, p.nrb,
                            p.row_tps, p.row_splits, ws, p.chunk_splits, part);
     }
-    const int row_wgs = p.row_splits > 1 ? a.pg.NKV * p.most * a.pg.n_seqs : 0;
-    const int wgs = row_wgs + (p.chunk_splits > PC_FEW ? a.pg.n_tokens * a.NQ : p.chunk_splits > 1 ? a.pg.n_tokens : 0);
+    const long long row_wgs = p.row_splits > 1 ? (long long)a.pg.NKV * p.most * a.pg.n_seqs : 0;
+    const long long wgs = row_wgs + (p.chunk_splits > PC_FEW ? (long long)a.pg.n_tokens * a.NQ
+                                     : p.chunk_splits > 1   ? a.pg.n_tokens
+                                                            : 0);
     typedef typename std::conditional<HL, float, TC>::type TO;
+    if (wgs > PG_WGS) return hipErrorInvalidConfiguration;
     if (wgs > 0)
-        hipLaunchKernelGGL((k_pg_join<TO, D, HL>), dim3(wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps, p.row_splits, ws,
-                           row_wgs, p.most, p.chunk_splits, part);
+        hipLaunchKernelGGL((k_pg_join<TO, D, HL>), dim3((unsigned)wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps,
+                           p.row_splits, ws, (int)row_wgs, p.most, p.chunk_splits, part);
     return hipGetLastError();
 }
 

@@ -142,6 +142,7 @@ class SyntheticDense:
         [sequences][pages] (host ints); logits [sequences][vocab] (device fp32)
         of each one's last token."""
         import torch
+        from . import paged
         ints = lambda v: np.ascontiguousarray(v, dtype=np.int32)   # noqa: E731
         n_new, kv_len, page_table, toks = ints(n_new), ints(kv_len), ints(page_table), ints(tokens)
         n = len(n_new)
@@ -149,6 +150,10 @@ class SyntheticDense:
             raise ValueError("n_new, kv_len and page_table: one row a sequence; tokens: the sum of n_new")
         if logits.numel() != n * self.cfg.vocab or logits.dtype != torch.float32 or not logits.is_contiguous():
             raise ValueError("logits: contiguous float32 [sequences][vocab]")
+        dev = paged._here(cache)
+        paged._on("logits", logits, dev)
+        if torch.cuda.is_current_stream_capturing():
+            raise ValueError("step is not for capture: a replay would repeat this call's tokens and lengths")
         need = int(lib().tbq_dense_step_workspace_size(C.byref(self.model), C.byref(cache), n, len(toks),
                                                        page_table.shape[1]))
         ws = getattr(self, "_step_ws", None)
@@ -160,7 +165,7 @@ class SyntheticDense:
         _check(lib().tbq_dense_step(C.byref(self.model), C.byref(cache), n, n_new.ctypes.data, kv_len.ctypes.data,
                                     page_table.ctypes.data, page_table.shape[1], toks.ctypes.data,
                                     None if rope is None else C.byref(rope), window, sinks, _ptr(logits), _ptr(ws),
-                                    0 if ws is None else ws.numel(), _stream(stream)), "tbq_dense_step")
+                                    0 if ws is None else ws.numel(), paged._to(stream, dev)), "tbq_dense_step")
         return logits
 
     def matvec_shapes(self):

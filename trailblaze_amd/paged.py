@@ -66,6 +66,13 @@ def _here(*owners):
     return cur
 
 
+def _to(stream, dev):
+    """_stream, of the device the tensors are on."""
+    if stream is not None and stream.device_index != dev:
+        raise ValueError(f"stream on cuda:{stream.device_index}, tensors on cuda:{dev}")
+    return _stream(stream)
+
+
 def _on(name, t, dev):
     if t.get_device() != dev:
         raise ValueError(f"{name}: tensor on {t.device}, current device is cuda:{dev}")
@@ -170,7 +177,7 @@ def kv_append(cache: KvCache, layer: int, batch: KvBatch, q, k, v, q_out, rope: 
         _on("positions", positions, dev)
     _check(lib().tbq_kv_append(C.byref(cache), layer, C.byref(batch), nq, None if rope is None else C.byref(rope),
                                _ptr(q_norm), _ptr(k_norm), eps, _ptr(positions), in_type, qp, qs, k.data_ptr(), ks,
-                               v.data_ptr(), vs, q_type, qo, _stream(stream)), "tbq_kv_append")
+                               v.data_ptr(), vs, q_type, qo, _to(stream, dev)), "tbq_kv_append")
     return q_out
 
 
@@ -200,7 +207,7 @@ def attn_paged(cache: KvCache, layer: int, batch: KvBatch, q, out, window: int =
             raise ValueError("workspace: contiguous")
     wp, wb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
     _check(lib().tbq_attn_paged(C.byref(cache), layer, C.byref(batch), nq, _type_id(q.dtype), q.data_ptr(), qs,
-                                out.data_ptr(), window, sinks, scale, wp, wb, _stream(stream)), "tbq_attn_paged")
+                                out.data_ptr(), window, sinks, scale, wp, wb, _to(stream, dev)), "tbq_attn_paged")
     return out
 
 
@@ -209,9 +216,9 @@ def kv_copy_pages(cache: KvCache, src, dst, stream=None):
     n = len(src)
     if len(dst) != n:
         raise ValueError(f"{n} sources, {len(dst)} destinations")
-    _here(cache)
+    dev = _here(cache)
     arr = C.c_int * n
-    _check(lib().tbq_kv_copy_pages(C.byref(cache), arr(*src), arr(*dst), n, _stream(stream)), "tbq_kv_copy_pages")
+    _check(lib().tbq_kv_copy_pages(C.byref(cache), arr(*src), arr(*dst), n, _to(stream, dev)), "tbq_kv_copy_pages")
 
 
 def kv_compact(cache: KvCache, page_table, keep_start, keep, stream=None):
@@ -226,8 +233,10 @@ def kv_compact(cache: KvCache, page_table, keep_start, keep, stream=None):
     _ints("keep", keep, (keep.numel(),))
     for name, t in (("page_table", page_table), ("keep_start", keep_start), ("keep", keep)):
         _on(name, t, dev)
+    if keep.numel() == 0:   # no row is kept, so none moves
+        return
     _check(lib().tbq_kv_compact(C.byref(cache), n, page_table.data_ptr(), page_table.shape[1], keep_start.data_ptr(),
-                                keep.data_ptr(), _stream(stream)), "tbq_kv_compact")
+                                keep.data_ptr(), _to(stream, dev)), "tbq_kv_compact")
 
 
 class PagePool:
@@ -264,6 +273,8 @@ class PagePool:
     def fork(self, positions: int, page_size: int, pages):
         """The child's pages, and (source, destination) of the page that is to
         be copied, or None."""
+        if positions < 0 or page_size < 1:
+            raise ValueError(f"{positions} positions in pages of {page_size}")
         n = -(-positions // page_size)
         if len(pages) < n:
             raise ValueError(f"{positions} positions need {n} pages, got {len(pages)}")
