@@ -276,6 +276,14 @@ def test_attention_chunks_split_over_the_positions(act, cache, q, heads, kv, pas
     run_attention(act, cache, 64, heads, kv, 64, [q, 1], [past, 900])
 
 
+@pytest.mark.parametrize("heads,kv,D", [(12, 3, 128), (33, 3, 64), (4, 1, 64)])
+def test_attention_joins_of_few_and_of_many_splits(heads, kv, D):
+    """As many splits as a row's lanes add in turn, and more (a workgroup a row); heads that leave a
+    joining workgroup partly empty."""
+    run_attention("f16", "f16", D, heads, kv, 64, [16], [9 * 64 * 4])
+    run_attention("f16", "f16", D, heads, kv, 64, [16], [36 * 64 * 4])
+
+
 def test_attention_bounds_leave_out_what_lies_beyond():
     """Lengths above max_q and max_kv: the rows within them are as ever where nothing of theirs is
     left out, nothing else is written or read."""

@@ -882,9 +882,11 @@ __device__ __forceinline__ int pg_chunk_splits(const PgAttn &a, int q0, int rows
 }
 
 // Joins the rows of token t (heads hd0 .. hd1 - 1) in a sequence of many rows: up to
-// PC_FEW splits D / 4 lanes have a head and load its records at once, else a
-// workgroup has a head.
-constexpr int PC_FEW = 8, PC_SPLITS = 256, PC_LEAST = 4;   // ..., most splits, tiles of one at least
+// PC_FEW splits D / 4 lanes have a head and load eight of its records at once, else
+// a workgroup has a head (384 tokens of 16 heads of 64 in 10 splits 24.8 and 37.4 us;
+// 64 tokens of 32 heads of 128 in 64 splits 74 and 66).
+constexpr int PC_FEW = 32, PC_SPLITS = 256, PC_LEAST = 4, PC_LONG = 16;   // ..., most splits, tiles of one at least
+__host__ __device__ constexpr int pj_heads(int D) { return PJ_THREADS / (D / 4); }   // of a workgroup
 template <typename TO, int D>
 __device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const float *__restrict__ part, int t, int hd0,
                                               int hd1) {
@@ -900,38 +902,43 @@ __device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const
         if (nz > 1) pg_join_row<TO, D>(part + at * nsplit * REC, nz, (TO *)a.out + at * D);
         return;
     }
-    for (int i = hd0 * (D / 4) + threadIdx.x; i < hd1 * (D / 4); i += PJ_THREADS) {
-        const int hd = i / (D / 4), d = i % (D / 4) * 4;
-        const int nz = pg_chunk_splits(a, q0, rows, base, t, hd, nsplit);
-        if (nz <= 1) continue;
-        const long long at = (long long)t * a.NQ + hd;
-        const float *rec = part + at * nsplit * REC;
-        float2 ml[PC_FEW];
-        float4 y[PC_FEW];
-        float M = PG_LOW;
+    const int hd = hd0 + threadIdx.x / (D / 4), d = threadIdx.x % (D / 4) * 4;
+    if (hd >= hd1) return;
+    const int nz = pg_chunk_splits(a, q0, rows, base, t, hd, nsplit);
+    if (nz <= 1) return;
+    const long long at = (long long)t * a.NQ + hd;
+    const float *rec = part + at * nsplit * REC;
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f, M = PG_LOW;
+    for (int z0 = 0; z0 < nz; z0 += 8) {
+        float2 ml[8];
+        float4 y[8];
+        float mn = M;
 #pragma unroll
-        for (int z = 0; z < PC_FEW; z++) {   // past the last: the last again, not added
-            ml[z] = *reinterpret_cast<const float2 *>(rec + min(z, nz - 1) * REC + D);
-            y[z] = *reinterpret_cast<const float4 *>(rec + min(z, nz - 1) * REC + d);
-            M = fmaxf(M, ml[z].x);
+        for (int z = 0; z < 8; z++) {   // past the last: the last again, not added
+            ml[z] = *reinterpret_cast<const float2 *>(rec + min(z0 + z, nz - 1) * REC + D);
+            y[z] = *reinterpret_cast<const float4 *>(rec + min(z0 + z, nz - 1) * REC + d);
+            mn = fmaxf(mn, ml[z].x);
         }
-        float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-        float den = 0.f;
+        const float c = __builtin_amdgcn_exp2f(M - mn);
+        M = mn;
+        x = make_float4(x.x * c, x.y * c, x.z * c, x.w * c);
+        den *= c;
 #pragma unroll
-        for (int z = 0; z < PC_FEW; z++) {
-            if (z >= nz) continue;
+        for (int z = 0; z < 8; z++) {
+            if (z0 + z >= nz) continue;
             const float f = __builtin_amdgcn_exp2f(ml[z].x - M);
             x = make_float4(fmaf(f, y[z].x, x.x), fmaf(f, y[z].y, x.y), fmaf(f, y[z].z, x.z), fmaf(f, y[z].w, x.w));
             den = fmaf(f, ml[z].y, den);
         }
-        const float inv = den == 0.f ? 0.f : 1.0f / den;
-        pg_st4((TO *)a.out + at * D + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
     }
+    const float inv = den == 0.f ? 0.f : 1.0f / den;
+    pg_st4((TO *)a.out + at * D + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
 }
 
 // grid: row_wgs = NKV * (most rows of a few-row sequence) * n_seqs workgroups for
-// few rows (0: they were not split), then one a token, or a token's head (none if
-// the many rows were not split).
+// few rows (0: they were not split), then one for pj_heads of a token's heads, or for
+// one of them (none if the many rows were not split).
 template <typename TO, int D, bool HL>
 __global__ __launch_bounds__(PJ_THREADS) void k_pg_join(const PgAttn a, int nrb, int tps, int row_splits,
                                                         const float *__restrict__ row_part, int row_wgs, int most,
@@ -939,7 +946,10 @@ __global__ __launch_bounds__(PJ_THREADS) void k_pg_join(const PgAttn a, int nrb,
     const int x = blockIdx.x, n = a.pg.NKV * most, y = x - row_wgs;
     if (x < row_wgs) pg_join_rows<TO, D, HL>(a, nrb, tps, row_splits, row_part, x % n, x / n);
     else if (nsplit > PC_FEW) pg_join_chunk<TO, D>(a, nsplit, part, y / a.NQ, y % a.NQ, y % a.NQ + 1);
-    else pg_join_chunk<TO, D>(a, nsplit, part, y, 0, a.NQ);
+    else {
+        const int hpw = pj_heads(D), g = (a.NQ + hpw - 1) / hpw;
+        pg_join_chunk<TO, D>(a, nsplit, part, y / g, y % g * hpw, min(y % g * hpw + hpw, a.NQ));
+    }
 }
 
 // ---------------------------------------------------------------------------
@@ -972,7 +982,12 @@ static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, boo
         // 351 us in 8 splits, 97 in 64; 40 tokens after 2500 27.2 us with 8 tiles at least, 21.7 with 4,
         // 4 prompts of 100 after 1000 32.8 and 33.4
         const long long t = (seen + PC_TS - 1) / PC_TS;
-        p.chunk_splits = (int)std::max(1ll, std::min(std::min((long long)PC_SPLITS, 2 * cu / w), t / PC_LEAST));
+        long long n = std::min(2 * cu / w, t / PC_LEAST);
+        // Heads of 64 leave room for three, which pays where a split keeps PC_LONG tiles: 16 ragged prompts
+        // of up to 300 after 3000 positions 66.8 us in one split, 49.5 in two; but 600 after 3000 with a
+        // window of 1024 34.3 in one, 35.7 in two.
+        if (D == 64) n = std::max(n, std::min(3 * cu / w, t / PC_LONG));
+        p.chunk_splits = (int)std::max(1ll, std::min((long long)PC_SPLITS, n));
     }
     const long long tiles = (seen + PR_TS - 1) / PR_TS + 1;
     // Two workgroups a CU run at once, so at least as many splits as fill them.  Longer ranges than
@@ -1010,13 +1025,13 @@ size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32) {
 
 // Rows: a batch of w workgroups a split has at most 512 / w + 1 splits to fill the
 // chip, or one for each `longest` tiles, where w / longest <= 2 PR_MANY / PR_LONG;
-// chunks: more than one split only while all of them fill two workgroups a CU.
+// chunks: more than one split only while all of them fill three workgroups a CU.
 size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int D, int NQ, bool f32) {
     const long long RB = f32 ? 8 : 16, w = (long long)NKV * (PR_MAX / RB) * n_seqs;
     const long long all = ((long long)max_kv + PR_TS - 1) / PR_TS + 1;
     const long long rows = std::max(512 + w, std::max(std::min(w, 2ll * PR_MANY) * ((all + PR_LONG - 1) / PR_LONG),
                                                       2ll * PR_MANY * all / PR_LONG + w));
-    const long long chunk = std::min((long long)n_tokens * NQ * PC_SPLITS, 512ll * PC_ROWS);
+    const long long chunk = std::min((long long)n_tokens * NQ * PC_SPLITS, 768ll * PC_ROWS);
     return (size_t)(rows * RB + chunk) * pg_rec(D) * 4;
 }
 
@@ -1047,7 +1062,7 @@ static hipError_t pg_attn(const PgAttn &a, float *ws, hipStream_t st) {
     }
     const long long row_wgs = p.row_splits > 1 ? (long long)a.pg.NKV * p.most * a.pg.n_seqs : 0;
     const long long wgs = row_wgs + (p.chunk_splits > PC_FEW ? (long long)a.pg.n_tokens * a.NQ
-                                     : p.chunk_splits > 1   ? a.pg.n_tokens
+                                     : p.chunk_splits > 1   ? (long long)a.pg.n_tokens * ((a.NQ + pj_heads(D) - 1) / pj_heads(D))
                                                             : 0);
     typedef typename std::conditional<HL, float, TC>::type TO;
     if (wgs > PG_WGS) return hipErrorInvalidConfiguration;
