@@ -284,6 +284,19 @@ def test_attention_joins_of_few_and_of_many_splits(heads, kv, D):
     run_attention("f16", "f16", D, heads, kv, 64, [16], [36 * 64 * 4])
 
 
+@pytest.mark.parametrize("wide", [False, True])
+@pytest.mark.parametrize("act,cache", ATTN_TYPES)
+def test_attention_drafts(act, cache, wide):
+    """Rows around the 16 and the 32 that a sequence of few rows has at most, in batches that may hold
+    little and more than 256 MiB of keys and values (wide tables)."""
+    def widen(table, P):
+        for r in table:
+            r.extend([-1] * 200)
+    for window in (0, 150):
+        run_attention(act, cache, 64, 16, 8, 256, [1, 4, 5, 8, 9, 16, 17], [300, 20, 0, 511, 300, 100, 250],
+                      window=window, spoil=widen if wide else None)
+
+
 def test_attention_bounds_leave_out_what_lies_beyond():
     """Lengths above max_q and max_kv: the rows within them are as ever where nothing of theirs is
     left out, nothing else is written or read."""

@@ -54,6 +54,7 @@ struct PgAttn {
     long long qs;
     void *out;             // [n_tokens][NQ][D]
     int NQ, window, sinks;
+    int few;               // rows up to which a sequence is one of few rows (launch_pg_attn sets it)
     float scale;           // of q . k, times log2(e): the softmax is in powers of two
 };
 

@@ -174,9 +174,14 @@ constexpr int pg_rec(int D) { return D + 4; }   // floats of a split's record: D
 // 6.8 us, which is the chain of lengths, page, rows and merge.
 // ---------------------------------------------------------------------------
 constexpr int PR_WAVES = 4, PR_TS = 32;
-// Rows up to which a sequence is one of few rows: 8 tokens of 4 heads a kv head
-// after 4000 positions 13.8 us as two row blocks, 28.6 as one of many; 16 tokens
-// of 8 sequences after 2000 40.0 us as four, 33.4 as many.
+// Rows up to which a sequence is one of few rows (PgAttn::few): PR_MAX, or half as
+// many where the batch's keys and values are more than the 256 MiB that the last
+// cache holds, so that each row block reads them from HBM again.  8 tokens of 4
+// heads a kv head, fp16, as two row blocks / as many rows: 1 sequence after 4096
+// positions 13.7 / 19.4 us, 32 after 1000 34.4 / 43.4, 32 after 4096 155 / 119, 64
+// after 4096 294 / 212; 16 tokens of 8 sequences after 2000 40.0 as four, 33.4 as
+// many.  fp32 as four blocks / as many: 24 after 1000 41.8 / 50.2, 64 after 4096
+// 417 / 284; 4 tokens as two / as many: 64 after 4096 267 / 275.
 constexpr int PR_MAX = 32;
 constexpr int PR_MIN = 4, PR_LONG = 64;   // tiles of a split: one a wave at least, 2048 positions at most
 constexpr int PR_MANY = 1024;              // (in batches of up to twice so many workgroups)
@@ -201,7 +206,7 @@ __device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int n
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
     if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
     const int rows = qn * G;
-    if (rows > PR_MAX || r0 >= rows) return;
+    if (rows > a.few || r0 >= rows) return;
     const int base = a.pg.kv_len[s] - qn;   // position of the first token
     const int t0 = r0 / G, t1 = (min(r0 + RB, rows) - 1) / G;   // the block's tokens
     const int plo = base + t0, phi = base + t1, last = min(phi, a.pg.max_kv - 1);
@@ -508,7 +513,7 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
     if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
     const int rows = qn * G;
-    if (rows > PR_MAX || r >= rows) return;
+    if (rows > a.few || r >= rows) return;
     const int base = a.pg.kv_len[s] - qn, r0 = r / RB * RB;
     const int nz = (pg_tiles<PR_TS>(base + r0 / G, base + (min(r0 + RB, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n +
                     tps - 1) / tps;
@@ -550,12 +555,12 @@ __device__ __forceinline__ pg_s4 pg_read_tr(uint32_t addr) {
 struct PcBlock {
     int s, q0, qn, len, yb;
 };
-__device__ __forceinline__ PcBlock pg_chunk_block(const PgArgs &a, int G, int y) {
+__device__ __forceinline__ PcBlock pg_chunk_block(const PgArgs &a, int few, int G, int y) {
     const int lane = threadIdx.x & 63;
     for (int i = 0; i < a.n_seqs; i += 64) {
         const int s = min(i + lane, a.n_seqs - 1), q0 = a.q_start[s], qn = a.q_start[s + 1] - q0, len = a.kv_len[s];
         const long long rows = i + lane < a.n_seqs ? (long long)qn * G : 0;
-        const int nb = rows > PR_MAX ? (int)((rows + PC_ROWS - 1) / PC_ROWS) : 0;
+        const int nb = rows > few ? (int)((rows + PC_ROWS - 1) / PC_ROWS) : 0;
         int sum = nb;   // inclusive over the lanes
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) {
@@ -586,7 +591,7 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
     constexpr float SH = PgVec<TC>::SHIFT;
     const int kvh = x % a.pg.NKV, G = a.NQ / a.pg.NKV;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 31, h = lane >> 5;
-    const PcBlock blk = pg_chunk_block(a.pg, G, x / a.pg.NKV);
+    const PcBlock blk = pg_chunk_block(a.pg, a.few, G, x / a.pg.NKV);
     const int s = blk.s, q0 = blk.q0, qn = blk.qn;
     if (s < 0 || q0 < 0 || qn > a.pg.n_tokens - q0) return;
     const int rows = qn * G, base = blk.len - qn;
@@ -894,7 +899,7 @@ __device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const
     const int s = pg_seq_of(a.pg.q_start, a.pg.n_seqs, t);
     if (s >= a.pg.n_seqs || t < a.pg.q_start[s]) return;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
-    if (q0 < 0 || qn > a.pg.n_tokens - q0 || (long long)qn * (a.NQ / a.pg.NKV) <= PR_MAX) return;
+    if (q0 < 0 || qn > a.pg.n_tokens - q0 || (long long)qn * (a.NQ / a.pg.NKV) <= a.few) return;
     const int rows = qn * (a.NQ / a.pg.NKV), base = a.pg.kv_len[s] - qn;
     if (nsplit > PC_FEW) {
         const long long at = (long long)t * a.NQ + hd0;
@@ -956,7 +961,7 @@ __global__ __launch_bounds__(PJ_THREADS) void k_pg_join(const PgAttn a, int nrb,
 // Host side: the splits, by what the host knows (max_q, max_kv, n_tokens).
 // ---------------------------------------------------------------------------
 struct PgPlan {
-    int most, nrb, row_tps, row_splits;   // few rows: most rows, row blocks, tiles of a split, splits
+    int few, most, nrb, row_tps, row_splits;   // few rows: up to, most there can be, row blocks, tiles of a split, splits
     bool chunks;                          // whether a sequence can have many rows
     int blocks, chunk_splits;
     size_t rows_bytes, bytes;             // workspace: the few rows' records, then the others'
@@ -965,18 +970,19 @@ struct PgPlan {
 static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32) {
     PgPlan p{};
     const int G = NQ / a.NKV, RB = f32 ? 8 : 16, cu = 256;
-    p.most = (int)std::min((long long)a.max_q * G, (long long)PR_MAX);
+    p.few = (double)a.n_seqs * a.max_kv * a.NKV * D * 4 > 256 << 20 ? PR_MAX / 2 : PR_MAX;
+    p.most = (int)std::min((long long)a.max_q * G, (long long)p.few);
     p.nrb = (p.most + RB - 1) / RB;
     // positions that one block can see
     long long seen = a.max_kv;
     if (window > 0) seen = std::min(seen, (long long)window + sinks + 2 * PC_TS + std::min(a.max_q, PC_ROWS));
-    p.chunks = (long long)a.max_q * G > PR_MAX;
+    p.chunks = (long long)a.max_q * G > p.few;
     p.chunk_splits = 1;
     if (p.chunks) {
-        // a last block that is not full for each sequence that has more than PR_MAX rows; half of them
+        // a last block that is not full for each sequence that has many rows; half of them
         // counted as there
         const long long full = ((long long)a.n_tokens * G + PC_ROWS - 1) / PC_ROWS;
-        p.blocks = (int)(full + std::min((long long)a.n_seqs, (long long)a.n_tokens * G / (PR_MAX + 1)));
+        p.blocks = (int)(full + std::min((long long)a.n_seqs, (long long)a.n_tokens * G / (p.few + 1)));
         const long long w = a.NKV * ((full + p.blocks) / 2);
         // two workgroups a CU, each with PC_LEAST tiles: 16 tokens of 32 / 8 heads after 100000 positions
         // 351 us in 8 splits, 97 in 64; 40 tokens after 2500 27.2 us with 8 tiles at least, 21.7 with 4,
@@ -1038,8 +1044,9 @@ size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int
 constexpr long long PG_WGS = (1ll << 32) / 256 - 1;   // a launch's threads along x stay below 2^32
 
 template <typename TC, int D, bool HL>
-static hipError_t pg_attn(const PgAttn &a, float *ws, hipStream_t st) {
+static hipError_t pg_attn(PgAttn a, float *ws, hipStream_t st) {
     const PgPlan p = pg_plan(a.pg, D, a.NQ, a.window, a.sinks, HL);
+    a.few = p.few;
     float *part = ws + p.rows_bytes / 4;
     if (!p.chunks) {
         const dim3 grid(a.pg.NKV * p.nrb, p.row_splits, a.pg.n_seqs);
