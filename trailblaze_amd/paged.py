@@ -37,15 +37,18 @@ class Rope(C.Structure):
     _fields_ = [("rot_dim", C.c_int), ("layout", C.c_int), ("mscale", C.c_double), ("freq", C.c_double * 64)]
 
 
-_torch, _ids = None, {}
+_torch, _raw, _device, _ids = None, None, None, {}
 
 
 def _init_torch():
     """torch, imported at the first use as everywhere in this package."""
-    global _torch
+    global _torch, _raw, _device
     if _torch is None:
         import torch
         _torch = torch
+        # (torch's own functions behind current_stream and current_device, 3 and 0.3 us a call less)
+        _raw = getattr(torch._C, "_cuda_getCurrentRawStream", None)
+        _device = getattr(torch._C, "_cuda_getDevice", torch.cuda.current_device)
         _ids.update({torch.float32: F32, torch.float16: F16, torch.bfloat16: BF16})
     return _torch
 
@@ -59,7 +62,8 @@ def _type_id(dtype):
 
 def _here(*owners):
     """The current device, whose stream the call takes: that of the cache and the batch."""
-    cur = _init_torch().cuda.current_device()
+    _init_torch()
+    cur = _device()
     for o in owners:
         if o._dev != cur:
             raise ValueError(f"tensors on device {o._dev}, current device is cuda:{cur}")
@@ -67,8 +71,10 @@ def _here(*owners):
 
 
 def _to(stream, dev):
-    """_stream, of the device the tensors are on."""
-    if stream is not None and stream.device_index != dev:
+    """_stream, of the current device, which the tensors are on."""
+    if stream is None:
+        return _stream() if _raw is None else _raw(dev)
+    if stream.device_index != dev:
         raise ValueError(f"stream on cuda:{stream.device_index}, tensors on cuda:{dev}")
     return _stream(stream)
 
