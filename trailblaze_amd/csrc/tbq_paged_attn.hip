@@ -169,9 +169,10 @@ constexpr int pg_rec(int D) { return D + 4; }   // floats of a split's record: D
 // congruent to j.  A tile's loads are issued a tile ahead.
 //
 // Bound by HBM: 64 ragged sequences of up to 8192 positions, 32 / 8 heads of 128,
-// read their 1.19 GB of keys and values once in 193 to 202 us (5.9 to 6.2 TB/s);
+// read their 1.19 GB of keys and values once in 196 to 203 us (5.9 to 6.1 TB/s);
 // one token over 131072 positions, 268 MB, 45 to 48 us; one over 4096, 16.8 MB,
-// 6.8 us, which is the chain of lengths, page, rows and merge.
+// 7 us: 3.6 of the bytes, and a launch with the chain of lengths, page, rows and
+// merge (the page looked up beside the lengths instead of after them: 0.2 less).
 // ---------------------------------------------------------------------------
 constexpr int PR_WAVES = 4, PR_TS = 32;
 // Rows up to which a sequence is one of few rows (PgAttn::few): PR_MAX, or half as
@@ -537,6 +538,13 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
 // Blocks are numbered over the batch (a sequence's last one first, its rows see
 // most); several workgroups share a block's tiles where there are few
 // blocks.
+//
+// Bound by the MFMAs and the softmax's VALU work: 2048 tokens after 8192 positions,
+// 32 / 8 heads of 128, fp16, 343 to 370 us (0.84 to 0.90 PFLOP/s), each of the two
+// half of a SIMD's cycles at the 1.65 GHz that the power limit leaves; batches of
+// less than a workgroup a CU by a tile's chain of products, maximum and powers, 0.95
+// us with heads of 64.  Slower: the next tile's scores under this one's softmax (382
+// us), sums by dot products; no faster: wave priorities, three tiles in LDS.
 // ---------------------------------------------------------------------------
 constexpr int PC_WAVES = 4, PC_TS = 64, PC_ROWS = 32 * PC_WAVES;
 
@@ -1006,7 +1014,7 @@ static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, boo
     long long tps = (tiles + want - 1) / want;
     // Beside many rows, ranges that take about as long as a split of theirs (a wave of few rows takes
     // half as long a position) fill the chip no worse, and rows that are not split need no join: 9
-    // mixed sequences with a window of 1024 41.3 -> 37.0 us.
+    // mixed sequences with a window of 1024 41.3 -> 37.1 us.
     if (p.chunks) tps = std::max(tps, (seen + PC_TS - 1) / PC_TS * 4 / p.chunk_splits);
     tps = std::max((long long)PR_MIN, std::min(longest, (tps + 3) / 4 * 4));
     if ((tiles + tps - 1) / tps > PJ_MAX) tps = (tiles + PJ_MAX - 1) / PJ_MAX;
