@@ -539,12 +539,14 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
 // most); several workgroups share a block's tiles where there are few
 // blocks.
 //
-// Bound by the MFMAs and the softmax's VALU work: 2048 tokens after 8192 positions,
-// 32 / 8 heads of 128, fp16, 343 to 370 us (0.84 to 0.90 PFLOP/s), each of the two
-// half of a SIMD's cycles at the 1.65 GHz that the power limit leaves; batches of
-// less than a workgroup a CU by a tile's chain of products, maximum and powers, 0.95
-// us with heads of 64.  Slower: the next tile's scores under this one's softmax (382
-// us), sums by dot products; no faster: wave priorities, three tiles in LDS.
+// Bound by power where it fills the chip: 2048 tokens after 8192 positions, 32 / 8
+// heads of 128, fp16, 343 to 370 us (0.84 to 0.90 PFLOP/s), MFMAs and VALU each half of
+// a SIMD's cycles at 1.65 GHz.  With a quarter more cycles a tile (added by counting
+// them) the clock rose to 2.0 GHz and a tile took as long; so fewer waits gain
+// nothing there: keys read ahead of their products -1 to 3%, copies between the products
+// -10%, the next tile's scores under this one's softmax -9%, three tiles in LDS 0 to
+// -4%.  Smaller batches are bound by a tile's chain of products, maximum and powers,
+// 0.95 us with heads of 64.
 // ---------------------------------------------------------------------------
 constexpr int PC_WAVES = 4, PC_TS = 64, PC_ROWS = 32 * PC_WAVES;
 
@@ -660,40 +662,27 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
         vo[i] = (uint32_t)((r & 15) * D * 2 + 16 * ((lane % SEG) ^ vswz(r)));
     }
     const uint32_t lk = lds_addr(st->k[0]), lv = lds_addr(st->v[0]);
-    int pages = -1;   // lane i: the page of block i % 4 of tile i / 4 (of 16 tiles)
-    uint64_t nopage = 0;   // bit i: lane i has none
-    auto look_up = [&](int n) {
-        const int it = it0 + n + (lane >> 2);
-        pages = it < it1 ? pg_block_page(a.pg, s, tiles.at(it) * PC_TS + 16 * (lane & 3), last) : -1;
-        nopage = __builtin_amdgcn_ballot_w64(pages < 0);
-    };
+    uint32_t off_lo = 0, off_hi = 0;   // lane i: bytes before block i % 4 of tile i / 4 (of 16 tiles)
+    uint64_t nopage = 0;               // bit i: lane i's has no page
     const int pmask = (1 << a.pg.shift) - 1;
     const long long hbytes = (long long)(2 * D) << a.pg.shift;   // bytes of a kv head in a page
+    auto look_up = [&](int n) {
+        const int it = it0 + n + (lane >> 2), pos = tiles.at(it) * PC_TS + 16 * (lane & 3);
+        const int page = it < it1 ? pg_block_page(a.pg, s, pos, last) : -1;
+        nopage = __builtin_amdgcn_ballot_w64(page < 0);
+        const long long off = ((long long)max(page, 0) * a.pg.NKV + kvh) * hbytes + (long long)(pos & pmask) * (2 * D);
+        off_lo = (uint32_t)off;
+        off_hi = (uint32_t)(off >> 32);
+    };
     auto copy = [&](int buf, int n) {
-        const int k0 = tiles.at(it0 + n) * PC_TS;
-        auto at = [&](int b) {   // bytes before block b's rows
-            const int page = max(__builtin_amdgcn_readlane(pages, 4 * (n & 15) + b), 0);
-            return ((long long)page * a.pg.NKV + kvh) * hbytes + (long long)((k0 + 16 * b) & pmask) * (2 * D);
-        };
-        const uint32_t to = buf * (PC_TS * D * 2);
-        if (pmask >= PC_TS - 1) {   // the tile lies in one page (uniform)
-            const long long off = at(0);
-            const dma_rsrc_t kr = dma_rsrc((const uint8_t *)a.pg.k + off, PC_TS * 2 * D);
-            const dma_rsrc_t vr = dma_rsrc((const uint8_t *)a.pg.v + off, PC_TS * 2 * D);
 #pragma unroll
-            for (int i = 0; i < CPW; i++) {
-                const int c = wave + PC_WAVES * i, blk = c * RPC / 16;
-                dma16(lk + to + c * 1024, ko[i], kr, blk * 32 * D);
-                dma16(lv + to + c * 1024, vo[i], vr, blk * 32 * D);
-            }
-        } else {
-#pragma unroll
-            for (int i = 0; i < CPW; i++) {
-                const int c = wave + PC_WAVES * i;
-                const long long off = at(c * RPC / 16);
-                dma16(lk + to + c * 1024, ko[i], dma_rsrc((const uint8_t *)a.pg.k + off, 32 * D), 0);
-                dma16(lv + to + c * 1024, vo[i], dma_rsrc((const uint8_t *)a.pg.v + off, 32 * D), 0);
-            }
+        for (int i = 0; i < CPW; i++) {
+            const int c = wave + PC_WAVES * i, at = 4 * (n & 15) + c * RPC / 16;
+            const long long off = (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)off_hi, at) << 32 |
+                                              (uint32_t)__builtin_amdgcn_readlane((int)off_lo, at));
+            const uint32_t to = buf * (PC_TS * D * 2) + c * 1024;
+            dma16(lk + to, ko[i], dma_rsrc((const uint8_t *)a.pg.k + off, 32 * D), 0);
+            dma16(lv + to, vo[i], dma_rsrc((const uint8_t *)a.pg.v + off, 32 * D), 0);
         }
     };
     // V's transposing reads: lane l of 16 addresses position kk = l / 4 of 4, dims 4 (l % 4) .. + 4
