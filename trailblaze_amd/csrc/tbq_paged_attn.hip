@@ -888,6 +888,7 @@ __device__ __forceinline__ int pg_chunk_splits(const PgAttn &a, int q0, int rows
 // a workgroup has a head (384 tokens of 16 heads of 64 in 10 splits 24.8 and 37.4 us;
 // 64 tokens of 32 heads of 128 in 64 splits 74 and 66).
 constexpr int PC_FEW = 32, PC_SPLITS = 256, PC_LEAST = 4, PC_LONG = 16;   // ..., most splits, tiles of one at least
+constexpr long long PC_SHORT = 8;
 __host__ __device__ constexpr int pj_heads(int D) { return PJ_THREADS / (D / 4); }   // of a workgroup
 template <typename TO, int D>
 __device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const float *__restrict__ part, int t, int hd0,
@@ -986,6 +987,10 @@ static PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, boo
         // 4 prompts of 100 after 1000 32.8 and 33.4
         const long long t = (seen + PC_TS - 1) / PC_TS;
         long long n = std::min(2 * cu / w, t / PC_LEAST);
+        // or half so many tiles, up to PC_SHORT splits that all run at once: 72 tokens after 393 14.9 -> 12.9,
+        // 835 tokens 21.4 -> 17.9, 15 sequences of 65 after 633 17.2 -> 18.5 (more splits, or of fewer than 8
+        // tiles, are slower)
+        if (t >= 2 * PC_LEAST) n = std::max(n, std::min(2 * cu / ((long long)a.NKV * p.blocks), std::min(2 * t / PC_LEAST, PC_SHORT)));
         // Heads of 64 leave room for three, which pays where a split keeps PC_LONG tiles: 16 ragged prompts
         // of up to 300 after 3000 positions 66.8 us in one split, 49.5 in two; but 600 after 3000 with a
         // window of 1024 34.3 in one, 35.7 in two.
