@@ -174,6 +174,13 @@ def test_append_many_sequences(seqs):
                layers=1, layer=0)
 
 
+@pytest.mark.parametrize("seqs", [4095, 4096, 4097, 5000])
+def test_append_thousands_of_sequences(seqs):
+    """Lookups of one, two and three rounds, a long run of empty sequences among them."""
+    run_append("f16", "f16", "f16", 64, 1, 1, 16, [0 if 100 < i < 1500 else (i * 7) % 3 for i in range(seqs)],
+               [i % 5 for i in range(seqs)], layers=1, layer=0)
+
+
 @pytest.mark.parametrize("T", [300, 2500])
 def test_append_long_prompt(T):
     run_append("f32", "f16", "f16", 128, 4, 2, 64, [T], [100], scaling="yarn", factor=4.0, orig=1024)

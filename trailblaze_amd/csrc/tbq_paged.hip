@@ -27,9 +27,9 @@ namespace tbq {
 // to fp16, 302 MB: 56 to 61 us (5.0 to 5.4 TB/s); one token 3.1 us.
 // ---------------------------------------------------------------------------
 constexpr int AP_THREADS = 256;
-template <typename TI, typename TQ, typename TC, int D, int HPT>
-__global__ __launch_bounds__(AP_THREADS) void k_pg_append(const PgAppend a) {
-    constexpr int LPH = D / 8, SL = AP_THREADS / LPH;
+template <typename TI, typename TQ, typename TC, int D, int HPT, int TH>
+__global__ __launch_bounds__(TH) void k_pg_append(const PgAppend a) {
+    constexpr int LPH = D / 8, SL = TH / LPH;
     const int t = blockIdx.x, l = threadIdx.x % LPH, rot = a.rope.rot;
     const int nslots = a.NQ + 2 * a.pg.NKV;
     const int s = pg_seq_of(a.pg.q_start, a.pg.n_seqs, t);
@@ -128,9 +128,14 @@ static hipError_t append_d(const PgAppend &a, hipStream_t st) {
     // (512 tokens) or faster (64 tokens 3.8 us, 4.8 with three).
     const int hpt = (long long)a.pg.n_tokens * nb >= 2048 ? std::min(nb, 3) : 1;
     const dim3 grid(a.pg.n_tokens, (nb + hpt - 1) / hpt);
-    if (hpt == 3) hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 3>), grid, dim3(AP_THREADS), 0, st, a);
-    else if (hpt == 2) hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 2>), grid, dim3(AP_THREADS), 0, st, a);
-    else hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 1>), grid, dim3(AP_THREADS), 0, st, a);
+    // Few heads (a shard of a model) leave most of a workgroup idle: one of 64 or 128 threads then.  12
+    // prompts of 410 tokens, 4 + 1 + 1 heads of 64: 10.7 -> 6 us.
+    const int th = nb > 1 ? AP_THREADS : (a.NQ + 2 * a.pg.NKV) * (D / 8);
+    if (hpt == 3) hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 3, AP_THREADS>), grid, dim3(AP_THREADS), 0, st, a);
+    else if (hpt == 2) hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 2, AP_THREADS>), grid, dim3(AP_THREADS), 0, st, a);
+    else if (th <= 64) hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 1, 64>), grid, dim3(64), 0, st, a);
+    else if (th <= 128) hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 1, 128>), grid, dim3(128), 0, st, a);
+    else hipLaunchKernelGGL((k_pg_append<TI, TQ, TC, D, 1, AP_THREADS>), grid, dim3(AP_THREADS), 0, st, a);
     return hipGetLastError();
 }
 
@@ -208,6 +213,7 @@ __global__ __launch_bounds__(CO_THREADS) void k_pg_compact(uint16_t *k, uint16_t
         const int b = j0 / lr & 1;
 #pragma unroll
         for (int i = 0; i < CO_LIST / CO_THREADS; i++) {
+            if (CO_THREADS * i >= n - j0 + jr) break;   // past the last step (uniform)
             const int e = threadIdx.x + CO_THREADS * i, j = j0 + e, jc = min(j, n - 1);
             const int from = keep[at + jc], p = max(from, 0), ps = pg_page(a, s, p), pd = pg_page(a, s, jc);
             const bool moves = j < n && from >= 0 && p != j && ps >= 0 && pd >= 0;

@@ -88,15 +88,19 @@ struct PgPairs {
 };
 
 // The sequence of token row t: the number of sequences that end at or before
-// it (n_seqs: none).  The whole wave calls it; uniform.
+// it (n_seqs: none).  The whole wave calls it; uniform.  Each round asks for every
+// step-th end, a lane each (4096 single tokens appended: 64 us with 64 rounds of
+// 64 ends side by side, 27 with two).
 __device__ __forceinline__ int pg_seq_of(const int *__restrict__ q_start, int n_seqs, int t) {
     const int lane = threadIdx.x & 63;
-    int s = 0;
-    for (int i = 0; i < n_seqs; i += 64) {
-        const bool ends = i + lane < n_seqs && q_start[i + lane + 1] <= t;
-        s += __builtin_popcountll(__builtin_amdgcn_ballot_w64(ends));
+    int lo = 0, hi = n_seqs;
+    while (lo < hi) {
+        const int step = (hi - lo + 63) >> 6, i = lo + (lane + 1) * step - 1;
+        const bool ends = i < hi && q_start[i + 1] <= t;
+        lo += __builtin_popcountll(__builtin_amdgcn_ballot_w64(ends)) * step;
+        hi = min(hi, lo + step - 1);
     }
-    return s;
+    return lo;
 }
 
 // The page of position p (>= 0) of sequence s, -1 where it has none.
