@@ -194,8 +194,8 @@ hipError_t launch_pg_copy(void *k, void *v, int n_layers, long long pbytes, long
 // Pages are looked up for CO_LIST rows at a time, into LDS: memory operations
 // complete in order, so a lookup per step would have waited for all of the
 // step's rows first.  16000 rows to 9001 in 36 layers, 4 heads of 128, 1.33 GB:
-// 265 to 314 us (4.2 to 5.0 TB/s; 803 with a step's lookups, loads and stores in
-// turn); 24 rows of 16 sequences to 9: 12 us, one step of each workgroup.
+// 261 to 313 us (4.2 to 5.1 TB/s; 803 with a step's lookups, loads and stores in
+// turn); 24 rows of 16 sequences to 9: 9.4 to 11 us, one step of each workgroup.
 // ---------------------------------------------------------------------------
 constexpr int CO_THREADS = 256, CO_V = 4, CO_UNITS = CO_THREADS / 8 * CO_V, CO_LIST = 1024;
 template <int D>

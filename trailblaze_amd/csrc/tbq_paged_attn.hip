@@ -169,7 +169,7 @@ constexpr int pg_rec(int D) { return D + 4; }   // floats of a split's record: D
 // congruent to j.  A tile's loads are issued a tile ahead.
 //
 // Bound by HBM: 64 ragged sequences of up to 8192 positions, 32 / 8 heads of 128,
-// read their 1.19 GB of keys and values once in 196 to 203 us (5.9 to 6.1 TB/s);
+// read their 1.19 GB of keys and values once in 191 to 203 us (5.9 to 6.2 TB/s);
 // one token over 131072 positions, 268 MB, 45 to 48 us; one over 4096, 16.8 MB,
 // 7 us: 3.6 of the bytes, and a launch with the chain of lengths, page, rows and
 // merge (the page looked up beside the lengths instead of after them: 0.2 less).
@@ -540,7 +540,7 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
 // blocks.
 //
 // Bound by power where it fills the chip: 2048 tokens after 8192 positions, 32 / 8
-// heads of 128, fp16, 343 to 370 us (0.84 to 0.90 PFLOP/s), MFMAs and VALU each half of
+// heads of 128, fp16, 341 to 371 us (0.83 to 0.91 PFLOP/s), MFMAs and VALU each half of
 // a SIMD's cycles at 1.65 GHz.  With a quarter more cycles a tile (added by counting
 // them) the clock rose to 2.0 GHz and a tile took as long; so fewer waits gain
 // nothing there: keys read ahead of their products -1 to 3%, copies between the products
@@ -856,7 +856,7 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
 
 // Sequences of many rows and, in the last workgroups, of few.  One launch: the few
 // rows' reads run beside the last of the many rows' products (9 mixed sequences
-// 39.8 us, 45.5 as two launches, 41.7 with the few rows first).
+// 39.8 us, 45.5 as two launches, 41.7 with the few rows first; 35 to 36 since).
 template <typename TC, int D, bool HL>
 __global__ __launch_bounds__(64 * PC_WAVES)
     __attribute__((amdgpu_waves_per_eu(D == 64 ? 3 : 2, D == 64 ? 3 : 2))) void k_pg_attn_chunk(
