@@ -545,8 +545,10 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
 // them) the clock rose to 2.0 GHz and a tile took as long; so fewer waits gain
 // nothing there: keys read ahead of their products -1 to 3%, copies between the products
 // -10%, the next tile's scores under this one's softmax -9%, three tiles in LDS 0 to
-// -4%.  Smaller batches are bound by a tile's chain of products, maximum and powers,
-// 0.95 us with heads of 64.
+// -4%.  Half the LDS reads would gain 15% (two row tiles a wave, for which 256
+// registers are too few), no copies at all 14%; eight waves on one tile gain 4% for 4096
+// tokens and lose 4 to 40% for fewer.  Smaller batches are bound by a tile's chain of
+// products, maximum and powers, 0.95 us with heads of 64.
 // ---------------------------------------------------------------------------
 constexpr int PC_WAVES = 4, PC_TS = 64, PC_ROWS = 32 * PC_WAVES;
 
