@@ -140,7 +140,8 @@ class SyntheticDense:
         """tbq_dense_step: n_new[s] tokens of every sequence s (side by side in
         `tokens`), kv_len[s] its positions with them, page_table
         [sequences][pages] (host ints); logits [sequences][vocab] (device fp32)
-        of each one's last token."""
+        of each one's last token.  The model has one workspace: steps on
+        several streams must wait for each other."""
         import torch
         from . import paged
         ints = lambda v: np.ascontiguousarray(v, dtype=np.int32)   # noqa: E731
