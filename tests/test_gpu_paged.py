@@ -562,6 +562,35 @@ def test_captured_decode_steps_follow_the_lengths(act, cache):
             assert torch.equal(s["out"], want) and torch.equal(s["K"], e["K"]) and torch.equal(s["V"], e["V"])
 
 
+@pytest.mark.parametrize("act,cache", ATTN_TYPES)
+def test_captured_chunks(act, cache):
+    """A chunk's append and attention, split and joined, captured with a workspace from the call itself
+    and replayed over new rows, with eager calls between."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(9)
+    kv, q_lens = [2500, 30], [40, 1]
+    table, P = make_table(kv, 64, g)
+    K, V = (torch.randn(1, P, 2, 64, 128, generator=g).to(TYPES[cache]).cuda() for _ in range(2))
+    c, b = paged.kv_cache(K, V), make_batch(q_lens, kv, table)
+    x = torch.randn(41, 12, 128, generator=g).to(TYPES[act]).cuda()
+    q, out = torch.empty_like(x[:, :8]).contiguous(), torch.empty(41, 8, 128, device="cuda", dtype=TYPES[act])
+    rope = paged.rope(128, 1e4)
+
+    def step(o):
+        paged.kv_append(c, 0, b, x[:, :8], x[:, 8:10], x[:, 10:], q, rope=rope)
+        paged.attn_paged(c, 0, b, q, o)
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        step(out)
+    for r in range(3):
+        x.copy_(torch.randn(41, 12, 128, generator=g))
+        gr.replay()
+        want = torch.empty_like(out)
+        step(want)
+        torch.cuda.synchronize()
+        assert torch.equal(out, want)
+
+
 def test_another_stream():
     torch = _torch()
     a, b = _decode_state(3), _decode_state(3)

@@ -1062,9 +1062,7 @@ static hipError_t pg_attn(PgAttn a, float *ws, hipStream_t st) {
                                p.row_splits, ws);
     } else {
         constexpr int lds = std::max(sizeof(PcLds<D>), sizeof(PrLds<D>));
-        static const hipError_t e = hipFuncSetAttribute((const void *)k_pg_attn_chunk<TC, D, HL>,
-                                                        hipFuncAttributeMaxDynamicSharedMemorySize, lds);
-        if (e != hipSuccess) return e;
+        static_assert(lds <= 65536, "what a launch may ask for without an attribute of the kernel");
         const long long wgs = (long long)a.pg.NKV * ((long long)p.nrb * p.row_splits * a.pg.n_seqs +
                                                      (long long)p.blocks * p.chunk_splits);
         if (wgs > PG_WGS) return hipErrorInvalidConfiguration;
