@@ -332,3 +332,58 @@ def test_built_copies_wait_for_lds_reads(tmp_path):
             seen.update(_copies(r.stdout.splitlines()))
     assert any("k_pg_attn_chunk" in k for k in seen)
     assert {k: c for k, c in seen.items() if c[1]} == {}
+
+
+# ---- workspaces made for a call ------------------------------------------------------
+class _Allocations:
+    """torch.empty and torch.cuda.stream on the CPU: the stream that each workspace is made on."""
+
+    def __init__(self, monkeypatch):
+        import torch
+        self.current, self.made = [], []
+        empty = torch.empty
+
+        class on:
+            def __init__(this, stream):
+                this.stream = stream
+
+            def __enter__(this):
+                self.current.append(this.stream)
+
+            def __exit__(this, *e):
+                self.current.pop()
+
+        def make(*a, device=None, **kw):
+            self.made.append(self.current[-1] if self.current else None)
+            return empty(*a, **kw)
+        paged._init_torch()
+        monkeypatch.setattr(torch.cuda, "stream", on)
+        monkeypatch.setattr(torch, "empty", make)
+        monkeypatch.setattr(torch.Tensor, "record_stream", lambda t, s: None)
+        monkeypatch.setattr(paged, "_device", lambda: -1)
+        monkeypatch.setattr(paged, "_raw", lambda dev: 0)
+
+
+class _Stream:
+    device_index, cuda_stream = -1, 7
+
+
+class _Lib:
+    """Every call succeeds; workspace sizes are 1000 bytes."""
+
+    def __getattr__(self, name):
+        return (lambda *a: 1000) if name.endswith("workspace_size") else (lambda *a: 1)
+
+
+@pytest.mark.parametrize("stream", [None, _Stream()])
+def test_attention_makes_its_workspace_on_the_calls_stream(monkeypatch, stream):
+    """The workspace comes from the pool of the stream that the kernels run on: a block of another
+    stream's pool may still be in use there by what was freed before."""
+    import torch
+    q, out = torch.zeros(3, 4, 128).half(), torch.zeros(3, 4, 128).half()
+    c, b = cache(), batch()
+    c._dev = b._dev = -1
+    allocations = _Allocations(monkeypatch)
+    monkeypatch.setattr(paged, "lib", _Lib)
+    paged.attn_paged(c, 0, b, q, out, stream=stream)
+    assert allocations.made == [stream]

@@ -169,6 +169,17 @@ def _stream(stream=None):
     return C.c_void_p(stream.cuda_stream)
 
 
+def _workspace(nbytes: int, stream=None):
+    """Device bytes for kernels on ``stream`` (None: torch's current one), from
+    that stream's own pool: what torch freed in another stream's may still be in
+    use there."""
+    import torch
+    if stream is None:
+        return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+    with torch.cuda.stream(stream):
+        return torch.empty(nbytes, dtype=torch.uint8, device="cuda")
+
+
 def dequant(W, qtype: int, nrows: int, K: int, out, stream=None):
     """out[nrows*K] (fp32 device tensor) = bit-exact dequantised weights."""
     _check(lib().tbq_dequant(_ptr(W), qtype, nrows, K, _ptr(out), _stream(stream)), "tbq_dequant")

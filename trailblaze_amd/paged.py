@@ -12,7 +12,7 @@ from __future__ import annotations
 
 import ctypes as C
 
-from . import TbqError, _check, _ptr, _stream, lib
+from . import TbqError, _check, _ptr, _stream, _workspace, lib
 
 F32, F16, BF16 = 0, 1, 30
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
@@ -201,19 +201,18 @@ def attn_paged(cache: KvCache, layer: int, batch: KvBatch, q, out, window: int =
     nq = q.shape[1]
     qs = _heads("q", q, T, nq, D, dev)
     _flat("out", out, (T, nq, D), q.dtype, dev)
+    to = _to(stream, dev)
     if workspace is None:
         n = attn_workspace_size(cache, batch, nq, q.dtype)
         if n:
-            workspace = _torch.empty(n, dtype=_torch.uint8, device=q.device)
-            if stream is not None:
-                workspace.record_stream(stream)
+            workspace = _workspace(n, stream)
     else:
         _on("workspace", workspace, dev)
         if not workspace.is_contiguous():
             raise ValueError("workspace: contiguous")
     wp, wb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
     _check(lib().tbq_attn_paged(C.byref(cache), layer, C.byref(batch), nq, _type_id(q.dtype), q.data_ptr(), qs,
-                                out.data_ptr(), window, sinks, scale, wp, wb, _to(stream, dev)), "tbq_attn_paged")
+                                out.data_ptr(), window, sinks, scale, wp, wb, to), "tbq_attn_paged")
     return out
 
 
