@@ -387,3 +387,21 @@ def test_attention_makes_its_workspace_on_the_calls_stream(monkeypatch, stream):
     monkeypatch.setattr(paged, "lib", _Lib)
     paged.attn_paged(c, 0, b, q, out, stream=stream)
     assert allocations.made == [stream]
+
+
+@pytest.mark.parametrize("stream", [None, _Stream()])
+def test_step_grows_its_workspace_on_the_calls_stream(monkeypatch, stream):
+    import torch
+    from types import SimpleNamespace
+    from trailblaze_amd import dense
+    m = object.__new__(dense.SyntheticDense)
+    m.cfg, m.model = SimpleNamespace(vocab=1000), _dense()
+    c, logits = cache(), torch.zeros(1, 1000)
+    c._dev = -1
+    allocations = _Allocations(monkeypatch)
+    monkeypatch.setattr(dense, "lib", _Lib)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: None)
+    m.step(c, [1], [1], [[0]], [3], logits, stream=stream)
+    m.step(c, [1], [2], [[0]], [4], logits)   # large enough: kept
+    assert allocations.made == [stream]

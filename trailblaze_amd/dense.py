@@ -12,7 +12,7 @@ from dataclasses import dataclass
 
 import numpy as np
 
-from . import _check, _ptr, _stream, formats as fm, lib, synth
+from . import _check, _ptr, _stream, _workspace, formats as fm, lib, synth
 
 _vp, _i, _f = C.c_void_p, C.c_int, C.c_float
 
@@ -153,20 +153,21 @@ class SyntheticDense:
             raise ValueError("logits: contiguous float32 [sequences][vocab]")
         dev = paged._here(cache)
         paged._on("logits", logits, dev)
+        to = paged._to(stream, dev)
         if torch.cuda.is_current_stream_capturing():
             raise ValueError("step is not for capture: a replay would repeat this call's tokens and lengths")
         need = int(lib().tbq_dense_step_workspace_size(C.byref(self.model), C.byref(cache), n, len(toks),
                                                        page_table.shape[1]))
         ws = getattr(self, "_step_ws", None)
         if need > (0 if ws is None else ws.numel()):
-            ws = self._step_ws = torch.empty(need, dtype=torch.uint8, device="cuda")
+            ws = self._step_ws = _workspace(need, stream)
         if ws is not None:   # used on this stream, whichever it was made on
             ws.record_stream(torch.cuda.current_stream() if stream is None else stream)
         # (need == 0: bad arguments, which the call itself reports)
         _check(lib().tbq_dense_step(C.byref(self.model), C.byref(cache), n, n_new.ctypes.data, kv_len.ctypes.data,
                                     page_table.ctypes.data, page_table.shape[1], toks.ctypes.data,
                                     None if rope is None else C.byref(rope), window, sinks, _ptr(logits), _ptr(ws),
-                                    0 if ws is None else ws.numel(), paged._to(stream, dev)), "tbq_dense_step")
+                                    0 if ws is None else ws.numel(), to), "tbq_dense_step")
         return logits
 
     def matvec_shapes(self):
