@@ -405,3 +405,23 @@ def test_step_grows_its_workspace_on_the_calls_stream(monkeypatch, stream):
     m.step(c, [1], [1], [[0]], [3], logits, stream=stream)
     m.step(c, [1], [2], [[0]], [4], logits)   # large enough: kept
     assert allocations.made == [stream]
+
+
+@pytest.mark.parametrize("stream", [None, _Stream()])
+def test_older_calls_make_their_workspaces_on_their_streams(monkeypatch, stream):
+    """gemm, SyntheticDense.prefill and gguf.dense_prefill, as the paged calls."""
+    import torch
+    from trailblaze_amd import dense, gguf
+    x = torch.zeros(4)
+    allocations = _Allocations(monkeypatch)
+    for mod in (tb, dense, gguf):
+        monkeypatch.setattr(mod, "lib", _Lib)
+        monkeypatch.setattr(mod, "_stream", lambda s=None: None)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: None)
+    monkeypatch.setattr(torch.cuda, "synchronize", lambda: None)
+    tb.gemm(x, 1, x, 2, 4, 256, x, stream=stream)
+    m = object.__new__(dense.SyntheticDense)
+    m.model = _dense()
+    m.prefill([1, 2, 3], 0, x, stream=stream)
+    gguf.dense_prefill(_dense(), [1, 2, 3], 0, x, stream=stream)
+    assert allocations.made == [stream] * 3

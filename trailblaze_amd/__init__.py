@@ -237,10 +237,9 @@ def moe_forward_noalloc(L: MoeLayer, T, xn, resid, out, sel_idx=None, sel_w=None
 def gemm(W, wqt: int, X16, T: int, N: int, K: int, C_out, ldc: int = 0, workspace=None, stream=None):
     """C_out[T][ldc or N] = X16[T][K] . W[N][K]^T with the batched prefill's
     GEMM (W fp16 halves, wqt = 1, or Q4_K rows, wqt = 12)."""
-    import torch
     if workspace is None:
         nb = int(lib().tbq_gemm_workspace_size(T, N, K))
-        workspace = torch.empty(max(nb, 1), dtype=torch.uint8, device="cuda") if nb else None
+        workspace = _workspace(nb, stream) if nb else None
     ws_bytes = 0 if workspace is None else workspace.numel() * workspace.element_size()
     _check(lib().tbq_gemm(wqt, _ptr(W), _ptr(X16), T, N, K, _ptr(C_out), ldc or N, _ptr(workspace), ws_bytes,
                           _stream(stream)), "tbq_gemm")

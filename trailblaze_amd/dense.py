@@ -115,8 +115,10 @@ class SyntheticDense:
         if ws is None or len(toks) > self._pf_len:   # a workspace serves every shorter prompt
             n = int(lib().tbq_dense_prefill_workspace_size(C.byref(self.model), len(toks)))
             if n > 0:
-                ws = self._pf_ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+                ws = self._pf_ws = _workspace(n, stream)
                 self._pf_len = len(toks)
+        if ws is not None:   # used on this stream, whichever it was made on
+            ws.record_stream(torch.cuda.current_stream() if stream is None else stream)
         self._pf_tokens = toks   # read by an asynchronous copy on the stream
         # (n == 0: bad arguments, which the call itself reports)
         _check(lib().tbq_dense_prefill(C.byref(self.model), toks.ctypes.data, len(toks), pos0, _ptr(logits),

@@ -12,7 +12,7 @@ import ctypes as C
 
 import numpy as np
 
-from . import MoeLayer, TbqError, _check, _ptr, _stream, lib
+from . import MoeLayer, TbqError, _check, _ptr, _stream, _workspace, lib
 
 
 class GgufFile:
@@ -126,7 +126,7 @@ def dense_prefill(m, tokens, pos0: int, logits, stream=None):
     toks = np.ascontiguousarray(tokens, dtype=np.int32)
     n = int(lib().tbq_dense_prefill_workspace_size(C.byref(m), len(toks)))
     _check(n > 0, "tbq_dense_prefill_workspace_size")
-    ws = torch.empty(n, dtype=torch.uint8, device="cuda")
+    ws = _workspace(n, stream)
     _check(lib().tbq_dense_prefill(C.byref(m), toks.ctypes.data, len(toks), pos0, _ptr(logits), _ptr(ws), n,
                                    _stream(stream)), "tbq_dense_prefill")
     torch.cuda.synchronize()   # the token copy has run before `toks` goes away
