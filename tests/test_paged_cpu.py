@@ -425,3 +425,21 @@ def test_older_calls_make_their_workspaces_on_their_streams(monkeypatch, stream)
     m.prefill([1, 2, 3], 0, x, stream=stream)
     gguf.dense_prefill(_dense(), [1, 2, 3], 0, x, stream=stream)
     assert allocations.made == [stream] * 3
+
+
+def test_step_refuses_capture_on_a_named_stream(monkeypatch):
+    """The stream that the step runs on is asked, not the current one."""
+    import torch
+    from types import SimpleNamespace
+    from trailblaze_amd import dense
+    m = object.__new__(dense.SyntheticDense)
+    m.cfg, m.model = SimpleNamespace(vocab=1000), _dense()
+    c, logits, stream = cache(), torch.zeros(1, 1000), _Stream()
+    c._dev = -1
+    allocations = _Allocations(monkeypatch)
+    monkeypatch.setattr(dense, "lib", _Lib)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: allocations.current[-1:] == [stream])
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: None)
+    with pytest.raises(ValueError, match="capture"):
+        m.step(c, [1], [1], [[0]], [3], logits, stream=stream)
+    m.step(c, [1], [1], [[0]], [3], logits)

@@ -156,7 +156,9 @@ class SyntheticDense:
         dev = paged._here(cache)
         paged._on("logits", logits, dev)
         to = paged._to(stream, dev)
-        if torch.cuda.is_current_stream_capturing():
+        with torch.cuda.stream(stream):   # (None: the current one)
+            capturing = torch.cuda.is_current_stream_capturing()
+        if capturing:
             raise ValueError("step is not for capture: a replay would repeat this call's tokens and lengths")
         need = int(lib().tbq_dense_step_workspace_size(C.byref(self.model), C.byref(cache), n, len(toks),
                                                        page_table.shape[1]))
