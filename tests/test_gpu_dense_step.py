@@ -315,3 +315,22 @@ def test_step_refusals(oracle):
                 m.step(*a, logits)
         finally:
             g.capture_end()
+
+
+def test_a_larger_workspace_changes_nothing():
+    """The logits' product of eight and more sequences splits its sums by the call's shape alone: with the
+    workspace that a call asks for and with one left from a longer prompt, the same bits.  Rows of 2048, 2048
+    of them at a time, in 8 slices, where the layers' products take 4 or fewer rows."""
+    import ctypes as C
+    import torch
+    from trailblaze_amd.dense import DenseConfig, SyntheticDense
+    m = SyntheticDense(DenseConfig(n_layers=1, hidden=2048, n_heads=4, n_kv_heads=2, head_dim=64, ffn=1024, vocab=4128,
+                                   max_ctx=16), 11)
+    for n in (8, 16):
+        cache = m.paged_cache(n, 16)
+        logits = [torch.empty(n, m.cfg.vocab, device="cuda") for _ in range(2)]
+        size = int(tb.lib().tbq_dense_step_workspace_size(C.byref(m.model), C.byref(cache), n, n, 1))
+        for spare, o in zip((0, 64 << 20), logits):
+            m._step_ws = torch.empty(size + spare, dtype=torch.uint8, device="cuda")
+            m.step(cache, [1] * n, [1] * n, [[i] for i in range(n)], list(range(3, 3 + n)), o)
+        assert torch.equal(*logits), n

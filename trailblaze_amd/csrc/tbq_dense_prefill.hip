@@ -961,13 +961,28 @@ struct StepWs {
 // Sequences from which the logits are one fp16 product with the lm_head, dequantised
 // as many rows at a time as the weights' buffer holds, instead of a matvec each.
 constexpr int STEP_LM_GEMM = 8;
+static int step_lm_rows(const tbq_dense_model *m, size_t wh_halves) {
+    return (int)std::min<size_t>(wh_halves / m->hidden, 1u << 20) / 16 * 16;
+}
+
+// Room for that product's partial sums: as much as its slices take by its shape
+// alone, so that they (and the logits' bits) do not depend on what is left of
+// the workspace.
+static size_t step_lm_partials(const tbq_dense_model *m, int n_seqs, size_t wh_halves) {
+    if (n_seqs < STEP_LM_GEMM || !wh_halves) return 0;
+    const int most = step_lm_rows(m, wh_halves), V = m->vocab, cu = hgemm_cus();
+    size_t gp = hgemm_partial_upto(n_seqs, std::min(most, V), m->hidden, cu);
+    if (V > most && V % most) gp = std::max(gp, hgemm_partial_upto(n_seqs, V % most, m->hidden, cu));
+    return gp;
+}
+
 static hipError_t step_logits(const tbq_dense_model *m, const StepWs &w, int n_seqs, int T, const int *q_start,
                               const float *ysrc, int yns, float *logits, hipStream_t st) {
     const int H = m->hidden, V = m->vocab, qt = canon_qt(m->qtype_embd), cu = hgemm_cus();
     hipLaunchKernelGGL(k_pf_last_rows, dim3((H + 255) / 256, n_seqs), dim3(256), 0, st, w.pf.x, ysrc, yns, (long long)T * H,
                        w.pf.sb, q_start, H, w.xg, w.yg);
     hipError_t err = launch_pf_norm(n_seqs, w.xg, w.yg, 1, 0, nullptr, m->output_norm, H, m->norm_eps, w.pf.h16, w.pf.sa, st);
-    const int most = (int)std::min<size_t>(w.pf.wh_halves / H, 1u << 20) / 16 * 16;
+    const int most = step_lm_rows(m, w.pf.wh_halves);
     const size_t rb = tbq_row_bytes(qt, H);
     for (int r = 0; r < V && err == hipSuccess; r += most) {
         const int n = std::min(most, V - r);
@@ -988,7 +1003,7 @@ static StepWs step_ws(const tbq_dense_model *m, int n_seqs, int T, int max_pages
     StepWs w{};
     size_t off = 0;
     // (the prefill's first, without their split-K partials, which are what is left at the end)
-    pf_ws(m, T, ws, 0, &off, true);
+    w.pf = pf_ws(m, T, ws, 0, &off, true);
     auto take = [&](size_t bytes) {
         void *r = (char *)ws + off;
         off += pf_up(bytes);
@@ -1009,8 +1024,9 @@ static size_t step_attn_bytes(const tbq_dense_model *m, int n_seqs, int T, long 
 
 size_t dense_step_workspace_bytes(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int T, int max_pages) {
     size_t t = 0;
-    step_ws(m, n_seqs, T, max_pages, nullptr, 0, &t);
-    return t + pf_up(step_attn_bytes(m, n_seqs, T, (long long)max_pages * c->page_size)) + pf_partials(m, T);
+    const StepWs w = step_ws(m, n_seqs, T, max_pages, nullptr, 0, &t);
+    return t + pf_up(step_attn_bytes(m, n_seqs, T, (long long)max_pages * c->page_size)) +
+           std::max(pf_partials(m, T), step_lm_partials(m, n_seqs, w.pf.wh_halves));
 }
 
 hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new,
