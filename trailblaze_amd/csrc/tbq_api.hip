@@ -544,6 +544,8 @@ int tbq_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, 
         rope = &own;
     }
     const tbq_dense_model p = uncached(m);
+    if (!dense_step_attn_fits(&p, c, n_seqs, n_new, kv_len, max_pages))
+        return fail("%s: the attention's records do not fit their part of the workspace", who);
     const size_t need = dense_step_workspace_bytes(&p, c, n_seqs, (int)T, max_pages);
     if (ws_bytes < need) return fail("%s: workspace %zu < %zu bytes", who, ws_bytes, need);
     if (!ensure_init()) return 0;

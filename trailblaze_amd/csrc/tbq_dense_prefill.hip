@@ -1029,6 +1029,29 @@ size_t dense_step_workspace_bytes(const tbq_dense_model *m, const tbq_kv_cache *
            std::max(pf_partials(m, T), step_lm_partials(m, n_seqs, w.pf.wh_halves));
 }
 
+// Whether the attention of every launch of this step has the room that the
+// workspace sets aside for it.
+bool dense_step_attn_fits(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new, const int *kv_len,
+                          int max_pages) {
+    PgArgs a = pg_layer(c, 0);
+    a.max_pages = max_pages;
+    for (int s = 0; s < n_seqs; s++) {
+        a.n_tokens += n_new[s];
+        a.max_q = std::max(a.max_q, n_new[s]);
+        a.max_kv = std::max(a.max_kv, kv_len[s]);
+    }
+    const size_t room = step_attn_bytes(m, n_seqs, a.n_tokens, (long long)max_pages * c->page_size);
+    if (dense_prefill_batched(m) && a.n_tokens >= 2) {
+        a.n_seqs = n_seqs;
+        return pg_attn_workspace_bytes(a, m->head_dim, m->n_heads, false) <= room;
+    }
+    a.n_seqs = a.n_tokens = a.max_q = 1;
+    for (int s = 0; s < n_seqs; s++)
+        for (a.max_kv = kv_len[s] - n_new[s] + 1; a.max_kv <= kv_len[s]; a.max_kv++)
+            if (pg_attn_workspace_bytes(a, m->head_dim, m->n_heads, true) > room) return false;
+    return true;
+}
+
 hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new,
                              const int *kv_len, const int *page_table, int max_pages, const int *tokens,
                              const tbq_rope &rope, int window, int sinks, float *logits, void *ws, size_t ws_bytes,

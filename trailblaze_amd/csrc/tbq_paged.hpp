@@ -148,6 +148,8 @@ hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const 
                                      const PgRope &rope, int window, int sinks, float *logits, void *ws, void *attn_ws,
                                      hipStream_t st);
 size_t dense_step_workspace_bytes(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int T, int max_pages);
+bool dense_step_attn_fits(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new, const int *kv_len,
+                          int max_pages);
 hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, const int *n_new,
                              const int *kv_len, const int *page_table, int max_pages, const int *tokens,
                              const tbq_rope &rope, int window, int sinks, float *logits, void *ws, size_t ws_bytes,
