@@ -334,3 +334,28 @@ def test_a_larger_workspace_changes_nothing():
             m._step_ws = torch.empty(size + spare, dtype=torch.uint8, device="cuda")
             m.step(cache, [1] * n, [1] * n, [[i] for i in range(n)], list(range(3, 3 + n)), o)
         assert torch.equal(*logits), n
+
+
+def test_small_values_over_many_positions(oracle):
+    """Values near the end of fp16: the attention's rows, averages of 500 of them, are an order of magnitude
+    smaller and reach the o product scaled, as the contiguous prefill's do.  attn_norm of 2^-21 leaves values
+    of 16 * 2^-21 = 7.6e-6 (rows of 256, weights N(0, 1); q and k are normalised), which the cache rounds to
+    steps of 2^-24: off by 2.2e-3 (rms), and so are their averages.  Averages in steps of 2^-24 would be off
+    by 3e-2 of themselves.  wo and the embedding are scaled so that the logits are what the attention adds."""
+    import torch
+    m, model = _model(oracle, seed=12, n_layers=1, qtype_layers=fm.F32, qtype_embd=fm.F32, norm_eps=1e-14, max_ctx=16)
+    L, dev = model.ref.layers[0], m._keep[0]
+    for name, f in (("attn_norm", 2.0 ** -21), ("wo", 2.0 ** 10), ("wdown", 2.0 ** -30)):
+        L[name] = L[name] * f
+        dev[name].view(torch.float32).mul_(f)
+    model.ref.lm = model.ref.lm * 2.0 ** -20
+    m.lm_head.view(torch.float32).mul_(2.0 ** -20)
+    rng = np.random.default_rng(12)
+    toks = _tokens(rng, 500)
+    cache, logits, ref = m.paged_cache(8), torch.empty(1, 512, device="cuda"), model.empty()
+    m.step(cache, [500], [500], [list(range(8))], toks, logits)
+    for t in toks:
+        want = model.decode(ref, t)
+    err = rel_l2(host(logits)[0], want)
+    print("error", err, flush=True)
+    assert err <= BATCH_TOL

@@ -738,8 +738,8 @@ static PfWs pf_ws(const tbq_dense_model *m, int T, void *ws, size_t ws_bytes, si
             w.cp = (m->max_ctx + PC_KC - 1) / PC_KC * PC_KC;
             w.k16 = (_Float16 *)take((size_t)m->n_kv_heads * w.cp * m->head_dim * 2);
             w.vt = (_Float16 *)take((size_t)m->n_kv_heads * w.cp * m->head_dim * 2);
-            w.att = (float *)take((size_t)T * QD * 4);
         }
+        w.att = (float *)take((size_t)T * QD * 4);
         w.gu = (float *)take((size_t)T * 2 * F * 4);
         w.h16 = (_Float16 *)take((size_t)T * wide * 2);
         w.sa = (float *)take((size_t)T * 4);
@@ -793,8 +793,8 @@ size_t dense_prefill_workspace_bytes(const tbq_dense_model *m, int T) {
 // The layers over T >= 2 tokens (w.tok: T device ints, in range).  attn(l, L, qsrc,
 // qns) takes layer l's q | k | v rows (qns split-K slices T * QKVR apart, scaled by
 // 1 / w.sa), appends to the cache and writes the o GEMM's operand to w.h16, with
-// the inverse row scales at the pointer it sets.  *last, *lns: the last layer's
-// output (slices T * H apart, scaled by 1 / w.sb), not yet added to w.x.
+// the inverse row scales to w.sb.  *last, *lns: the last layer's output (slices
+// T * H apart, scaled by 1 / w.sb), not yet added to w.x.
 template <typename Attn>
 static hipError_t pf_layers(const tbq_dense_model *m, const PfWs &w, int T, Attn attn, const float **last, int *lns,
                             hipStream_t st) {
@@ -829,11 +829,10 @@ static hipError_t pf_layers(const tbq_dense_model *m, const PfWs &w, int T, Attn
             if (err == hipSuccess) err = gemm(qt_of(L.qt_v), L.wv, KD, H, w.qkv + QD + KD, QKVR);
         }
         if (err != hipSuccess) break;
-        const float *osc = w.sb;   // inverse scales of the attention's rows
-        if ((err = attn(l, L, qns > 1 ? w.gpart : w.qkv, qns, &osc)) != hipSuccess) break;
+        if ((err = attn(l, L, qns > 1 ? w.gpart : w.qkv, qns)) != hipSuccess) break;
         if ((err = gemm(qt_of(L.qt_o), L.wo, H, QD, w.y, H, &yns)) != hipSuccess) break;
         ysrc = yns > 1 ? w.gpart : w.y;
-        if ((err = launch_pf_norm(T, w.x, ysrc, yns, (long long)T * H, osc, L.ffn_norm, H, m->norm_eps, w.h16,
+        if ((err = launch_pf_norm(T, w.x, ysrc, yns, (long long)T * H, w.sb, L.ffn_norm, H, m->norm_eps, w.h16,
                                   w.sa, st)) != hipSuccess)
             break;
         // a fused gate|up matrix: SwiGLU in the GEMM's epilogue, then the
@@ -882,8 +881,7 @@ static hipError_t pf_batched(const tbq_dense_model *m, const PfWs &w, int T, int
     hipLaunchKernelGGL(k_pf_rope, dim3(T), dim3(64), 0, st, pos0, m->rope_theta, D, w.rope);
     const float *ysrc = nullptr;
     int yns = 1;
-    const hipError_t err = pf_layers(m, w, T, [&](int l, const tbq_dense_layer &L, const float *qsrc, int qns,
-                                                  const float **) {
+    const hipError_t err = pf_layers(m, w, T, [&](int l, const tbq_dense_layer &L, const float *qsrc, int qns) {
         const size_t kvoff = (size_t)l * NKV * m->max_ctx * D;
         float *kc = m->k_cache + kvoff, *vc = m->v_cache + kvoff;
         if (D == 128) {
@@ -922,11 +920,6 @@ hipError_t launch_dense_prefill(const tbq_dense_model *m, const int *tokens_host
 // ---------------------------------------------------------------------------
 // The forward over a paged cache (tbq_dense_step).
 // ---------------------------------------------------------------------------
-__global__ __launch_bounds__(256) void k_pf_ones(float *__restrict__ p, int n) {
-    const int i = blockIdx.x * 256 + threadIdx.x;
-    if (i < n) p[i] = 1.f;
-}
-
 // Row s of xg and yg: the residual and the last layer's output (its ny slices added
 // in slice order, scaled) of sequence s's last token.  grid = (ceil(H / 256), n_seqs).
 __global__ __launch_bounds__(256) void k_pf_last_rows(const float *__restrict__ x, const float *__restrict__ y, int ny,
@@ -949,12 +942,12 @@ __global__ __launch_bounds__(256) void k_pf_scale_rows(float *__restrict__ p, in
     for (int j = blockIdx.x * 1024 + threadIdx.x; j < min(n, (int)(blockIdx.x + 1) * 1024); j += 256) row[j] *= f;
 }
 
-// Behind the prefill's regions: the batch's ints, ones for the attention's row
-// scales, the last tokens' rows, and the attention's workspace.
+// Behind the prefill's regions: the batch's ints, the last tokens' rows, and the
+// attention's workspace.
 struct StepWs {
     PfWs pf;
     int *ints;
-    float *ones, *xg, *yg;
+    float *xg, *yg;
     void *attn;
 };
 
@@ -1010,7 +1003,6 @@ static StepWs step_ws(const tbq_dense_model *m, int n_seqs, int T, int max_pages
         return r;
     };
     w.ints = (int *)take(((size_t)n_seqs * (max_pages + 2) + 1) * 4);
-    w.ones = (float *)take((size_t)T * 4);
     w.xg = (float *)take((size_t)n_seqs * m->hidden * 4);
     w.yg = (float *)take((size_t)n_seqs * m->hidden * 4);
     *total = off;
@@ -1115,7 +1107,6 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
         }
     }
     if ((err = launch_put_ints(len, kv_len, n_seqs, st)) != hipSuccess) return err;
-    hipLaunchKernelGGL(k_pf_ones, dim3((T + 255) / 256), dim3(256), 0, st, w.ones, T);
     const int D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads, QKVR = (NQ + 2 * NKV) * D;
     PgAppend ap{};
     ap.pg = pg;
@@ -1126,18 +1117,21 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
     ap.rs = w.pf.sa;
     ap.slstride = (long long)T * QKVR;
     ap.rope = rp;
-    // the attention's fp16 rows are averages of fp16 values: the o GEMM takes them as they are
+    // Averages of many values can be far smaller than the values, below fp16's normal numbers: the
+    // attention's rows are fp32 and go to the o GEMM scaled, as the contiguous prefill's do (500 values of
+    // 8e-6: logits off by 2.2e-3, 2.3e-2 with fp16 rows as they are; 0.1 ms of a step of 36 layers).
     PgAttn at{};
     at.q = w.pf.qb;
     at.qs = NQ * D;
-    at.out = w.pf.h16;
+    at.out = w.pf.att;
+    at.f32_out = 1;
     at.NQ = NQ;
     at.window = window;
     at.sinks = sinks;
     at.scale = pg_scale(0.f, D);
     const float *ysrc = nullptr;
     int yns = 1;
-    err = pf_layers(m, w.pf, T, [&](int l, const tbq_dense_layer &L, const float *qsrc, int qns, const float **osc) {
+    err = pf_layers(m, w.pf, T, [&](int l, const tbq_dense_layer &L, const float *qsrc, int qns) {
         ap.pg.k = (char *)pg.k + l * layer_bytes;
         ap.pg.v = (char *)pg.v + l * layer_bytes;
         ap.q = qsrc;
@@ -1147,9 +1141,9 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
         ap.qn = L.q_norm;
         ap.kn = L.k_norm;
         at.pg = ap.pg;
-        *osc = w.ones;
-        const hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F16, TBQ_KV_F16, st);
-        return e != hipSuccess ? e : launch_pg_attn(at, D, TBQ_KV_F16, TBQ_KV_F16, w.attn, st);
+        hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F16, TBQ_KV_F16, st);
+        if (e == hipSuccess) e = launch_pg_attn(at, D, TBQ_KV_F16, TBQ_KV_F16, w.attn, st);
+        return e != hipSuccess ? e : launch_rows_f16(w.pf.att, T, NQ * D, w.pf.h16, w.pf.sb, st);
     }, &ysrc, &yns, st);
     if (err != hipSuccess) return err;
     if (n_seqs >= STEP_LM_GEMM && m->vocab % 4 == 0 && ((uintptr_t)logits & 15) == 0)

@@ -52,8 +52,8 @@ struct PgAttn {
     PgArgs pg;
     const void *q;         // heads of row t side by side at base + t * stride
     long long qs;
-    void *out;             // [n_tokens][NQ][D]
-    int NQ, window, sinks;
+    void *out;             // [n_tokens][NQ][D], of q's type or (f32_out) fp32
+    int NQ, window, sinks, f32_out;
     int few;               // rows up to which a sequence is one of few rows (launch_pg_attn sets it)
     float scale;           // of q . k, times log2(e): the softmax is in powers of two
 };

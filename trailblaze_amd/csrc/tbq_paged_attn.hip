@@ -422,7 +422,7 @@ __device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int n
             const float inv = den == 0.f ? 0.f : 1.0f / den;   // a row that sees nothing is 0
             const long long at = ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D + d;
             sum = make_float4(sum.x * inv, sum.y * inv, sum.z * inv, sum.w * inv);
-            if constexpr (HL) pg_st4((float *)a.out + at, sum);
+            if (HL || a.f32_out) pg_st4((float *)a.out + at, sum);
             else pg_st4((TC *)a.out + at, sum);
         } else {
             float *rec = part + ((((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit + z) * pg_rec(D);
@@ -819,8 +819,10 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
         float *rec = part + (to * nsplit + z) * pg_rec(D);
 #pragma unroll
         for (int i = 0; i < D / 64; i++) {
-            if (nz <= 1) ((TA *)a.out)[to * D + lane + 64 * i] = (TA)(sl == 0.f ? 0.f : so[i] / sl);
-            else rec[lane + 64 * i] = so[i];
+            const float x = nz > 1 ? so[i] : sl == 0.f ? 0.f : so[i] / sl;
+            if (nz > 1) rec[lane + 64 * i] = x;
+            else if (HL || a.f32_out) ((float *)a.out)[to * D + lane + 64 * i] = x;
+            else ((TC *)a.out)[to * D + lane + 64 * i] = (TC)x;
         }
         if (nz > 1 && lane == 0) {
             rec[D] = sm;
@@ -838,7 +840,7 @@ __device__ __forceinline__ void pg_chunk(const PgAttn &a, int nsplit, float *__r
             for (int r = 0; r < 4; r++) {
                 const float4 x = make_float4(o[j][4 * r] * inv, o[j][4 * r + 1] * inv, o[j][4 * r + 2] * inv, o[j][4 * r + 3] * inv);
                 const long long d = at * D + 32 * j + 8 * r + 4 * h;
-                if constexpr (HL) pg_st4((float *)a.out + d, x);
+                if (HL || a.f32_out) pg_st4((float *)a.out + d, x);
                 else pg_st4((TC *)a.out + d, x);
             }
         return;
@@ -1073,10 +1075,12 @@ static hipError_t pg_attn(PgAttn a, float *ws, hipStream_t st) {
     const long long wgs = row_wgs + (p.chunk_splits > PC_FEW ? (long long)a.pg.n_tokens * a.NQ
                                      : p.chunk_splits > 1   ? (long long)a.pg.n_tokens * ((a.NQ + pj_heads(D) - 1) / pj_heads(D))
                                                             : 0);
-    typedef typename std::conditional<HL, float, TC>::type TO;
     if (wgs > PG_WGS) return hipErrorInvalidConfiguration;
-    if (wgs > 0)
-        hipLaunchKernelGGL((k_pg_join<TO, D, HL>), dim3((unsigned)wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps,
+    if (wgs > 0 && (HL || a.f32_out))
+        hipLaunchKernelGGL((k_pg_join<float, D, HL>), dim3((unsigned)wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps,
+                           p.row_splits, ws, (int)row_wgs, p.most, p.chunk_splits, part);
+    else if (wgs > 0)
+        hipLaunchKernelGGL((k_pg_join<TC, D, HL>), dim3((unsigned)wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps,
                            p.row_splits, ws, (int)row_wgs, p.most, p.chunk_splits, part);
     return hipGetLastError();
 }
