@@ -359,3 +359,38 @@ def test_small_values_over_many_positions(oracle):
     err = rel_l2(host(logits)[0], want)
     print("error", err, flush=True)
     assert err <= BATCH_TOL
+
+
+@pytest.mark.parametrize("qt", [fm.Q6_K, fm.Q4_K, fm.GGML | fm.Q4_K, fm.Q8_0, fm.F32])
+@pytest.mark.parametrize("n,hidden", [(33, 256), (64, 2048)])
+def test_logits_of_many_sequences_are_as_exact_as_of_few(n, hidden, qt):
+    """The product that forms the logits of many sequences, against the matvecs on the same rows (what a
+    vocabulary that is no multiple of 4 takes): each within the matvecs' 1e-5 of the formula."""
+    import dataclasses
+    import torch
+    from trailblaze_amd.dense import DenseConfig, SyntheticDense
+    m = SyntheticDense(DenseConfig(n_layers=1, hidden=hidden, n_heads=4, n_kv_heads=2, head_dim=64, ffn=512, vocab=2068,
+                                   max_ctx=16, qtype_embd=qt), 13)
+    cache, got = m.paged_cache(n, 16), []
+    for vocab in (2068, 2066):
+        m.model.vocab, m.cfg = vocab, dataclasses.replace(m.cfg, vocab=vocab)
+        logits = torch.full((n, vocab), float("nan"), device="cuda")
+        m.step(cache, [1] * n, [1] * n, [[i] for i in range(n)], list(range(5, 5 + n)), logits)
+        got.append(host(logits))
+    for i in range(n):
+        assert rel_l2(got[0][i, :2066], got[1][i]) <= 2e-5, i
+
+
+def test_logits_do_not_depend_on_their_address():
+    """logits 4 bytes into an allocation: the same product, the same bits."""
+    import torch
+    from trailblaze_amd.dense import DenseConfig, SyntheticDense
+    m = SyntheticDense(DenseConfig(n_layers=1, hidden=256, n_heads=4, n_kv_heads=2, head_dim=64, ffn=512, vocab=512,
+                                   max_ctx=16), 14)
+    cache, buf = m.paged_cache(40, 16), torch.empty(40 * 512 + 1, device="cuda")
+    got = []
+    for off in (0, 1):
+        logits = buf[off:off + 40 * 512].view(40, 512)
+        m.step(cache, [1] * 40, [1] * 40, [[i] for i in range(40)], list(range(40)), logits)
+        got.append(host(logits))
+    assert np.array_equal(*got)

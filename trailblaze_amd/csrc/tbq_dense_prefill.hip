@@ -920,77 +920,152 @@ hipError_t launch_dense_prefill(const tbq_dense_model *m, const int *tokens_host
 // ---------------------------------------------------------------------------
 // The forward over a paged cache (tbq_dense_step).
 // ---------------------------------------------------------------------------
-// Row s of xg and yg: the residual and the last layer's output (its ny slices added
-// in slice order, scaled) of sequence s's last token.  grid = (ceil(H / 256), n_seqs).
-__global__ __launch_bounds__(256) void k_pf_last_rows(const float *__restrict__ x, const float *__restrict__ y, int ny,
-                                                      long long ystride, const float *__restrict__ ys,
-                                                      const int *__restrict__ q_start, int H, float *__restrict__ xg,
-                                                      float *__restrict__ yg) {
-    const int j = blockIdx.x * 256 + threadIdx.x, s = blockIdx.y, t = q_start[s + 1] - 1;
-    if (j >= H) return;
-    const long long at = (long long)t * H + j;
-    float a = y[at];
-    for (int z = 1; z < ny; z++) a = a + y[at + z * ystride];
-    xg[(long long)s * H + j] = x[at];
-    yg[(long long)s * H + j] = a * ys[t];
+// Sequence s's last token: h = rmsnorm(x + y) * w (y: its ny slices added in slice
+// order, scaled by ys), times the power of two 2^e that puts max |h| in [2^14, 2^15)
+// and inv[s] = 2^-e, as pairs of halves h = hi + lo against the weights' pairs of
+// k_dequant_f16_pair: row s of X is hi, then hi 2^-11 (the weights' lo halves are
+// times 2^11), row n + s is lo, then 0.  grid = n.
+__global__ __launch_bounds__(PN_THREADS) void k_pf_last_rows(const float *__restrict__ x, const float *__restrict__ y, int ny,
+                                                             long long ystride, const float *__restrict__ ys,
+                                                             const int *__restrict__ q_start, const float *__restrict__ w,
+                                                             int H, float eps, int n, _Float16 *__restrict__ X,
+                                                             float *__restrict__ inv) {
+    typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+    __shared__ float red[PN_THREADS / 64];
+    const int s = blockIdx.x, t = q_start[s + 1] - 1, tid = threadIdx.x, n4 = H / 4;
+    const float4 *xr = reinterpret_cast<const float4 *>(x + (long long)t * H);
+    const float4 *yr = reinterpret_cast<const float4 *>(y + (long long)t * H);
+    const float f = ys[t];
+    float4 v[PN_V];
+    float ss = 0.f;
+#pragma unroll
+    for (int i = 0; i < PN_V; i++) {
+        const int j = tid + PN_THREADS * i;
+        if (j >= n4) continue;
+        float4 a = yr[j];
+        for (int z = 1; z < ny; z++) {
+            const float4 b = yr[j + z * (ystride / 4)];
+            a = make_float4(a.x + b.x, a.y + b.y, a.z + b.z, a.w + b.w);
+        }
+        const float4 r = xr[j];
+        v[i] = make_float4(r.x + a.x * f, r.y + a.y * f, r.z + a.z * f, r.w + a.w * f);
+        ss += v[i].x * v[i].x + v[i].y * v[i].y + v[i].z * v[i].z + v[i].w * v[i].w;
+    }
+    const float r = 1.0f / sqrtf(pf_block_sum(ss, red) / (float)H + eps);
+    float mx = 0.f;
+#pragma unroll
+    for (int i = 0; i < PN_V; i++) {
+        const int j = tid + PN_THREADS * i;
+        if (j >= n4) continue;
+        const float4 g = reinterpret_cast<const float4 *>(w)[j];
+        v[i] = make_float4(v[i].x * r * g.x, v[i].y * r * g.y, v[i].z * r * g.z, v[i].w * r * g.w);
+        mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v[i].x), fabsf(v[i].y)), fmaxf(fabsf(v[i].z), fabsf(v[i].w))));
+    }
+    mx = pf_block_max(mx, red);
+    int e = 0;
+    frexpf(mx, &e);
+    const int sh = min(max(mx > 0.f ? 15 - e : 0, -126), 126);
+    const float sc = ldexpf(1.f, sh);
+    h4 *hr = reinterpret_cast<h4 *>(X + (long long)s * 2 * H), *lr = reinterpret_cast<h4 *>(X + (long long)(n + s) * 2 * H);
+#pragma unroll
+    for (int i = 0; i < PN_V; i++) {
+        const int j = tid + PN_THREADS * i;
+        if (j >= n4) continue;
+        const float a[4] = {v[i].x * sc, v[i].y * sc, v[i].z * sc, v[i].w * sc};
+        h4 hi, lo, hs;
+#pragma unroll
+        for (int k = 0; k < 4; k++) {
+            hi[k] = (_Float16)a[k];
+            lo[k] = (_Float16)(a[k] - (float)hi[k]);
+            hs[k] = (_Float16)((float)hi[k] * (1.f / 2048.f));
+        }
+        hr[j] = hi;
+        hr[n4 + j] = hs;
+        lr[j] = lo;
+        lr[n4 + j] = h4{};
+    }
+    if (tid == 0) inv[s] = ldexpf(1.f, -sh);
 }
 
-// Row s of n floats times sc[s].  grid = (ceil(n / 1024), rows).
-__global__ __launch_bounds__(256) void k_pf_scale_rows(float *__restrict__ p, int n, const float *__restrict__ sc) {
-    const float f = sc[blockIdx.y];
-    float *row = p + (long long)blockIdx.y * n;
-    for (int j = blockIdx.x * 1024 + threadIdx.x; j < min(n, (int)(blockIdx.x + 1) * 1024); j += 256) row[j] *= f;
+// out[s][r] = inv[s] (row s + row n + s of P), each the sum of its ns slices in slice
+// order; P [ns][2 n][N], rows of out are ldo apart.  grid = (ceil(N / 256), n).
+__global__ __launch_bounds__(256) void k_pf_lm_join(const float *__restrict__ P, int ns, int n, int N,
+                                                    const float *__restrict__ inv, float *__restrict__ out, long long ldo) {
+    const int j = blockIdx.x * 256 + threadIdx.x, s = blockIdx.y;
+    if (j >= N) return;
+    const float *hi = P + (long long)s * N + j, *lo = hi + (long long)n * N;
+    const long long slice = 2ll * n * N;
+    float a = hi[0], b = lo[0];
+    for (int z = 1; z < ns; z++) {
+        a += hi[z * slice];
+        b += lo[z * slice];
+    }
+    out[s * ldo + j] = (a + b) * inv[s];
 }
 
-// Behind the prefill's regions: the batch's ints, the last tokens' rows, and the
-// attention's workspace.
+// Behind the prefill's regions: the batch's ints, the last tokens' rows (k_pf_last_rows),
+// and the attention's workspace.
 struct StepWs {
     PfWs pf;
     int *ints;
-    float *xg, *yg;
+    _Float16 *rows;
     void *attn;
 };
 
-// Sequences from which the logits are one fp16 product with the lm_head, dequantised
-// as many rows at a time as the weights' buffer holds, instead of a matvec each.
-constexpr int STEP_LM_GEMM = 8;
+// The logits of many sequences as one product with the lm_head instead of a matvec
+// each.  Rows and weights are pairs of halves (~22 bits), which make the product as
+// exact as the matvecs (logits of single halves are off by 3e-4): K is [hi | lo] of
+// the weights, and a sequence has a row of its hi halves and one of its lo.  The
+// weights' buffer holds part of the lm_head at a time.
 static int step_lm_rows(const tbq_dense_model *m, size_t wh_halves) {
-    return (int)std::min<size_t>(wh_halves / m->hidden, 1u << 20) / 16 * 16;
+    return (int)std::min<size_t>(wh_halves / (2 * m->hidden), 1u << 20) / 16 * 16;
 }
 
-// Room for that product's partial sums: as much as its slices take by its shape
-// alone, so that they (and the logits' bits) do not depend on what is left of
-// the workspace.
+// From as many sequences as there are parts, and 8: a part (three launches) takes
+// about as long as a matvec.  A step of one layer, matvecs / product: 151936 rows of
+// 2560 in 16 parts, 12 sequences 0.99 / 1.01 ms, 16 1.28 / 1.02, 64 4.85 / 1.13;
+// 32000 rows in 4 parts, 8 0.24 / 0.26, 10 0.28 / 0.26, 64 1.29 / 0.30; 151936 rows
+// of 1024 in 54 parts, 32 0.91 / 1.32, 64 1.75 / 1.37.
+static bool step_lm_product(const tbq_dense_model *m, int n_seqs, size_t wh_halves) {
+    if (!wh_halves || m->vocab % 4) return false;   // (rows that the product takes)
+    const int most = step_lm_rows(m, wh_halves);
+    return n_seqs >= std::max(8, (m->vocab + most - 1) / most);
+}
+
+// Room for that product's sums: as much as its slices take by its shape alone, so
+// that they (and the logits' bits) do not depend on what is left of the workspace.
 static size_t step_lm_partials(const tbq_dense_model *m, int n_seqs, size_t wh_halves) {
-    if (n_seqs < STEP_LM_GEMM || !wh_halves) return 0;
+    if (!step_lm_product(m, n_seqs, wh_halves)) return 0;
     const int most = step_lm_rows(m, wh_halves), V = m->vocab, cu = hgemm_cus();
-    size_t gp = hgemm_partial_upto(n_seqs, std::min(most, V), m->hidden, cu);
-    if (V > most && V % most) gp = std::max(gp, hgemm_partial_upto(n_seqs, V % most, m->hidden, cu));
-    return gp;
+    auto room = [&](int n) {
+        return std::max(hgemm_partial_upto(2 * n_seqs, n, 2 * m->hidden, cu), (size_t)2 * n_seqs * n * 4);
+    };
+    return V > most && V % most ? std::max(room(most), room(V % most)) : room(std::min(most, V));
 }
 
 static hipError_t step_logits(const tbq_dense_model *m, const StepWs &w, int n_seqs, int T, const int *q_start,
                               const float *ysrc, int yns, float *logits, hipStream_t st) {
     const int H = m->hidden, V = m->vocab, qt = canon_qt(m->qtype_embd), cu = hgemm_cus();
-    hipLaunchKernelGGL(k_pf_last_rows, dim3((H + 255) / 256, n_seqs), dim3(256), 0, st, w.pf.x, ysrc, yns, (long long)T * H,
-                       w.pf.sb, q_start, H, w.xg, w.yg);
-    hipError_t err = launch_pf_norm(n_seqs, w.xg, w.yg, 1, 0, nullptr, m->output_norm, H, m->norm_eps, w.pf.h16, w.pf.sa, st);
+    hipLaunchKernelGGL(k_pf_last_rows, dim3(n_seqs), dim3(PN_THREADS), 0, st, w.pf.x, ysrc, yns, (long long)T * H, w.pf.sb,
+                       q_start, m->output_norm, H, m->norm_eps, n_seqs, w.rows, w.pf.sa);
+    hipError_t err = hipGetLastError();
     const int most = step_lm_rows(m, w.pf.wh_halves);
     const size_t rb = tbq_row_bytes(qt, H);
     for (int r = 0; r < V && err == hipSuccess; r += most) {
         const int n = std::min(most, V - r);
-        const void *W = (const uint8_t *)m->lm_head + r * rb;
-        if (qt != QT_Q4_K) {
-            if ((err = launch_dequant_f16(qt, W, (long long)n * H, w.pf.wh, st)) != hipSuccess) break;
-            W = w.pf.wh;
-        }
-        err = launch_hgemm(qt == QT_Q4_K ? QT_Q4_K : QT_F16, W, w.pf.h16, n_seqs, n, H, logits + r, V, w.pf.gpart,
-                           w.pf.gpart_bytes, cu, st);
+        int ns = 1;
+        err = launch_dequant_f16_pair(qt, (const uint8_t *)m->lm_head + r * rb, n, H, w.pf.wh, st);
+        if (err == hipSuccess)
+            err = launch_hgemm(QT_F16, w.pf.wh, w.rows, 2 * n_seqs, n, 2 * H, w.pf.gpart, n, w.pf.gpart, w.pf.gpart_bytes,
+                               cu, st, &ns);
+        if (err != hipSuccess) break;
+        hipLaunchKernelGGL(k_pf_lm_join, dim3((n + 255) / 256, n_seqs), dim3(256), 0, st, w.pf.gpart, ns, n_seqs, n, w.pf.sa,
+                           logits + r, V);
+        err = hipGetLastError();
     }
-    if (err != hipSuccess) return err;
-    hipLaunchKernelGGL(k_pf_scale_rows, dim3((V + 1023) / 1024, n_seqs), dim3(256), 0, st, logits, V, w.pf.sa);
-    return hipGetLastError();
+    return err;
 }
+
 static StepWs step_ws(const tbq_dense_model *m, int n_seqs, int T, int max_pages, void *ws, size_t ws_bytes,
                       size_t *total) {
     StepWs w{};
@@ -1003,8 +1078,7 @@ static StepWs step_ws(const tbq_dense_model *m, int n_seqs, int T, int max_pages
         return r;
     };
     w.ints = (int *)take(((size_t)n_seqs * (max_pages + 2) + 1) * 4);
-    w.xg = (float *)take((size_t)n_seqs * m->hidden * 4);
-    w.yg = (float *)take((size_t)n_seqs * m->hidden * 4);
+    w.rows = (_Float16 *)take((size_t)n_seqs * m->hidden * 8);
     *total = off;
     return w;
 }
@@ -1146,7 +1220,7 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
         return e != hipSuccess ? e : launch_rows_f16(w.pf.att, T, NQ * D, w.pf.h16, w.pf.sb, st);
     }, &ysrc, &yns, st);
     if (err != hipSuccess) return err;
-    if (n_seqs >= STEP_LM_GEMM && m->vocab % 4 == 0 && ((uintptr_t)logits & 15) == 0)
+    if (step_lm_product(m, n_seqs, w.pf.wh_halves))
         return step_logits(m, w, n_seqs, T, q_start, ysrc, yns, logits, st);
     for (int s = 0, t = -1; s < n_seqs && err == hipSuccess; s++) {
         t += n_new[s];

@@ -60,6 +60,7 @@ struct MoeArgs {
 hipError_t launch_dequant(int qt, const void *W, long long nweights, float *out, hipStream_t s);
 hipError_t launch_dequant_rows(int qt, const void *W, const int *idx, int nrows, int K, float *out, hipStream_t s);
 hipError_t launch_dequant_f16(int qt, const void *W, long long nweights, _Float16 *out, hipStream_t s);
+hipError_t launch_dequant_f16_pair(int qt, const void *W, int nrows, int K, _Float16 *out, hipStream_t s);
 hipError_t launch_matvec_generic(int qt, const void *W, int M, int K, const float *x, float *y,
                                  hipStream_t s, int n_cu);
 // The Q4_K kernels read the reference's layout, or ggml's (QT_GQ4_K) when ggml.
