@@ -636,3 +636,13 @@ def test_python_refusals():
     if paged.attn_workspace_size(c, b, 4, torch.float32) > 16:
         with pytest.raises(tb.TbqError, match="workspace"):
             paged.attn_paged(c, 0, b, s["q"], s["out"], workspace=s["ws"][:16])
+
+
+@pytest.mark.parametrize("act,cache,size", [("bf16", "bf16", 3e38), ("f16", "f16", 65504.0), ("f32", "f16", 65504.0)])
+@pytest.mark.parametrize("past", [60, 2500])
+def test_attention_values_at_the_end_of_their_type(act, cache, size, past):
+    """Averages of values whose sum fp32 does not hold: few rows and many, split or not."""
+    def big(K, V, table, kv):
+        V.copy_(_torch().where(_torch().isnan(V), V, V.sign() * size))
+        V[:, :, :, :, :8] = V[:, :, :, :, :8].abs()   # dims where they are all alike
+    run_attention(act, cache, 64, 4, 1, 64, [1, 40], [past, past], spoil_pool=big)

@@ -15,7 +15,8 @@
 // [2^13, 2^14), and the probabilities are each taken as two halves, x = hi + lo,
 // which keeps ~22 bits; the keys and values are halves already.  16-bit rows
 // round the probabilities to the cache's type.  Half probabilities are scaled by
-// 2^14, so those that a half cannot hold are below 2^-38 of the largest.
+// 2^14, so those that a half cannot hold are below 2^-38 of the largest; bf16's by
+// 2^-32, so that sums of values near their type's end stay within fp32.
 //
 // What a row does not see must not reach it, NaN and infinities included.
 // Scores are replaced before the maximum.  In the product with V an unseen
@@ -45,7 +46,7 @@ struct PgVec<pg_f16> {
 template <>
 struct PgVec<pg_bf16> {
     typedef pg_bf16 h8 __attribute__((ext_vector_type(8)));
-    static constexpr float SHIFT = 0.f;
+    static constexpr float SHIFT = -32.f;
 };
 typedef float pg_f4 __attribute__((ext_vector_type(4)));
 typedef float pg_f16x __attribute__((ext_vector_type(16)));
