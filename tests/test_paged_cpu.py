@@ -476,3 +476,62 @@ def test_steps_attention_has_its_room():
         ok = tb.lib().tbq_dense_step(C.byref(mod), C.byref(c), n, ptr(n_new), ptr(kv_len), ptr(table), most, ptr(tokens),
                                      None, rng.choice([0, 100]), 0, FAKE, FAKE, 100, None)
         refused(ok, "workspace 100 <")
+
+
+# ---- numbers that a C int does not hold --------------------------------------------------
+@pytest.mark.parametrize("bad", [2 ** 32, 2 ** 31, -2 ** 32, 1.0])
+def test_numbers_beyond_an_int_are_refused(monkeypatch, bad):
+    """None of them is taken as the number that its low 32 bits are."""
+    import torch
+    allocations = _Allocations(monkeypatch)
+    monkeypatch.setattr(paged, "_device", lambda: -1)
+    c, b = cache(), batch()
+    c._dev = b._dev = -1
+    pool = paged.PagePool(4)
+    pool.alloc(2)
+    monkeypatch.setattr(paged, "lib", _Lib)
+    q, out = torch.zeros(3, 4, 128).half(), torch.zeros(3, 4, 128).half()
+    kv = torch.zeros(3, 2, 128).half()
+    i32 = lambda *v: torch.tensor(v, dtype=torch.int32)   # noqa: E731
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: 0)
+    for call in (lambda: paged.kv_copy_pages(c, [bad], [1]), lambda: paged.kv_copy_pages(c, [0, 1], [2, bad]),
+                 lambda: paged.kv_batch(i32(0, 1), i32(1), i32(0)[None], bad),
+                 lambda: paged.kv_batch(i32(0, 1), i32(1), i32(0)[None], 1, max_q=bad),
+                 lambda: paged.kv_batch(i32(0, 1), i32(1), i32(0)[None], 1, max_kv=bad)):
+        with pytest.raises((ValueError, TypeError)):
+            call()
+    monkeypatch.setattr(torch.Tensor, "get_device", lambda t: -1)
+    if bad != 1.0:   # (an argument of a call: ctypes refuses a float itself)
+        for call in (lambda: paged.attn_paged(c, bad, b, q, out), lambda: paged.attn_paged(c, 0, b, q, out, window=bad),
+                     lambda: paged.attn_paged(c, 0, b, q, out, window=4, sinks=bad),
+                     lambda: paged.kv_append(c, bad, b, q, kv, kv, out)):
+            with pytest.raises(ValueError):
+                call()
+    monkeypatch.undo()
+    for call in (lambda: pool.share([0, bad]), lambda: pool.release([bad]), lambda: pool.fork(16, 16, [bad]),
+                 lambda: pool.alloc(bad), lambda: pool.defrag(bad), lambda: pool.holders(bad)):
+        with pytest.raises((ValueError, TypeError)):
+            call()
+    assert [pool.holders(p) for p in range(4)] == [1, 1, 0, 0]
+
+
+@pytest.mark.parametrize("kw", [dict(n_new=[2 ** 32 + 1]), dict(kv_len=[2 ** 32 + 1]), dict(page_table=[[2 ** 32]]),
+                                dict(tokens=[2 ** 32 + 3]), dict(tokens=[3.5])])
+def test_step_refuses_numbers_beyond_an_int(monkeypatch, kw):
+    import numpy as np
+    import torch
+    from types import SimpleNamespace
+    from trailblaze_amd import dense
+    m = object.__new__(dense.SyntheticDense)
+    m.cfg, m.model = SimpleNamespace(vocab=1000), _dense()
+    c, logits = cache(), torch.zeros(1, 1000)
+    c._dev = -1
+    _Allocations(monkeypatch)
+    monkeypatch.setattr(dense, "lib", _Lib)
+    monkeypatch.setattr(torch.cuda, "is_current_stream_capturing", lambda: False)
+    monkeypatch.setattr(torch.cuda, "current_stream", lambda: None)
+    a = dict(n_new=[1], kv_len=[1], page_table=[[0]], tokens=[3])
+    m.step(c, *a.values(), logits)
+    for form in (lambda v: v, np.array):
+        with pytest.raises(ValueError):
+            m.step(c, *{**a, **{k: form(v) for k, v in kw.items()}}.values(), logits)

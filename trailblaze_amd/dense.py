@@ -146,8 +146,14 @@ class SyntheticDense:
         several streams must wait for each other."""
         import torch
         from . import paged
-        ints = lambda v: np.ascontiguousarray(v, dtype=np.int32)   # noqa: E731
-        n_new, kv_len, page_table, toks = ints(n_new), ints(kv_len), ints(page_table), ints(tokens)
+
+        def ints(name, v):
+            v = np.asarray(v)
+            if v.size and (v.dtype.kind not in "iu" or v.min() < -0x80000000 or v.max() > 0x7FFFFFFF):
+                raise ValueError(f"{name}: 32-bit ints")
+            return np.ascontiguousarray(v, dtype=np.int32)
+        n_new, kv_len, page_table = ints("n_new", n_new), ints("kv_len", kv_len), ints("page_table", page_table)
+        toks = ints("tokens", tokens)
         n = len(n_new)
         if page_table.ndim != 2 or kv_len.shape != (n,) or len(page_table) != n or len(toks) != n_new.sum():
             raise ValueError("n_new, kv_len and page_table: one row a sequence; tokens: the sum of n_new")
@@ -155,7 +161,7 @@ class SyntheticDense:
             raise ValueError("logits: contiguous float32 [sequences][vocab]")
         dev = paged._here(cache)
         paged._on("logits", logits, dev)
-        to = paged._to(stream, dev)
+        to, window, sinks = paged._to(stream, dev), paged._int("window", window), paged._int("sinks", sinks)
         with torch.cuda.stream(stream):   # (None: the current one)
             capturing = torch.cuda.is_current_stream_capturing()
         if capturing:

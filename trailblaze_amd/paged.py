@@ -11,6 +11,8 @@ unless ``stream`` names one.
 from __future__ import annotations
 
 import ctypes as C
+from array import array
+from operator import index
 
 from . import TbqError, _check, _ptr, _stream, _workspace, lib
 
@@ -38,6 +40,7 @@ class Rope(C.Structure):
 
 
 _torch, _raw, _device, _ids = None, None, None, {}
+_INT = 1 << 31
 
 
 def _init_torch():
@@ -58,6 +61,23 @@ def _type_id(dtype):
     if dtype not in _ids:
         raise ValueError(f"{dtype}: float32, float16 or bfloat16")
     return _ids[dtype]
+
+
+def _int(name, v):
+    """v, where a C int holds it (ctypes would pass on its low 32 bits)."""
+    v = index(v)
+    if not -_INT <= v < _INT:
+        raise ValueError(f"{name}: {v} is no 32-bit int")
+    return v
+
+
+def _c_ints(name, values):
+    """A C array of a list of ints."""
+    try:
+        a = array("i", values)
+    except OverflowError:
+        raise ValueError(f"{name}: a number that is no 32-bit int") from None
+    return (C.c_int * len(a)).from_buffer(a) if a else (C.c_int * 0)()
 
 
 def _here(*owners):
@@ -132,6 +152,8 @@ def kv_batch(q_start, kv_len, page_table, n_tokens: int, max_q: int = 0, max_kv:
     dev = kv_len.get_device()
     if dev < 0 or q_start.get_device() != dev or page_table.get_device() != dev:
         raise ValueError("q_start, kv_len and page_table: on one device")
+    for name, v in (("n_tokens", n_tokens), ("max_q", max_q), ("max_kv", max_kv)):
+        _int(name, v)
     b = KvBatch(n, n_tokens, page_table.shape[1], max_q, max_kv, q_start.data_ptr(), kv_len.data_ptr(),
                 page_table.data_ptr())
     b._keep, b._dev = (q_start, kv_len, page_table), dev
@@ -160,6 +182,8 @@ def kv_append(cache: KvCache, layer: int, batch: KvBatch, q, k, v, q_out, rope: 
     """Rotate and append the batch's new rows: q [tokens][heads][D] to q_out
     (both may be None), k and v [tokens][kv heads][D] to their pages."""
     dev = _here(cache, batch)
+    if not -_INT <= layer < _INT:
+        _int("layer", layer)
     T, D, nkv = batch.n_tokens, cache.head_dim, cache.n_kv_heads
     in_type = _type_id(k.dtype)
     if v.dtype != k.dtype or (q is not None and q.dtype != k.dtype):
@@ -195,6 +219,9 @@ def attn_paged(cache: KvCache, layer: int, batch: KvBatch, q, out, window: int =
                scale: float = 0.0, workspace=None, stream=None):
     """out[token][head] = attention of q over the pages the token sees."""
     dev = _here(cache, batch)
+    if not (-_INT <= layer < _INT and -_INT <= window < _INT and -_INT <= sinks < _INT):
+        for name, v in (("layer", layer), ("window", window), ("sinks", sinks)):
+            _int(name, v)
     T, D = batch.n_tokens, cache.head_dim
     if q.dim() != 3:
         raise ValueError("q: [tokens][heads][head dim]")
@@ -222,8 +249,8 @@ def kv_copy_pages(cache: KvCache, src, dst, stream=None):
     if len(dst) != n:
         raise ValueError(f"{n} sources, {len(dst)} destinations")
     dev = _here(cache)
-    arr = C.c_int * n
-    _check(lib().tbq_kv_copy_pages(C.byref(cache), arr(*src), arr(*dst), n, _to(stream, dev)), "tbq_kv_copy_pages")
+    _check(lib().tbq_kv_copy_pages(C.byref(cache), _c_ints("src", src), _c_ints("dst", dst), n, _to(stream, dev)),
+           "tbq_kv_copy_pages")
 
 
 def kv_compact(cache: KvCache, page_table, keep_start, keep, stream=None):
@@ -248,7 +275,7 @@ class PagePool:
     """Which pages of a cache are held, and how often (tbq_kv_pool_*)."""
 
     def __init__(self, n_pages: int):
-        self._p = lib().tbq_kv_pool_create(n_pages)
+        self._p = lib().tbq_kv_pool_create(_int("n_pages", n_pages))
         _check(self._p, "tbq_kv_pool_create")
 
     def close(self):
@@ -262,36 +289,36 @@ class PagePool:
         return lib().tbq_kv_pool_free_pages(self._p)
 
     def holders(self, page: int) -> int:
-        return lib().tbq_kv_pool_holders(self._p, page)
+        return lib().tbq_kv_pool_holders(self._p, _int("page", page))
 
     def alloc(self, n: int) -> list:
-        a = (C.c_int * max(n, 1))()
+        a = (C.c_int * max(_int("n", n), 1))()
         _check(lib().tbq_kv_pool_alloc(self._p, n, a), "tbq_kv_pool_alloc")
         return list(a[:n])
 
     def share(self, pages):
-        _check(lib().tbq_kv_pool_share(self._p, len(pages), (C.c_int * len(pages))(*pages)), "tbq_kv_pool_share")
+        _check(lib().tbq_kv_pool_share(self._p, len(pages), _c_ints("pages", pages)), "tbq_kv_pool_share")
 
     def release(self, pages):
-        _check(lib().tbq_kv_pool_release(self._p, len(pages), (C.c_int * len(pages))(*pages)), "tbq_kv_pool_release")
+        _check(lib().tbq_kv_pool_release(self._p, len(pages), _c_ints("pages", pages)), "tbq_kv_pool_release")
 
     def fork(self, positions: int, page_size: int, pages):
         """The child's pages, and (source, destination) of the page that is to
         be copied, or None."""
-        if positions < 0 or page_size < 1:
+        if _int("positions", positions) < 0 or _int("page_size", page_size) < 1:
             raise ValueError(f"{positions} positions in pages of {page_size}")
         n = -(-positions // page_size)
         if len(pages) < n:
             raise ValueError(f"{positions} positions need {n} pages, got {len(pages)}")
         child, copy = (C.c_int * max(n, 1))(), (C.c_int * 2)()
-        _check(lib().tbq_kv_pool_fork(self._p, positions, page_size, (C.c_int * len(pages))(*pages), child, copy),
+        _check(lib().tbq_kv_pool_fork(self._p, positions, page_size, _c_ints("pages", pages), child, copy),
                "tbq_kv_pool_fork")
         return list(child[:n]), (copy[0], copy[1]) if copy[0] >= 0 else None
 
     def defrag(self, most: int):
         """[(source, destination)] of the moves that bring the held pages to
         the lowest numbers, at most `most`."""
-        src, dst = (C.c_int * max(most, 1))(), (C.c_int * max(most, 1))()
+        src, dst = ((C.c_int * max(_int("most", most), 1))() for _ in range(2))
         n = lib().tbq_kv_pool_defrag(self._p, most, src, dst)
         if n < 0:
             raise TbqError(f"tbq_kv_pool_defrag failed: {lib().tbq_last_error().decode()}")
