@@ -394,3 +394,25 @@ def test_logits_do_not_depend_on_their_address():
         m.step(cache, [1] * 40, [1] * 40, [[i] for i in range(40)], list(range(40)), logits)
         got.append(host(logits))
     assert np.array_equal(*got)
+
+
+@pytest.mark.parametrize("n,vocab,qt", [(300, 2068, fm.Q8_0), (40, 2068, fm.Q6_K), (9, 2068, fm.Q8_0), (9, 514, fm.Q6_K)])
+def test_many_sequences_within_the_stated_bound(oracle, n, vocab, qt):
+    """Weights without a mean (Q8_0 and Q6_K quants are symmetric), whose sums do not cancel against each
+    other: the stated 1e-2 without exception; an lm_head in five parts of 512 rows, the last of 20."""
+    import torch
+    m, model = _model(oracle, seed=15, n_layers=1, vocab=vocab, qtype_layers=qt)
+    cache, rng = m.paged_cache(n), np.random.default_rng(15)
+    n_new = [1 + i % 3 for i in range(n)]
+    toks = _tokens(rng, sum(n_new))
+    logits = torch.empty(n, vocab, device="cuda")
+    m.step(cache, n_new, n_new, [[i] for i in range(n)], toks, logits)
+    got, at, errs = host(logits), 0, []
+    for i in range(n):
+        ref = model.empty()
+        for t in toks[at:at + n_new[i]]:
+            want = model.decode(ref, t)
+        at += n_new[i]
+        errs.append(rel_l2(got[i], want))
+    print("errors", n, vocab, max(errs), float(np.mean(errs)), flush=True)
+    assert max(errs) <= BATCH_TOL

@@ -646,3 +646,86 @@ def test_attention_values_at_the_end_of_their_type(act, cache, size, past):
         V.copy_(_torch().where(_torch().isnan(V), V, V.sign() * size))
         V[:, :, :, :, :8] = V[:, :, :, :, :8].abs()   # dims where they are all alike
     run_attention(act, cache, 64, 4, 1, 64, [1, 40], [past, past], spoil_pool=big)
+
+
+# ---- long loops: lists, lookups and splits that follow the first ------------------------------
+def check_sampled(got, K, V, layer, st, kv, table, Q, rows, window, sinks, ta, tc):
+    """The sampled token rows against the 64-bit form, each as a batch of its own."""
+    for t, s, pos in tokens(st, kv):
+        if t in rows:
+            o, spread, size = attention(K, V, layer, [0, 1], [pos + 1], [table[s]], Q[t:t + 1], window, sinks)[0]
+            tol = attention_tolerance(o, spread, size, ta, tc)
+            assert bool(((got[t].double() - o).abs() <= tol).all()), (t, s, pos)
+
+
+@pytest.mark.parametrize("act,cache", ATTN_TYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (3001, 150)])
+def test_attention_chunk_of_many_tiles(act, cache, window, sinks):
+    """A prompt's chunk of enough blocks that none is split (100 of 8 kv heads): up to 91 tiles one after
+    the other on shuffled pages, looked up 16 at a time, the sinks' in front of a window's."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(31)
+    T, past, page, NQ, NKV, D = 3200, 2600, 64, 32, 8, 64
+    ta, tc = TYPES[act], TYPES[cache]
+    table, P = make_table([T + past], page, g, spare=3)
+    K, V = (torch.full((1, P, NKV, page, D), float("nan"), dtype=tc) for _ in range(2))
+    for t in (K, V):
+        t[:, table[0]] = torch.randn(1, len(table[0]), NKV, page, D, generator=g).to(tc)
+        t[:, table[0][-1], :, (T + past - 1) % page + 1:] = float("nan")
+    Q = torch.randn(T, NQ, D, generator=g).to(ta)
+    out = torch.empty(T, NQ, D, dtype=ta, device="cuda")
+    b = make_batch([T], [T + past], table)
+    paged.attn_paged(paged.kv_cache(K.cuda(), V.cuda()), 0, b, Q.cuda(), out, window=window, sinks=sinks)
+    rows = {0, 1, 31, 32, 700, 1023, 1555, 2048, 3000, 3198, 3199}
+    assert bool(torch.isfinite(out).all())
+    check_sampled(out.cpu(), K, V, 0, [0, T], [T + past], table, Q, rows, window, sinks, ta, tc)
+
+
+@pytest.mark.parametrize("act,cache", ATTN_TYPES)
+@pytest.mark.parametrize("window,sinks", [(0, 0), (6000, 70)])
+def test_attention_single_tokens_of_many_tiles(act, cache, window, sinks):
+    """Enough workgroups (400 sequences of 8 kv heads) that a split has 192 tiles, 48 a wave, whose pages
+    are looked up 32 tiles at a time; the sequences share a few pages in orders of their own."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(32)
+    S, page, P, NQ, NKV, D, most = 400, 256, 40, 16, 8, 64, 30
+    ta, tc = TYPES[act], TYPES[cache]
+    K, V = (torch.randn(1, P, NKV, page, D, generator=g).to(tc) for _ in range(2))
+    kv = torch.randint(1, most * page + 1, (S,), generator=g).tolist()
+    kv[:6] = [most * page, 4096, 4097, 4128, 6144, 6145]
+    table = [torch.randint(0, P, (most,), generator=g).tolist() for _ in range(S)]
+    Q = torch.randn(S, NQ, D, generator=g).to(ta)
+    out = torch.empty(S, NQ, D, dtype=ta, device="cuda")
+    b = make_batch([1] * S, kv, table)
+    paged.attn_paged(paged.kv_cache(K.cuda(), V.cuda()), 0, b, Q.cuda(), out, window=window, sinks=sinks)
+    rows = set(range(6)) | set(range(50, S, 60))
+    check_sampled(out.cpu(), K, V, 0, list(range(S + 1)), kv, table, Q, rows, window, sinks, ta, tc)
+
+
+# layers and sequences that give a workgroup 1, 2, 3, 5, 16, 33 and 64 columns; rows beyond one and two lists
+@pytest.mark.parametrize("D,NKV,layers,lens,kept", [
+    (64, 1, 1, [4000], [2500]), (128, 1, 512, [1500], [1100]), (64, 3, 512, [1300], [1030]), (64, 5, 512, [1200], [1001]),
+    (128, 8, 512, [1200], [1030]), (64, 33, 32, [90, 40, 70, 7] * 4, [50, 1, 70, 0] * 4),
+    (128, 32, 32, [90, 40, 70, 7] * 4, [50, 1, 69, 3] * 4)])
+def test_compact_many_rows_and_columns(D, NKV, layers, lens, kept):
+    torch = _torch()
+    g = torch.Generator().manual_seed(sum(lens) + NKV)
+    page = 16
+    table, P = make_table(lens, page, g, spare=1)
+    gg = torch.Generator(device="cuda").manual_seed(5)
+    k, v = (torch.randint(-2 ** 15, 2 ** 15, (layers, P, NKV, page, D), generator=gg, device="cuda", dtype=torch.int16)
+            for _ in range(2))
+    keep = [sorted(torch.randperm(n, generator=g)[:m].tolist()) for n, m in zip(lens, kept)]
+    want = []
+    for t in (k, v):
+        w = t.clone()
+        for s, r in enumerate(keep):
+            at = lambda ps: (torch.tensor([table[s][p // page] for p in ps], dtype=torch.int64).cuda(),   # noqa: E731
+                             torch.tensor([p % page for p in ps], dtype=torch.int64).cuda())
+            if r:
+                (ps, rs), (pd, rd) = at(r), at(range(len(r)))
+                w.transpose(2, 3)[:, pd, rd] = t.transpose(2, 3)[:, ps, rs]
+        want.append(w)
+    c = paged.kv_cache(k.view(torch.float16), v.view(torch.float16))
+    paged.kv_compact(c, ints(table), ints(starts(kept)), ints([x for r in keep for x in r]))
+    assert torch.equal(k, want[0]) and torch.equal(v, want[1])
