@@ -119,8 +119,11 @@ int tbq_kv_append(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n
  * q [n_tokens][n_heads][head_dim] with q_stride elements between tokens (a
  * multiple of 8), out contiguous, not overlapping q, both of type q_type: the
  * cache's type, or F32 with an F16 cache.  Scores, softmax and sums are fp32.
- * 16-bit products round the probabilities to the cache's type; F32 takes q and
- * the probabilities as pairs of halves (~22 bits, relative to a row's largest
+ * 16-bit rows of a sequence with up to 32 of them a kv head (new tokens times
+ * n_heads / n_kv_heads; 16 where the batch may hold more than 256 MiB of keys
+ * and values) are rounded once, at the output; with more rows the
+ * probabilities are rounded to the cache's type too.  F32 takes q and the
+ * probabilities as pairs of halves (~22 bits, relative to a row's largest
  * element), so its rows are exact to about 1e-6.
  * workspace: tbq_attn_paged_workspace_size() bytes, 16-byte aligned, no
  * zero-fill needed; calls that share one must not overlap. */

@@ -729,3 +729,29 @@ def test_compact_many_rows_and_columns(D, NKV, layers, lens, kept):
     c = paged.kv_cache(k.view(torch.float16), v.view(torch.float16))
     paged.kv_compact(c, ints(table), ints(starts(kept)), ints([x for r in keep for x in r]))
     assert torch.equal(k, want[0]) and torch.equal(v, want[1])
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("D,heads,kv,q_lens,past", [(128, 32, 8, [1, 1, 1], [299, 4999, 8]), (64, 8, 1, [1], [20000]),
+                                                    (64, 4, 1, [8, 3, 1], [700, 40, 5000]), (128, 17, 1, [1], [3000])])
+@pytest.mark.parametrize("window", [0, 256])
+def test_attention_of_few_rows_rounds_only_its_output(act, D, heads, kv, q_lens, past, window):
+    """Single tokens and drafts (up to 32 rows a kv head) of 16-bit rows: the probabilities are pairs (each
+    half off by half a step of what it rounds), so what is left is fp32's (attention_tolerance's first terms)
+    and the one rounding of the output."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(D + heads)
+    t, page, kvl = TYPES[act], 64, [n + p for n, p in zip(q_lens, past)]
+    table, P = make_table(kvl, page, g)
+    K, V = (torch.randn(1, P, kv, page, D, generator=g).to(t) for _ in range(2))
+    T = sum(q_lens)
+    Q = torch.randn(T, heads, D, generator=g).to(t)
+    out = torch.empty(T, heads, D, dtype=t, device="cuda")
+    paged.attn_paged(paged.kv_cache(K.cuda(), V.cuda()), 0, make_batch(q_lens, kvl, table), Q.cuda(), out, window=window)
+    ref = attention(K, V, 0, starts(q_lens), kvl, table, Q, window)
+    for r in ref:
+        o, spread, size = ref[r]
+        tol = attention_tolerance(o, spread, size, torch.float32, t)
+        tol = tol + half_step(t) ** 2 * spread
+        tol = tol + half_step(t) * (o.abs() + tol) + least(t)
+        assert bool(((out[r].cpu().double() - o).abs() <= tol).all()), r

@@ -13,10 +13,15 @@
 //
 // F32 rows (HL): q, scaled by the power of two that puts its largest element in
 // [2^13, 2^14), and the probabilities are each taken as two halves, x = hi + lo,
-// which keeps ~22 bits; the keys and values are halves already.  16-bit rows
-// round the probabilities to the cache's type.  Half probabilities are scaled by
-// 2^14, so those that a half cannot hold are below 2^-38 of the largest; bf16's by
-// 2^-32, so that sums of values near their type's end stay within fp32.
+// which keeps ~22 bits; the keys and values are halves already.  16-bit rows: few
+// take the probabilities as two of the cache's type as well, in a second product
+// (0 to 3% of the time, bound by the bytes: 64 sequences of up to 8192 213.4 -> 214.1
+// us); many round them once, which adds a third to the output's own rounding (errors
+// against 64 bits 2.7e-4 with fp16, 2.1e-4 without): two would take 462 us instead of
+// 344 for 2048 tokens after 8192, 44 instead of 35 for 9 mixed sequences.  Half
+// probabilities are scaled by 2^14, so those that a half cannot hold are below 2^-38
+// of the largest; bf16's by 2^-32, so that sums of values near their type's end stay
+// within fp32.
 //
 // What a row does not see must not reach it, NaN and infinities included.
 // Scores are replaced before the maximum.  In the product with V an unseen
@@ -328,15 +333,19 @@ __device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int n
 #pragma unroll
             for (int j = 0; j < ND; j++) o[j] *= corr;
         }
-        h8 pf;
+        h8 pf, pl;   // (F32 rows' lo halves are columns of their own)
         const float mb = SH - m;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][e % 4], cs, mb));
             l += p;
             const TC hi = (TC)p;
-            if constexpr (HL) pf[e] = li < 8 ? hi : (TC)(p - (float)hi);
-            else pf[e] = hi;
+            const TC lo = (TC)(p - (float)hi);
+            if constexpr (HL) pf[e] = li < 8 ? hi : lo;
+            else {
+                pf[e] = hi;
+                pl[e] = lo;
+            }
         }
         if (!whole) {   // values that no row of the block sees
             const uint32_t any = seen(plo, phi);
@@ -350,6 +359,7 @@ __device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int n
 #pragma unroll
                 for (int e = 0; e < 8; e++) v[e] = vf[buf][e][j];
                 o[j] = pg_mfma16(v, pf, o[j]);
+                if constexpr (!HL) o[j] = pg_mfma16(v, pl, o[j]);
             }
         } else {
             for (int t = t0; t <= t1; t++) {
@@ -362,7 +372,8 @@ __device__ __forceinline__ void pg_rows(const PgAttn &a, int nrb, int tps, int n
                     h8 v;
 #pragma unroll
                     for (int e = 0; e < 8; e++) v[e] = w[e][j];
-                    const pg_f4 u = pg_mfma16(v, pf, o[j]);
+                    pg_f4 u = pg_mfma16(v, pf, o[j]);
+                    if constexpr (!HL) u = pg_mfma16(v, pl, u);
                     if (tok == t) o[j] = u;
                 }
             }
