@@ -107,7 +107,9 @@ int tbq_rope_init(tbq_rope *r, int rot_dim, int layout, double theta, int scalin
     r->rot_dim = rot_dim;
     r->layout = layout;
     r->mscale = scaling == TBQ_ROPE_YARN ? 0.1 * log(factor) + 1 : 1;
-    // the pair that turns beta times in orig_ctx positions
+    // The pair that turns beta times in orig_ctx positions.  (The whole pairs that bound the ramp, their
+    // limits 0 and rot_dim - 1 and the 0.001 between equal ones are not the paper's: models are trained
+    // with them.)
     auto pair = [&](double beta) { return rot_dim * log(orig_ctx / (beta * 2 * M_PI)) / (2 * log(theta)); };
     double lo = 0, hi = 0;
     if (scaling == TBQ_ROPE_YARN) {

@@ -188,7 +188,10 @@ constexpr int PR_WAVES = 4, PR_TS = 32;
 // positions 13.7 / 19.4 us, 32 after 1000 34.4 / 43.4, 32 after 4096 155 / 119, 64
 // after 4096 294 / 212; 16 tokens of 8 sequences after 2000 40.0 as four, 33.4 as
 // many.  fp32 as four blocks / as many: 24 after 1000 41.8 / 50.2, 64 after 4096
-// 417 / 284; 4 tokens as two / as many: 64 after 4096 267 / 275.
+// 417 / 284; 4 tokens as two / as many: 64 after 4096 267 / 275.  One token of 17 to 32
+// heads a kv head, fp16, as two / as many: 32 heads of 64 sequences over 4096 260 / 211, of
+// 5 over 65536 202 / 172, of 9 over 16384 142 / 156; 17 heads of 64 over 2000 114 / 120;
+// fp32 (four blocks) 32 heads of 64 over 4096 362 / 280, of 9 over 16384 207 / 182.
 constexpr int PR_MAX = 32;
 constexpr int PR_MIN = 4, PR_LONG = 64;   // tiles of a split: one a wave at least, 2048 positions at most
 constexpr int PR_MANY = 1024;              // (in batches of up to twice so many workgroups)
