@@ -197,9 +197,9 @@ int tbq_kv_pool_defrag(tbq_kv_pool *p, int max, int *src, int *dst);
  * each included.  Those products leave the logits within 1e-2 relative L2 (1.5e-3
  * at most in 300 prompts of one to three tokens) unless the weights' sums nearly
  * cancel: weights whose rows have a mean took 1 prompt in 100 to 1e-2 .. 8e-2.
- * The lm_head is as exact as the decode step's for any number of sequences.  Two
- * single tokens take longer in one step than in two (Qwen3-4B's shape at 4096: 3.9
- * ms and 1.65 each), three less.
+ * The lm_head (weights within fp16's 65504) is as exact as the decode step's for
+ * any number of sequences.  Two single tokens take longer in one step than in two
+ * (Qwen3-4B's shape at 4096: 3.9 ms and 1.65 each), three less.
  * A captured call repeats its tokens, lengths and pages at every replay, so a
  * step is not for capture.
  * The workspace size covers every call with at most that many sequences, tokens

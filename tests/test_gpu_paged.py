@@ -755,3 +755,27 @@ def test_attention_of_few_rows_rounds_only_its_output(act, D, heads, kv, q_lens,
         tol = tol + half_step(t) ** 2 * spread
         tol = tol + half_step(t) * (o.abs() + tol) + least(t)
         assert bool(((out[r].cpu().double() - o).abs() <= tol).all()), r
+
+
+def test_named_stream_without_a_workspace():
+    """Calls on a stream that is not the current one, workspaces their own, while the current one's
+    memory comes and goes."""
+    torch = _torch()
+    a, b = _decode_state(3), _decode_state(3)
+    want, st = _step(a).clone(), torch.cuda.Stream()
+    for _ in range(3):
+        st.wait_stream(torch.cuda.current_stream())
+        paged.kv_append(b["c"], 0, b["b"], b["x"][:, :4], b["x"][:, 4:6], b["x"][:, 6:], b["q"], rope=b["rope"], stream=st)
+        paged.attn_paged(b["c"], 0, b["b"], b["q"], b["out"], stream=st)
+        for _ in range(4):
+            torch.full((1 << 16,), float("nan"), device="cuda")
+        st.synchronize()
+        assert torch.equal(b["out"], want)
+    X, W = torch.randn(40, 2048, device="cuda").half(), torch.randn(64, 2048, device="cuda").half()
+    got = [torch.empty(40, 64, device="cuda") for _ in range(2)]
+    st.wait_stream(torch.cuda.current_stream())
+    tb.gemm(W, 1, X, 40, 64, 2048, got[0], stream=st)
+    tb.gemm(W, 1, X, 40, 64, 2048, got[1])
+    st.synchronize()
+    torch.cuda.synchronize()
+    assert torch.equal(*got)
