@@ -23,19 +23,37 @@
 extern "C" {
 #endif
 
-/* Element types, as tbq.h's ids: 0 F32, 1 F16 (IEEE halves), 30 BF16. */
+/* Element types, as tbq.h's ids: 0 F32, 1 F16 (IEEE halves), 30 BF16; 39 MXFP4
+ * (a cache's type only). */
 #define TBQ_KV_F32 0
 #define TBQ_KV_F16 1
 #define TBQ_KV_BF16 30
+#define TBQ_KV_MXFP4 39
 
 /* The cache: K and V are [n_layers][n_pages][n_kv_heads][page_size][head_dim]
  * of `type` (F16 or BF16), 16-byte aligned.  head_dim 64 or 128; page_size
  * 16, 32, 64, 128 or 256 positions.  Position p of a sequence is row
- * p % page_size of the page that its page table names at p / page_size. */
+ * p % page_size of the page that its page table names at p / page_size.
+ *
+ * type MXFP4 (4.25 bits a value): K and V are [n_layers][n_pages][n_kv_heads]
+ * [tbq_kv_head_bytes()] bytes, 16-byte aligned.  32 values side by side in a row
+ * are a block (OCP Microscaling Formats, MXFP4): one byte b for the scale 2^(b -
+ * 127) and 32 codes of 4 bits, a sign and 0, 0.5, 1, 1.5, 2, 3, 4 or 6.  A kv
+ * head's page of K is its codes [position][dim] (two a byte, the even dim in the
+ * low half), then its scale bytes [position][dim / 32]; V's codes lie [position /
+ * 4][dim / 8][position % 4][dim % 8], its scales [position / 4][dim / 32]
+ * [position % 4].  Append writes the least scale 2^E, E from -23 to 13, with
+ * max |x| <= 7 * 2^E, and the nearest codes (ties to the even one; larger values
+ * become 6 * 2^E), so every value held is an IEEE half.  A block with an infinity
+ * or a NaN gets the scale byte 255: all its values are NaN. */
 typedef struct {
     int n_layers, n_pages, n_kv_heads, page_size, head_dim, type;
     void *k, *v;
 } tbq_kv_cache;
+
+/* Bytes of one kv head in a page of K (or of V); 0 for a type, page_size or
+ * head_dim that a cache cannot have.  Host only. */
+size_t tbq_kv_head_bytes(int type, int page_size, int head_dim);
 
 /* New tokens of n_seqs sequences side by side (device arrays of int, which a
  * captured call reads again at every replay).  Sequence s has the token rows
@@ -93,7 +111,9 @@ int tbq_rope_init(tbq_rope *rope, int rot_dim, int layout, double theta, int sca
  * fp64), rounded once.
  * q, k, v: heads of row t side by side at base + t * stride elements (strides
  * multiples of 8, 16-byte aligned bases).  in_type is theirs, q_type q_out's:
- * in_type F32 with q_type F32 or the cache's type, or both the cache's type.
+ * in_type F32 with q_type F32 or the cache's type, or both the cache's type; with
+ * an MXFP4 cache in_type F32 with any q_type, or both F16, or both BF16 (keys are
+ * then normalised and rotated in fp64, so that their codes are the nearest ones).
  * q (with q_out) may be NULL; q_out may be q itself where types and strides
  * agree (q_stride = n_heads * head_dim), and must overlap no other input.
  * positions: NULL, or [n_tokens] ints that rotate in place of the positions in
@@ -118,7 +138,8 @@ int tbq_kv_append(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n
  * free: the kernel reads nothing of theirs that enters a result.
  * q [n_tokens][n_heads][head_dim] with q_stride elements between tokens (a
  * multiple of 8), out contiguous, not overlapping q, both of type q_type: the
- * cache's type, or F32 with an F16 cache.  Scores, softmax and sums are fp32.
+ * cache's type, or F32 with an F16 cache; any of the three with an MXFP4 cache,
+ * whose values enter the products exactly.  Scores, softmax and sums are fp32.
  * 16-bit rows of a sequence with up to 32 of them a kv head (new tokens times
  * n_heads / n_kv_heads; 16 where the batch may hold more than 256 MiB of keys
  * and values) are rounded once, at the output; with more rows the
@@ -131,6 +152,14 @@ size_t tbq_attn_paged_workspace_size(const tbq_kv_cache *c, const tbq_kv_batch *
 int tbq_attn_paged(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n_heads, int q_type, const void *q,
                    long long q_stride, void *out, int window, int sinks, float scale, void *workspace,
                    size_t workspace_bytes, void *stream);
+
+/* ---- values of an MXFP4 cache --------------------------------------------- */
+/* The values that pages of `layer` hold, exactly: k_out, v_out [n]
+ * [n_kv_heads][page_size][head_dim] of out_type (F32, F16 or BF16), 16-byte
+ * aligned.  pages: n device ints, a page outside the cache gives zeros; or NULL:
+ * the first n pages. */
+int tbq_kv_dequant(const tbq_kv_cache *c, int layer, const int *pages, int n, int out_type, void *k_out, void *v_out,
+                   void *stream);
 
 /* ---- pages and rows moved ---------------------------------------------------- */
 /* Page src[i] of every layer, K and V, is copied to page dst[i], for n pairs
@@ -188,7 +217,7 @@ int tbq_kv_pool_defrag(tbq_kv_pool *p, int max, int *src, int *dst);
  * the call returns.  Writes every
  * layer's K and V rows and logits[s][vocab] of each sequence's last token.  A
  * row of a page that two new tokens would write is refused.
- * The cache is F16 and has the model's layers, kv heads and head_dim.  rope
+ * The cache is F16 or MXFP4 and has the model's layers, kv heads and head_dim.  rope
  * NULL: the model's theta on the whole head in halves.  window, sinks: as
  * tbq_attn_paged, in every layer.  One token of one sequence runs on the
  * decode step's matvecs (logits as exact as the fp16 cache lets them be),

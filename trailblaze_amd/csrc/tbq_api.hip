@@ -468,7 +468,7 @@ int tbq_kv_check_cache(const char *who, const tbq_kv_cache *c);
 
 static int check_step(const char *who, const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int max_pages) {
     if (!check_dense(m, true) || !tbq_kv_check_cache(who, c)) return 0;
-    if (c->type != TBQ_KV_F16) return fail("%s: cache type %d (F16)", who, c->type);
+    if (c->type != TBQ_KV_F16 && c->type != TBQ_KV_MXFP4) return fail("%s: cache type %d (F16 or MXFP4)", who, c->type);
     if (c->n_layers != m->n_layers || c->n_kv_heads != m->n_kv_heads || c->head_dim != m->head_dim)
         return fail("%s: a cache of %d layers, %d kv heads of %d for a model of %d, %d of %d", who, c->n_layers,
                     c->n_kv_heads, c->head_dim, m->n_layers, m->n_kv_heads, m->head_dim);

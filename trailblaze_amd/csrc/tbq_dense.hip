@@ -596,7 +596,7 @@ hipError_t launch_dense_decode(const tbq_dense_model *m, int token, int pos, flo
 
 // The same step over a paged cache: pg is a batch of one sequence with one token
 // (layer 0's pages), layer_bytes lies between two layers of K (of V).
-hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const PgArgs &pg, size_t layer_bytes,
+hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const PgArgs &pg, int c_type, size_t layer_bytes,
                                      const PgRope &rope, int window, int sinks, float *logits, void *ws, void *attn_ws,
                                      hipStream_t st) {
     const int D = m->head_dim, NQ = m->n_heads, NKV = m->n_kv_heads;
@@ -625,8 +625,8 @@ hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const 
         ap.qn = L.q_norm;
         ap.kn = L.k_norm;
         at.pg = ap.pg;
-        const hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F32, TBQ_KV_F16, st);
-        return e != hipSuccess ? e : launch_pg_attn(at, D, TBQ_KV_F32, TBQ_KV_F16, attn_ws, st);
+        const hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F32, c_type, st);
+        return e != hipSuccess ? e : launch_pg_attn(at, D, TBQ_KV_F32, c_type, attn_ws, st);
     }, st);
 }
 

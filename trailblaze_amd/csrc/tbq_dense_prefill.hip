@@ -1109,12 +1109,12 @@ bool dense_step_attn_fits(const tbq_dense_model *m, const tbq_kv_cache *c, int n
     const size_t room = step_attn_bytes(m, n_seqs, a.n_tokens, (long long)max_pages * c->page_size);
     if (dense_prefill_batched(m) && a.n_tokens >= 2) {
         a.n_seqs = n_seqs;
-        return pg_attn_workspace_bytes(a, m->head_dim, m->n_heads, false) <= room;
+        return pg_attn_workspace_bytes(a, m->head_dim, m->n_heads, false, c->type) <= room;
     }
     a.n_seqs = a.n_tokens = a.max_q = 1;
     for (int s = 0; s < n_seqs; s++)
         for (a.max_kv = kv_len[s] - n_new[s] + 1; a.max_kv <= kv_len[s]; a.max_kv++)
-            if (pg_attn_workspace_bytes(a, m->head_dim, m->n_heads, true) > room) return false;
+            if (pg_attn_workspace_bytes(a, m->head_dim, m->n_heads, true, c->type) > room) return false;
     return true;
 }
 
@@ -1135,7 +1135,7 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
     w.pf = pf_ws(m, T, ws, ws_bytes, nullptr, true);
     w.pf.gpart_bytes = ws_bytes > off ? ws_bytes - off : 0;
     w.pf.gpart = w.pf.gpart_bytes ? (float *)((char *)ws + off) : nullptr;
-    const size_t layer_bytes = (size_t)c->n_pages * c->n_kv_heads * c->page_size * c->head_dim * 2;
+    const size_t layer_bytes = pg_layer_bytes(c);
     PgArgs pg = pg_layer(c, 0);
     PgRope rp{};
     pg_rope(rope, rp);
@@ -1156,7 +1156,7 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
                 pg.kv_len = q_start + 2;   // q_start and its length side by side
                 const int three[3] = {one[0], one[1], pg.max_kv};
                 if ((err = launch_put_ints(q_start, three, 3, st)) != hipSuccess) return err;
-                if ((err = launch_dense_decode_paged(m, tokens[t], pg, layer_bytes, rp, window, sinks,
+                if ((err = launch_dense_decode_paged(m, tokens[t], pg, c->type, layer_bytes, rp, window, sinks,
                                                      logits + (size_t)s * m->vocab, w.pf.dec, w.attn, st)) != hipSuccess)
                     return err;
             }
@@ -1215,8 +1215,8 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
         ap.qn = L.q_norm;
         ap.kn = L.k_norm;
         at.pg = ap.pg;
-        hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F16, TBQ_KV_F16, st);
-        if (e == hipSuccess) e = launch_pg_attn(at, D, TBQ_KV_F16, TBQ_KV_F16, w.attn, st);
+        hipError_t e = launch_pg_append(ap, D, TBQ_KV_F32, TBQ_KV_F16, c->type, st);
+        if (e == hipSuccess) e = launch_pg_attn(at, D, TBQ_KV_F16, c->type, w.attn, st);
         return e != hipSuccess ? e : launch_rows_f16(w.pf.att, T, NQ * D, w.pf.h16, w.pf.sb, st);
     }, &ysrc, &yns, st);
     if (err != hipSuccess) return err;

@@ -35,12 +35,16 @@ bool aligned(const void *p, unsigned n) { return ((uintptr_t)p & (n - 1)) == 0; 
 
 hipStream_t S(void *s) { return reinterpret_cast<hipStream_t>(s); }
 
+bool cache_type(int t) { return t == TBQ_KV_F16 || t == TBQ_KV_BF16 || t == TBQ_KV_MXFP4; }
+bool float_type(int t) { return t == TBQ_KV_F32 || t == TBQ_KV_F16 || t == TBQ_KV_BF16; }
+bool head_dim(int d) { return d == 64 || d == 128; }
+bool page_size(int n) { return n == 16 || n == 32 || n == 64 || n == 128 || n == 256; }
+
 int check_cache(const char *who, const tbq_kv_cache *c) {
     if (!c) return fail("%s: null cache", who);
-    if (c->type != TBQ_KV_F16 && c->type != TBQ_KV_BF16) return fail("%s: cache type %d (F16 or BF16)", who, c->type);
-    if (c->head_dim != 64 && c->head_dim != 128) return fail("%s: head_dim %d (64 or 128)", who, c->head_dim);
-    if (c->page_size != 16 && c->page_size != 32 && c->page_size != 64 && c->page_size != 128 && c->page_size != 256)
-        return fail("%s: page_size %d (16, 32, 64, 128 or 256)", who, c->page_size);
+    if (!cache_type(c->type)) return fail("%s: cache type %d (F16, BF16 or MXFP4)", who, c->type);
+    if (!head_dim(c->head_dim)) return fail("%s: head_dim %d (64 or 128)", who, c->head_dim);
+    if (!page_size(c->page_size)) return fail("%s: page_size %d (16, 32, 64, 128 or 256)", who, c->page_size);
     if (c->n_layers < 1 || c->n_layers > 16384 || c->n_pages < 1 || c->n_kv_heads < 1 || c->n_kv_heads > 65535)
         return fail("%s: cache of %d layers, %d pages, %d kv heads", who, c->n_layers, c->n_pages, c->n_kv_heads);
     if ((long long)c->n_pages * c->n_kv_heads * c->page_size > 0x7FFFFFFF)
@@ -62,7 +66,9 @@ int check_batch(const char *who, const tbq_kv_batch *b) {
     return 1;
 }
 
-long long page_elems(const tbq_kv_cache *c) { return (long long)c->n_kv_heads * c->page_size * c->head_dim; }
+long long page_bytes(const tbq_kv_cache *c) {
+    return (long long)c->n_kv_heads * c->page_size * pg_row_bytes(c->type, c->head_dim);
+}
 
 PgArgs pg_args(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b) {
     PgArgs a = pg_layer(c, layer);
@@ -86,6 +92,10 @@ extern "C" {
 // For tbq_api.hip (hidden): the checks of a cache.
 __attribute__((visibility("hidden"))) int tbq_kv_check_cache(const char *who, const tbq_kv_cache *c) {
     return check_cache(who, c);
+}
+
+size_t tbq_kv_head_bytes(int type, int page, int dim) {
+    return cache_type(type) && page_size(page) && head_dim(dim) ? (size_t)page * pg_row_bytes(type, dim) : 0;
 }
 
 int tbq_rope_init(tbq_rope *r, int rot_dim, int layout, double theta, int scaling, double factor, int orig_ctx,
@@ -136,9 +146,12 @@ int tbq_kv_append(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n
     const char *who = "tbq_kv_append";
     if (!check_cache(who, c) || !check_layer(who, c, layer) || !check_batch(who, b)) return 0;
     const int D = c->head_dim;
-    if (in_type != TBQ_KV_F32 && in_type != c->type) return fail("%s: in_type %d (F32 or the cache's)", who, in_type);
+    const bool mx = c->type == TBQ_KV_MXFP4;
+    if (mx ? !float_type(in_type) : in_type != TBQ_KV_F32 && in_type != c->type)
+        return fail("%s: in_type %d (F32 or the cache's; F32, F16 or BF16 with MXFP4)", who, in_type);
     if (!q != !q_out) return fail("%s: q and q_out go together", who);
-    if (q && q_type != c->type && !(q_type == TBQ_KV_F32 && in_type == TBQ_KV_F32))
+    if (q && (mx ? !float_type(q_type) || (in_type != TBQ_KV_F32 && q_type != in_type)
+                 : q_type != c->type && !(q_type == TBQ_KV_F32 && in_type == TBQ_KV_F32)))
         return fail("%s: q_type %d with in_type %d and cache type %d", who, q_type, in_type, c->type);
     if (q && (n_heads < 1 || n_heads > 65535)) return fail("%s: n_heads %d", who, n_heads);
     if (rope) {
@@ -174,7 +187,8 @@ int tbq_kv_append(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n
     a.NQ = q ? n_heads : 0;
     a.nsl = 1;
     if (rope) pg_rope(*rope, a.rope);
-    return hip_ok(launch_pg_append(a, D, in_type, q ? q_type : c->type, c->type, S(stream)), "kv append launch");
+    return hip_ok(launch_pg_append(a, D, in_type, q ? q_type : mx ? in_type : c->type, c->type, S(stream)),
+                  "kv append launch");
 }
 
 static int check_attn(const char *who, const tbq_kv_cache *c, const tbq_kv_batch *b, int n_heads, int q_type) {
@@ -182,14 +196,15 @@ static int check_attn(const char *who, const tbq_kv_cache *c, const tbq_kv_batch
     if (n_heads < 1 || n_heads > 65535 || n_heads % c->n_kv_heads)
         return fail("%s: n_heads %d, a multiple of the %d kv heads", who, n_heads, c->n_kv_heads);
     if ((long long)b->n_tokens * n_heads >= 1ll << 30) return fail("%s: %d tokens of %d heads", who, b->n_tokens, n_heads);
-    if (q_type != c->type && !(q_type == TBQ_KV_F32 && c->type == TBQ_KV_F16))
-        return fail("%s: q_type %d with cache type %d (the cache's type, or F32 with an F16 cache)", who, q_type, c->type);
+    if (c->type == TBQ_KV_MXFP4 ? !float_type(q_type) : q_type != c->type && !(q_type == TBQ_KV_F32 && c->type == TBQ_KV_F16))
+        return fail("%s: q_type %d with cache type %d (the cache's type, F32 with an F16 cache, any with MXFP4)", who, q_type,
+                    c->type);
     return 1;
 }
 
 size_t tbq_attn_paged_workspace_size(const tbq_kv_cache *c, const tbq_kv_batch *b, int n_heads, int q_type) {
     if (!check_attn("tbq_attn_paged_workspace_size", c, b, n_heads, q_type)) return 0;
-    return pg_attn_workspace_bytes(pg_args(c, 0, b), c->head_dim, n_heads, q_type == TBQ_KV_F32);
+    return pg_attn_workspace_bytes(pg_args(c, 0, b), c->head_dim, n_heads, q_type == TBQ_KV_F32, c->type);
 }
 
 int tbq_attn_paged(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n_heads, int q_type, const void *q,
@@ -203,7 +218,7 @@ int tbq_attn_paged(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int 
     if (qs % 8 || qs < (long long)n_heads * c->head_dim) return fail("%s: q_stride %lld", who, qs);
     PgAttn a{};
     a.pg = pg_args(c, layer, b);
-    const size_t need = pg_attn_workspace_bytes(a.pg, c->head_dim, n_heads, q_type == TBQ_KV_F32);
+    const size_t need = pg_attn_workspace_bytes(a.pg, c->head_dim, n_heads, q_type == TBQ_KV_F32, c->type);
     if (need && (!ws || ws_bytes < need || !aligned(ws, 16)))
         return fail("%s: workspace %zu < %zu bytes, or not 16-byte aligned", who, ws ? ws_bytes : 0, need);
     if (!tbq_init()) return 0;
@@ -215,6 +230,24 @@ int tbq_attn_paged(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int 
     a.sinks = window > 0 ? pg_window(sinks) : 0;
     a.scale = pg_scale(scale, c->head_dim);
     return hip_ok(launch_pg_attn(a, c->head_dim, q_type, c->type, ws, S(stream)), "paged attention launch");
+}
+
+int tbq_kv_dequant(const tbq_kv_cache *c, int layer, const int *pages, int n, int out_type, void *k_out, void *v_out,
+                   void *stream) {
+    const char *who = "tbq_kv_dequant";
+    if (!check_cache(who, c) || !check_layer(who, c, layer)) return 0;
+    if (c->type != TBQ_KV_MXFP4) return fail("%s: cache type %d (MXFP4)", who, c->type);
+    if (!float_type(out_type)) return fail("%s: out_type %d (F32, F16 or BF16)", who, out_type);
+    // (a workgroup for 16 rows at most: their number, times 256 threads, stays below 2^32)
+    if (n < 0 || n > (1 << 20) || (!pages && n > c->n_pages)) return fail("%s: %d pages of %d", who, n, c->n_pages);
+    if (n == 0) return 1;
+    if (!k_out || !v_out || !aligned(k_out, 16) || !aligned(v_out, 16))
+        return fail("%s: null or misaligned output (16 bytes)", who);
+    if (!tbq_init()) return 0;
+    tbq_kv_batch b{};
+    b.max_pages = 1;
+    return hip_ok(launch_mx_dequant(pg_args(c, layer, &b), c->head_dim, pages, n, out_type, k_out, v_out, S(stream)),
+                  "kv dequant launch");
 }
 
 int tbq_kv_copy_pages(const tbq_kv_cache *c, const int *src, const int *dst, int n, void *stream) {
@@ -237,7 +270,7 @@ int tbq_kv_copy_pages(const tbq_kv_cache *c, const int *src, const int *dst, int
     free(seen);
     if (bad >= 0) return fail("%s: page %d is written twice, or read and written", who, dst[bad]);
     if (!tbq_init()) return 0;
-    const long long pbytes = page_elems(c) * 2, lbytes = pbytes * c->n_pages;
+    const long long pbytes = page_bytes(c), lbytes = pbytes * c->n_pages;
     for (int i = 0; i < n; i += PG_PAIRS) {
         PgPairs p;
         const int m = n - i < PG_PAIRS ? n - i : PG_PAIRS;
@@ -260,8 +293,11 @@ int tbq_kv_compact(const tbq_kv_cache *c, int n_seqs, const int *page_table, int
     b.n_seqs = n_seqs;
     b.max_pages = max_pages;
     b.page_table = page_table;
-    return hip_ok(launch_pg_compact(c->k, c->v, c->n_layers, page_elems(c) * c->n_pages, c->head_dim, pg_args(c, 0, &b),
-                                    keep_start, keep, S(stream)),
+    const long long lbytes = page_bytes(c) * c->n_pages;
+    const PgArgs a = pg_args(c, 0, &b);
+    return hip_ok(c->type == TBQ_KV_MXFP4
+                      ? launch_mx_compact(c->k, c->v, c->n_layers, lbytes, c->head_dim, a, keep_start, keep, S(stream))
+                      : launch_pg_compact(c->k, c->v, c->n_layers, lbytes / 2, c->head_dim, a, keep_start, keep, S(stream)),
                   "compact launch");
 }
 

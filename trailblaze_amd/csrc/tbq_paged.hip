@@ -141,6 +141,7 @@ static hipError_t append_d(const PgAppend &a, hipStream_t st) {
 
 hipError_t launch_pg_append(const PgAppend &a, int D, int in_type, int q_type, int c_type, hipStream_t st) {
 #define TBQ_AP(TI, TQ, TC) return D == 128 ? append_d<TI, TQ, TC, 128>(a, st) : append_d<TI, TQ, TC, 64>(a, st)
+    if (c_type == TBQ_KV_MXFP4) return launch_mx_append(a, D, in_type, q_type, st);
     const bool fi = in_type == TBQ_KV_F32, fq = q_type == TBQ_KV_F32;
     if (c_type == TBQ_KV_F16) {
         if (fi && fq) TBQ_AP(float, float, pg_f16);

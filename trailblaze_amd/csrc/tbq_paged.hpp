@@ -22,12 +22,14 @@ struct PgRope {
     int rot, interleaved;
     float mscale;
     double turns[64];      // freq[j] / 2 pi
+    double mscale64;
 };
 
 inline void pg_rope(const tbq_rope &r, PgRope &o) {
     o.rot = r.rot_dim;
     o.interleaved = r.layout == TBQ_ROPE_INTERLEAVED;
     o.mscale = (float)r.mscale;
+    o.mscale64 = r.mscale;
     for (int j = 0; j < r.rot_dim / 2; j++) o.turns[j] = r.freq[j] * 0.15915494309189533577;
 }
 
@@ -70,12 +72,17 @@ inline int pg_log2(int n) {
     return s;
 }
 
+// Bytes of a row (of K or of V: one position of a kv head) and of a layer of K.
+inline int pg_row_bytes(int type, int D) { return type == TBQ_KV_MXFP4 ? D / 2 + D / 32 : 2 * D; }
+inline long long pg_layer_bytes(const tbq_kv_cache *c) {
+    return (long long)c->n_pages * c->n_kv_heads * c->page_size * pg_row_bytes(c->type, c->head_dim);
+}
+
 // Layer `layer` of a cache.
 inline PgArgs pg_layer(const tbq_kv_cache *c, int layer) {
     PgArgs a{};
-    const long long off = (long long)layer * c->n_pages * c->n_kv_heads * c->page_size * c->head_dim;
-    a.k = (uint16_t *)c->k + off;
-    a.v = (uint16_t *)c->v + off;
+    a.k = (uint8_t *)c->k + layer * pg_layer_bytes(c);
+    a.v = (uint8_t *)c->v + layer * pg_layer_bytes(c);
     a.n_pages = c->n_pages;
     a.NKV = c->n_kv_heads;
     a.shift = pg_log2(c->page_size);
@@ -140,11 +147,11 @@ hipError_t launch_pg_copy(void *k, void *v, int n_layers, long long pbytes, long
                           hipStream_t st);
 hipError_t launch_pg_compact(void *k, void *v, int n_layers, long long lelems, int D, const PgArgs &a, const int *keep_start,
                              const int *keep, hipStream_t st);
-size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32);
+size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32, int c_type);
 // at least that of every batch of up to n_seqs sequences, n_tokens tokens and max_kv positions
 size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int D, int NQ, bool f32);
 // One token of one sequence (tbq_dense.hip), a batch of sequences (tbq_dense_prefill.hip).
-hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const PgArgs &pg, size_t layer_bytes,
+hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const PgArgs &pg, int c_type, size_t layer_bytes,
                                      const PgRope &rope, int window, int sinks, float *logits, void *ws, void *attn_ws,
                                      hipStream_t st);
 size_t dense_step_workspace_bytes(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int T, int max_pages);
@@ -157,5 +164,13 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
 // *dst = n host ints, through kernel arguments (the host array is free at once)
 hipError_t launch_put_ints(int *dst, const int *src, long long n, hipStream_t st);
 hipError_t launch_pg_attn(const PgAttn &a, int D, int q_type, int c_type, void *ws, hipStream_t st);
+// The same over MXFP4 pages (tbq_paged_mx.hip, tbq_paged_mx_attn.hip; launch_pg_append and
+// launch_pg_attn hand on to them).
+hipError_t launch_mx_append(const PgAppend &a, int D, int in_type, int q_type, hipStream_t st);
+hipError_t launch_mx_attn(const PgAttn &a, int D, int q_type, void *ws, hipStream_t st);
+hipError_t launch_mx_dequant(const PgArgs &a, int D, const int *pages, int n, int out_type, void *k, void *v,
+                             hipStream_t st);
+hipError_t launch_mx_compact(void *k, void *v, int n_layers, long long lbytes, int D, const PgArgs &a,
+                             const int *keep_start, const int *keep, hipStream_t st);
 
 }  // namespace tbq

@@ -129,11 +129,14 @@ class SyntheticDense:
     def prefill_batched(self) -> bool:
         return bool(lib().tbq_dense_prefill_batched(C.byref(self.model)))
 
-    def paged_cache(self, n_pages: int, page_size: int = 64):
-        """An F16 ``paged.KvCache`` of this model's shape, for ``step``."""
+    def paged_cache(self, n_pages: int, page_size: int = 64, mxfp4: bool = False):
+        """An F16 (or MXFP4) ``paged.KvCache`` of this model's shape, for ``step``."""
         import torch
         from . import paged
         c = self.cfg
+        if mxfp4:
+            shape = (c.n_layers, n_pages, c.n_kv_heads, paged.kv_head_bytes(page_size, c.head_dim))
+            return paged.kv_cache(*(torch.zeros(shape, dtype=torch.uint8, device="cuda") for _ in range(2)), head_dim=c.head_dim)
         shape = (c.n_layers, n_pages, c.n_kv_heads, page_size, c.head_dim)
         return paged.kv_cache(*(torch.zeros(shape, dtype=torch.float16, device="cuda") for _ in range(2)))
 

@@ -3,7 +3,8 @@ with rotary positions, attention over the pages, page copies, compaction and
 the host-side page pool.
 
 A cache is two tensors [layers][pages][kv heads][page size][head dim] of
-float16 or bfloat16; a batch is int32 tensors on the same device.  Every call
+float16 or bfloat16, or [layers][pages][kv heads][bytes] of uint8 (MXFP4, 4.25
+bits a value); a batch is int32 tensors on the same device.  Every call
 checks its tensors (device, type, shape, strides) and raises TbqError or
 ValueError before anything is launched; work goes to torch's current stream
 unless ``stream`` names one.
@@ -16,7 +17,7 @@ from operator import index
 
 from . import TbqError, _check, _ptr, _stream, _workspace, lib
 
-F32, F16, BF16 = 0, 1, 30
+F32, F16, BF16, MXFP4 = 0, 1, 30, 39
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
 _LAYOUTS = {"half": ROPE_HALF, "interleaved": ROPE_INTERLEAVED}
 _SCALINGS = {"none": 0, "linear": 1, "yarn": 2}
@@ -126,16 +127,38 @@ def _flat(name, t, shape, dtype, dev):
     _on(name, t, dev)
 
 
-def kv_cache(k, v) -> KvCache:
-    """A ``tbq_kv_cache`` over two device tensors."""
-    if k.dim() != 5 or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or not v.is_contiguous():
-        raise ValueError("k and v: contiguous [layers][pages][kv heads][page size][head dim], alike")
-    if _type_id(k.dtype) == F32:
-        raise ValueError("k and v: float16 or bfloat16")
+def kv_head_bytes(page_size: int, head_dim: int, type_id: int = MXFP4) -> int:
+    """Bytes of one kv head in a page of K (or of V): the last size of an MXFP4 cache's tensors."""
+    n = int(lib().tbq_kv_head_bytes(type_id, _int("page_size", page_size), _int("head_dim", head_dim)))
+    if n == 0:
+        raise ValueError(f"no cache of type {type_id} has pages of {page_size} positions of {head_dim}")
+    return n
+
+
+def kv_cache(k, v, head_dim: int = 0) -> KvCache:
+    """A ``tbq_kv_cache`` over two device tensors.  uint8 tensors [layers][pages]
+    [kv heads][kv_head_bytes(page size, head_dim)] are an MXFP4 cache of head_dim."""
+    _init_torch()
+    mx = k.dtype == _torch.uint8
+    if k.dim() != (4 if mx else 5) or k.shape != v.shape or k.dtype != v.dtype or not k.is_contiguous() or \
+            not v.is_contiguous():
+        raise ValueError("k and v: contiguous [layers][pages][kv heads][page size][head dim] "
+                         "(MXFP4: [layers][pages][kv heads][bytes]), alike")
+    if not mx and _type_id(k.dtype) == F32:
+        raise ValueError("k and v: float16 or bfloat16 (or uint8, MXFP4)")
     if k.get_device() < 0 or k.get_device() != v.get_device():
         raise ValueError(f"k and v: on one device, got {k.device} and {v.device}")
-    L, P, H, S, D = k.shape
-    c = KvCache(L, P, H, S, D, _type_id(k.dtype), k.data_ptr(), v.data_ptr())
+    if mx:
+        L, P, H, n = k.shape
+        D = _int("head_dim", head_dim)
+        S = next((p for p in (16, 32, 64, 128, 256) if D in (64, 128) and kv_head_bytes(p, D) == n), 0)
+        if not S:
+            raise ValueError(f"k and v: {n} bytes a kv head are no page of MXFP4 rows of head_dim {head_dim}")
+    else:
+        L, P, H, S, D = k.shape
+        if head_dim not in (0, D):
+            raise ValueError(f"head_dim {head_dim}, but k and v have {D}")
+    c = KvCache(L, P, H, S, D, MXFP4 if mx else _type_id(k.dtype), k.data_ptr(), v.data_ptr())
     c._keep, c._dev = (k, v), k.get_device()
     return c
 
@@ -243,6 +266,24 @@ def attn_paged(cache: KvCache, layer: int, batch: KvBatch, q, out, window: int =
     return out
 
 
+def kv_dequant(cache: KvCache, layer: int, k_out, v_out, pages=None, stream=None):
+    """The values of an MXFP4 cache's pages of `layer`: k_out, v_out [n][kv heads]
+    [page size][head dim] of one floating type.  pages: int32 device tensor [n]
+    (None: the first n pages)."""
+    dev = _here(cache)
+    _int("layer", layer)
+    shape = (k_out.shape[0] if k_out.dim() else 0, cache.n_kv_heads, cache.page_size, cache.head_dim)
+    out_type = _type_id(k_out.dtype)
+    _flat("k_out", k_out, shape, k_out.dtype, dev)
+    _flat("v_out", v_out, shape, k_out.dtype, dev)
+    if pages is not None:
+        _ints("pages", pages, (shape[0],))
+        _on("pages", pages, dev)
+    _check(lib().tbq_kv_dequant(C.byref(cache), layer, None if pages is None else pages.data_ptr(), shape[0], out_type,
+                                k_out.data_ptr(), v_out.data_ptr(), _to(stream, dev)), "tbq_kv_dequant")
+    return k_out, v_out
+
+
 def kv_copy_pages(cache: KvCache, src, dst, stream=None):
     """Pages src[i] -> dst[i] of every layer (lists of int)."""
     n = len(src)
@@ -325,5 +366,5 @@ class PagePool:
         return list(zip(src[:n], dst[:n]))
 
 
-__all__ = ["KvCache", "KvBatch", "Rope", "PagePool", "kv_cache", "kv_batch", "rope", "kv_append", "attn_paged",
-           "attn_workspace_size", "kv_copy_pages", "kv_compact"]
+__all__ = ["KvCache", "KvBatch", "Rope", "PagePool", "kv_cache", "kv_head_bytes", "kv_batch", "rope", "kv_append", "attn_paged",
+           "attn_workspace_size", "kv_dequant", "kv_copy_pages", "kv_compact"]
