@@ -208,6 +208,74 @@ int tbq_kv_pool_fork(tbq_kv_pool *p, int positions, int page_size, const int *pa
  * number (-1: error). */
 int tbq_kv_pool_defrag(tbq_kv_pool *p, int max, int *src, int *dst);
 
+/* ---- a step's tables from request lengths ------------------------------------ */
+/* What the host pool and the host's batch arrays are to a server that decides on the
+ * host, on the device: lengths that a kernel produced (tbq_draft_verify's n_drop)
+ * become the next batch without a copy to the host.  The free list is device
+ * memory: free_pages[0 .. n_free[0] - 1] are pages with no holder, for instance
+ * those of a tbq_kv_pool_alloc that the host lends (pages with several holders stay
+ * in the host's books).
+ * First every sequence s drops its last n_drop[s] positions (NULL: none; at most
+ * kv_len[s]): pages behind the last position kept go to the list's end, in the order of
+ * sequences and positions (entries that name no page do not).  Then each gets
+ * n_new[s] positions more, and pages for them from the list's end, the last one
+ * first, in the order of sequences and positions, as long as all of its pages are
+ * there, its positions fit max_pages and the tokens so far fit n_tokens: from the first
+ * sequence where they do not, none gets any (its drop still holds), and served[0]
+ * says how many were served.
+ * kv_len_out[s]: positions with the new ones; q_start [n_seqs + 1]: a batch's;
+ * page_table_out: -1 behind a sequence's last page; free_out: -1 from n_free_out[0]
+ * on; positions and slots [n_tokens]: a token's position, and page * page_size +
+ * row in it, -1 for rows behind the last sequence (or without a page).
+ * Outputs may be the inputs of the same meaning (free_out with n_free_out), else
+ * overlap none.  n_pages: of the cache and entries of free_pages and free_out.
+ * Lengths below 0 count as 0, above max_pages * page_size as that; n_free above n_pages as that. */
+typedef struct {
+    int n_seqs, max_pages, page_size, n_pages, n_tokens;
+    const int *kv_len;      /* [n_seqs] */
+    const int *n_drop;      /* [n_seqs], or NULL */
+    const int *n_new;       /* [n_seqs] */
+    const int *page_table;  /* [n_seqs][max_pages] */
+    const int *free_pages;  /* [n_pages] */
+    const int *n_free;      /* [1] */
+    int *kv_len_out, *page_table_out, *free_out, *n_free_out;
+    int *q_start;           /* [n_seqs + 1] */
+    int *slots, *positions; /* [n_tokens], or NULL */
+    int *served;            /* [1], or NULL */
+} tbq_kv_tables;
+int tbq_kv_build_tables(const tbq_kv_tables *t, void *stream);
+
+/* ---- verification of drafted tokens ------------------------------------------- */
+/* Sequence s has the rows q_start[s] .. q_start[s + 1] - 1 of logits [n_rows]
+ * [vocab] (stride elements between rows, of `type`: F32, F16 or BF16), one for each
+ * token of the step that made them: row r predicts the token behind tokens[r], so
+ * the draft tokens[r + 1] is judged by row r, for all rows of a sequence but its
+ * last.  With p = softmax(logits[r] / temperature[s]) (temperature NULL: 1; not
+ * above 0: all weight on the largest logit, of equal ones the first) and q the
+ * same of draft_logits[r] (NULL: the draft was certain, q = 1 at it), drafts stay
+ * as long as u_accept[r] * q(draft) < p(draft).  n_accept[s]: how many;
+ * next[s]: the token behind them, the first v whose sum of weights 0 .. v is above
+ * u_next[s] times the sum of all, weights max(p - q, 0) of the row that rejected
+ * its draft (p, if all of those are 0), or p of the last row; n_drop[s] (NULL: not
+ * written): drafts that did not stay.  So tokens are distributed as the target's,
+ * for independent u_accept and u_next uniform in [0, 1) (others count as the nearest
+ * float there, a NaN as 0).
+ * Weights and sums are fp64.  A NaN logit counts as -infinity; among infinite
+ * ones the +infinities share the weight.  A row without weight rejects its draft,
+ * and next is -1 if it is drawn from.  Drafts outside the vocabulary are rejected.
+ * A sequence without rows (or with rows outside n_rows) has 0, -1 and 0.  Starts do
+ * not fall; where they do, the sequences that share rows get no defined tokens, but
+ * none outside the vocabulary.
+ * draft_logits: [n_rows][vocab] with draft_stride, of the same type; rows that
+ * judge no draft are not read.
+ * workspace: tbq_draft_verify_workspace_size() bytes, 16-byte aligned, no
+ * zero-fill needed; calls that share one must not overlap. */
+size_t tbq_draft_verify_workspace_size(int n_seqs, int n_rows, int vocab, int type, int with_draft);
+int tbq_draft_verify(int n_seqs, int n_rows, int vocab, int type, const int *q_start, const int *tokens,
+                     const void *logits, long long stride, const void *draft_logits, long long draft_stride,
+                     const float *temperature, const float *u_accept, const float *u_next, int *n_accept, int *next,
+                     int *n_drop, void *workspace, size_t workspace_bytes, void *stream);
+
 /* ---- dense model over a paged cache ------------------------------------------- */
 /* The forward of tbq_dense_decode / tbq_dense_prefill (same model struct; its
  * max_ctx, k_cache and v_cache are not used) for n_seqs sequences at once:

@@ -68,6 +68,9 @@ SYMBOLS = {
     "tbq_attn_paged": (_i, [_vp, _i, _vp, _i, _i, _vp, _ll, _vp, _i, _i, _f, _vp, _sz, _vp]),
     "tbq_kv_head_bytes": (_sz, [_i, _i, _i]),
     "tbq_kv_dequant": (_i, [_vp, _i, _vp, _i, _i, _vp, _vp, _vp]),
+    "tbq_kv_build_tables": (_i, [_vp, _vp]),
+    "tbq_draft_verify_workspace_size": (_sz, [_i, _i, _i, _i, _i]),
+    "tbq_draft_verify": (_i, [_i, _i, _i, _i, _vp, _vp, _vp, _ll, _vp, _ll, _vp, _vp, _vp, _vp, _vp, _vp, _vp, _sz, _vp]),
     "tbq_kv_copy_pages": (_i, [_vp, _vp, _vp, _i, _vp]),
     "tbq_kv_compact": (_i, [_vp, _i, _vp, _i, _vp, _vp, _vp]),
     "tbq_dense_step_workspace_size": (_sz, [_vp, _vp, _i, _i, _i]),

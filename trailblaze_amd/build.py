@@ -28,7 +28,7 @@ C_FLAGS = ["-std=c11", "-O2", "-fPIC", "-Wall", "-Wextra", "-ffp-contract=off",
 
 HIP_SOURCES = ["tbq_matvec.hip", "tbq_mv_q4k.hip", "tbq_mv_kq.hip", "tbq_moe.hip", "tbq_moe_q4k.hip", "tbq_moe_prefill.hip", "tbq_dense.hip", "tbq_dense_prefill.hip", "tbq_gemm.hip", "tbq_api.hip",
                "tbq_noalloc.hip", "tbq_paged.hip", "tbq_paged_attn.hip", "tbq_paged_mx.hip",
-               "tbq_paged_mx_attn.hip", "tbq_kv_api.hip"]
+               "tbq_paged_mx_attn.hip", "tbq_tables.hip", "tbq_verify.hip", "tbq_kv_api.hip"]
 C_SOURCES = ["tb_cuda_abi.c", "tbq_moe_host.c", "tbq_gguf.c", "tbq_kv_pool.c"]
 
 

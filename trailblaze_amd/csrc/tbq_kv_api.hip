@@ -12,6 +12,7 @@
 #include "../../include/tbq_kv.h"
 #include "tbq_kernels.h"
 #include "tbq_paged.hpp"
+#include "tbq_serve.hpp"
 
 using namespace tbq;
 
@@ -299,6 +300,76 @@ int tbq_kv_compact(const tbq_kv_cache *c, int n_seqs, const int *page_table, int
                       ? launch_mx_compact(c->k, c->v, c->n_layers, lbytes, c->head_dim, a, keep_start, keep, S(stream))
                       : launch_pg_compact(c->k, c->v, c->n_layers, lbytes / 2, c->head_dim, a, keep_start, keep, S(stream)),
                   "compact launch");
+}
+
+int tbq_kv_build_tables(const tbq_kv_tables *t, void *stream) {
+    const char *who = "tbq_kv_build_tables";
+    if (!t) return fail("%s: null tables", who);
+    if (!page_size(t->page_size)) return fail("%s: page_size %d (16, 32, 64, 128 or 256)", who, t->page_size);
+    if (t->n_seqs < 0 || t->n_seqs > 65535 || t->n_tokens < 0 || t->n_tokens > 1 << 30 || t->max_pages < 1 ||
+        t->n_pages < 1 || (long long)t->max_pages * t->page_size > 1 << 30 ||
+        (long long)t->n_seqs * t->max_pages > 0x7FFFFFFF || (long long)t->n_pages * t->page_size > 0x7FFFFFFF)
+        return fail("%s: %d sequences of %d pages, %d tokens, %d pages of %d", who, t->n_seqs, t->max_pages, t->n_tokens,
+                    t->n_pages, t->page_size);
+    if (!t->q_start || !t->free_pages || !t->n_free || !t->free_out || !t->n_free_out ||
+        (t->n_seqs && (!t->kv_len || !t->n_new || !t->page_table || !t->kv_len_out || !t->page_table_out)))
+        return fail("%s: null array", who);
+    if ((t->free_out == t->free_pages) != (t->n_free_out == t->n_free))
+        return fail("%s: free_out and n_free_out go together: both in place, or neither", who);
+    if (!tbq_init()) return 0;
+    return hip_ok(launch_tables({*t, pg_log2(t->page_size)}, S(stream)), "tables launch");
+}
+
+static int check_verify(const char *who, int n_seqs, int n_rows, int vocab, int type, bool draft) {
+    if (n_seqs < 0 || n_seqs > 65535 || n_rows < 0 || vocab < 1 || vocab > 1 << 28)
+        return fail("%s: %d sequences, %d rows of %d", who, n_seqs, n_rows, vocab);
+    if (!float_type(type)) return fail("%s: type %d (F32, F16 or BF16)", who, type);
+    // a workgroup of 256 a chunk: their threads stay below 2^32
+    const long long chunks = (vocab + DV_CHUNK - 1) / DV_CHUNK;
+    if (chunks * (n_rows > n_seqs ? n_rows : n_seqs) * (draft ? 2 : 1) > (1 << 24) - 1)
+        return fail("%s: %d rows of %d", who, n_rows, vocab);
+    return 1;
+}
+
+size_t tbq_draft_verify_workspace_size(int n_seqs, int n_rows, int vocab, int type, int draft) {
+    if (!check_verify("tbq_draft_verify_workspace_size", n_seqs, n_rows, vocab, type, draft)) return 0;
+    return verify_workspace_bytes(n_seqs, n_rows, vocab, draft);
+}
+
+int tbq_draft_verify(int n_seqs, int n_rows, int vocab, int type, const int *q_start, const int *tokens,
+                     const void *logits, long long stride, const void *draft, long long dstride, const float *temperature,
+                     const float *u_accept, const float *u_next, int *n_accept, int *next, int *n_drop, void *ws,
+                     size_t ws_bytes, void *stream) {
+    const char *who = "tbq_draft_verify";
+    if (!check_verify(who, n_seqs, n_rows, vocab, type, draft != nullptr)) return 0;
+    if (n_seqs == 0) return 1;
+    if (!q_start || !u_next || !n_accept || !next || (n_rows && (!tokens || !logits || !u_accept)))
+        return fail("%s: null pointer", who);
+    const unsigned size = type == TBQ_KV_F32 ? 4 : 2;
+    if (!aligned(logits, size) || !aligned(draft, size)) return fail("%s: misaligned logits", who);
+    if (n_rows && (stride < vocab || (draft && dstride < vocab))) return fail("%s: a stride is shorter than its row", who);
+    const size_t need = verify_workspace_bytes(n_seqs, n_rows, vocab, draft != nullptr);
+    if (need && (!ws || ws_bytes < need || !aligned(ws, 16)))
+        return fail("%s: workspace %zu < %zu bytes, or not 16-byte aligned", who, ws ? ws_bytes : 0, need);
+    if (!tbq_init()) return 0;
+    SvVerify a{};
+    a.n_seqs = n_seqs;
+    a.n_rows = n_rows;
+    a.vocab = vocab;
+    a.chunks = (vocab + DV_CHUNK - 1) / DV_CHUNK;
+    a.q_start = q_start;
+    a.tokens = tokens;
+    a.logits = logits;
+    a.draft = draft;
+    a.stride = stride;
+    a.dstride = dstride;
+    a.temperature = temperature;
+    a.u_accept = u_accept;
+    a.u_next = u_next;
+    a.n_accept = n_accept;
+    a.next = next;
+    a.n_drop = n_drop;
+    return hip_ok(launch_verify(a, type, ws, S(stream)), "draft verify launch");
 }
 
 }  // extern "C"

@@ -40,6 +40,13 @@ class Rope(C.Structure):
     _fields_ = [("rot_dim", C.c_int), ("layout", C.c_int), ("mscale", C.c_double), ("freq", C.c_double * 64)]
 
 
+class KvTables(C.Structure):
+    """Mirror of ``tbq_kv_tables``."""
+    _fields_ = [(n, C.c_int) for n in ("n_seqs", "max_pages", "page_size", "n_pages", "n_tokens")] + \
+        [(n, C.c_void_p) for n in ("kv_len", "n_drop", "n_new", "page_table", "free_pages", "n_free", "kv_len_out",
+                                   "page_table_out", "free_out", "n_free_out", "q_start", "slots", "positions", "served")]
+
+
 _torch, _raw, _device, _ids = None, None, None, {}
 _INT = 1 << 31
 
@@ -312,6 +319,101 @@ def kv_compact(cache: KvCache, page_table, keep_start, keep, stream=None):
                                 keep.data_ptr(), _to(stream, dev)), "tbq_kv_compact")
 
 
+def kv_tables(page_size: int, kv_len, n_new, page_table, free_pages, n_free, *, q_start, n_drop=None, kv_len_out=None,
+              table_out=None, free_out=None, n_free_out=None, slots=None, positions=None, served=None) -> KvTables:
+    """A ``tbq_kv_tables`` over int32 device tensors, for ``kv_build_tables``: kv_len,
+    n_new, n_drop [sequences], page_table [sequences][pages], free_pages [pages of the
+    cache], n_free [1]; outputs that are not given are the inputs of the same meaning.
+    slots and positions have a row a token of the batch."""
+    _init_torch()
+    kv_len_out, table_out = kv_len if kv_len_out is None else kv_len_out, page_table if table_out is None else table_out
+    free_out, n_free_out = free_pages if free_out is None else free_out, n_free if n_free_out is None else n_free_out
+    n = kv_len.numel()
+    if page_table.dim() != 2:
+        raise ValueError("page_table: [sequences][pages]")
+    rows = next((t.numel() for t in (slots, positions) if t is not None), None)
+    if rows is None:
+        rows = 1 << 30   # no rows to fill, so no bound on them
+    one, table, pages = (1,), (n, page_table.shape[1]), (free_pages.numel(),)
+    given = dict(kv_len=(kv_len, (n,)), n_drop=(n_drop, (n,)), n_new=(n_new, (n,)), page_table=(page_table, table),
+                 free_pages=(free_pages, pages), n_free=(n_free, one), kv_len_out=(kv_len_out, (n,)),
+                 page_table_out=(table_out, table), free_out=(free_out, pages), n_free_out=(n_free_out, one),
+                 q_start=(q_start, (n + 1,)), slots=(slots, (rows,)), positions=(positions, (rows,)), served=(served, one))
+    dev = kv_len.get_device()
+    for name, (t, shape) in given.items():
+        if t is not None:
+            _ints(name, t, shape)
+    for name, (t, _) in given.items():
+        if dev < 0 or (t is not None and t.get_device() != dev):
+            raise ValueError(f"{name}: tensors on one device, got {kv_len.device if t is None else t.device}")
+    t = KvTables(n, page_table.shape[1], _int("page_size", page_size), free_pages.numel(), rows,
+                 *(None if t is None else t.data_ptr() for t, _ in given.values()))
+    t._keep, t._dev = tuple(t for t, _ in given.values()), dev
+    return t
+
+
+def kv_build_tables(tables: KvTables, stream=None):
+    """Pages of dropped positions go back, pages for new ones are taken; the batch's q_start, lengths, page
+    table, slots and positions (tbq_kv_build_tables)."""
+    dev = _here(tables)
+    _check(lib().tbq_kv_build_tables(C.byref(tables), _to(stream, dev)), "tbq_kv_build_tables")
+
+
+def draft_verify_workspace_size(n_seqs: int, n_rows: int, vocab: int, dtype, with_draft: bool) -> int:
+    return int(lib().tbq_draft_verify_workspace_size(_int("n_seqs", n_seqs), _int("n_rows", n_rows), _int("vocab", vocab),
+                                                     _type_id(dtype), bool(with_draft)))
+
+
+def _rows_of(name, t, rows, vocab, dev):
+    """Elements between the rows of logits [rows][vocab]."""
+    if t.dim() != 2 or t.shape != (rows, vocab) or (vocab > 1 and t.stride(1) != 1):
+        raise ValueError(f"{name}: {(rows, vocab)} with the elements of a row side by side expected, got {tuple(t.shape)}")
+    _on(name, t, dev)
+    return t.stride(0) if rows > 1 else vocab
+
+
+def draft_verify(q_start, tokens, logits, u_accept, u_next, n_accept, next_token, n_drop=None, draft_logits=None,
+                 temperature=None, workspace=None, stream=None):
+    """Which drafts stay, and the token behind them (tbq_draft_verify).  q_start [sequences + 1], tokens [rows],
+    n_accept, next_token, n_drop [sequences]: int32; logits, draft_logits [rows][vocab] of one type; u_accept
+    [rows], u_next, temperature [sequences]: float32."""
+    _init_torch()
+    dev, n = _device(), next_token.numel()
+    if logits.dim() != 2:
+        raise ValueError("logits: [rows][vocab]")
+    rows, vocab = logits.shape
+    type_id = _type_id(logits.dtype)
+    stride = _rows_of("logits", logits, rows, vocab, dev)
+    dstride = 0
+    if draft_logits is not None:
+        if draft_logits.dtype != logits.dtype:
+            raise ValueError("logits and draft_logits: one type")
+        dstride = _rows_of("draft_logits", draft_logits, rows, vocab, dev)
+    for name, t, m in (("q_start", q_start, n + 1), ("tokens", tokens, rows), ("n_accept", n_accept, n),
+                       ("next_token", next_token, n), ("n_drop", n_drop, n)):
+        if t is not None:
+            _ints(name, t, (m,))
+            _on(name, t, dev)
+    for name, t, m in (("u_accept", u_accept, rows), ("u_next", u_next, n), ("temperature", temperature, n)):
+        if t is not None:
+            _flat(name, t, (m,), _torch.float32, dev)
+    to = _to(stream, dev)
+    if workspace is None:
+        size = draft_verify_workspace_size(n, rows, vocab, logits.dtype, draft_logits is not None)
+        if size:
+            workspace = _workspace(size, stream)
+    else:
+        _on("workspace", workspace, dev)
+        if not workspace.is_contiguous():
+            raise ValueError("workspace: contiguous")
+    wp, wb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
+    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
+    _check(lib().tbq_draft_verify(n, rows, vocab, type_id, ptr(q_start), ptr(tokens), ptr(logits), stride, ptr(draft_logits),
+                                  dstride, ptr(temperature), ptr(u_accept), ptr(u_next), ptr(n_accept), ptr(next_token),
+                                  ptr(n_drop), wp, wb, to), "tbq_draft_verify")
+    return next_token
+
+
 class PagePool:
     """Which pages of a cache are held, and how often (tbq_kv_pool_*)."""
 
@@ -366,5 +468,6 @@ class PagePool:
         return list(zip(src[:n], dst[:n]))
 
 
-__all__ = ["KvCache", "KvBatch", "Rope", "PagePool", "kv_cache", "kv_head_bytes", "kv_batch", "rope", "kv_append", "attn_paged",
+__all__ = ["KvCache", "KvBatch", "KvTables", "Rope", "PagePool", "kv_tables", "kv_build_tables", "draft_verify",
+           "draft_verify_workspace_size", "kv_cache", "kv_head_bytes", "kv_batch", "rope", "kv_append", "attn_paged",
            "attn_workspace_size", "kv_dequant", "kv_copy_pages", "kv_compact"]
