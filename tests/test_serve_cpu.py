@@ -63,8 +63,8 @@ def test_verify_refusals(kw, words):
 def test_verify_of_nothing_and_sizes():
     assert verify(n_seqs=0, q_start=None, ws=None) == 1
     size = tb.lib().tbq_draft_verify_workspace_size
-    assert size(2, 5, 8192, 0, 0) == 5 * 16 and size(2, 5, 8193, 0, 0) == 10 * 16
-    assert size(2, 5, 8193, 30, 1) == 20 * 16 + 2 * 2 * 8
+    assert 0 < size(2, 5, 8192, 0, 0) < size(2, 6, 8192, 0, 0) < size(2, 6, 90000, 0, 0) < size(2, 6, 90000, 0, 1)
+    assert size(1, 1, 1, 30, 0) >= 16
     assert size(2, 5, 0, 0, 0) == 0 and size(2, 5, 10, 39, 0) == 0
 
 

@@ -368,10 +368,43 @@ __device__ __forceinline__ void pg_join_row(const float *__restrict__ rec, int n
     out[tid] = (TO)(den == 0.f ? 0.f : num / den);
 }
 
-// A row of a sequence of few rows.  x: kv head + NKV * row; s: sequence.
-template <typename TO, int D, bool HL>
+// Joins nz records by D / 4 lanes, dims d .. d + 3 each, eight records at once.
+template <typename TO, int D>
+__device__ __forceinline__ void pg_join_few(const float *__restrict__ rec, int nz, int d, TO *out) {
+    constexpr int REC = pg_rec(D);
+    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
+    float den = 0.f, M = PG_LOW;
+    for (int z0 = 0; z0 < nz; z0 += 8) {
+        float2 ml[8];
+        float4 y[8];
+        float mn = M;
+#pragma unroll
+        for (int z = 0; z < 8; z++) {   // past the last: the last again, not added
+            ml[z] = *reinterpret_cast<const float2 *>(rec + min(z0 + z, nz - 1) * REC + D);
+            y[z] = *reinterpret_cast<const float4 *>(rec + min(z0 + z, nz - 1) * REC + d);
+            mn = fmaxf(mn, ml[z].x);
+        }
+        const float c = __builtin_amdgcn_exp2f(M - mn);
+        M = mn;
+        x = make_float4(x.x * c, x.y * c, x.z * c, x.w * c);
+        den *= c;
+#pragma unroll
+        for (int z = 0; z < 8; z++) {
+            if (z0 + z >= nz) continue;
+            const float f = __builtin_amdgcn_exp2f(ml[z].x - M);
+            x = make_float4(fmaf(f, y[z].x, x.x), fmaf(f, y[z].y, x.y), fmaf(f, y[z].z, x.z), fmaf(f, y[z].w, x.w));
+            den = fmaf(f, ml[z].y, den);
+        }
+    }
+    const float inv = den == 0.f ? 0.f : 1.0f / den;
+    pg_st4(out + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+}
+
+// A row of a sequence of few rows.  x: kv head + NKV * row; s: sequence; d: of FEW lanes'
+// dims the first.
+template <typename TO, int D, bool HL, bool FEW>
 __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, int nsplit, const float *__restrict__ part,
-                                             int x, int s) {
+                                             int x, int s, int d) {
     constexpr int RB = HL ? 8 : 16;
     const int kvh = x % a.pg.NKV, r = x / a.pg.NKV, G = a.NQ / a.pg.NKV;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
@@ -381,9 +414,11 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
     const int base = a.pg.kv_len[s] - qn, r0 = r / RB * RB;
     const int nz = (pg_tiles<PR_TS>(base + r0 / G, base + (min(r0 + RB, rows) - 1) / G, a.window, a.sinks, a.pg.max_kv).n +
                     tps - 1) / tps;
-    if (nz > 1)
-        pg_join_row<TO, D>(part + (((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit * pg_rec(D), nz,
-                           (TO *)a.out + ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D);
+    const float *rec = part + (((long long)s * a.pg.NKV + kvh) * nrb * RB + r) * nsplit * pg_rec(D);
+    TO *out = (TO *)a.out + ((long long)(q0 + r / G) * a.NQ + kvh * G + r % G) * D;
+    if (nz <= 1) return;
+    if constexpr (FEW) pg_join_few<TO, D>(rec, nz, d, out);
+    else pg_join_row<TO, D>(rec, nz, out);
 }
 
 // ---------------------------------------------------------------------------
@@ -742,44 +777,22 @@ __device__ __forceinline__ void pg_join_chunk(const PgAttn &a, int nsplit, const
     const int nz = pg_chunk_splits(a, q0, rows, base, t, hd, nsplit);
     if (nz <= 1) return;
     const long long at = (long long)t * a.NQ + hd;
-    const float *rec = part + at * nsplit * REC;
-    float4 x = make_float4(0.f, 0.f, 0.f, 0.f);
-    float den = 0.f, M = PG_LOW;
-    for (int z0 = 0; z0 < nz; z0 += 8) {
-        float2 ml[8];
-        float4 y[8];
-        float mn = M;
-#pragma unroll
-        for (int z = 0; z < 8; z++) {   // past the last: the last again, not added
-            ml[z] = *reinterpret_cast<const float2 *>(rec + min(z0 + z, nz - 1) * REC + D);
-            y[z] = *reinterpret_cast<const float4 *>(rec + min(z0 + z, nz - 1) * REC + d);
-            mn = fmaxf(mn, ml[z].x);
-        }
-        const float c = __builtin_amdgcn_exp2f(M - mn);
-        M = mn;
-        x = make_float4(x.x * c, x.y * c, x.z * c, x.w * c);
-        den *= c;
-#pragma unroll
-        for (int z = 0; z < 8; z++) {
-            if (z0 + z >= nz) continue;
-            const float f = __builtin_amdgcn_exp2f(ml[z].x - M);
-            x = make_float4(fmaf(f, y[z].x, x.x), fmaf(f, y[z].y, x.y), fmaf(f, y[z].z, x.z), fmaf(f, y[z].w, x.w));
-            den = fmaf(f, ml[z].y, den);
-        }
-    }
-    const float inv = den == 0.f ? 0.f : 1.0f / den;
-    pg_st4((TO *)a.out + at * D + d, make_float4(x.x * inv, x.y * inv, x.z * inv, x.w * inv));
+    pg_join_few<TO, D>(part + at * nsplit * REC, nz, d, (TO *)a.out + at * D);
 }
 
 // grid: row_wgs = NKV * (most rows of a few-row sequence) * n_seqs workgroups for
-// few rows (0: they were not split), then one for pj_heads of a token's heads, or for
-// one of them (none if the many rows were not split).
-template <typename TO, int D, bool HL>
+// few rows (0: they were not split; FEW: one for pj_heads of them), then one for
+// pj_heads of a token's heads, or for one of them (none if the many rows were not split).
+template <typename TO, int D, bool HL, bool FEW>
 __global__ __launch_bounds__(PJ_THREADS) void k_pg_join(const PgAttn a, int nrb, int tps, int row_splits,
                                                         const float *__restrict__ row_part, int row_wgs, int most,
                                                         int nsplit, const float *__restrict__ part) {
     const int x = blockIdx.x, n = a.pg.NKV * most, y = x - row_wgs;
-    if (x < row_wgs) pg_join_rows<TO, D, HL>(a, nrb, tps, row_splits, row_part, x % n, x / n);
+    if (FEW && x < row_wgs) {
+        const int i = x * pj_heads(D) + threadIdx.x / (D / 4), s = i / n;
+        if (s < a.pg.n_seqs)
+            pg_join_rows<TO, D, HL, true>(a, nrb, tps, row_splits, row_part, i % n, s, threadIdx.x % (D / 4) * 4);
+    } else if (x < row_wgs) pg_join_rows<TO, D, HL, false>(a, nrb, tps, row_splits, row_part, x % n, x / n, 0);
     else if (nsplit > PC_FEW) pg_join_chunk<TO, D>(a, nsplit, part, y / a.NQ, y % a.NQ, y % a.NQ + 1);
     else {
         const int hpw = pj_heads(D), g = (a.NQ + hpw - 1) / hpw;
@@ -869,30 +882,32 @@ size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int
 }
 
 // Adds the split ranges of a launch, where there are any.
-template <typename TC, int D, bool HL>
-static hipError_t pg_join(const PgAttn &a, const PgPlan &p, bool f32_out, const float *ws, hipStream_t st) {
+template <typename TO, int D, bool HL, bool FEW>
+static hipError_t pg_join(const PgAttn &a, const PgPlan &p, const float *ws, hipStream_t st) {
     const float *part = ws + p.rows_bytes / 4;
-    const long long row_wgs = p.row_splits > 1 ? (long long)a.pg.NKV * p.most * a.pg.n_seqs : 0;
+    long long row_wgs = p.row_splits > 1 ? (long long)a.pg.NKV * p.most * a.pg.n_seqs : 0;
+    if (FEW) row_wgs = (row_wgs + pj_heads(D) - 1) / pj_heads(D);
     const long long wgs = row_wgs + (p.chunk_splits > PC_FEW ? (long long)a.pg.n_tokens * a.NQ
                                      : p.chunk_splits > 1   ? (long long)a.pg.n_tokens * ((a.NQ + pj_heads(D) - 1) / pj_heads(D))
                                                             : 0);
     if (wgs > PG_WGS) return hipErrorInvalidConfiguration;
-    if (wgs > 0 && f32_out)
-        hipLaunchKernelGGL((k_pg_join<float, D, HL>), dim3((unsigned)wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps,
-                           p.row_splits, ws, (int)row_wgs, p.most, p.chunk_splits, part);
-    else if (wgs > 0)
-        hipLaunchKernelGGL((k_pg_join<TC, D, HL>), dim3((unsigned)wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps,
+    if (wgs > 0)
+        hipLaunchKernelGGL((k_pg_join<TO, D, HL, FEW>), dim3((unsigned)wgs), dim3(PJ_THREADS), 0, st, a, p.nrb, p.row_tps,
                            p.row_splits, ws, (int)row_wgs, p.most, p.chunk_splits, part);
     return hipGetLastError();
 }
 
-hipError_t launch_pg_join(const PgAttn &a, int D, const PgPlan &p, bool f32, int out_type, const float *ws,
-                          hipStream_t st) {
-    const bool o32 = out_type == TBQ_KV_F32;
-    if (f32) return D == 128 ? pg_join<pg_f16, 128, true>(a, p, true, ws, st) : pg_join<pg_f16, 64, true>(a, p, true, ws, st);
-    if (out_type == TBQ_KV_BF16)
-        return D == 128 ? pg_join<pg_bf16, 128, false>(a, p, false, ws, st) : pg_join<pg_bf16, 64, false>(a, p, false, ws, st);
-    return D == 128 ? pg_join<pg_f16, 128, false>(a, p, o32, ws, st) : pg_join<pg_f16, 64, false>(a, p, o32, ws, st);
+// Over 4-bit pages.  A batch's few splits a row: D / 4 lanes a row (64 sequences of up to 8192 positions
+// 7.2 -> 3.x us); the hundreds of a long context a workgroup.
+template <typename TO, int D, bool HL>
+static hipError_t mx_join(const PgAttn &a, const PgPlan &p, const float *ws, hipStream_t st) {
+    return p.row_splits <= PC_FEW ? pg_join<TO, D, HL, true>(a, p, ws, st) : pg_join<TO, D, HL, false>(a, p, ws, st);
+}
+hipError_t launch_mx_join(const PgAttn &a, int D, const PgPlan &p, bool f32, int out_type, const float *ws, hipStream_t st) {
+    if (f32) return D == 128 ? mx_join<float, 128, true>(a, p, ws, st) : mx_join<float, 64, true>(a, p, ws, st);
+    if (out_type == TBQ_KV_F32) return D == 128 ? mx_join<float, 128, false>(a, p, ws, st) : mx_join<float, 64, false>(a, p, ws, st);
+    if (out_type == TBQ_KV_F16) return D == 128 ? mx_join<pg_f16, 128, false>(a, p, ws, st) : mx_join<pg_f16, 64, false>(a, p, ws, st);
+    return D == 128 ? mx_join<pg_bf16, 128, false>(a, p, ws, st) : mx_join<pg_bf16, 64, false>(a, p, ws, st);
 }
 
 template <typename TC, int D, bool HL>
@@ -918,7 +933,8 @@ static hipError_t pg_attn(PgAttn a, float *ws, hipStream_t st) {
                            p.row_tps, p.row_splits, ws, p.chunk_splits, part);
     }
     const hipError_t e = hipGetLastError();
-    return e != hipSuccess ? e : pg_join<TC, D, HL>(a, p, HL || a.f32_out, ws, st);
+    if (e != hipSuccess) return e;
+    return HL || a.f32_out ? pg_join<float, D, HL, false>(a, p, ws, st) : pg_join<TC, D, HL, false>(a, p, ws, st);
 }
 
 hipError_t launch_pg_attn(const PgAttn &a, int D, int q_type, int c_type, void *ws, hipStream_t st) {

@@ -118,10 +118,14 @@ struct PrLds {
 // and written (nz <= 1), or kept as split z's record of each row in part.  o[j],
 // register r of lane (li, h): row li, dims ND (4 h + r) + j; HL: rows 8 .. 15 are the lo
 // halves' shares.
-template <typename TO, int D, bool HL>
+// fix: called by every wave between its stores and the workgroup's sum (rows formed again).
+struct PgNoFix {
+    __device__ __forceinline__ void operator()() const {}
+};
+template <typename TO, int D, bool HL, typename Fix = PgNoFix>
 __device__ __forceinline__ void pg_rows_out(const PgAttn &a, pg_f4 (&o)[D / 16], float m, float l, int r0, int rows, int G,
                                             int kvh, int q0, int s, int z, int nz, int nrb, int nsplit, float *__restrict__ part,
-                                            PrLds<D> *lds) {
+                                            PrLds<D> *lds, Fix fix = Fix{}) {
     constexpr int RB = HL ? 8 : 16, ND = D / 16, OST = D + 4;
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, h = lane >> 4;
     l = swap32_sum(swap16_sum(l));
@@ -136,6 +140,7 @@ __device__ __forceinline__ void pg_rows_out(const PgAttn &a, pg_f4 (&o)[D / 16],
         lds->m[wave][li] = m;
         lds->l[wave][li] = l;
     }
+    fix();
     __syncthreads();
     for (int i = threadIdx.x; i < RB * D / 4; i += 64 * PR_WAVES) {
         const int c = i / (D / 4), d = i % (D / 4) * 4, r = r0 + c;
@@ -222,9 +227,8 @@ PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, 
 
 constexpr long long PG_WGS = (1ll << 32) / 256 - 1;   // a launch's threads along x stay below 2^32
 
-// Adds the split ranges of a launch (nothing to do where there are none): row_part
-// the few rows' records, which the others' follow.  out_type: TBQ_KV_*.
-hipError_t launch_pg_join(const PgAttn &a, int D, const PgPlan &p, bool f32, int out_type, const float *row_part,
-                          hipStream_t st);
+// Adds the split ranges of a launch over 4-bit pages (nothing to do where there are none): the few rows'
+// records in ws, the others' behind them.  out_type: TBQ_KV_*.
+hipError_t launch_mx_join(const PgAttn &a, int D, const PgPlan &p, bool f32, int out_type, const float *ws, hipStream_t st);
 
 }  // namespace tbq

@@ -18,22 +18,23 @@ namespace tbq {
 
 constexpr float MX_SH = PgVec<pg_f16>::SHIFT;   // probabilities are scaled by 2^14
 
-// One row by one wave from what it sees only, as pg_slow_row.
-template <typename TA, int D>
+// One row by one wave, 64 positions at a time, from what the row sees only, as
+// pg_slow_row; key(i): the lane's position of the i-th 64 (-1: none).  *m, *l:
+// maximum and sum; probabilities, sum and output are scaled by 2^14.
+template <typename TA, int D, typename Key>
 __device__ __forceinline__ void mx_slow_row(const PgArgs &pg, const TA *q, float cs, int s, int kvh, int pos, int back,
-                                            int sinks, PgTiles tiles, int it0, int it1, float (&o)[D / 64], float *m,
-                                            float *l) {
+                                            int sinks, int n, Key key, float (&o)[D / 64], float *m, float *l) {
     const int lane = threadIdx.x & 63, last = min(pos, pg.max_kv - 1), mask = (1 << pg.shift) - 1;
     const int codes = (D / 2) << pg.shift;
 #pragma unroll
     for (int i = 0; i < D / 64; i++) o[i] = 0.f;
     *m = PG_LOW;
     *l = 0.f;
-    for (int it = it0; it < it1; it++) {
-        const int k0 = tiles.at(it) * 64, key = k0 + lane, in = key & mask;
-        const int page = pg_block_page(pg, s, key, last);
+    for (int it = 0; it < n; it++) {
+        const int k = key(it), in = k & mask;
+        const int page = k >= 0 ? pg_block_page(pg, s, k, last) : -1;
         const uint8_t *kp = (const uint8_t *)pg.k + mx_head<D>(pg, max(page, 0), kvh);
-        const bool sees = page >= 0 && ((pg_seen(k0, pos - back, last, sinks) >> lane) & 1);
+        const bool sees = page >= 0 && k <= last && (k > pos - back || k < sinks);
         float dot = 0.f;
         for (int g = 0; g < D / 8; g++) {
             const mx_h8 y = mx_eight(*reinterpret_cast<const uint32_t *>(kp + mx_k_code<D>(in, g)),
@@ -51,14 +52,14 @@ __device__ __forceinline__ void mx_slow_row(const PgArgs &pg, const TA *q, float
 #pragma unroll
         for (int i = 0; i < D / 64; i++) o[i] *= corr;
         for (unsigned long long left = __builtin_amdgcn_ballot_w64(sees); left; left &= left - 1) {
-            const int k = __builtin_ctzll(left), kin = (k0 + k) & mask;
-            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), k));
-            const uint8_t *vp = (const uint8_t *)pg.v + mx_head<D>(pg, __builtin_amdgcn_readlane(page, k), kvh);
+            const int c = __builtin_ctzll(left), kin = __builtin_amdgcn_readlane(in, c);
+            const float w = __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, p), c));
+            const uint8_t *vp = (const uint8_t *)pg.v + mx_head<D>(pg, __builtin_amdgcn_readlane(page, c), kvh);
 #pragma unroll
             for (int i = 0; i < D / 64; i++) {
                 const int d = lane + 64 * i;
-                const uint32_t c = *reinterpret_cast<const uint32_t *>(vp + mx_v_code<D>(kin, d / 8)) >> (4 * (d % 8));
-                o[i] = fmaf(w, (float)mx_pair<0>(c, mx_scale(vp[codes + mx_v_scale<D>(kin, d / 32)]))[0], o[i]);
+                const uint32_t x = *reinterpret_cast<const uint32_t *>(vp + mx_v_code<D>(kin, d / 8)) >> (4 * (d % 8));
+                o[i] = fmaf(w, (float)mx_pair<0>(x, mx_scale(vp[codes + mx_v_scale<D>(kin, d / 32)]))[0], o[i]);
             }
         }
     }
@@ -112,10 +113,11 @@ template <int D>
 struct MxRaw {
     uint32_t kc[2][D / 32], vc[2][4], ks[2], vs[2];
     int k0;          // first position of the tile
-    uint32_t has;    // positions whose block has a page
+    uint32_t has;    // bit b: block b has a page
 };
 
-template <typename TA, int D>
+// ONCE: one row block reads the pages, so they need not stay in the caches.
+template <typename TA, int D, bool ONCE>
 __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int nsplit, float *__restrict__ part, int x, int z,
                                         int s, PrLds<D> *lds) {
     constexpr bool HL = std::is_same<TA, float>::value;
@@ -147,46 +149,55 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
                 if (li >= 8) qf[i] = lo[i];
         }
     }
-    const int hbytes = mx_row(D) << a.pg.shift, codes = (D / 2) << a.pg.shift, mask = (1 << a.pg.shift) - 1;
-    const uint32_t koff = li * (D / 2) + D / 8 * h, ksoff = li * (D / 32) + h * (D / 32) / 4;
-    const uint32_t voff = 2 * D * h + 16 * (li * ND / 8), vsoff = D / 8 * h + 4 * (li * ND / 32);
-    int pages = -1;   // lane i: the page of block i % 2 of the wave's tile i / 2 (of 32 tiles)
     const int nt = (it1 - it0 - wave + PR_WAVES - 1) / PR_WAVES;   // this wave's tiles
     auto tile_at = [&](int n) { return tiles.at(it0 + wave + PR_WAVES * n) * PR_TS; };
+    const uint32_t koff = li * (D / 2) + D / 8 * h, ksoff = li * (D / 32) + h * (D / 32) / 4;
+    const uint32_t voff = 2 * D * h + 16 * (li * ND / 8), vsoff = D / 8 * h + 4 * (li * ND / 32);
+    // lane i, of block i % 2 of the wave's tile i / 2 (of 32 tiles): bytes before its codes, from them to
+    // its scales; bit i of pages: whether it has a page
+    uint32_t off_lo = 0, off_hi = 0, to_scales = 0;
+    uint64_t pages = 0;
+    auto get = [](const auto *p) {
+        if constexpr (ONCE) return __builtin_nontemporal_load(p);
+        else return *p;
+    };
     auto load = [&](MxRaw<D> &w, int n) {
         if ((n & 31) == 0) {
-            const int k = n + (lane >> 1);
-            pages = k < nt ? pg_block_page(a.pg, s, tile_at(k) + 16 * (lane & 1), last) : -1;
+            const int k = n + (lane >> 1), p = tile_at(k) + 16 * (lane & 1), in = p & ((1 << a.pg.shift) - 1);
+            const int page = k < nt ? pg_block_page(a.pg, s, p, last) : -1;
+            const long long off = mx_head<D>(a.pg, max(page, 0), kvh) + in * (D / 2);
+            pages = __builtin_amdgcn_ballot_w64(page >= 0);
+            off_lo = (uint32_t)off;
+            off_hi = (uint32_t)(off >> 32);
+            to_scales = ((D / 2) << a.pg.shift) - in * (D / 2 - D / 32);
         }
         w.k0 = tile_at(n);
-        w.has = 0;
+        w.has = (uint32_t)(pages >> (2 * (n & 31))) & 3;
 #pragma unroll
         for (int b = 0; b < 2; b++) {
-            const int page = __builtin_amdgcn_readlane(pages, 2 * (n & 31) + b), in = (w.k0 + 16 * b) & mask;
-            w.has |= page >= 0 ? 0xFFFFu << (16 * b) : 0u;
-            const long long off = ((long long)max(page, 0) * a.pg.NKV + kvh) * hbytes;
+            const int at = 2 * (n & 31) + b;
+            const long long off = (long long)((uint64_t)(uint32_t)__builtin_amdgcn_readlane((int)off_hi, at) << 32 |
+                                              (uint32_t)__builtin_amdgcn_readlane((int)off_lo, at));
+            const uint32_t sc = __builtin_amdgcn_readlane((int)to_scales, at);
             const uint8_t *kp = (const uint8_t *)a.pg.k + off, *vp = (const uint8_t *)a.pg.v + off;
-            const kvec kc = *reinterpret_cast<const kvec *>(kp + in * (D / 2) + koff);
+            const kvec kc = get(reinterpret_cast<const kvec *>(kp + koff));
 #pragma unroll
             for (int i = 0; i < NS; i++) w.kc[b][i] = kc[i];
-            const pg_u4 vc = *reinterpret_cast<const pg_u4 *>(vp + in * (D / 2) + voff);
+            const pg_u4 vc = get(reinterpret_cast<const pg_u4 *>(vp + voff));
 #pragma unroll
             for (int i = 0; i < 4; i++) w.vc[b][i] = vc[i];
-            w.ks[b] = kp[codes + in * (D / 32) + ksoff];
-            w.vs[b] = *reinterpret_cast<const uint32_t *>(vp + codes + in * (D / 32) + vsoff);
+            w.ks[b] = (kp + sc)[ksoff];
+            w.vs[b] = *reinterpret_cast<const uint32_t *>(vp + sc + vsoff);
         }
     };
     pg_f4 o[ND];
-    float m, l;
-    auto compute = [&](MxRaw<D> &w, bool safe) {
+    float m = PG_LOW, l = 0.f;
+#pragma unroll
+    for (int j = 0; j < ND; j++) o[j] = pg_f4{};
+    auto compute = [&](MxRaw<D> &w) {
         const int k0 = w.k0;
-        const bool whole = w.has == 0xFFFFFFFFu && k0 + PR_TS - 1 <= min(plo, a.pg.max_kv - 1) &&
+        const bool whole = w.has == 3 && k0 + PR_TS - 1 <= min(plo, a.pg.max_kv - 1) &&
                            (k0 > phi - back || k0 + PR_TS <= a.sinks);
-        // the lane's positions that tokens at lo .. hi see: element e is bit 16 (e / 4) + e % 4
-        auto seen = [&](int lo, int hi) {
-            return ((uint32_t)pg_seen(k0, lo - back, min(hi, last), a.sinks) & w.has) >> (4 * h);
-        };
-        auto bit = [](int e) { return 16 * (e / 4) + e % 4; };
         pg_f4 sc[2] = {pg_f4{}, pg_f4{}};
 #pragma unroll
         for (int b = 0; b < 2; b++)
@@ -199,9 +210,21 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
                 for (int r = 0; r < 4; r++) sc[b][r] += dpp_f32<0x128>(sc[b][r]);   // row_ror:8
         }
         if (!whole) {
-            const uint32_t mine = seen(pos, pos);
+            // the lane's positions that tokens at lo .. hi see: element e is bit 16 (e / 4) + e % 4
+            const uint32_t has = (w.has & 1 ? 0xFFFFu : 0u) | (w.has & 2 ? 0xFFFF0000u : 0u);
+            auto seen = [&](int lo, int hi) {
+                return ((uint32_t)pg_seen(k0, lo - back, min(hi, last), a.sinks) & has) >> (4 * h);
+            };
+            const uint32_t mine = seen(pos, pos), any = seen(plo, phi);
 #pragma unroll
-            for (int e = 0; e < 8; e++) sc[e / 4][e % 4] = pg_hide(sc[e / 4][e % 4], pg_ones(mine, bit(e)));
+            for (int e = 0; e < 8; e++) {
+                const int bit = 16 * (e / 4) + e % 4;
+                sc[e / 4][e % 4] = pg_hide(sc[e / 4][e % 4], pg_ones(mine, bit));
+                // values that no row of the block sees are 0 (under whatever scale but NaN)
+                const uint32_t on = pg_ones(any, bit);
+                w.vc[e / 4][e % 4] &= on;
+                w.vs[e / 4] &= on | ~(0xFFu << (8 * (e % 4)));
+            }
         }
         float mx = sc[0][0];
 #pragma unroll
@@ -214,100 +237,88 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
 #pragma unroll
             for (int j = 0; j < ND; j++) o[j] *= corr;
         }
-        mx_h8 pf, pl;   // (fp32 rows' lo halves are columns of their own)
+        mx_h8 pf;   // (fp32 rows' lo halves are columns of their own)
         const float mb = MX_SH - m;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][e % 4], cs, mb));
             l += p;
-            const pg_f16 hi = (pg_f16)p, lo = (pg_f16)(p - (float)hi);
-            if constexpr (HL) pf[e] = li < 8 ? hi : lo;
-            else {
-                pf[e] = hi;
-                pl[e] = lo;
-            }
+            const pg_f16 hi = (pg_f16)p;
+            if constexpr (HL) pf[e] = li < 8 ? hi : (pg_f16)(p - (float)hi);
+            else pf[e] = hi;
         }
-        uint32_t vc[8];
-        float vs[8];
-        auto values = [&](uint32_t ones) {   // those of hidden positions are 0
+        auto two = [&](auto S) {   // dims 2 S and 2 S + 1 of the lane's ND
+            constexpr int I = decltype(S)::value;
+            mx_h8 va, vb;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
-                const uint32_t on = pg_ones(ones, bit(e));
-                vc[e] = (w.vc[e / 4][e % 4] >> (D == 64 ? 16 * (li & 1) : 0)) & on;
-                vs[e] = __builtin_bit_cast(float, (((w.vs[e / 4] >> (8 * (e % 4))) & 0xFFu) << 23) & on);
+                const uint32_t c = w.vc[e / 4][e % 4] >> (D == 64 ? 16 * (li & 1) : 0);
+                const mx_h2 y = mx_pair<I>(c, mx_scale((w.vs[e / 4] >> (8 * (e % 4))) & 0xFFu));
+                va[e] = y[0];
+                vb[e] = y[1];
             }
+            o[2 * I] = pg_mfma16(va, pf, o[2 * I]);
+            o[2 * I + 1] = pg_mfma16(vb, pf, o[2 * I + 1]);
         };
-        auto products = [&](pg_f4 (&u)[ND]) {
-            auto two = [&](auto S) {
-                constexpr int I = decltype(S)::value;
-                mx_h8 va, vb;
-#pragma unroll
-                for (int e = 0; e < 8; e++) {
-                    const mx_h2 y = mx_pair<I>(vc[e], vs[e]);
-                    va[e] = y[0];
-                    vb[e] = y[1];
-                }
-                u[2 * I] = pg_mfma16(va, pf, u[2 * I]);
-                u[2 * I + 1] = pg_mfma16(vb, pf, u[2 * I + 1]);
-                if constexpr (!HL) {
-                    u[2 * I] = pg_mfma16(va, pl, u[2 * I]);
-                    u[2 * I + 1] = pg_mfma16(vb, pl, u[2 * I + 1]);
-                }
-            };
-            two(std::integral_constant<int, 0>{});
-            two(std::integral_constant<int, 1>{});
-            if constexpr (ND == 8) {
-                two(std::integral_constant<int, 2>{});
-                two(std::integral_constant<int, 3>{});
-            }
-        };
-        if (whole || !safe) {
-            values(whole ? ~0u : seen(plo, phi));
-            products(o);
-        } else {
-            for (int t = t0; t <= t1; t++) {
-                values(seen(base + t, base + t));
-                pg_f4 u[ND];
-#pragma unroll
-                for (int j = 0; j < ND; j++) u[j] = o[j];
-                products(u);
-#pragma unroll
-                for (int j = 0; j < ND; j++)
-                    if (tok == t) o[j] = u[j];
-            }
+        two(std::integral_constant<int, 0>{});
+        two(std::integral_constant<int, 1>{});
+        if constexpr (ND == 8) {
+            two(std::integral_constant<int, 2>{});
+            two(std::integral_constant<int, 3>{});
         }
     };
-    for (int safe = 0;; safe = 1) {
-        m = PG_LOW;
-        l = 0.f;
-#pragma unroll
-        for (int j = 0; j < ND; j++) o[j] = pg_f4{};
-        MxRaw<D> w[3];
-        if (nt > 0) load(w[0], 0);
-        if (nt > 1) load(w[1], 1);
-        for (int n = 0; n < nt; n += 3) {
-            if (n + 2 < nt) load(w[2], n + 2);
-            compute(w[0], safe);
+    if (nt > 0) {
+        // (a last load is of a tile that was there already: as many loads are in flight on every way to a
+        // product, or the compiler would wait for all of them)
+        MxRaw<D> w[2];
+        load(w[0], 0);
+        for (int n = 0;; n += 2) {
+            load(w[1], min(n + 1, nt - 1));
+            compute(w[0]);
             if (n + 1 >= nt) break;
-            if (n + 3 < nt) load(w[0], n + 3);
-            compute(w[1], safe);
+            load(w[0], min(n + 2, nt - 1));
+            compute(w[1]);
             if (n + 2 >= nt) break;
-            if (n + 4 < nt) load(w[1], n + 4);
-            compute(w[2], safe);
         }
-        float sum = 0.f;
-#pragma unroll
-        for (int j = 0; j < ND; j++) sum += (o[j][0] - o[j][0]) + (o[j][1] - o[j][1]) + (o[j][2] - o[j][2]) + (o[j][3] - o[j][3]);
-        if (safe || !__builtin_amdgcn_ballot_w64(row < rows && sum != 0.f)) break;   // no NaN or infinity
     }
-    pg_rows_out<TA, D, HL>(a, o, m, l, r0, rows, G, kvh, q0, s, z, nz, nrb, nsplit, part, lds);
+    // rows with an output that is not finite are formed again, one at a time
+    float odd = 0.f;   // NaN where an output is NaN or infinite
+#pragma unroll
+    for (int j = 0; j < ND; j++) odd += (o[j][0] - o[j][0]) + (o[j][1] - o[j][1]) + (o[j][2] - o[j][2]) + (o[j][3] - o[j][3]);
+    const bool again = row < rows && !(odd == 0.f);
+    pg_rows_out<TA, D, HL>(a, o, m, l, r0, rows, G, kvh, q0, s, z, nz, nrb, nsplit, part, lds, [&] {
+        uint64_t left = __builtin_amdgcn_ballot_w64(again);   // lane bits: a row's are li (HL: and li + 8) of each 16
+        left |= left >> 32;
+        left |= left >> 16;
+        left = (HL ? left | left >> 8 : left) & (HL ? 0xFF : 0xFFFF);
+        for (; left; left &= left - 1) {
+            const int c = __builtin_ctzll(left), r = r0 + c, t = r / G;
+            float so[D / 64], sm, sl;
+            mx_slow_row<TA, D>(a.pg, (const TA *)a.q + (long long)(q0 + t) * a.qs + (long long)(kvh * G + r % G) * D, a.scale,
+                               s, kvh, base + t, back, a.sinks, (nt + 1) / 2,
+                               [&](int i) {
+                                   const int n = 2 * i + (lane >> 5);
+                                   return n < nt ? tile_at(n) + (lane & 31) : -1;
+                               },
+                               so, &sm, &sl);
+#pragma unroll
+            for (int i = 0; i < D / 64; i++) {
+                lds->o[wave][c * (D + 4) + lane + 64 * i] = so[i];
+                if constexpr (HL) lds->o[wave][(c + 8) * (D + 4) + lane + 64 * i] = 0.f;
+            }
+            if (lane == 0) {
+                lds->m[wave][c] = sm;
+                lds->l[wave][c] = sl;
+            }
+        }
+    });
 }
 
-template <typename TA, int D>
-__global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(2, 2))) void k_mx_attn_rows(
+template <typename TA, int D, bool ONCE>
+__global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(3, 3))) void k_mx_attn_rows(
     const PgAttn a, int nrb, int tps, int nsplit, float *__restrict__ part) {
     __shared__ __attribute__((aligned(16))) PrLds<D> lds;
-    mx_rows<TA, D>(a, nrb, tps, nsplit, part, blockIdx.x, blockIdx.y, blockIdx.z, &lds);
+    mx_rows<TA, D, ONCE>(a, nrb, tps, nsplit, part, blockIdx.x, blockIdx.y, blockIdx.z, &lds);
 }
 
 // ---------------------------------------------------------------------------
@@ -536,7 +547,8 @@ __device__ __forceinline__ void mx_chunk(const PgAttn &a, int nsplit, float *__r
         const int c = __builtin_ctzll(left), r = r0 + wave * 32 + c, t = r / G;
         float so[D / 64], sm, sl;
         mx_slow_row<TA, D>(a.pg, (const TA *)a.q + (long long)(q0 + t) * a.qs + (long long)(kvh * G + r % G) * D, a.scale, s,
-                           kvh, base + t, back, a.sinks, tiles, it0, it1, so, &sm, &sl);
+                           kvh, base + t, back, a.sinks, it1 - it0,
+                           [&](int i) { return tiles.at(it0 + i) * PC_TS + lane; }, so, &sm, &sl);
         const long long to = (long long)(q0 + t) * a.NQ + kvh * G + r % G;
         float *rec = part + (to * nsplit + z) * pg_rec(D);
 #pragma unroll
@@ -579,7 +591,7 @@ __global__ __launch_bounds__(64 * PC_WAVES)
     const int nrows = a.pg.NKV * nrb, chunks = (int)gridDim.x - nrows * row_splits * a.pg.n_seqs, x = blockIdx.x;
     if (x >= chunks) {
         const int y = (x - chunks) / nrows;
-        mx_rows<TA, D>(a, nrb, tps, row_splits, row_part, (x - chunks) % nrows, y % row_splits, y / row_splits,
+        mx_rows<TA, D, false>(a, nrb, tps, row_splits, row_part, (x - chunks) % nrows, y % row_splits, y / row_splits,
                        reinterpret_cast<PrLds<D> *>(mx_lds));
     } else {
         const int y = x / a.pg.NKV;
@@ -596,7 +608,12 @@ static hipError_t mx_attn(PgAttn a, int out_type, float *ws, hipStream_t st) {
     float *part = ws + p.rows_bytes / 4;
     if (!p.chunks) {
         const dim3 grid(a.pg.NKV * p.nrb, p.row_splits, a.pg.n_seqs);
-        hipLaunchKernelGGL((k_mx_attn_rows<TA, D>), grid, dim3(64 * PR_WAVES), 0, st, a, p.nrb, p.row_tps, p.row_splits, ws);
+        if (p.nrb == 1)
+            hipLaunchKernelGGL((k_mx_attn_rows<TA, D, true>), grid, dim3(64 * PR_WAVES), 0, st, a, p.nrb, p.row_tps,
+                               p.row_splits, ws);
+        else
+            hipLaunchKernelGGL((k_mx_attn_rows<TA, D, false>), grid, dim3(64 * PR_WAVES), 0, st, a, p.nrb, p.row_tps,
+                               p.row_splits, ws);
     } else {
         constexpr int lds = std::max(sizeof(McLds<D>), sizeof(PrLds<D>));
         static_assert(lds <= 65536, "what a launch may ask for without an attribute of the kernel");
@@ -607,7 +624,7 @@ static hipError_t mx_attn(PgAttn a, int out_type, float *ws, hipStream_t st) {
                            p.row_splits, ws, p.chunk_splits, part);
     }
     const hipError_t e = hipGetLastError();
-    return e != hipSuccess ? e : launch_pg_join(a, D, p, HL, a.f32_out ? TBQ_KV_F32 : out_type, ws, st);
+    return e != hipSuccess ? e : launch_mx_join(a, D, p, HL, a.f32_out ? TBQ_KV_F32 : out_type, ws, st);
 }
 
 hipError_t launch_mx_attn(const PgAttn &a, int D, int q_type, void *ws, hipStream_t st) {

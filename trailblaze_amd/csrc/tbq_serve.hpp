@@ -21,7 +21,9 @@ struct SvVerify {
     const float *temperature, *u_accept, *u_next;
     int *n_accept, *next, *n_drop;
 };
-constexpr int DV_CHUNK = 8192;           // elements of a row that a workgroup takes at a time
+// Elements of a row that a workgroup takes at a time: the longer ones where there are many.
+constexpr int DV_SHORT = 2048, DV_LONG = 8192;
+int verify_chunk(int n_rows, int vocab, bool draft);
 size_t verify_workspace_bytes(int n_seqs, int n_rows, int vocab, bool draft);
 hipError_t launch_verify(const SvVerify &a, int type, void *ws, hipStream_t st);
 

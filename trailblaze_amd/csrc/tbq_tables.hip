@@ -10,34 +10,52 @@
 
 namespace tbq {
 
-constexpr int TB_THREADS = 1024;
+constexpr int TB_THREADS = 1024, TB_WAVES = TB_THREADS / 64;
 struct TbLds {
-    long long wave[TB_THREADS / 64];
+    int3 wave[2][TB_WAVES];                   // sums of the waves' sequences (by turns)
+    int count[2][TB_WAVES];
     int end[TB_THREADS], first[TB_THREADS];   // inclusive sums of a chunk's entries; each sequence's first entry
-    int fail;
-    long long take, tokens;
+    int fail, take, tokens;
 };
 
-// Inclusive sum over the workgroup, and the whole one.
-__device__ __forceinline__ long long tb_scan(long long v, TbLds *lds, long long *total) {
+constexpr int TB_MOST = 1 << 30;   // tokens of a call; sums of them stop behind it
+__device__ __forceinline__ int3 tb_add(int3 a, int3 b) {
+    return make_int3(a.x + b.x, a.y + b.y, (int)min((unsigned)a.z + (unsigned)b.z, (unsigned)TB_MOST + 1u));
+}
+// Inclusive sums over the workgroup of pages given, pages taken (below 2^31: a table has no more entries)
+// and tokens; and the whole ones.  One barrier; turn: 0 and 1 by turns.
+__device__ __forceinline__ int3 tb_scan(int3 v, TbLds *lds, int turn, int3 *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
-        const long long o = __shfl_up(v, d);
-        if (lane >= d) v += o;
+        const int3 o = make_int3(__shfl_up(v.x, d), __shfl_up(v.y, d), __shfl_up(v.z, d));
+        if (lane >= d) v = tb_add(v, o);
     }
+    if (lane == 63) lds->wave[turn][wave] = v;
     __syncthreads();
-    if (lane == 63) lds->wave[wave] = v;
-    __syncthreads();
-    long long before = 0, all = 0;
+    int3 before = make_int3(0, 0, 0), all = before;
 #pragma unroll
-    for (int w = 0; w < TB_THREADS / 64; w++) {
-        const long long x = lds->wave[w];
-        before += w < wave ? x : 0;
-        all += x;
+    for (int w = 0; w < TB_WAVES; w++) {
+        if (w == wave) before = all;
+        all = tb_add(all, lds->wave[turn][w]);
     }
     *total = all;
-    return before + v;
+    return tb_add(before, v);
+}
+// How many threads up to this one say yes, and how many do.
+__device__ __forceinline__ int tb_count(bool yes, TbLds *lds, int turn, int *total) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t b = __builtin_amdgcn_ballot_w64(yes);
+    if (lane == 0) lds->count[turn][wave] = __builtin_popcountll(b);
+    __syncthreads();
+    int before = 0, all = 0;
+#pragma unroll
+    for (int w = 0; w < TB_WAVES; w++) {
+        if (w == wave) before = all;
+        all += lds->count[turn][w];
+    }
+    *total = all;
+    return before + __builtin_popcountll(b & (lane == 63 ? ~0ull : (2ull << lane) - 1));
 }
 
 // The sequence of a chunk that entry j belongs to: the first whose end is above j.
@@ -51,89 +69,92 @@ __device__ __forceinline__ int tb_find(const TbLds *lds, int n, int j) {
     return lo;
 }
 
-// Sequence s before the call: positions kept and held, pages of both, new tokens.
+// Sequence s before the call: positions kept, pages of them and of all, new tokens; the pages it needs
+// then (-1: more than the table has).
 struct TbSeq {
-    int base, held, kept, add;
+    int base, held, kept, add, need;
 };
-__device__ __forceinline__ TbSeq tb_seq(const SvTables &a, int s) {
+__device__ __forceinline__ TbSeq tb_seq(const SvTables &a, int s, bool there) {
+    if (!there) return {0, 0, 0, 0, 0};
     const int round = (1 << a.shift) - 1, room = a.t.max_pages << a.shift;
     const int len = min(max(a.t.kv_len[s], 0), room);
-    const int drop = a.t.n_drop ? min(max(a.t.n_drop[s], 0), len) : 0;
-    return {len - drop, (len + round) >> a.shift, (len - drop + round) >> a.shift, max(a.t.n_new[s], 0)};
+    const int drop = a.t.n_drop ? min(max(a.t.n_drop[s], 0), len) : 0, add = max(a.t.n_new[s], 0), base = len - drop;
+    return {base, (len + round) >> a.shift, (base + round) >> a.shift, min(add, TB_MOST + 1),
+            add > room - base ? -1 : (base + add + round) >> a.shift};
+}
+__device__ __forceinline__ int3 tb_sums(const TbSeq &q) {
+    return make_int3(q.held - q.kept, q.need < 0 ? 0 : q.need - q.kept, q.add);
 }
 
 __global__ __launch_bounds__(TB_THREADS) void k_tables_plan(const SvTables a) {
     __shared__ TbLds lds;
     const tbq_kv_tables &t = a.t;
     const int tid = threadIdx.x, listed = min(max(t.n_free[0], 0), t.n_pages);
-    long long total;
+    TbSeq q{};
+    int3 sum{}, all{};
     // pages behind the last kept position go to the list, in the sequences' order
-    int have = listed;
+    int have = listed, turn = 0;
     for (int s0 = 0; s0 < t.n_seqs; s0 += TB_THREADS) {
         const int n = min(TB_THREADS, t.n_seqs - s0);
-        const TbSeq q = tid < n ? tb_seq(a, s0 + tid) : TbSeq{0, 0, 0, 0};
-        const int end = (int)tb_scan(q.held - q.kept, &lds, &total);   // (sums of entries stay below 2^31: the table has no more)
-        lds.end[tid] = end;
-        lds.first[tid] = q.kept - (end - (q.held - q.kept));
+        q = tb_seq(a, s0 + tid, tid < n);
+        sum = tb_scan(tb_sums(q), &lds, turn ^= 1, &all);
+        if (all.x == 0) continue;   // uniform
+        lds.end[tid] = sum.x;
+        lds.first[tid] = q.kept - (sum.x - (q.held - q.kept));
         __syncthreads();
-        const int back = (int)total;
-        for (int j0 = 0; j0 < back; j0 += TB_THREADS) {
+        for (int j0 = 0; j0 < all.x; j0 += TB_THREADS) {
             const int j = j0 + tid;
-            int page = -1;
-            if (j < back) {
+            int page = -1, count;
+            if (j < all.x) {
                 const int i = tb_find(&lds, n, j);
                 page = t.page_table[(long long)(s0 + i) * t.max_pages + lds.first[i] + j];
             }
             const bool is = (unsigned)page < (unsigned)t.n_pages;
-            const int at = have + (int)tb_scan(is, &lds, &total) - 1;
+            const int at = have + tb_count(is, &lds, turn ^= 1, &count) - 1;
             if (is && at < t.n_pages) t.free_out[at] = page;
-            have = min(have + (int)total, t.n_pages);
+            have = min(have + count, t.n_pages);
         }
-        __syncthreads();
     }
     __threadfence_block();
-    __syncthreads();
     // then sequences take pages from its end, until one does not get what it needs
     long long taken = 0, rows = 0;
     int served = 0;
     bool going = true;
     for (int s0 = 0; s0 < t.n_seqs; s0 += TB_THREADS) {
         const int n = min(TB_THREADS, t.n_seqs - s0);
-        const TbSeq q = tid < n ? tb_seq(a, s0 + tid) : TbSeq{0, 0, 0, 0};
-        const long long len = (long long)q.base + q.add, need = (len + (1 << a.shift) - 1) >> a.shift;
-        const bool fits = need <= t.max_pages;
-        const int take = fits ? (int)need - q.kept : 0;
-        long long all_take, all_rows;
-        const long long end = tb_scan(take, &lds, &all_take), end_rows = tb_scan(q.add, &lds, &all_rows);
+        if (t.n_seqs > TB_THREADS) {
+            q = tb_seq(a, s0 + tid, tid < n);
+            sum = tb_scan(tb_sums(q), &lds, turn ^= 1, &all);
+        }
         if (tid == 0) lds.fail = n;
         __syncthreads();
-        if (tid < n && (!going || !fits || taken + end > have || rows + end_rows > t.n_tokens)) atomicMin(&lds.fail, tid);
+        if (tid < n && (!going || q.need < 0 || taken + sum.y > have || rows + sum.z > t.n_tokens)) atomicMin(&lds.fail, tid);
         __syncthreads();
-        const int fail = lds.fail;
-        if (tid == fail) {
-            lds.take = end - take;
-            lds.tokens = end_rows - q.add;
-        }
-        lds.end[tid] = tid < fail ? (int)end : 0x7FFFFFFF;
-        lds.first[tid] = q.kept - (int)(end - take);
+        const int fail = lds.fail, take = q.need < 0 ? 0 : q.need - q.kept;
+        if (tid == fail) lds.take = sum.y - take;
+        // (the tokens before the first that fails are its predecessor's sum: its own may have stopped)
+        if (tid + 1 == fail) lds.tokens = sum.z;
+        lds.end[tid] = tid < fail ? sum.y : 0x7FFFFFFF;
+        lds.first[tid] = q.kept - (sum.y - take);
         __syncthreads();
+        int all_take = all.y, all_rows = all.z;
         if (fail < n) {
             all_take = lds.take;
-            all_rows = lds.tokens;
+            all_rows = fail == 0 ? 0 : lds.tokens;
         }
         if (tid < n) {
             t.kv_len_out[s0 + tid] = q.base + (tid < fail ? q.add : 0);
-            t.q_start[s0 + tid + 1] = (int)(rows + (tid < fail ? end_rows : all_rows));
+            t.q_start[s0 + tid + 1] = (int)(rows + (tid < fail ? sum.z : all_rows));
         }
-        for (int j = tid; j < (int)all_take; j += TB_THREADS) {
+        for (int j = tid; j < all_take; j += TB_THREADS) {
             const int i = tb_find(&lds, n, j), at = have - 1 - (int)taken - j;
-            t.page_table_out[(long long)(s0 + i) * t.max_pages + lds.first[i] + j] = at < listed ? t.free_pages[at] : t.free_out[at];
+            t.page_table_out[(long long)(s0 + i) * t.max_pages + lds.first[i] + j] =
+                at < listed ? t.free_pages[at] : t.free_out[at];
         }
         taken += all_take;
         rows += all_rows;
         served += fail;
         going = going && fail == n;
-        __syncthreads();
     }
     if (tid == 0) {
         t.q_start[0] = 0;
