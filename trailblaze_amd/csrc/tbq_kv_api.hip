@@ -325,7 +325,7 @@ static int check_verify(const char *who, int n_seqs, int n_rows, int vocab, int 
         return fail("%s: %d sequences, %d rows of %d", who, n_seqs, n_rows, vocab);
     if (!float_type(type)) return fail("%s: type %d (F32, F16 or BF16)", who, type);
     // a workgroup of 256 a chunk: their threads stay below 2^32
-    const long long ch = verify_chunk(n_rows, vocab, draft), chunks = (vocab + ch - 1) / ch;
+    const long long chunks = (vocab + DV_CHUNK - 1) / DV_CHUNK;
     if (chunks * (n_rows > n_seqs ? n_rows : n_seqs) * (draft ? 2 : 1) > (1 << 24) - 1)
         return fail("%s: %d rows of %d", who, n_rows, vocab);
     return 1;
@@ -356,6 +356,7 @@ int tbq_draft_verify(int n_seqs, int n_rows, int vocab, int type, const int *q_s
     a.n_seqs = n_seqs;
     a.n_rows = n_rows;
     a.vocab = vocab;
+    a.chunks = (vocab + DV_CHUNK - 1) / DV_CHUNK;
     a.q_start = q_start;
     a.tokens = tokens;
     a.logits = logits;

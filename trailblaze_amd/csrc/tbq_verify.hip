@@ -16,7 +16,8 @@
 
 namespace tbq {
 
-constexpr int DV_THREADS = 256, DV_PICK = 1024;
+constexpr int DV_THREADS = 256, DV_CHOOSE = 1024, DV_PICK = 512;
+
 
 struct DvRec {      // of a chunk of a row: the largest logit, where first, and the sum of the weights 2^(k (l - m))
     float m;
@@ -25,29 +26,40 @@ struct DvRec {      // of a chunk of a row: the largest logit, where first, and 
 };
 typedef DvRec DvRow;   // of a row: the same
 
-// 2^t for t <= 0: t = k + r, |r| <= 1/2, and the series of 2^r up to the term in which the next
-// one, (ln 2 / 2)^12 / 12!, is below 2^-47 of the whole; a NaN gives 0.  (The library's exp takes twice as
-// long: 218 + 154 rows of 151936 113 us, 5x with this one.)
-__device__ __forceinline__ double dv_exp2(double t) {
-    t = fmax(t, -1100.);
-    const double k = __builtin_rint(t), r = t - k;
-    double p = 4.4455382718708116e-10;   // (ln 2)^11 / 11!
-    p = fma(p, r, 7.0549116208011234e-9);
-    p = fma(p, r, 1.0178086009239699e-7);
-    p = fma(p, r, 1.3215486790144309e-6);
-    p = fma(p, r, 1.5252733804059841e-5);
-    p = fma(p, r, 1.5403530393381609e-4);
-    p = fma(p, r, 1.3333558146428443e-3);
-    p = fma(p, r, 9.6181291076284772e-3);
-    p = fma(p, r, 5.5504108664821580e-2);
-    p = fma(p, r, 2.4022650695910071e-1);
-    p = fma(p, r, 6.9314718055994531e-1);
-    return ldexp(fma(p, r, 1.), (int)k);
+// The weights exp((l - m) / T) of a row whose largest logit is m, by k = log2(e) / T: 2^t, t = k (l - m).
+// t is split into the nearest whole number, which adding 1.5 * 2^52 leaves in the low bits, and r, |r| <= 1/2;
+// 2^r is the polynomial of degree 8 that meets it at the nine Chebyshev points, off by 1.1e-12 of it at most; the
+// whole number goes to the exponent.  Logits from low on have no weight (2^-1000 of the largest, -infinity, NaN);
+// where m is infinite, all below it; k is 0 where only m itself has weight.  With Least set, they have up to 2^-999, for sums alone (k > 0).
+// (218 + 154 rows of 151936: 113 us with the library's exp, NN with this.)
+struct DvLaw {
+    double k, m;
+    float low;
+};
+__device__ __forceinline__ DvLaw dv_law(float m, double k) {
+    const float most = 3.402823466e38f;
+    if (!(m <= most)) return {0., most, most};
+    const double x = (double)m - 1000. / k;
+    float low = (float)fmax(x, -(double)most);
+    if ((double)low < x) low = nextafterf(low, most);   // (not below x)
+    // where that leaves no float below m, m alone has weight
+    return low < m ? DvLaw{k, m, low} : DvLaw{0., m, nextafterf(m, -__builtin_huge_valf())};
 }
-// The weight exp((l - m) / T) for l <= m, k = log2(e) / T: 1 for the largest itself (also where it is infinite), 0 for
-// -infinity and NaN.
-__device__ __forceinline__ double dv_weight(float l, float m, double k) {
-    return l == m ? 1. : dv_exp2(((double)l - (double)m) * k);
+template <bool Least = false>
+__device__ __forceinline__ double dv_weight(const DvLaw &w, float l) {
+    const double t = ((double)__builtin_amdgcn_fmed3f(l, w.low, 3.402823466e38f) - w.m) * w.k, magic = 6755399441055744.;
+    const double n = t + magic, r = t - (n - magic);
+    double p = 1.3255179556479267e-6;
+    p = fma(p, r, 1.5310080611926545e-5);
+    p = fma(p, r, 1.5403456082633648e-4);
+    p = fma(p, r, 1.3333450563173552e-3);
+    p = fma(p, r, 9.618129159053034e-3);
+    p = fma(p, r, 5.5504109412108156e-2);
+    p = fma(p, r, 2.4022650695814518e-1);
+    p = fma(p, r, 6.931471805459332e-1);
+    p = fma(p, r, 1.);
+    const uint64_t b = __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, n) << 52);
+    return Least || l > w.low ? __builtin_bit_cast(double, b) : 0.;
 }
 
 __device__ __forceinline__ double dv_sum64(double v) {
@@ -82,20 +94,21 @@ __device__ __forceinline__ double dv_random(float u) { return fminf(fmaxf(u, 0.f
 // log2(e) over the temperature; 0: all weight on the largest logit.
 __device__ __forceinline__ double dv_rate(const SvVerify &a, int s) {
     const double t = a.temperature ? a.temperature[s] : 1.;
-    return t > 0. ? fmax(1.4426950408889634 / t, 1e-300) : 0.;
+    return t > 0. ? fmax(1.4426950408889634 / t, 1e-34) : 0.;   // (1e-34 of any two finite ones is alike)
 }
 
 // Block x: chunk, row, and (draft) whose logits.  Bound by HBM and the exponentials' fp64.
-template <typename T, int CH>
-__global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec *__restrict__ rec) {
-    constexpr int N = CH / DV_THREADS < 16 / (int)sizeof(T) ? CH / DV_THREADS : 16 / sizeof(T), R = CH / DV_THREADS / N;
+template <typename T>
+__global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec *__restrict__ rec,
+                                                         float *__restrict__ drafted) {
+    constexpr int N = 16 / sizeof(T), R = DV_CHUNK / DV_THREADS / N;
     __shared__ float ms[DV_THREADS / 64];
     __shared__ int at[DV_THREADS / 64];
     __shared__ double sums[DV_THREADS / 64];
     const int c = blockIdx.x % a.chunks, r = blockIdx.x / a.chunks % a.n_rows, which = blockIdx.x / a.chunks / a.n_rows;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *row = (const T *)(which ? a.draft : a.logits) + r * (which ? a.dstride : a.stride);
-    const int v0 = c * CH + (int)threadIdx.x * N;
+    const int v0 = c * DV_CHUNK + (int)threadIdx.x * N;
     float x[R][N];
 #pragma unroll
     for (int i = 0; i < R; i++) dv_load(row, v0 + i * DV_THREADS * N, a.vocab, x[i]);
@@ -124,10 +137,18 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) first = min(first, __shfl_xor(first, d));
     } else if (m > -__builtin_huge_valf()) {
+        const DvLaw law = dv_law(m, k);
+        if (law.k > 0.) {   // uniform
 #pragma unroll
-        for (int i = 0; i < R; i++)
+            for (int i = 0; i < R; i++)
 #pragma unroll
-            for (int e = 0; e < N; e++) sum += dv_weight(x[i][e], m, k);
+                for (int e = 0; e < N; e++) sum += dv_weight<true>(law, x[i][e]);
+        } else {
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int e = 0; e < N; e++) sum += x[i][e] == m ? 1. : 0.;
+        }
         sum = dv_sum64(sum);
     }
     if (lane == 0) {
@@ -144,6 +165,11 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
         }
         rec[((long long)which * a.n_rows + r) * a.chunks + c] = {m, first, sum};
     }
+    // the judged draft's logit, for the choice
+    if (threadIdx.x == 64 && r + 1 < q0 + n) {
+        const int v = a.tokens[r + 1];
+        if ((unsigned)v < (unsigned)a.vocab && v / DV_CHUNK == c) drafted[(long long)which * a.n_rows + r] = (float)row[v];
+    }
 }
 
 // A row's records as one, by a wave.
@@ -152,11 +178,12 @@ __device__ __forceinline__ DvRow dv_row(const DvRec *rec, int chunks, double k) 
     float m = -__builtin_huge_valf();
     for (int c = lane; c < chunks; c += 64) m = fmaxf(m, rec[c].m);
     m = wave_max(m);
+    const DvLaw law = dv_law(m, k);
     int at = 0x7FFFFFFF;
     double sum = 0.;
     for (int c = lane; c < chunks; c += 64) {
         const DvRec x = rec[c];
-        if (k > 0.) sum += x.sum * dv_weight(x.m, m, k);
+        if (k > 0.) sum += x.sum * dv_weight(law, x.m);
         else if (x.m == m) at = min(at, x.at);
     }
     if (k > 0.) return {m, -1, dv_sum64(sum)};
@@ -177,84 +204,77 @@ struct DvChoice {
 // The probability of token x where its row's logit is l.
 __device__ __forceinline__ double dv_prob(const DvRow &r, float l, int x, double k) {
     if (!(k > 0.)) return x == r.at && r.m > -__builtin_huge_valf() ? 1. : 0.;
-    return r.sum > 0. ? dv_weight(l, r.m, k) / r.sum : 0.;
+    return r.sum > 0. ? dv_weight(dv_law(r.m, k), l) / r.sum : 0.;
 }
-template <typename T>
-__device__ __forceinline__ float dv_logit(const void *base, long long stride, int r, int x) {
-    return (float)((const T *)base)[r * stride + x];
-}
-
-// By a whole workgroup of WAVES waves, a row a wave at a time.
-template <typename T, int WAVES>
-__device__ __forceinline__ bool dv_choose(const SvVerify &a, const DvRec *rec, int s, DvChoice *out) {
-    __shared__ DvChoice ch[WAVES];
+// By a whole workgroup of WAVES waves, a row a wave at a time (n 0: no rows).
+template <int WAVES>
+__device__ __forceinline__ DvChoice dv_choose(const SvVerify &a, const DvRec *rec, const float *drafted, int s) {
+    __shared__ DvRow lp[WAVES], lq[WAVES];
     __shared__ int stays[WAVES];
     int q0, n;
-    if (!dv_rows(a, s, &q0, &n)) return false;
-    const int wave = threadIdx.x >> 6;
+    if (!dv_rows(a, s, &q0, &n)) return {0, 0, -1, 0, {}, {}, 0., 0};
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const double k = dv_rate(a, s);
     for (int i0 = 0;; i0 += WAVES) {   // uniform
-        const int i = i0 + wave, r = q0 + i;
-        int stay = 0;
-        if (i < n) {
-            DvChoice c;
-            c.kept = i;
-            c.n = n;
-            c.row = r;
-            c.k = k;
-            c.p = dv_row(rec + (long long)r * a.chunks, a.chunks, k);
-            c.q = {0.f, -1, 0.};
-            c.x = -1;
-            c.rest = 0;
-            if (i + 1 < n) {
-                const int x = a.tokens[r + 1];
-                const bool is = (unsigned)x < (unsigned)a.vocab;
-                double px = 0., qx = is ? 1. : 0.;
-                if (is) px = dv_prob(c.p, dv_logit<T>(a.logits, a.stride, r, x), x, k);
-                if (a.draft) {
-                    c.q = dv_row(rec + (long long)(a.n_rows + r) * a.chunks, a.chunks, k);
-                    qx = is ? dv_prob(c.q, dv_logit<T>(a.draft, a.dstride, r, x), x, k) : 0.;
-                }
-                stay = dv_random(a.u_accept[r]) * qx < px;
-                c.x = x;
-                c.rest = 1;
+        const int r = q0 + i0 + wave;
+        const bool judges = i0 + wave + 1 < n;
+        if (i0 + wave < n) {
+            const int x = judges ? a.tokens[r + 1] : -1;
+            const bool is = (unsigned)x < (unsigned)a.vocab;
+            const float u = judges ? a.u_accept[r] : 0.f, lx = is ? drafted[r] : 0.f;
+            const float ly = is && a.draft ? drafted[a.n_rows + r] : 0.f;
+            const DvRow p = dv_row(rec + (long long)r * a.chunks, a.chunks, k);
+            DvRow q = {0.f, -1, 0.};
+            double qx = 1.;
+            if (judges && a.draft) {
+                q = dv_row(rec + (long long)(a.n_rows + r) * a.chunks, a.chunks, k);
+                qx = dv_prob(q, ly, x, k);
             }
-            if ((threadIdx.x & 63) == 0) ch[wave] = c;
-        }
-        if ((threadIdx.x & 63) == 0) stays[wave] = stay;
+            if (lane == 0) {
+                lp[wave] = p;
+                lq[wave] = q;
+                stays[wave] = is && dv_random(u) * qx < dv_prob(p, lx, x, k);
+            }
+        } else if (lane == 0) stays[wave] = 1;
         __syncthreads();
-#pragma unroll 1
-        for (int w = 0; w < WAVES; w++)
-            if (!stays[w]) {   // (the last row of a sequence never stays)
-                *out = ch[w];
-                return true;
-            }
+        // the first row that does not stay (the last row of a sequence never does)
+        const uint64_t ends = __builtin_amdgcn_ballot_w64(lane < WAVES && !stays[lane % WAVES]);
+        if (ends) {   // uniform
+            const int w = __builtin_ctzll(ends);
+            const int row = q0 + i0 + w, rest = i0 + w + 1 < n;
+            return {i0 + w, n, rest ? a.tokens[row + 1] : -1, row, lp[w], lq[w], k, rest};
+        }
         __syncthreads();
     }
 }
 
 // The weight of token v in max(p - q, 0), or in p; pi, qi: 1 / the rows' sums (0: no weight).
-__device__ __forceinline__ double dv_rest(const DvChoice &c, double pi, double qi, bool draft, float l, float d, int v) {
-    const double p = dv_weight(l, c.p.m, c.k) * pi;
-    if (!c.rest) return p;
-    if (!draft) return v == c.x ? 0. : p;
-    return fmax(p - dv_weight(d, c.q.m, c.k) * qi, 0.);
+__device__ __forceinline__ double dv_rest(const DvChoice &c, const DvLaw &p, const DvLaw &q, double pi, double qi, bool draft,
+                                          float l, float d, int v) {
+    const double w = dv_weight(p, l) * pi;
+    if (!c.rest) return w;
+    if (!draft) return v == c.x ? 0. : w;
+    return fmax(w - dv_weight(q, d) * qi, 0.);
 }
 
-// With a draft model: what each sequence comes to, and the sums of its weights a chunk.  x: chunk,
-// sequence.
-template <typename T, int CH>
-__global__ __launch_bounds__(DV_THREADS) void k_dv_rest(const SvVerify a, const DvRec *__restrict__ rec,
-                                                        DvChoice *__restrict__ choice, double *__restrict__ rest) {
-    constexpr int N = CH / DV_THREADS < 16 / (int)sizeof(T) ? CH / DV_THREADS : 16 / sizeof(T), R = CH / DV_THREADS / N;
+// With a draft model: what each sequence comes to (n 0: no rows), by a workgroup each.
+__global__ __launch_bounds__(DV_CHOOSE) void k_dv_choose(const SvVerify a, const DvRec *__restrict__ rec,
+                                                       const float *__restrict__ drafted, DvChoice *__restrict__ choice) {
+    const DvChoice c = dv_choose<DV_CHOOSE / 64>(a, rec, drafted, blockIdx.x);
+    if (threadIdx.x == 0) choice[blockIdx.x] = c;
+}
+
+// And the sums of its weights a chunk.  x: chunk, sequence.
+template <typename T>
+__global__ __launch_bounds__(DV_THREADS) void k_dv_rest(const SvVerify a, const DvChoice *__restrict__ choice,
+                                                        double *__restrict__ rest) {
+    constexpr int N = 16 / sizeof(T), R = DV_CHUNK / DV_THREADS / N;
     __shared__ double sums[DV_THREADS / 64];
     const int ck = blockIdx.x % a.chunks, s = blockIdx.x / a.chunks;
-    DvChoice c;
-    if (!dv_choose<T, DV_THREADS / 64>(a, rec, s, &c)) return;
-    if (ck == 0 && threadIdx.x == 0) choice[s] = c;
+    const DvChoice c = choice[s];
     if (!c.rest || !(c.k > 0.) || !(c.p.sum > 0.)) return;   // the draw does without
     const T *l = (const T *)a.logits + c.row * a.stride, *d = (const T *)a.draft + c.row * a.dstride;
-    const int v0 = ck * CH + (int)threadIdx.x * N;
+    const int v0 = ck * DV_CHUNK + (int)threadIdx.x * N;
     float x[R][N], y[R][N];
 #pragma unroll
     for (int i = 0; i < R; i++) {
@@ -262,11 +282,12 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_rest(const SvVerify a, const 
         dv_load(d, v0 + i * DV_THREADS * N, a.vocab, y[i]);
     }
     const double pi = 1. / c.p.sum, qi = c.q.sum > 0. ? 1. / c.q.sum : 0.;
+    const DvLaw p = dv_law(c.p.m, c.k), q = dv_law(c.q.m, c.k);
     double sum = 0.;
 #pragma unroll
     for (int i = 0; i < R; i++)
 #pragma unroll
-        for (int e = 0; e < N; e++) sum += dv_rest(c, pi, qi, true, x[i][e], y[i][e], 0);
+        for (int e = 0; e < N; e++) sum += dv_rest(c, p, q, pi, qi, true, x[i][e], y[i][e], 0);
     sum = dv_sum64(sum);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
@@ -278,7 +299,8 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_rest(const SvVerify a, const 
     }
 }
 
-// Inclusive sum over the workgroup of DV_PICK threads, and the whole one.
+// Inclusive sum over the workgroup of WAVES waves, and the whole one.
+template <int WAVES>
 __device__ __forceinline__ double dv_scan(double v, double *lds, double *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
 #pragma unroll
@@ -290,29 +312,49 @@ __device__ __forceinline__ double dv_scan(double v, double *lds, double *total) 
     if (lane == 63) lds[wave] = v;
     __syncthreads();
     double before = 0., all = 0.;
-    for (int w = 0; w < DV_PICK / 64; w++) {
-        before += w < wave ? lds[w] : 0.;
+#pragma unroll
+    for (int w = 0; w < WAVES; w++) {
+        if (w == wave) before = all;
         all += lds[w];
     }
     *total = all;
     return before + v;
 }
+// The first thread that says yes: its value (and x); -1 where none does.  Of the last one with LAST.
+template <int WAVES, bool LAST>
+__device__ __forceinline__ int dv_which(bool yes, int v, double x, int *li, double *ld, double *out) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    const uint64_t b = __builtin_amdgcn_ballot_w64(yes);
+    const int l = b ? LAST ? 63 - __builtin_clzll(b) : __builtin_ctzll(b) : 0;
+    __syncthreads();
+    if (lane == l) {
+        li[wave] = b ? v : -1;
+        ld[wave] = x;
+    }
+    __syncthreads();
+    int found = -1;
+#pragma unroll
+    for (int i = 0; i < WAVES; i++) {
+        const int w = LAST ? WAVES - 1 - i : i;
+        if (found < 0 && li[w] >= 0) {
+            found = li[w];
+            *out = ld[w];
+        }
+    }
+    return found;
+}
 
 // The draw, a workgroup a sequence.
-template <typename T, int CH>
+template <typename T>
 __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvRec *__restrict__ rec,
+                                                     const float *__restrict__ drafted,
                                                      const DvChoice *__restrict__ choice, const double *__restrict__ rest) {
-    constexpr int EACH = CH / DV_PICK;
-    __shared__ double red[DV_PICK / 64], before;
-    __shared__ int found, last;
+    constexpr int EACH = DV_CHUNK / DV_PICK, WAVES = DV_PICK / 64, N = 16 / sizeof(T);
+    __shared__ double red[WAVES];
+    __shared__ int who[WAVES];
     const int s = blockIdx.x, tid = threadIdx.x;
-    DvChoice c;
-    bool is;
-    if (choice) {
-        int q0, n;
-        is = dv_rows(a, s, &q0, &n);
-        if (is) c = choice[s];
-    } else is = dv_choose<T, DV_PICK / 64>(a, rec, s, &c);
+    DvChoice c = choice ? choice[s] : dv_choose<WAVES>(a, rec, drafted, s);
+    const bool is = c.n > 0;
     int next = -1;
     if (is && !(c.k > 0.)) {
         if (c.p.m > -__builtin_huge_valf()) next = c.p.at;
@@ -320,92 +362,79 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
         const T *l = (const T *)a.logits + c.row * a.stride;
         const T *d = a.draft ? (const T *)a.draft + c.row * a.dstride : nullptr;
         const double u = dv_random(a.u_next[s]), pi = 1. / c.p.sum, qi = c.q.sum > 0. ? 1. / c.q.sum : 0.;
+        const DvLaw p = dv_law(c.p.m, c.k), q = dv_law(c.q.m, c.k);
         double w[EACH];
         // the weights of a chunk's elements, EACH side by side a thread, and their sum
         auto weights = [&](int ck) {
-            const int v0 = ck * CH + tid * EACH;
-            float x[EACH], y[EACH];
-            dv_load(l, v0, a.vocab, x);
-            if (d && c.rest) dv_load(d, v0, a.vocab, y);
+            const int v0 = ck * DV_CHUNK + tid * EACH;
             double sum = 0.;
 #pragma unroll
-            for (int e = 0; e < EACH; e++) {
-                w[e] = dv_rest(c, pi, qi, d != nullptr, x[e], y[e], v0 + e);
-                sum += w[e];
+            for (int i = 0; i < EACH; i += N) {
+                float x[N], y[N];
+                dv_load(l, v0 + i, a.vocab, x);
+                if (d && c.rest) dv_load(d, v0 + i, a.vocab, y);
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    w[i + e] = dv_rest(c, p, q, pi, qi, d != nullptr, x[e], y[e], v0 + i + e);
+                    sum += w[i + e];
+                }
             }
             return sum;
         };
         // a chunk's sum: as the record has it, or k_dv_rest, or (the rejected guess's own chunk) anew
-        const int own = c.rest && !d && (unsigned)c.x < (unsigned)a.vocab ? c.x / CH : -1;
+        const int own = c.rest && !d && (unsigned)c.x < (unsigned)a.vocab ? c.x / DV_CHUNK : -1;
         double anew = 0., total = 0.;
-        if (own >= 0) dv_scan(weights(own), red, &anew);
+        if (own >= 0) dv_scan<WAVES>(weights(own), red, &anew);
         auto mass = [&](int k) {
             if (c.rest && d) return rest[(long long)s * a.chunks + k];
             if (c.rest && k == own) return anew;
             const DvRec r = rec[(long long)c.row * a.chunks + k];
-            return r.sum * dv_weight(r.m, c.p.m, c.k) * pi;
+            return r.sum * dv_weight(p, r.m) * pi;
         };
         // a thread's chunks lie side by side
         const int per = (a.chunks + DV_PICK - 1) / DV_PICK, k0 = min(tid * per, a.chunks), k1 = min(k0 + per, a.chunks);
-        double mine = 0., run = 0.;
+        double run = 0.;
         for (int round = 0; round < 2; round++) {   // (nothing left of p - q: p itself)
-            mine = 0.;
+            double mine = 0.;
             for (int k = k0; k < k1; k++) mine += mass(k);
-            run = dv_scan(mine, red, &total) - mine;
+            run = dv_scan<WAVES>(mine, red, &total) - mine;
             if (total > 0.) break;
             c.rest = 0;
         }
-        if (tid == 0) {
-            found = 0x7FFFFFFF;
-            last = -1;
-        }
-        __syncthreads();
         // the first chunk whose end is above u * total; the last that has any weight, where rounding
         // leaves none
-        double at[2] = {0., 0.};
-        int f = 0x7FFFFFFF, z = -1;
+        double at = 0., end = 0., before = 0.;
+        int f = -1, z = -1;
         for (int k = k0; k < k1; k++) {
             const double m = mass(k);
-            if (m > 0. && run + m > u * total && f == 0x7FFFFFFF) {
+            if (m > 0. && run + m > u * total && f < 0) {
                 f = k;
-                at[0] = run;
+                at = run;
             }
             if (m > 0.) {
                 z = k;
-                at[1] = run;
+                end = run;
             }
             run += m;
         }
-        if (f != 0x7FFFFFFF) atomicMin(&found, f);
-        if (z >= 0) atomicMax(&last, z);
-        __syncthreads();
-        const int ck = found != 0x7FFFFFFF ? found : last;
-        if (ck == f) before = at[0];
-        else if (found == 0x7FFFFFFF && ck >= 0 && ck == z) before = at[1];
-        __syncthreads();
+        int ck = dv_which<WAVES, false>(f >= 0, f, at, who, red, &before);
+        if (ck < 0) ck = dv_which<WAVES, true>(z >= 0, z, end, who, red, &before);
         if (ck >= 0) {
-            if (tid == 0) {
-                found = 0x7FFFFFFF;
-                last = -1;
-            }
-            mine = weights(ck);
+            const double mine = weights(ck);
             double all;
-            run = before + (dv_scan(mine, red, &all) - mine);
-            f = 0x7FFFFFFF;
-            z = -1;
+            run = before + (dv_scan<WAVES>(mine, red, &all) - mine);
+            f = z = -1;
 #pragma unroll
             for (int e = 0; e < EACH; e++) {
                 run += w[e];
                 if (w[e] > 0.) {
                     z = e;
-                    if (run > u * total && f == 0x7FFFFFFF) f = e;
+                    if (run > u * total && f < 0) f = e;
                 }
             }
-            const int v0 = ck * CH + tid * EACH;
-            if (f != 0x7FFFFFFF) atomicMin(&found, v0 + f);
-            if (z >= 0) atomicMax(&last, v0 + z);
-            __syncthreads();
-            next = found != 0x7FFFFFFF ? found : last;
+            const int v0 = ck * DV_CHUNK + tid * EACH;
+            next = dv_which<WAVES, false>(f >= 0, v0 + f, 0., who, red, &before);
+            if (next < 0) next = dv_which<WAVES, true>(z >= 0, v0 + z, 0., who, red, &before);
         }
     }
     if (tid == 0) {
@@ -415,41 +444,52 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
     }
 }
 
-int verify_chunk(int n_rows, int vocab, bool draft) {
-    return (long long)n_rows * (draft ? 2 : 1) * vocab <= 512ll * DV_LONG ? DV_SHORT : DV_LONG;
+// Records, choices, sums of the rest a chunk, the drafts' logits.
+struct DvWs {
+    DvRec *rec;
+    DvChoice *choice;
+    double *rest;
+    float *drafted;
+    size_t bytes;
+};
+static DvWs verify_ws(void *ws, int n_seqs, int n_rows, int vocab, bool draft) {
+    const size_t chunks = ((size_t)vocab + DV_CHUNK - 1) / DV_CHUNK;
+    const size_t rows = (size_t)n_rows * (draft ? 2 : 1);
+    DvWs w{};
+    w.rec = (DvRec *)ws;
+    size_t at = rows * chunks * sizeof(DvRec);
+    if (draft) {
+        w.choice = (DvChoice *)((char *)ws + at);
+        at += (size_t)n_seqs * sizeof(DvChoice);
+        w.rest = (double *)((char *)ws + at);
+        at += (size_t)n_seqs * chunks * sizeof(double);
+    }
+    w.drafted = (float *)((char *)ws + at);
+    w.bytes = at + rows * sizeof(float);
+    return w;
 }
-
 size_t verify_workspace_bytes(int n_seqs, int n_rows, int vocab, bool draft) {
-    const size_t ch = verify_chunk(n_rows, vocab, draft), chunks = ((size_t)vocab + ch - 1) / ch;
-    const size_t n = (size_t)n_rows * (draft ? 2 : 1) * chunks * sizeof(DvRec);
-    return draft ? n + (size_t)n_seqs * (chunks * sizeof(double) + sizeof(DvChoice)) : n;
-}
-
-template <typename T, int CH>
-static hipError_t verify(SvVerify a, void *ws, hipStream_t st) {
-    a.chunks = (a.vocab + CH - 1) / CH;
-    const long long wgs = (long long)a.n_rows * (a.draft ? 2 : 1) * a.chunks;
-    if (wgs > (1ll << 32) / DV_THREADS - 1 || (long long)a.n_seqs * a.chunks > (1ll << 32) / DV_THREADS - 1)
-        return hipErrorInvalidConfiguration;
-    DvRec *rec = (DvRec *)ws;
-    DvChoice *choice = a.draft ? (DvChoice *)(rec + wgs) : nullptr;
-    double *rest = a.draft ? (double *)(choice + a.n_seqs) : nullptr;
-    if (wgs > 0) hipLaunchKernelGGL((k_dv_stats<T, CH>), dim3((unsigned)wgs), dim3(DV_THREADS), 0, st, a, rec);
-    if (a.draft && wgs > 0)
-        hipLaunchKernelGGL((k_dv_rest<T, CH>), dim3((unsigned)(a.n_seqs * a.chunks)), dim3(DV_THREADS), 0, st, a, rec, choice,
-                           rest);
-    hipLaunchKernelGGL((k_dv_pick<T, CH>), dim3(a.n_seqs), dim3(DV_PICK), 0, st, a, rec, choice, rest);
-    return hipGetLastError();
+    return verify_ws(nullptr, n_seqs, n_rows, vocab, draft).bytes;
 }
 
 template <typename T>
-static hipError_t verify_t(const SvVerify &a, void *ws, hipStream_t st) {
-    return verify_chunk(a.n_rows, a.vocab, a.draft != nullptr) == DV_SHORT ? verify<T, DV_SHORT>(a, ws, st)
-                                                                          : verify<T, DV_LONG>(a, ws, st);
+static hipError_t verify(const SvVerify &a, void *ws, hipStream_t st) {
+    const long long wgs = (long long)a.n_rows * (a.draft ? 2 : 1) * a.chunks;
+    if (wgs > (1ll << 32) / DV_THREADS - 1 || (long long)a.n_seqs * a.chunks > (1ll << 32) / DV_THREADS - 1)
+        return hipErrorInvalidConfiguration;
+    const DvWs w = verify_ws(ws, a.n_seqs, a.n_rows, a.vocab, a.draft != nullptr);
+    if (wgs > 0) hipLaunchKernelGGL(k_dv_stats<T>, dim3((unsigned)wgs), dim3(DV_THREADS), 0, st, a, w.rec, w.drafted);
+    if (a.draft) {
+        hipLaunchKernelGGL(k_dv_choose, dim3(a.n_seqs), dim3(DV_CHOOSE), 0, st, a, w.rec, w.drafted, w.choice);
+        hipLaunchKernelGGL(k_dv_rest<T>, dim3((unsigned)(a.n_seqs * a.chunks)), dim3(DV_THREADS), 0, st, a, w.choice,
+                           w.rest);
+    }
+    hipLaunchKernelGGL(k_dv_pick<T>, dim3(a.n_seqs), dim3(DV_PICK), 0, st, a, w.rec, w.drafted, w.choice, w.rest);
+    return hipGetLastError();
 }
 
 hipError_t launch_verify(const SvVerify &a, int type, void *ws, hipStream_t st) {
-    return type == TBQ_KV_F32 ? verify_t<float>(a, ws, st) : type == TBQ_KV_F16 ? verify_t<pg_f16>(a, ws, st) : verify_t<pg_bf16>(a, ws, st);
+    return type == TBQ_KV_F32 ? verify<float>(a, ws, st) : type == TBQ_KV_F16 ? verify<pg_f16>(a, ws, st) : verify<pg_bf16>(a, ws, st);
 }
 
 }  // namespace tbq
