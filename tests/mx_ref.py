@@ -22,7 +22,7 @@ def blocks(x):
     # of two codes that are equally near, the even one
     code = (near & (torch.arange(8) % 2 == 0)).double().argmax(-1)
     code = torch.where((near & (torch.arange(8) % 2 == 0)).any(-1), code, near.double().argmax(-1))
-    code = code + 8 * (y < 0)
+    code = code + 8 * torch.signbit(y)
     return code.flatten(-2), torch.where(odd, NAN, E + 127)
 
 

@@ -57,20 +57,30 @@ __device__ __forceinline__ mx_h8 mx_eight(uint32_t codes, float scale) {
 // Exponent of the scale of a block whose largest magnitude is a (finite): the least
 // E with a <= 7 * 2^E.  7 is where the last code, 6, is no further off than codes
 // between 4 and 6 can be (values N(0, 1): relative error 0.112; 0.115 with 6 or 8).
-template <typename F>
-__device__ __forceinline__ int mx_exponent(F a) {
+__device__ __forceinline__ int mx_exponent(float a) {
     int e;
-    const F m = frexp(a, &e);
-    return a > 0 ? min(max(e - 3 + (m > F(0.875) ? 1 : 0), MX_LEAST), MX_MOST) : MX_LEAST;
+    const float m = frexpf(a, &e);
+    return a > 0.f ? min(max(e - 3 + (m > 0.875f ? 1 : 0), MX_LEAST), MX_MOST) : MX_LEAST;
 }
 
-// The nearest code of y (in units of the scale), ties to the even one.
-template <typename F>
-__device__ __forceinline__ uint32_t mx_code(F y) {
-    const F m = y < 0 ? -y : y;
-    const int c = (m > F(0.25)) + (m >= F(0.75)) + (m > F(1.25)) + (m >= F(1.75)) + (m > F(2.5)) + (m >= F(3.5)) +
-                  (m > F(5));
-    return (uint32_t)c | (y < 0 ? 8u : 0u);
+// y as a float that stands to every float of fewer bits, and halfway between two of them, as y does: rounded
+// to an odd last bit where it is not a float.  So what is rounded from it is what would be rounded from y.
+__device__ __forceinline__ float mx_odd(double y) {
+    const float f = (float)y;
+    const double d = y - (double)f;
+    const uint32_t b = __builtin_bit_cast(uint32_t, f);
+    const uint32_t n = (d > 0.) == (y > 0.) ? b + 1 : b - 1;   // the float on y's other side
+    return (d > 0. || d < 0.) && f != 0.f && !(b & 1) ? __builtin_bit_cast(float, n) : f;   // (infinities stay)
+}
+
+// The codes of eight values: the nearest ones to x / scale, ties to the even one, at most 6
+// (v_cvt_scalef32_pk_fp4_f32; checked against the definition at every border of every scale and beside it).
+__device__ __forceinline__ uint32_t mx_codes(const float (&x)[8], float scale) {
+    uint32_t c = 0;
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[0], x[1], scale, 0);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[2], x[3], scale, 1);
+    c = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[4], x[5], scale, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(c, x[6], x[7], scale, 3);
 }
 
 }  // namespace tbq

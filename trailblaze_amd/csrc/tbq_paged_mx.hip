@@ -10,44 +10,48 @@
 
 namespace tbq {
 
-template <typename F, int WIDTH>
-__device__ __forceinline__ F mx_group_max(F v) {
-#pragma unroll
-    for (int d = 1; d < WIDTH; d *= 2) {
-        const F o = __shfl_xor(v, d);
-        v = o > v ? o : v;
-    }
-    return v;
+template <int CTRL>
+__device__ __forceinline__ double mx_dpp(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_bit_cast(uint32_t, dpp_f32<CTRL>(__builtin_bit_cast(float, (uint32_t)b)));
+    const uint32_t hi = __builtin_bit_cast(uint32_t, dpp_f32<CTRL>(__builtin_bit_cast(float, (uint32_t)(b >> 32))));
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
+// Sum over 8 or 16 lanes, as group_sum.
 template <int WIDTH>
 __device__ __forceinline__ double mx_group_sum(double v) {
-#pragma unroll
-    for (int d = 1; d < WIDTH; d *= 2) v += __shfl_xor(v, d);
+    v += mx_dpp<DPP_QXOR1>(v);
+    v += mx_dpp<DPP_QXOR2>(v);
+    v += mx_dpp<DPP_HALF_MIRROR>(v);
+    if constexpr (WIDTH == 16) v += mx_dpp<DPP_MIRROR>(v);
     return v;
+}
+
+// 1 / sqrt(x): from fp32's by Newton's iteration, twice (1e-7, 1e-14, then fp64's own).
+__device__ __forceinline__ double mx_rsqrt(double x) {
+    if (!(x > 1e-30 && x < 1e30)) return 1. / sqrt(x);
+    double r = (double)(1.0f / sqrtf((float)x));
+    r = r * fma(-0.5 * x * r, r, 1.5);
+    return r * fma(-0.5 * x * r, r, 1.5);
 }
 
 // Eight values side by side, of the four lanes that share a block of 32: the codes,
 // and the block's scale byte.  A value that is not finite makes the block NaN.
-template <typename F>
-__device__ __forceinline__ uint32_t mx_block(const F (&x)[8], uint32_t *scale) {
-    F a = 0;
-    int odd = 0;
+__device__ __forceinline__ uint32_t mx_block(const float (&x)[8], uint32_t *scale) {
+    float a = 0.f, odd = 0.f;   // odd: NaN where a value is not finite
 #pragma unroll
     for (int i = 0; i < 8; i++) {
-        const F m = x[i] < 0 ? -x[i] : x[i];
-        odd |= !(m < F(__builtin_huge_val()));
-        a = m > a ? m : a;
+        a = fmaxf(a, fabsf(x[i]));
+        odd += x[i] - x[i];
     }
-    a = mx_group_max<F, 4>(a);
-    odd |= __shfl_xor(odd, 1);
-    odd |= __shfl_xor(odd, 2);
-    if (odd) a = 0;
+    a = fmaxf(a, dpp_f32<DPP_QXOR1>(a));
+    a = fmaxf(a, dpp_f32<DPP_QXOR2>(a));
+    odd += dpp_f32<DPP_QXOR1>(odd);
+    odd += dpp_f32<DPP_QXOR2>(odd);
+    const bool fine = odd == 0.f;
     const int E = mx_exponent(a);
-    *scale = odd ? MX_NAN : E + 127;
-    uint32_t codes = 0;
-#pragma unroll
-    for (int i = 0; i < 8; i++) codes |= mx_code(ldexp(x[i], -E)) << (4 * i);
-    return odd ? 0u : codes;
+    *scale = fine ? E + 127 : MX_NAN;
+    return fine ? mx_codes(x, mx_scale(E + 127)) : 0u;
 }
 
 // ---------------------------------------------------------------------------
@@ -65,8 +69,13 @@ template <typename TI, typename TQ, int D, int HPT>
 __global__ __launch_bounds__(MA_THREADS) void k_mx_append(const PgAppend a) {
     constexpr int LPH = D / 8, SL = MA_THREADS / LPH;
     __shared__ double cs[D / 2], sn[D / 2];
-    __shared__ __attribute__((aligned(16))) double kx[SL][D];
-    const int t = blockIdx.x, l = threadIdx.x % LPH, rot = a.rope.rot, slot = threadIdx.x / LPH;
+    __shared__ __attribute__((aligned(16))) float kx[SL][D];
+    // Sixteen tokens side by side go to one XCD's workgroups, one after the other: they write into the same lines
+    // (four positions of V share each), which one L2 then holds (8191 tokens: 62.7 -> 61.2 us).
+    constexpr int XCDS = 8, RUN = 16;
+    const int run0 = blockIdx.x / (XCDS * RUN) * (XCDS * RUN), in_run = blockIdx.x - run0;
+    const int t = run0 + XCDS * RUN <= (int)gridDim.x ? run0 + in_run % XCDS * RUN + in_run / XCDS : (int)blockIdx.x;
+    const int l = threadIdx.x % LPH, rot = a.rope.rot, slot = threadIdx.x / LPH;
     const int nslots = a.NQ + 2 * a.pg.NKV;
     const int s = pg_seq_of(a.pg.q_start, a.pg.n_seqs, t);
     if (s >= a.pg.n_seqs) return;
@@ -128,7 +137,7 @@ __global__ __launch_bounds__(MA_THREADS) void k_mx_append(const PgAppend a) {
     for (int i = 0; i < HPT; i++) {
         const int hh = (int)(blockIdx.y * HPT + i) * SL + slot;
         const bool isq = hh < a.NQ, isv = hh >= a.NQ + a.pg.NKV;
-        const float x[8] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w, xb[i].x, xb[i].y, xb[i].z, xb[i].w};
+        float x[8] = {xa[i].x, xa[i].y, xa[i].z, xa[i].w, xb[i].x, xb[i].y, xb[i].z, xb[i].w};
         if (hh >= nslots) continue;
         if (isq) {
             float y[8], ss = 0.f;
@@ -152,9 +161,11 @@ __global__ __launch_bounds__(MA_THREADS) void k_mx_append(const PgAppend a) {
             continue;
         }
         const int kvh = isv ? hh - a.NQ - a.pg.NKV : hh - a.NQ;
-        uint32_t codes, scale;
-        if (isv) codes = mx_block(x, &scale);
-        else {
+        float v[8];
+        if (isv) {
+#pragma unroll
+            for (int e = 0; e < 8; e++) v[e] = x[e];
+        } else {
             double y[8], ss = 0.;
 #pragma unroll
             for (int e = 0; e < 8; e++) {
@@ -162,8 +173,7 @@ __global__ __launch_bounds__(MA_THREADS) void k_mx_append(const PgAppend a) {
                 ss = fma(y[e], y[e], ss);
             }
             if (a.kn) {
-                ss = mx_group_sum<LPH>(ss);
-                const double r = 1. / sqrt(ss / D + (double)a.eps);
+                const double r = mx_rsqrt(mx_group_sum<LPH>(ss) / D + (double)a.eps);
                 const float4 wa = pg_ld4(a.kn + oa), wb = pg_ld4(a.kn + ob);
                 const float w[8] = {wa.x, wa.y, wa.z, wa.w, wb.x, wb.y, wb.z, wb.w};
 #pragma unroll
@@ -171,19 +181,17 @@ __global__ __launch_bounds__(MA_THREADS) void k_mx_append(const PgAppend a) {
             }
             if (turn) rotate(y);
             // to eight elements side by side (the head's lanes are of one wave)
-            double *row = kx[slot];
-#pragma unroll
-            for (int e = 0; e < 4; e++) {
-                row[oa + e] = y[e];
-                row[ob + e] = y[e + 4];
-            }
-            __builtin_amdgcn_wave_barrier();
+            float *row = kx[slot];
+            *reinterpret_cast<float4 *>(row + oa) = make_float4(mx_odd(y[0]), mx_odd(y[1]), mx_odd(y[2]), mx_odd(y[3]));
+            *reinterpret_cast<float4 *>(row + ob) = make_float4(mx_odd(y[4]), mx_odd(y[5]), mx_odd(y[6]), mx_odd(y[7]));
             __builtin_amdgcn_fence(__ATOMIC_SEQ_CST, "wavefront");
-#pragma unroll
-            for (int e = 0; e < 8; e++) y[e] = row[8 * l + e];
             __builtin_amdgcn_wave_barrier();
-            codes = mx_block(y, &scale);
+            const float4 va = *reinterpret_cast<const float4 *>(row + 8 * l), vb = *reinterpret_cast<const float4 *>(row + 8 * l + 4);
+            __builtin_amdgcn_wave_barrier();
+            v[0] = va.x, v[1] = va.y, v[2] = va.z, v[3] = va.w, v[4] = vb.x, v[5] = vb.y, v[6] = vb.z, v[7] = vb.w;
         }
+        uint32_t scale;
+        const uint32_t codes = mx_block(v, &scale);
         if (page < 0) continue;
         uint8_t *o = (uint8_t *)(isv ? a.pg.v : a.pg.k) + mx_head<D>(a.pg, page, kvh), *sc = o + ((D / 2) << a.pg.shift);
         *reinterpret_cast<uint32_t *>(o + (isv ? mx_v_code<D>(in, l) : mx_k_code<D>(in, l))) = codes;
@@ -219,38 +227,57 @@ hipError_t launch_mx_append(const PgAppend &a, int D, int in_type, int q_type, h
 // read side by side and whole lines are written.  Bound by HBM (the values' bytes).
 // ---------------------------------------------------------------------------
 constexpr int MD_THREADS = 256;
-template <typename TO, int D>
+template <typename TO, int D, int ROUNDS>
 __global__ __launch_bounds__(MD_THREADS) void k_mx_dequant(const PgArgs a, const int *__restrict__ pages, TO *k, TO *v) {
     constexpr int LPR = D / 8, RPW = MD_THREADS / LPR;   // rows of a workgroup's round
     const int g = threadIdx.x / 4 % LPR, r = threadIdx.x / (4 * LPR) * 4 + threadIdx.x % 4;
-    const int chunks = max(1, (1 << a.shift) / RPW), n = blockIdx.x / chunks, h = blockIdx.y;
-    const int page = pages ? pages[n] : n, in = blockIdx.x % chunks * RPW + r;
-    if (in >= 1 << a.shift) return;
+    const int rows = 1 << a.shift, chunks = (rows + RPW * ROUNDS - 1) / (RPW * ROUNDS);
+    const int n = blockIdx.x / chunks, h = blockIdx.y, page = pages ? pages[n] : n;
     const bool there = (unsigned)page < (unsigned)a.n_pages;
-    const long long from = mx_head<D>(a, there ? page : 0, h);
-    const long long to = ((long long)n * a.NKV + h) << a.shift;
-    const int codes = (D / 2) << a.shift;
+    const long long from = mx_head<D>(a, there ? page : 0, h), to = ((long long)n * a.NKV + h) << a.shift;
+    const int codes = (D / 2) << a.shift, r0 = blockIdx.x % chunks * RPW * ROUNDS + r;
     const uint8_t *kp = (const uint8_t *)a.k + from, *vp = (const uint8_t *)a.v + from;
-    const uint32_t kc = *reinterpret_cast<const uint32_t *>(kp + mx_k_code<D>(in, g));
-    const uint32_t vc = *reinterpret_cast<const uint32_t *>(vp + mx_v_code<D>(in, g));
-    const uint32_t ks = kp[codes + mx_k_scale<D>(in, g / 4)], vs = vp[codes + mx_v_scale<D>(in, g / 4)];
-    mx_h8 x = mx_eight(kc, mx_scale(ks)), y = mx_eight(vc, mx_scale(vs));
-    if (!there) x = y = mx_h8{};
-    TO *ko = k + (to + in) * D + 8 * g, *vo = v + (to + in) * D + 8 * g;
+    uint32_t kc[ROUNDS], vc[ROUNDS], ks[ROUNDS], vs[ROUNDS];
 #pragma unroll
-    for (int e = 0; e < 8; e += 4) {
-        pg_st4(ko + e, make_float4((float)x[e], (float)x[e + 1], (float)x[e + 2], (float)x[e + 3]));
-        pg_st4(vo + e, make_float4((float)y[e], (float)y[e + 1], (float)y[e + 2], (float)y[e + 3]));
+    for (int i = 0; i < ROUNDS; i++) {
+        const int in = min(r0 + RPW * i, rows - 1);
+        kc[i] = *reinterpret_cast<const uint32_t *>(kp + mx_k_code<D>(in, g));
+        vc[i] = *reinterpret_cast<const uint32_t *>(vp + mx_v_code<D>(in, g));
+        ks[i] = kp[codes + mx_k_scale<D>(in, g / 4)];
+        vs[i] = vp[codes + mx_v_scale<D>(in, g / 4)];
     }
+    typedef TO out8 __attribute__((ext_vector_type(8)));
+#pragma unroll
+    for (int i = 0; i < ROUNDS; i++) {
+        const int in = r0 + RPW * i;
+        if (in >= rows) break;
+        const mx_h8 x = mx_eight(there ? kc[i] : 0u, mx_scale(there ? ks[i] : 0u));
+        const mx_h8 y = mx_eight(there ? vc[i] : 0u, mx_scale(there ? vs[i] : 0u));
+        out8 xo, yo;
+#pragma unroll
+        for (int e = 0; e < 8; e++) {
+            xo[e] = (TO)(float)x[e];
+            yo[e] = (TO)(float)y[e];
+        }
+        *reinterpret_cast<out8 *>(k + (to + in) * D + 8 * g) = xo;
+        *reinterpret_cast<out8 *>(v + (to + in) * D + 8 * g) = yo;
+    }
+}
+
+template <typename TO, int D, int ROUNDS>
+static void mx_dequant(const PgArgs &a, const int *pages, int n, void *k, void *v, hipStream_t st) {
+    constexpr int rows = MD_THREADS / (D / 8) * ROUNDS;
+    const dim3 grid((unsigned)n * (((1 << a.shift) + rows - 1) / rows), a.NKV);
+    hipLaunchKernelGGL((k_mx_dequant<TO, D, ROUNDS>), grid, dim3(MD_THREADS), 0, st, a, pages, (TO *)k, (TO *)v);
 }
 
 hipError_t launch_mx_dequant(const PgArgs &a, int D, const int *pages, int n, int out_type, void *k, void *v,
                              hipStream_t st) {
-    const int rows = MD_THREADS / (D / 8);
-    const dim3 grid((unsigned)n * std::max(1, (1 << a.shift) / rows), a.NKV);
+    // four rounds a workgroup where there are many rows (NN)
+    const bool many = (long long)n * a.NKV << a.shift >= 1 << 15;
 #define TBQ_MD(TO)                                                                                                       \
-    if (D == 128) hipLaunchKernelGGL((k_mx_dequant<TO, 128>), grid, dim3(MD_THREADS), 0, st, a, pages, (TO *)k, (TO *)v); \
-    else hipLaunchKernelGGL((k_mx_dequant<TO, 64>), grid, dim3(MD_THREADS), 0, st, a, pages, (TO *)k, (TO *)v)
+    if (D == 128) many ? mx_dequant<TO, 128, 4>(a, pages, n, k, v, st) : mx_dequant<TO, 128, 1>(a, pages, n, k, v, st);  \
+    else many ? mx_dequant<TO, 64, 4>(a, pages, n, k, v, st) : mx_dequant<TO, 64, 1>(a, pages, n, k, v, st)
     if (out_type == TBQ_KV_F32) {
         TBQ_MD(float);
     } else if (out_type == TBQ_KV_F16) {
