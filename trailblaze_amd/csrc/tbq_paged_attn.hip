@@ -897,11 +897,12 @@ static hipError_t pg_join(const PgAttn &a, const PgPlan &p, const float *ws, hip
     return hipGetLastError();
 }
 
-// Over 4-bit pages.  A batch's few splits a row: D / 4 lanes a row (64 sequences of up to 8192 positions
-// 7.2 -> 3.x us); the hundreds of a long context a workgroup.
+// Over 4-bit pages.  A batch's few splits of many rows: D / 4 lanes a row (2048 rows of up to 5 splits 7.2 -> 4.6 us);
+// else a workgroup (256 rows of 17 2.9 against 4.2, of 33 2.9 against 6.2).
 template <typename TO, int D, bool HL>
 static hipError_t mx_join(const PgAttn &a, const PgPlan &p, const float *ws, hipStream_t st) {
-    return p.row_splits <= PC_FEW ? pg_join<TO, D, HL, true>(a, p, ws, st) : pg_join<TO, D, HL, false>(a, p, ws, st);
+    const bool few = p.row_splits <= 8 && (long long)a.pg.NKV * p.most * a.pg.n_seqs > 512;
+    return few ? pg_join<TO, D, HL, true>(a, p, ws, st) : pg_join<TO, D, HL, false>(a, p, ws, st);
 }
 hipError_t launch_mx_join(const PgAttn &a, int D, const PgPlan &p, bool f32, int out_type, const float *ws, hipStream_t st) {
     if (f32) return D == 128 ? mx_join<float, 128, true>(a, p, ws, st) : mx_join<float, 64, true>(a, p, ws, st);
