@@ -239,6 +239,45 @@ __device__ __forceinline__ float group_sum(float v) {
     return v;
 }
 
+// The same on doubles, whose halves move apart.
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ double dpp_f64(double v) {   // rows of 16 lanes outside ROWS and lanes without a source: 0
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, ROWS, 0xF, false);
+    const uint32_t hi = __builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, ROWS, 0xF, false);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
+}
+template <int WIDTH>
+__device__ __forceinline__ double group_sum(double v) {
+    if constexpr (WIDTH >= 2) v += dpp_f64<DPP_QXOR1>(v);
+    if constexpr (WIDTH >= 4) v += dpp_f64<DPP_QXOR2>(v);
+    if constexpr (WIDTH >= 8) v += dpp_f64<DPP_HALF_MIRROR>(v);
+    if constexpr (WIDTH >= 16) v += dpp_f64<DPP_MIRROR>(v);
+    if constexpr (WIDTH >= 32) {
+#pragma unroll
+        for (int w = 32; w <= WIDTH; w *= 2) {
+            const uint64_t b = __builtin_bit_cast(uint64_t, v);
+            const uint32_t lo = (uint32_t)b, hi = (uint32_t)(b >> 32);
+            const auto x = w == 32 ? __builtin_amdgcn_permlane16_swap(lo, lo, false, false)
+                                   : __builtin_amdgcn_permlane32_swap(lo, lo, false, false);
+            const auto y = w == 32 ? __builtin_amdgcn_permlane16_swap(hi, hi, false, false)
+                                   : __builtin_amdgcn_permlane32_swap(hi, hi, false, false);
+            const uint32_t x0 = x[0], x1 = x[1], y0 = y[0], y1 = y[1];
+            v = __builtin_bit_cast(double, (uint64_t)y0 << 32 | x0) + __builtin_bit_cast(double, (uint64_t)y1 << 32 | x1);
+        }
+    }
+    return v;
+}
+// Inclusive sums over the lanes of a wave, all of them active.
+__device__ __forceinline__ double wave_scan(double v) {
+    v += dpp_f64<0x111>(v);        // row_shr 1, 2, 4, 8
+    v += dpp_f64<0x112>(v);
+    v += dpp_f64<0x114>(v);
+    v += dpp_f64<0x118>(v);
+    v += dpp_f64<0x142, 0xA>(v);   // row_bcast 15: into rows 1 and 3
+    return v + dpp_f64<0x143, 0xC>(v);   // row_bcast 31: into rows 2 and 3
+}
+
 // Sum of one float per thread over the workgroup (blockDim.x a multiple of
 // 64, at most 2048), in a fixed order; every thread gets it.
 __device__ __forceinline__ float pro_block_sum(float v) {

@@ -31,7 +31,7 @@ typedef DvRec DvRow;   // of a row: the same
 // 2^r is the polynomial of degree 8 that meets it at the nine Chebyshev points, off by 1.1e-12 of it at most; the
 // whole number goes to the exponent.  Logits from low on have no weight (2^-1000 of the largest, -infinity, NaN);
 // where m is infinite, all below it; k is 0 where only m itself has weight.  With Least set, they have up to 2^-999, for sums alone (k > 0).
-// (218 + 154 rows of 151936: 113 us with the library's exp, NN with this.)
+// (218 + 154 rows of 151936: 113 us with the library's exp, 53 with this.)
 struct DvLaw {
     double k, m;
     float low;
@@ -60,12 +60,6 @@ __device__ __forceinline__ double dv_weight(const DvLaw &w, float l) {
     p = fma(p, r, 1.);
     const uint64_t b = __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, n) << 52);
     return Least || l > w.low ? __builtin_bit_cast(double, b) : 0.;
-}
-
-__device__ __forceinline__ double dv_sum64(double v) {
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) v += __shfl_xor(v, d);
-    return v;
 }
 
 // N elements of a row from element i on (-infinity behind the end).
@@ -100,22 +94,29 @@ __device__ __forceinline__ double dv_rate(const SvVerify &a, int s) {
 // Block x: chunk, row, and (draft) whose logits.  Bound by HBM and the exponentials' fp64.
 template <typename T>
 __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec *__restrict__ rec,
-                                                         float *__restrict__ drafted) {
+                                                         float *__restrict__ drafted, double *__restrict__ others) {
     constexpr int N = 16 / sizeof(T), R = DV_CHUNK / DV_THREADS / N;
     __shared__ float ms[DV_THREADS / 64];
     __shared__ int at[DV_THREADS / 64];
-    __shared__ double sums[DV_THREADS / 64];
+    __shared__ double sums[DV_THREADS / 64], buts[DV_THREADS / 64];
     const int c = blockIdx.x % a.chunks, r = blockIdx.x / a.chunks % a.n_rows, which = blockIdx.x / a.chunks / a.n_rows;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *row = (const T *)(which ? a.draft : a.logits) + r * (which ? a.dstride : a.stride);
     const int v0 = c * DV_CHUNK + (int)threadIdx.x * N;
     float x[R][N];
+    auto load = [&] {
 #pragma unroll
-    for (int i = 0; i < R; i++) dv_load(row, v0 + i * DV_THREADS * N, a.vocab, x[i]);
+        for (int i = 0; i < R; i++) dv_load(row, v0 + i * DV_THREADS * N, a.vocab, x[i]);
+    };
+    if (!which) load();   // (nearly all of the target's rows are some sequence's)
+    const int behind = a.tokens[min(r + 1, a.n_rows - 1)];
     const int s = pg_seq_of(a.q_start, a.n_seqs, r);
     int q0, n;
     if (s >= a.n_seqs || !dv_rows(a, s, &q0, &n) || r < q0 || (which && r + 1 == q0 + n)) return;
+    if (which) load();
     const double k = dv_rate(a, s);
+    const int guess = r + 1 < q0 + n ? behind : -1;   // judged by this row
+    const bool has = (unsigned)guess < (unsigned)a.vocab && guess / DV_CHUNK == c, apart = has && !a.draft;
     float m = -__builtin_huge_valf();
 #pragma unroll
     for (int i = 0; i < R; i++)
@@ -127,7 +128,7 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
 #pragma unroll
     for (int w = 0; w < DV_THREADS / 64; w++) m = fmaxf(m, ms[w]);
     int first = 0x7FFFFFFF;
-    double sum = 0.;
+    double sum = 0., but = 0.;   // of all; of all but the guess, which the draw takes (not a difference: it may be nearly all)
     if (!(k > 0.)) {
 #pragma unroll
         for (int i = R - 1; i >= 0; i--)
@@ -138,7 +139,17 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
         for (int d = 1; d < 64; d *= 2) first = min(first, __shfl_xor(first, d));
     } else if (m > -__builtin_huge_valf()) {
         const DvLaw law = dv_law(m, k);
-        if (law.k > 0.) {   // uniform
+        if (apart) {   // uniform
+#pragma unroll
+            for (int i = 0; i < R; i++)
+#pragma unroll
+                for (int e = 0; e < N; e++) {
+                    const double w = dv_weight(law, x[i][e]);
+                    sum += w;
+                    but += v0 + i * DV_THREADS * N + e == guess ? 0. : w;
+                }
+            but = group_sum<64>(but);
+        } else if (law.k > 0.) {
 #pragma unroll
             for (int i = 0; i < R; i++)
 #pragma unroll
@@ -149,44 +160,44 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
 #pragma unroll
                 for (int e = 0; e < N; e++) sum += x[i][e] == m ? 1. : 0.;
         }
-        sum = dv_sum64(sum);
+        sum = group_sum<64>(sum);
     }
     if (lane == 0) {
         sums[wave] = sum;
+        buts[wave] = but;
         at[wave] = first;
     }
     __syncthreads();
     if (threadIdx.x == 0) {
-        sum = 0.;
+        sum = but = 0.;
 #pragma unroll
         for (int w = 0; w < DV_THREADS / 64; w++) {
             sum += sums[w];
+            but += buts[w];
             first = min(first, at[w]);
         }
         rec[((long long)which * a.n_rows + r) * a.chunks + c] = {m, first, sum};
+        if (apart) others[r] = but;
     }
-    // the judged draft's logit, for the choice
-    if (threadIdx.x == 64 && r + 1 < q0 + n) {
-        const int v = a.tokens[r + 1];
-        if ((unsigned)v < (unsigned)a.vocab && v / DV_CHUNK == c) drafted[(long long)which * a.n_rows + r] = (float)row[v];
-    }
+    // the guess's logit, for the choice
+    if (threadIdx.x == 64 && has) drafted[(long long)which * a.n_rows + r] = (float)row[guess];
 }
 
-// A row's records as one, by a wave.
-__device__ __forceinline__ DvRow dv_row(const DvRec *rec, int chunks, double k) {
+// A row's records as one, by a wave; mine: the lane's first (lane below chunks).
+__device__ __forceinline__ DvRow dv_row(const DvRec *rec, const DvRec &mine, int chunks, double k) {
     const int lane = threadIdx.x & 63;
-    float m = -__builtin_huge_valf();
-    for (int c = lane; c < chunks; c += 64) m = fmaxf(m, rec[c].m);
+    float m = mine.m;
+    for (int c = lane + 64; c < chunks; c += 64) m = fmaxf(m, rec[c].m);
     m = wave_max(m);
     const DvLaw law = dv_law(m, k);
     int at = 0x7FFFFFFF;
     double sum = 0.;
     for (int c = lane; c < chunks; c += 64) {
-        const DvRec x = rec[c];
+        const DvRec x = c == lane ? mine : rec[c];
         if (k > 0.) sum += x.sum * dv_weight(law, x.m);
         else if (x.m == m) at = min(at, x.at);
     }
-    if (k > 0.) return {m, -1, dv_sum64(sum)};
+    if (k > 0.) return {m, -1, group_sum<64>(sum)};
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) at = min(at, __shfl_xor(at, d));
     return {m, at, 0.};
@@ -223,11 +234,14 @@ __device__ __forceinline__ DvChoice dv_choose(const SvVerify &a, const DvRec *re
             const bool is = (unsigned)x < (unsigned)a.vocab;
             const float u = judges ? a.u_accept[r] : 0.f, lx = is ? drafted[r] : 0.f;
             const float ly = is && a.draft ? drafted[a.n_rows + r] : 0.f;
-            const DvRow p = dv_row(rec + (long long)r * a.chunks, a.chunks, k);
+            const DvRec *rp = rec + (long long)r * a.chunks, *rq = rec + (long long)(a.n_rows + r) * a.chunks;
+            const DvRec none = {-__builtin_huge_valf(), 0x7FFFFFFF, 0.};
+            const DvRec mp = lane < a.chunks ? rp[lane] : none, mq = lane < a.chunks && judges && a.draft ? rq[lane] : none;
+            const DvRow p = dv_row(rp, mp, a.chunks, k);
             DvRow q = {0.f, -1, 0.};
             double qx = 1.;
             if (judges && a.draft) {
-                q = dv_row(rec + (long long)(a.n_rows + r) * a.chunks, a.chunks, k);
+                q = dv_row(rq, mq, a.chunks, k);
                 qx = dv_prob(q, ly, x, k);
             }
             if (lane == 0) {
@@ -288,7 +302,7 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_rest(const SvVerify a, const 
     for (int i = 0; i < R; i++)
 #pragma unroll
         for (int e = 0; e < N; e++) sum += dv_rest(c, p, q, pi, qi, true, x[i][e], y[i][e], 0);
-    sum = dv_sum64(sum);
+    sum = group_sum<64>(sum);
     if ((threadIdx.x & 63) == 0) sums[threadIdx.x >> 6] = sum;
     __syncthreads();
     if (threadIdx.x == 0) {
@@ -303,11 +317,7 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_rest(const SvVerify a, const 
 template <int WAVES>
 __device__ __forceinline__ double dv_scan(double v, double *lds, double *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const double o = __shfl_up(v, d);
-        if (lane >= d) v += o;
-    }
+    v = wave_scan(v);
     __syncthreads();
     if (lane == 63) lds[wave] = v;
     __syncthreads();
@@ -348,7 +358,8 @@ __device__ __forceinline__ int dv_which(bool yes, int v, double x, int *li, doub
 template <typename T>
 __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvRec *__restrict__ rec,
                                                      const float *__restrict__ drafted,
-                                                     const DvChoice *__restrict__ choice, const double *__restrict__ rest) {
+                                                     const DvChoice *__restrict__ choice, const double *__restrict__ rest,
+                                                     const double *__restrict__ others) {
     constexpr int EACH = DV_CHUNK / DV_PICK, WAVES = DV_PICK / 64, N = 16 / sizeof(T);
     __shared__ double red[WAVES];
     __shared__ int who[WAVES];
@@ -381,21 +392,20 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
             }
             return sum;
         };
-        // a chunk's sum: as the record has it, or k_dv_rest, or (the rejected guess's own chunk) anew
+        // a chunk's sum: as the record has it, or k_dv_rest, or (the rejected guess's own chunk) without the guess
         const int own = c.rest && !d && (unsigned)c.x < (unsigned)a.vocab ? c.x / DV_CHUNK : -1;
-        double anew = 0., total = 0.;
-        if (own >= 0) dv_scan<WAVES>(weights(own), red, &anew);
+        const double but = own >= 0 ? others[c.row] : 0.;
+        double total = 0.;
         auto mass = [&](int k) {
             if (c.rest && d) return rest[(long long)s * a.chunks + k];
-            if (c.rest && k == own) return anew;
             const DvRec r = rec[(long long)c.row * a.chunks + k];
-            return r.sum * dv_weight(p, r.m) * pi;
+            return (c.rest && k == own ? but : r.sum) * dv_weight(p, r.m) * pi;
         };
         // a thread's chunks lie side by side
         const int per = (a.chunks + DV_PICK - 1) / DV_PICK, k0 = min(tid * per, a.chunks), k1 = min(k0 + per, a.chunks);
-        double run = 0.;
+        double run = 0., mine = 0.;
         for (int round = 0; round < 2; round++) {   // (nothing left of p - q: p itself)
-            double mine = 0.;
+            mine = 0.;
             for (int k = k0; k < k1; k++) mine += mass(k);
             run = dv_scan<WAVES>(mine, red, &total) - mine;
             if (total > 0.) break;
@@ -406,7 +416,7 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
         double at = 0., end = 0., before = 0.;
         int f = -1, z = -1;
         for (int k = k0; k < k1; k++) {
-            const double m = mass(k);
+            const double m = per == 1 ? mine : mass(k);
             if (m > 0. && run + m > u * total && f < 0) {
                 f = k;
                 at = run;
@@ -420,7 +430,7 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
         int ck = dv_which<WAVES, false>(f >= 0, f, at, who, red, &before);
         if (ck < 0) ck = dv_which<WAVES, true>(z >= 0, z, end, who, red, &before);
         if (ck >= 0) {
-            const double mine = weights(ck);
+            mine = weights(ck);
             double all;
             run = before + (dv_scan<WAVES>(mine, red, &all) - mine);
             f = z = -1;
@@ -444,11 +454,11 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
     }
 }
 
-// Records, choices, sums of the rest a chunk, the drafts' logits.
+// Records, choices and sums of the rest a chunk or (no draft model) of a chunk without the guess, the drafts' logits.
 struct DvWs {
     DvRec *rec;
     DvChoice *choice;
-    double *rest;
+    double *rest, *others;
     float *drafted;
     size_t bytes;
 };
@@ -463,6 +473,9 @@ static DvWs verify_ws(void *ws, int n_seqs, int n_rows, int vocab, bool draft) {
         at += (size_t)n_seqs * sizeof(DvChoice);
         w.rest = (double *)((char *)ws + at);
         at += (size_t)n_seqs * chunks * sizeof(double);
+    } else {
+        w.others = (double *)((char *)ws + at);
+        at += (size_t)n_rows * sizeof(double);
     }
     w.drafted = (float *)((char *)ws + at);
     w.bytes = at + rows * sizeof(float);
@@ -478,13 +491,14 @@ static hipError_t verify(const SvVerify &a, void *ws, hipStream_t st) {
     if (wgs > (1ll << 32) / DV_THREADS - 1 || (long long)a.n_seqs * a.chunks > (1ll << 32) / DV_THREADS - 1)
         return hipErrorInvalidConfiguration;
     const DvWs w = verify_ws(ws, a.n_seqs, a.n_rows, a.vocab, a.draft != nullptr);
-    if (wgs > 0) hipLaunchKernelGGL(k_dv_stats<T>, dim3((unsigned)wgs), dim3(DV_THREADS), 0, st, a, w.rec, w.drafted);
+    if (wgs > 0) hipLaunchKernelGGL(k_dv_stats<T>, dim3((unsigned)wgs), dim3(DV_THREADS), 0, st, a, w.rec, w.drafted, w.others);
     if (a.draft) {
         hipLaunchKernelGGL(k_dv_choose, dim3(a.n_seqs), dim3(DV_CHOOSE), 0, st, a, w.rec, w.drafted, w.choice);
         hipLaunchKernelGGL(k_dv_rest<T>, dim3((unsigned)(a.n_seqs * a.chunks)), dim3(DV_THREADS), 0, st, a, w.choice,
                            w.rest);
     }
-    hipLaunchKernelGGL(k_dv_pick<T>, dim3(a.n_seqs), dim3(DV_PICK), 0, st, a, w.rec, w.drafted, w.choice, w.rest);
+    hipLaunchKernelGGL(k_dv_pick<T>, dim3(a.n_seqs), dim3(DV_PICK), 0, st, a, w.rec, w.drafted, w.choice, w.rest,
+                       w.others);
     return hipGetLastError();
 }
 
