@@ -108,6 +108,17 @@ __device__ __forceinline__ void mx_load_q(const TA *q, Spread spread, mx_h8 (&hi
 // operands when the product's dims are taken in that order, and of V D / 16 dims of the
 // positions 4 h .. 4 h + 3, whose probabilities it computed; the codes become halves in
 // registers.
+//
+// Bound by HBM where there are many positions: 64 ragged sequences to 8192, 32 / 8 heads
+// of 128, fp16 rows 60 us, 5.3 TB/s.  What that took (a first form: 81):
+//   codes of one row block loaded past the caches: 73 -> 67.5;
+//   16-bit rows' probabilities as halves, one product a tile of V (fp32 rows: two columns'
+//   worth, at no cost): 67.5 -> 62.5.  Over 16-bit pages, four times the bytes hide the
+//   second product; here it is the longer part.  It costs 2^-11 of a probability;
+//   loads without a condition, so that a whole tile stays in flight, and three waves a
+//   SIMD: 62.5 -> 60.
+// One sequence of 131072: 16 us (4.5 TB/s), of 4096: 6, a chain of page, codes, products and
+// the workgroup's own join.
 // ---------------------------------------------------------------------------
 template <int D>
 struct MxRaw {
@@ -325,6 +336,13 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(3
 // Many rows.  pg_chunk's products over LDS tiles of 64 positions as halves; a tile's codes
 // come to registers two tiles ahead and to LDS as halves one tile ahead, each wave
 // those of one 16-position block.
+//
+// 2048 tokens after 8192, 32 / 8 heads of 128, fp16: 335 us, 0.92 PFLOP/s, where power
+// bounds it, as over fp16 pages (337); shorter chunks take 3-10% longer than over those,
+// for the codes' conversions.  Nine mixed sequences under a window of 1024 + 4, heads of 64,
+// bf16: 39, about 19 tiles one after the other in 304 workgroups on 256 CUs.  Not kept for
+// it: three waves a SIMD (no change), codes two tiles ahead in two sets of registers (no
+// change), the positions in two ranges (32, and 9.5 the join).
 // ---------------------------------------------------------------------------
 template <int D>
 struct McLds {

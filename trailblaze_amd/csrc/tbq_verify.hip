@@ -11,6 +11,8 @@
 // Three launches: a chunk's largest logit and sum of exponentials, for all rows;
 // with a draft model, the sums of max(p - q, 0) a chunk for the one row of a
 // sequence that is drawn from; and the draw, which looks for its token in one chunk.
+// (A launch of its own says, with a draft model, which row that is: in every workgroup of
+// the sums' launch it cost more than it spared.)
 #include "tbq_kernels.h"
 #include "tbq_serve.hpp"
 
@@ -91,7 +93,9 @@ __device__ __forceinline__ double dv_rate(const SvVerify &a, int s) {
     return t > 0. ? fmax(1.4426950408889634 / t, 1e-34) : 0.;   // (1e-34 of any two finite ones is alike)
 }
 
-// Block x: chunk, row, and (draft) whose logits.  Bound by HBM and the exponentials' fp64.
+// Block x: chunk, row, and (draft) whose logits.  Bound by the vector units: 29 instructions a
+// logit, 14 of them fp64, 88% of the cycles (218 + 154 rows of 151936, fp32: 59 us, 3.8 TB/s;
+// loads past the caches changed nothing).
 template <typename T>
 __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec *__restrict__ rec,
                                                          float *__restrict__ drafted, double *__restrict__ others) {
@@ -354,7 +358,9 @@ __device__ __forceinline__ int dv_which(bool yes, int v, double x, int *li, doub
     return found;
 }
 
-// The draw, a workgroup a sequence.
+// The draw, a workgroup a sequence: a chain of records, the scan of the chunks, one chunk's logits and
+// the scan of its weights (5 rows of 151936, the choice within: 6.8 us; with sums by shuffles and the
+// guess's chunk formed again 9.4).
 template <typename T>
 __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvRec *__restrict__ rec,
                                                      const float *__restrict__ drafted,
