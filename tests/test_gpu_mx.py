@@ -500,6 +500,32 @@ def test_streams_and_repeats():
     assert torch.equal(b["out"], want) and torch.equal(b["K"], a["K"])
 
 
+def test_two_steps_at_once():
+    """Two caches' steps on two streams, none waiting for the other."""
+    torch = _torch()
+    sets = [_state(7, "f16"), _state(8, "bf16")]
+    want = [_step(s).clone() for s in sets]
+    streams = [torch.cuda.Stream() for _ in sets]
+    torch.cuda.synchronize()
+    for _ in range(5):
+        for s, st in zip(sets, streams):
+            _step(s, stream=st)
+        torch.cuda.synchronize()
+        for s, w in zip(sets, want):
+            assert torch.equal(s["out"], w)
+
+
+@pytest.mark.parametrize("act", ACTS)
+def test_append_writes_over_its_own_q(act):
+    torch = _torch()
+    a, b = _state(9, act), _state(9, act)
+    _step(a)
+    q = b["x"][:, :4].clone()
+    paged.kv_append(b["c"], 0, b["b"], q, b["x"][:, 4:6], b["x"][:, 6:], q, rope=b["rope"])
+    torch.cuda.synchronize()
+    assert torch.equal(q, a["q"]) and torch.equal(b["K"], a["K"]) and torch.equal(b["V"], a["V"])
+
+
 @pytest.mark.parametrize("hidden", [256, 8448])
 def test_dense_step_over_an_mxfp4_cache(oracle, hidden):
     """Prompts, chunks and single tokens of two sequences through the model's forward: the keys and values

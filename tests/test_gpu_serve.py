@@ -262,6 +262,36 @@ def test_verify_infinite_and_missing_logits(act, draft):
         run_verify(rng, [2, 2, 3, 2, 4, 1, 1, 3], 9000, act, draft, T, change=odd)
 
 
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("act", ["f32", "bf16"])
+def test_verify_guesses_at_the_borders_of_chunks(act, draft):
+    """Rejected guesses at the ends of the parts that a row is summed in, guesses that are the largest of their
+    part or the only weight in it, and a part that has no other weight."""
+    at = [0, 4095, 4096, 8191, 8192, 12287, 12288, 5, 5000]
+
+    def change(logits, dl, tokens, ua, un):
+        for i, x in enumerate(at):
+            tokens[2 * i + 1] = x
+            if i % 3 == 1:   # nearly all of the row's weight
+                logits[2 * i, x] = 14.0
+            if i % 3 == 2:   # the only weight of its part
+                logits[2 * i, x // 4096 * 4096:(x // 4096 + 1) * 4096] = -float("inf")
+                logits[2 * i, x] = 9.0
+        tokens[-1] = 8190    # a row of nothing else, whose guess is outside its weight
+        logits[-2] = -float("inf")
+        logits[-2, 8189] = 1.0
+    for T in (None, [0.05] * 10, [3.0] * 10):
+        for seed in range(3):
+            rng = np.random.default_rng(seed)
+            run_verify(rng, [2] * 10, 12289, act, draft, T, change=change, u=(1 - 2.0 ** -24, float(rng.random())))
+
+
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_more_chunks_than_threads(draft):
+    """A vocabulary of 537 parts."""
+    run_verify(np.random.default_rng(8), [2, 1], 2200003, draft=draft, T=[0.8, 1.0], u=(1 - 2.0 ** -24, 0.75))
+
+
 def test_verify_draft_equal_to_the_target():
     """p = q: nothing is rejected, whatever the numbers; where a draft has no weight at all, p is drawn from."""
     rng = np.random.default_rng(5)
@@ -329,6 +359,43 @@ def test_verify_is_captured_and_repeats():
     call(b, stream=st)
     st.synchronize()
     assert [x.tolist() for x in b["o"]] == [x.tolist() for x in e["o"]]
+
+
+def test_two_verifications_and_tables_at_once():
+    """Calls on two streams with workspaces and outputs of their own, none waiting for the other."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(5)
+    S, R, V = 8, 32, 50001
+    q = ints(list(range(0, 33, 4)))
+    l = 3 * torch.randn(R, V, generator=g).cuda()
+    d = l + 0.5 * torch.randn(R, V, generator=g).cuda()
+    tok = torch.cat([torch.zeros(1, device="cuda"), l.argmax(-1)[:-1].float()]).int()
+    ua, un = torch.rand(R, generator=g).cuda(), torch.rand(S, generator=g).cuda()
+    sets = []
+    for dl in (d, None):
+        n = paged.draft_verify_workspace_size(S, R, V, torch.float32, dl is not None)
+        t = dict(kv_len=ints([100 * i for i in range(S)]), new=ints([4] * S), drop=ints([i % 3 for i in range(S)]),
+                 table=ints([[64 * s + e for e in range(64)] for s in range(S)]), free=ints(list(range(512, 1024))), n_free=ints([500]),
+                 q_start=ints([0] * (S + 1)), lens=ints([0] * S), out=ints([[0] * 64] * S), fo=ints([0] * 512), no=ints([0]))
+        h = paged.kv_tables(16, t["kv_len"], t["new"], t["table"], t["free"], t["n_free"], q_start=t["q_start"], n_drop=t["drop"],
+                            kv_len_out=t["lens"], table_out=t["out"], free_out=t["fo"], n_free_out=t["no"])
+        sets.append((dl, torch.empty(n, dtype=torch.uint8, device="cuda"), [ints([77] * S) for _ in range(3)], t, h))
+
+    def call(x, stream=None):
+        dl, ws, o, t, h = x
+        paged.draft_verify(q, tok, l, ua, un, o[0], o[1], n_drop=o[2], draft_logits=dl, workspace=ws, stream=stream)
+        paged.kv_build_tables(h, stream=stream)
+        return [*o, t["lens"], t["out"], t["fo"], t["no"], t["q_start"]]
+    want = [[y.clone() for y in call(x)] for x in sets]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(5):
+        for x, st in zip(sets, streams):
+            call(x, stream=st)
+        torch.cuda.synchronize()
+    for x, w in zip(sets, want):
+        for y, z in zip([*x[2], x[3]["lens"], x[3]["out"], x[3]["fo"], x[3]["no"], x[3]["q_start"]], w):
+            assert torch.equal(y, z)
 
 
 # ---- together ------------------------------------------------------------------------
