@@ -87,6 +87,17 @@ def test_tables(seqs, page, past, drop, new, place):
 
 
 @pytest.mark.parametrize("place", ["apart", "in place"])
+@pytest.mark.parametrize("seqs,page,past,new", [(40, 16, 5000, 5000), (1030, 16, 200, 100), (1, 16, 150000, 150000), (65, 16, 1200, 1200)])
+def test_tables_of_many_pages(seqs, page, past, new, place):
+    """More pages given and taken in a call than the workgroup has threads, by some multiples."""
+    rng = np.random.default_rng(seqs)
+    lens, table, free, n = state(rng, seqs, page, past, seqs * (new // page + 1), width=2 + new // page)
+    d, a = rng.integers(0, past + 1, seqs).tolist(), rng.integers(0, new + 1, seqs).tolist()
+    assert check(page, sum(a), lens, d, a, table, free, n, place=place)["served"] == [seqs]
+    check(page, sum(a), lens, [past] * seqs, a, table, free, 5, place=place)
+
+
+@pytest.mark.parametrize("place", ["apart", "in place"])
 @pytest.mark.parametrize("spare", [0, 1, 30])
 def test_tables_not_all_served(spare, place):
     """Too few pages, rows or entries of a table: from the first sequence they do not suffice for on, none is

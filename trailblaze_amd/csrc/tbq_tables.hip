@@ -5,72 +5,96 @@
 // free list, of the pages that are taken from its end, of the new tokens.  One
 // workgroup forms them, 1024 sequences at a time, and moves the pages (whose number
 // is small beside the tables); a launch over tokens and table entries follows.
-// Bound by the first one's chain of dependent loads: lengths, pages that go back, the
-// list's end (64 sequences of 8000 positions: 6.0 + 2.5 us; 1000 of 6000, 30 prompts among
-// them: 10.6 + 4.  A scan each for pages given, pages taken and tokens, instead of one: 11
-// and 20 in all.)
+// Bound by the first one's chain of dependent loads and barriers: lengths, pages that go
+// back, the list's end (64 sequences of 8000 positions: 4.0 + 2.5 us; 1000 of 6000, 30
+// prompts among them: 6.7 + 4).  LDS is what the 16 waves of one workgroup wait for: with
+// wave sums that every thread adds for itself and searches in waves without an entry,
+// 6.0 and 10.6 in the first launch; with a scan each for pages given, pages taken and tokens
+// 11 and 20 in all.
+#include <type_traits>
+
 #include "tbq_kernels.h"
 #include "tbq_serve.hpp"
 
 namespace tbq {
 
-constexpr int TB_THREADS = 1024, TB_WAVES = TB_THREADS / 64;
+constexpr int TB_THREADS = 1024, TB_WAVES = TB_THREADS / 64, TB_EACH = 4;   // most entries of a thread at a time
 struct TbLds {
     int3 wave[2][TB_WAVES];                   // sums of the waves' sequences (by turns)
-    int count[2][TB_WAVES];
-    int end[TB_THREADS], first[TB_THREADS];   // inclusive sums of a chunk's entries; each sequence's first entry
-    int fail, take, tokens;
+    int count[2][TB_EACH * TB_WAVES];
+    int3 fail[TB_WAVES];                      // a wave's first sequence that is not served, pages taken and tokens before it
+    // of a chunk's sequences, inclusive sums of the entries that each gives back and takes, and its first entry less
+    // those before it
+    int given[TB_THREADS], give[TB_THREADS], taken[TB_THREADS], take[TB_THREADS];
 };
 
 constexpr int TB_MOST = 1 << 30;   // tokens of a call; sums of them stop behind it
 __device__ __forceinline__ int3 tb_add(int3 a, int3 b) {
     return make_int3(a.x + b.x, a.y + b.y, (int)min((unsigned)a.z + (unsigned)b.z, (unsigned)TB_MOST + 1u));
 }
-// Inclusive sums over the workgroup of pages given, pages taken (below 2^31: a table has no more entries)
-// and tokens; and the whole ones.  One barrier; turn: 0 and 1 by turns.
-__device__ __forceinline__ int3 tb_scan(int3 v, TbLds *lds, int turn, int3 *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-        const int3 o = make_int3(__shfl_up(v.x, d), __shfl_up(v.y, d), __shfl_up(v.z, d));
-        if (lane >= d) v = tb_add(v, o);
-    }
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ int tb_dpp(int v) { return __builtin_amdgcn_update_dpp(0, v, CTRL, ROWS, 0xF, false); }
+template <int CTRL, int ROWS = 0xF>
+__device__ __forceinline__ int3 tb_dpp(int3 v) {
+    return make_int3(tb_dpp<CTRL, ROWS>(v.x), tb_dpp<CTRL, ROWS>(v.y), tb_dpp<CTRL, ROWS>(v.z));
+}
+__device__ __forceinline__ int tb_add(int a, int b) { return a + b; }
+__device__ __forceinline__ int tb_lane(int v, int l) { return __builtin_amdgcn_readlane(v, l); }
+__device__ __forceinline__ int3 tb_lane(int3 v, int l) { return make_int3(tb_lane(v.x, l), tb_lane(v.y, l), tb_lane(v.z, l)); }
+// Inclusive sums over rows of 16 lanes; over the wave.
+template <typename T>
+__device__ __forceinline__ T tb_row_scan(T v) {
+    v = tb_add(v, tb_dpp<0x111>(v));   // row_shr 1, 2, 4, 8
+    v = tb_add(v, tb_dpp<0x112>(v));
+    v = tb_add(v, tb_dpp<0x114>(v));
+    return tb_add(v, tb_dpp<0x118>(v));
+}
+template <typename T>
+__device__ __forceinline__ T tb_wave_scan(T v) {
+    v = tb_row_scan(v);
+    v = tb_add(v, tb_dpp<0x142, 0xA>(v));   // row_bcast 15, 31
+    return tb_add(v, tb_dpp<0x143, 0xC>(v));
+}
+// Sums over the workgroup, in front of each thread, of pages given, pages taken (below 2^31: a table has no more
+// entries) and tokens; and the whole ones.  One barrier; turn: 0 and 1 by turns.
+__device__ __forceinline__ int3 tb_scan(int3 own, TbLds *lds, int turn, int3 *total) {
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const int3 v = tb_wave_scan(own), before = tb_dpp<0x138>(v);   // wave_shr 1
     if (lane == 63) lds->wave[turn][wave] = v;
     __syncthreads();
-    int3 before = make_int3(0, 0, 0), all = before;
-#pragma unroll
-    for (int w = 0; w < TB_WAVES; w++) {
-        if (w == wave) before = all;
-        all = tb_add(all, lds->wave[turn][w]);
-    }
-    *total = all;
-    return tb_add(before, v);
+    const int3 w = tb_row_scan(lds->wave[turn][lane % TB_WAVES]);
+    *total = tb_lane(w, TB_WAVES - 1);
+    return wave ? tb_add(tb_lane(w, wave - 1), before) : before;
 }
-// How many threads up to this one say yes, and how many do.
-__device__ __forceinline__ int tb_count(bool yes, TbLds *lds, int turn, int *total) {
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const uint64_t b = __builtin_amdgcn_ballot_w64(yes);
-    if (lane == 0) lds->count[turn][wave] = __builtin_popcountll(b);
-    __syncthreads();
-    int before = 0, all = 0;
+// How many yeses there are before each of the threads' N, the threads' first ones coming first; and how many in all.
+template <int N>
+__device__ __forceinline__ void tb_count(const bool (&yes)[N], TbLds *lds, int turn, int (&before)[N], int *total) {
+    static_assert(N * TB_WAVES <= 64, "a lane a count");
+    const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
 #pragma unroll
-    for (int w = 0; w < TB_WAVES; w++) {
-        if (w == wave) before = all;
-        all += lds->count[turn][w];
+    for (int i = 0; i < N; i++) {
+        const uint64_t b = __builtin_amdgcn_ballot_w64(yes[i]);
+        before[i] = __builtin_popcountll(b & ((1ull << lane) - 1));
+        if (lane == 0) lds->count[turn][TB_WAVES * i + wave] = __builtin_popcountll(b);
     }
-    *total = all;
-    return before + __builtin_popcountll(b & (lane == 63 ? ~0ull : (2ull << lane) - 1));
+    __syncthreads();
+    const int own = lds->count[turn][lane % (N * TB_WAVES)], sum = N == 1 ? tb_row_scan(own) : tb_wave_scan(own);
+    *total = tb_lane(sum, N * TB_WAVES - 1);
+#pragma unroll
+    for (int i = 0; i < N; i++) before[i] += tb_lane(sum - own, TB_WAVES * i + wave);
 }
 
-// The sequence of a chunk that entry j belongs to: the first whose end is above j.
-__device__ __forceinline__ int tb_find(const TbLds *lds, int n, int j) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {
-        const int mid = (lo + hi) >> 1;
-        if (lds->end[mid] > j) hi = mid;
-        else lo = mid + 1;
+// The sequences (of n, 1 to 1024) that the entries j belong to: the first whose end is above j, which there is.
+template <int N>
+__device__ __forceinline__ void tb_find(const int *end, int n, const int (&j)[N], int (&at)[N]) {
+#pragma unroll
+    for (int i = 0; i < N; i++) at[i] = 0;
+    for (int step = 512; step; step >>= 1) {
+        if (step >= n) continue;   // uniform
+#pragma unroll
+        for (int i = 0; i < N; i++)
+            if (end[min(at[i] + step, n) - 1] <= j[i]) at[i] += step;
     }
-    return lo;
 }
 
 // Sequence s before the call: positions kept, pages of them and of all, new tokens; the pages it needs
@@ -93,76 +117,102 @@ __device__ __forceinline__ int3 tb_sums(const TbSeq &q) {
 __global__ __launch_bounds__(TB_THREADS) void k_tables_plan(const SvTables a) {
     __shared__ TbLds lds;
     const tbq_kv_tables &t = a.t;
-    const int tid = threadIdx.x, listed = min(max(t.n_free[0], 0), t.n_pages);
+    const int tid = threadIdx.x, lane = tid & 63, listed = min(max(t.n_free[0], 0), t.n_pages);
     TbSeq q{};
-    int3 sum{}, all{};
+    int3 own{}, sum{}, all{};   // the sequence's, those before it, the chunk's
+    int turn = 0;
+    // a chunk's sequences and where their entries begin
+    auto chunk = [&](int s0, int n) {
+        q = tb_seq(a, s0 + tid, tid < n);
+        own = tb_sums(q);
+        sum = tb_scan(own, &lds, turn ^= 1, &all);
+        lds.given[tid] = sum.x + own.x;
+        lds.give[tid] = q.kept - sum.x;
+        lds.taken[tid] = sum.y + own.y;
+        lds.take[tid] = q.kept - sum.y;
+        __syncthreads();
+    };
+    // n entries: one a thread, or TB_EACH while there are more than threads
+    auto rounds = [&](int n, auto f) {
+        int j0 = 0;
+        for (; n - j0 > TB_THREADS; j0 += TB_EACH * TB_THREADS) f(j0, std::integral_constant<int, TB_EACH>{});
+        if (j0 < n) f(j0, std::integral_constant<int, 1>{});
+    };
     // pages behind the last kept position go to the list, in the sequences' order
-    int have = listed, turn = 0;
+    int have = listed;
     for (int s0 = 0; s0 < t.n_seqs; s0 += TB_THREADS) {
         const int n = min(TB_THREADS, t.n_seqs - s0);
-        q = tb_seq(a, s0 + tid, tid < n);
-        sum = tb_scan(tb_sums(q), &lds, turn ^= 1, &all);
-        if (all.x == 0) continue;   // uniform
-        lds.end[tid] = sum.x;
-        lds.first[tid] = q.kept - (sum.x - (q.held - q.kept));
-        __syncthreads();
-        for (int j0 = 0; j0 < all.x; j0 += TB_THREADS) {
-            const int j = j0 + tid;
-            int page = -1, count;
-            if (j < all.x) {
-                const int i = tb_find(&lds, n, j);
-                page = t.page_table[(long long)(s0 + i) * t.max_pages + lds.first[i] + j];
+        chunk(s0, n);
+        rounds(all.x, [&](int j0, auto each) {
+            constexpr int N = decltype(each)::value;
+            int j[N], i[N], page[N], before[N], count;
+            bool is[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                j[e] = min(j0 + e * TB_THREADS + tid, all.x - 1);
+                page[e] = -1;
             }
-            const bool is = (unsigned)page < (unsigned)t.n_pages;
-            const int at = have + tb_count(is, &lds, turn ^= 1, &count) - 1;
-            if (is && at < t.n_pages) t.free_out[at] = page;
+            if (j0 + (tid & ~63) < all.x) {   // the wave has some
+                tb_find(lds.given, n, j, i);
+#pragma unroll
+                for (int e = 0; e < N; e++)
+                    page[e] = t.page_table[(long long)(s0 + i[e]) * t.max_pages + lds.give[i[e]] + j[e]];
+            }
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                is[e] = j0 + e * TB_THREADS + tid < all.x && (unsigned)page[e] < (unsigned)t.n_pages;
+            tb_count(is, &lds, turn ^= 1, before, &count);
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (is[e] && have + before[e] < t.n_pages) t.free_out[have + before[e]] = page[e];
             have = min(have + count, t.n_pages);
-        }
+        });
+        if (t.n_seqs > TB_THREADS) __syncthreads();   // the sums are rewritten
     }
     __threadfence_block();
     // then sequences take pages from its end, until one does not get what it needs
-    long long taken = 0, rows = 0;
-    int served = 0;
+    int taken = 0, rows = 0, served = 0;
     bool going = true;
     for (int s0 = 0; s0 < t.n_seqs; s0 += TB_THREADS) {
         const int n = min(TB_THREADS, t.n_seqs - s0);
-        if (t.n_seqs > TB_THREADS) {
-            q = tb_seq(a, s0 + tid, tid < n);
-            sum = tb_scan(tb_sums(q), &lds, turn ^= 1, &all);
-        }
-        if (tid == 0) lds.fail = n;
+        if (t.n_seqs > TB_THREADS) chunk(s0, n);
+        const bool fails = tid < n && (!going || q.need < 0 || sum.y + own.y > have - taken || tb_add(sum, own).z > t.n_tokens - rows);
+        const uint64_t b = __builtin_amdgcn_ballot_w64(fails);
+        if (lane == (b ? __builtin_ctzll(b) : 0)) lds.fail[tid >> 6] = b ? make_int3(tid, sum.y, sum.z) : make_int3(n, 0, 0);
         __syncthreads();
-        if (tid < n && (!going || q.need < 0 || taken + sum.y > have || rows + sum.z > t.n_tokens)) atomicMin(&lds.fail, tid);
-        __syncthreads();
-        const int fail = lds.fail, take = q.need < 0 ? 0 : q.need - q.kept;
-        if (tid == fail) lds.take = sum.y - take;
-        // (the tokens before the first that fails are its predecessor's sum: its own may have stopped)
-        if (tid + 1 == fail) lds.tokens = sum.z;
-        lds.end[tid] = tid < fail ? sum.y : 0x7FFFFFFF;
-        lds.first[tid] = q.kept - (sum.y - take);
-        __syncthreads();
-        int all_take = all.y, all_rows = all.z;
-        if (fail < n) {
-            all_take = lds.take;
-            all_rows = fail == 0 ? 0 : lds.tokens;
-        }
+        const int3 f = lds.fail[lane % TB_WAVES];
+        const uint64_t w = __builtin_amdgcn_ballot_w64(f.x < n);
+        const int3 first = tb_lane(f, w ? __builtin_ctzll(w) : 0);   // (a wave's fails are behind those of the waves before)
+        const int fail = w ? first.x : n, all_take = w ? first.y : all.y, all_rows = w ? first.z : all.z;
         if (tid < n) {
             t.kv_len_out[s0 + tid] = q.base + (tid < fail ? q.add : 0);
-            t.q_start[s0 + tid + 1] = (int)(rows + (tid < fail ? sum.z : all_rows));
+            t.q_start[s0 + tid + 1] = rows + (tid < fail ? sum.z + own.z : all_rows);
         }
-        for (int j = tid; j < all_take; j += TB_THREADS) {
-            const int i = tb_find(&lds, n, j), at = have - 1 - (int)taken - j;
-            t.page_table_out[(long long)(s0 + i) * t.max_pages + lds.first[i] + j] =
-                at < listed ? t.free_pages[at] : t.free_out[at];
-        }
+        rounds(all_take, [&](int j0, auto each) {
+            constexpr int N = decltype(each)::value;
+            if (j0 + (tid & ~63) >= all_take) return;   // the wave has none
+            int j[N], i[N], page[N];
+#pragma unroll
+            for (int e = 0; e < N; e++) {
+                j[e] = min(j0 + e * TB_THREADS + tid, all_take - 1);
+                const int at = have - 1 - taken - j[e];
+                page[e] = *(at < listed ? t.free_pages + at : t.free_out + at);
+            }
+            tb_find(lds.taken, n, j, i);
+#pragma unroll
+            for (int e = 0; e < N; e++)
+                if (j0 + e * TB_THREADS + tid < all_take)
+                    t.page_table_out[(long long)(s0 + i[e]) * t.max_pages + lds.take[i[e]] + j[e]] = page[e];
+        });
         taken += all_take;
         rows += all_rows;
         served += fail;
         going = going && fail == n;
+        if (t.n_seqs > TB_THREADS) __syncthreads();   // the sums are rewritten
     }
     if (tid == 0) {
         t.q_start[0] = 0;
-        t.n_free_out[0] = have - (int)taken;
+        t.n_free_out[0] = have - taken;
         if (t.served) t.served[0] = served;
     }
 }
