@@ -15,7 +15,7 @@ import ctypes as C
 from array import array
 from operator import index
 
-from . import TbqError, _check, _ptr, _stream, _workspace, lib
+from . import TbqError, _check, _stream, _workspace, lib
 
 F32, F16, BF16, MXFP4 = 0, 1, 30, 39
 ROPE_HALF, ROPE_INTERLEAVED = 0, 1
@@ -121,17 +121,30 @@ def _heads(name, t, rows, n_heads, D, dev):
     """Elements between the rows of [rows][heads][D], whose heads lie side by side."""
     if t.shape != (rows, n_heads, D):
         raise ValueError(f"{name}: {(rows, n_heads, D)} expected, got {tuple(t.shape)}")
-    _on(name, t, dev)
-    st = t.stride()
-    if st[2] != 1 or (n_heads > 1 and st[1] != D):
+    if t.get_device() != dev:
+        _on(name, t, dev)
+    row, head, one = t.stride()
+    if one != 1 or (n_heads > 1 and head != D):
         raise ValueError(f"{name}: the heads of a row must lie side by side")
-    return st[0] if rows > 1 else n_heads * D
+    return row if rows > 1 else n_heads * D
 
 
 def _flat(name, t, shape, dtype, dev):
-    if t.shape != shape or t.dtype != dtype or not t.is_contiguous():
+    """The address of a contiguous tensor."""
+    if t.dtype is not dtype or t.shape != shape or not t.is_contiguous():
         raise ValueError(f"{name}: contiguous {dtype} {shape} expected, got {t.dtype} {tuple(t.shape)}")
-    _on(name, t, dev)
+    if t.get_device() != dev:
+        _on(name, t, dev)
+    return t.data_ptr()
+
+
+def _vec(name, t, n, dtype, dev):
+    """_flat of n elements, or nothing (t None)."""
+    if t is None:
+        return None
+    if t.dtype is not dtype or t.numel() != n or t.dim() != 1 or not t.is_contiguous() or t.get_device() != dev:
+        _flat(name, t, (n,), dtype, dev)
+    return t.data_ptr()
 
 
 def kv_head_bytes(page_size: int, head_dim: int, type_id: int = MXFP4) -> int:
@@ -226,17 +239,14 @@ def kv_append(cache: KvCache, layer: int, batch: KvBatch, q, k, v, q_out, rope: 
         nq = q.shape[1]
         qs = _heads("q", q, T, nq, D, dev)
         q_type = _type_id(q_out.dtype)
-        _flat("q_out", q_out, (T, nq, D), q_out.dtype, dev)
-        qp, qo = q.data_ptr(), q_out.data_ptr()
-    if q_norm is not None:
-        _flat("q_norm", q_norm, (D,), _torch.float32, dev)
-    if k_norm is not None:
-        _flat("k_norm", k_norm, (D,), _torch.float32, dev)
+        qp, qo = q.data_ptr(), _flat("q_out", q_out, (T, nq, D), q_out.dtype, dev)
+    f32 = _torch.float32
+    qn, kn = _vec("q_norm", q_norm, D, f32, dev), _vec("k_norm", k_norm, D, f32, dev)
     if positions is not None:
         _ints("positions", positions, (T,))
         _on("positions", positions, dev)
     _check(lib().tbq_kv_append(C.byref(cache), layer, C.byref(batch), nq, None if rope is None else C.byref(rope),
-                               _ptr(q_norm), _ptr(k_norm), eps, _ptr(positions), in_type, qp, qs, k.data_ptr(), ks,
+                               qn, kn, eps, None if positions is None else positions.data_ptr(), in_type, qp, qs, k.data_ptr(), ks,
                                v.data_ptr(), vs, q_type, qo, _to(stream, dev)), "tbq_kv_append")
     return q_out
 
@@ -278,16 +288,16 @@ def kv_dequant(cache: KvCache, layer: int, k_out, v_out, pages=None, stream=None
     [page size][head dim] of one floating type.  pages: int32 device tensor [n]
     (None: the first n pages)."""
     dev = _here(cache)
-    _int("layer", layer)
+    if not -_INT <= layer < _INT:
+        _int("layer", layer)
     shape = (k_out.shape[0] if k_out.dim() else 0, cache.n_kv_heads, cache.page_size, cache.head_dim)
     out_type = _type_id(k_out.dtype)
-    _flat("k_out", k_out, shape, k_out.dtype, dev)
-    _flat("v_out", v_out, shape, k_out.dtype, dev)
+    kp, vp = _flat("k_out", k_out, shape, k_out.dtype, dev), _flat("v_out", v_out, shape, k_out.dtype, dev)
     if pages is not None:
         _ints("pages", pages, (shape[0],))
         _on("pages", pages, dev)
     _check(lib().tbq_kv_dequant(C.byref(cache), layer, None if pages is None else pages.data_ptr(), shape[0], out_type,
-                                k_out.data_ptr(), v_out.data_ptr(), _to(stream, dev)), "tbq_kv_dequant")
+                                kp, vp, _to(stream, dev)), "tbq_kv_dequant")
     return k_out, v_out
 
 
@@ -389,14 +399,11 @@ def draft_verify(q_start, tokens, logits, u_accept, u_next, n_accept, next_token
         if draft_logits.dtype != logits.dtype:
             raise ValueError("logits and draft_logits: one type")
         dstride = _rows_of("draft_logits", draft_logits, rows, vocab, dev)
-    for name, t, m in (("q_start", q_start, n + 1), ("tokens", tokens, rows), ("n_accept", n_accept, n),
-                       ("next_token", next_token, n), ("n_drop", n_drop, n)):
-        if t is not None:
-            _ints(name, t, (m,))
-            _on(name, t, dev)
-    for name, t, m in (("u_accept", u_accept, rows), ("u_next", u_next, n), ("temperature", temperature, n)):
-        if t is not None:
-            _flat(name, t, (m,), _torch.float32, dev)
+    i32, f32 = _torch.int32, _torch.float32
+    starts, toks = _vec("q_start", q_start, n + 1, i32, dev), _vec("tokens", tokens, rows, i32, dev)
+    outs = _vec("n_accept", n_accept, n, i32, dev), _vec("next_token", next_token, n, i32, dev), _vec("n_drop", n_drop, n, i32, dev)
+    temp = _vec("temperature", temperature, n, f32, dev)
+    us = _vec("u_accept", u_accept, rows, f32, dev), _vec("u_next", u_next, n, f32, dev)
     to = _to(stream, dev)
     if workspace is None:
         size = draft_verify_workspace_size(n, rows, vocab, logits.dtype, draft_logits is not None)
@@ -407,10 +414,9 @@ def draft_verify(q_start, tokens, logits, u_accept, u_next, n_accept, next_token
         if not workspace.is_contiguous():
             raise ValueError("workspace: contiguous")
     wp, wb = (None, 0) if workspace is None else (workspace.data_ptr(), workspace.numel() * workspace.element_size())
-    ptr = lambda t: None if t is None else t.data_ptr()   # noqa: E731
-    _check(lib().tbq_draft_verify(n, rows, vocab, type_id, ptr(q_start), ptr(tokens), ptr(logits), stride, ptr(draft_logits),
-                                  dstride, ptr(temperature), ptr(u_accept), ptr(u_next), ptr(n_accept), ptr(next_token),
-                                  ptr(n_drop), wp, wb, to), "tbq_draft_verify")
+    _check(lib().tbq_draft_verify(n, rows, vocab, type_id, starts, toks, logits.data_ptr(), stride,
+                                  None if draft_logits is None else draft_logits.data_ptr(), dstride, temp, *us, *outs, wp, wb,
+                                  to), "tbq_draft_verify")
     return next_token
 
 
