@@ -298,6 +298,33 @@ def test_verify_guesses_at_the_borders_of_chunks(act, draft):
 
 
 @pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("size", [1e-43, 1e-36, 1e-20, 1e20, 1e36])
+def test_verify_sizes_of_logits_and_temperatures(size, draft):
+    """Logits and temperatures far from 1, in proportion: the probabilities are ordinary ones."""
+    def change(logits, dl, tokens, ua, un):
+        for t in (logits,) if dl is None else (logits, dl):
+            t *= size
+    T = [float(np.float32(size * x)) for x in (0.5, 1.0, 2.0, 0.3)]
+    run_verify(np.random.default_rng(11), [4, 1, 6, 3], 9000, draft=draft, T=T, change=change)
+
+
+@pytest.mark.parametrize("draft", [False, True])
+@pytest.mark.parametrize("T", [1e33, 1e35, 1e37, 3e38, float("inf")])
+def test_verify_hot_temperatures_over_masks(T, draft):
+    """Where every finite logit has weight, the lowest one too, masked ones (-infinity, NaN) still have none."""
+    low = float(np.finfo(np.float32).min)
+
+    def change(logits, dl, tokens, ua, un):
+        for t in (logits,) if dl is None else (logits, dl):
+            t[:, ::3] = -float("inf")
+            t[:, 1::9] = low
+            t[:, 2::27] = 1e35
+            t[0:3, 50:6000] = float("nan")
+            t[3, 4096:8192] = low
+    run_verify(np.random.default_rng(12), [4, 1, 6, 3], 9000, draft=draft, T=[T] * 4, change=change)
+
+
+@pytest.mark.parametrize("draft", [False, True])
 def test_verify_more_chunks_than_threads(draft):
     """A vocabulary of 537 parts."""
     run_verify(np.random.default_rng(8), [2, 1], 2200003, draft=draft, T=[0.8, 1.0], u=(1 - 2.0 ** -24, 0.75))

@@ -18,8 +18,8 @@
 
 namespace tbq {
 
-constexpr int DV_THREADS = 256, DV_CHOOSE = 1024, DV_PICK = 512;
-
+constexpr int DV_THREADS = 256, DV_WIDE = 128, DV_CHOOSE = 1024, DV_PICK = 512;
+constexpr int DV_MANY = 4096;   // chunks
 
 struct DvRec {      // of a chunk of a row: the largest logit, where first, and the sum of the weights 2^(k (l - m))
     float m;
@@ -31,21 +31,27 @@ typedef DvRec DvRow;   // of a row: the same
 // The weights exp((l - m) / T) of a row whose largest logit is m, by k = log2(e) / T: 2^t, t = k (l - m).
 // t is split into the nearest whole number, which adding 1.5 * 2^52 leaves in the low bits, and r, |r| <= 1/2;
 // 2^r is the polynomial of degree 8 that meets it at the nine Chebyshev points, off by 1.1e-12 of it at most; the
-// whole number goes to the exponent.  Logits from low on have no weight (2^-1000 of the largest, -infinity, NaN);
-// where m is infinite, all below it; k is 0 where only m itself has weight.  With Least set, they have up to 2^-999, for sums alone (k > 0).
+// whole number goes to the exponent.  Logits from none on have no weight (2^-1000 of the largest, -infinity, NaN); where
+// m is infinite, all below it; k is 0 where only m itself has weight.  Those below low count as low: it is none, but for
+// temperatures so high that every finite logit has weight (all).  With Least set, logits without weight have up to
+// 2^-999, for sums alone (k > 0 and not all).
 // (218 + 154 rows of 151936: 113 us with the library's exp, 53 with this.)
 struct DvLaw {
     double k, m;
-    float low;
+    float low, none;
+    __device__ bool all() const { return none < low; }
 };
 __device__ __forceinline__ DvLaw dv_law(float m, double k) {
-    const float most = 3.402823466e38f;
-    if (!(m <= most)) return {0., most, most};
-    const double x = (double)m - 1000. / k;
-    float low = (float)fmax(x, -(double)most);
+    const float most = 3.402823466e38f, inf = __builtin_huge_valf();
+    if (!(m <= most)) return {0., most, most, most};
+    const double x = (double)m - 1000. * __builtin_amdgcn_rcp(k);   // (the instruction's reciprocal: 1000 or nearly)
+    if (x < -(double)most) return {k, m, -most, -inf};
+    float low = (float)x;
     if ((double)low < x) low = nextafterf(low, most);   // (not below x)
     // where that leaves no float below m, m alone has weight
-    return low < m ? DvLaw{k, m, low} : DvLaw{0., m, nextafterf(m, -__builtin_huge_valf())};
+    if (low < m) return {k, m, low, low};
+    low = nextafterf(m, -inf);
+    return {0., m, low, low};
 }
 template <bool Least = false>
 __device__ __forceinline__ double dv_weight(const DvLaw &w, float l) {
@@ -61,7 +67,7 @@ __device__ __forceinline__ double dv_weight(const DvLaw &w, float l) {
     p = fma(p, r, 6.931471805459332e-1);
     p = fma(p, r, 1.);
     const uint64_t b = __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, n) << 52);
-    return Least || l > w.low ? __builtin_bit_cast(double, b) : 0.;
+    return Least || l > w.none ? __builtin_bit_cast(double, b) : 0.;
 }
 
 // N elements of a row from element i on (-infinity behind the end).
@@ -90,19 +96,19 @@ __device__ __forceinline__ double dv_random(float u) { return fminf(fmaxf(u, 0.f
 // log2(e) over the temperature; 0: all weight on the largest logit.
 __device__ __forceinline__ double dv_rate(const SvVerify &a, int s) {
     const double t = a.temperature ? a.temperature[s] : 1.;
-    return t > 0. ? fmax(1.4426950408889634 / t, 1e-34) : 0.;   // (1e-34 of any two finite ones is alike)
+    return t > 0. ? fmax(1.4426950408889634 / t, 1e-60) : 0.;   // (1e-60 of any two finite ones is alike)
 }
 
-// Block x: chunk, row, and (draft) whose logits.  Bound by the vector units: 29 instructions a
-// logit, 14 of them fp64, 88% of the cycles (218 + 154 rows of 151936, fp32: 59 us, 3.8 TB/s;
-// loads past the caches changed nothing).
-template <typename T>
-__global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec *__restrict__ rec,
+// Block x: chunk, row, and (draft) whose logits.  Bound by the vector units, which have 18 instructions a
+// logit to do, 14 of them fp64, and about 170 a wave (218 + 154 rows of 151936, fp32: 53.5 us, 4.2 TB/s; with 16
+// logits a thread 59, where they were busy for 88% of the cycles; loads past the caches changed nothing).
+template <typename T, int THREADS>
+__global__ __launch_bounds__(THREADS) void k_dv_stats(const SvVerify a, DvRec *__restrict__ rec,
                                                          float *__restrict__ drafted, double *__restrict__ others) {
-    constexpr int N = 16 / sizeof(T), R = DV_CHUNK / DV_THREADS / N;
-    __shared__ float ms[DV_THREADS / 64];
-    __shared__ int at[DV_THREADS / 64];
-    __shared__ double sums[DV_THREADS / 64], buts[DV_THREADS / 64];
+    constexpr int N = 16 / sizeof(T), R = DV_CHUNK / THREADS / N;
+    __shared__ float ms[THREADS / 64];
+    __shared__ int at[THREADS / 64];
+    __shared__ double sums[THREADS / 64], buts[THREADS / 64];
     const int c = blockIdx.x % a.chunks, r = blockIdx.x / a.chunks % a.n_rows, which = blockIdx.x / a.chunks / a.n_rows;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const T *row = (const T *)(which ? a.draft : a.logits) + r * (which ? a.dstride : a.stride);
@@ -110,7 +116,7 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
     float x[R][N];
     auto load = [&] {
 #pragma unroll
-        for (int i = 0; i < R; i++) dv_load(row, v0 + i * DV_THREADS * N, a.vocab, x[i]);
+        for (int i = 0; i < R; i++) dv_load(row, v0 + i * THREADS * N, a.vocab, x[i]);
     };
     if (!which) load();   // (nearly all of the target's rows are some sequence's)
     const int behind = a.tokens[min(r + 1, a.n_rows - 1)];
@@ -130,7 +136,7 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
     if (lane == 0) ms[wave] = m;
     __syncthreads();
 #pragma unroll
-    for (int w = 0; w < DV_THREADS / 64; w++) m = fmaxf(m, ms[w]);
+    for (int w = 0; w < THREADS / 64; w++) m = fmaxf(m, ms[w]);
     int first = 0x7FFFFFFF;
     double sum = 0., but = 0.;   // of all; of all but the guess, which the draw takes (not a difference: it may be nearly all)
     if (!(k > 0.)) {
@@ -138,19 +144,19 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
         for (int i = R - 1; i >= 0; i--)
 #pragma unroll
             for (int e = N - 1; e >= 0; e--)
-                if (x[i][e] == m) first = v0 + i * DV_THREADS * N + e;
+                if (x[i][e] == m) first = v0 + i * THREADS * N + e;
 #pragma unroll
         for (int d = 1; d < 64; d *= 2) first = min(first, __shfl_xor(first, d));
     } else if (m > -__builtin_huge_valf()) {
         const DvLaw law = dv_law(m, k);
-        if (apart) {   // uniform
+        if (apart || law.all()) {   // uniform
 #pragma unroll
             for (int i = 0; i < R; i++)
 #pragma unroll
                 for (int e = 0; e < N; e++) {
                     const double w = dv_weight(law, x[i][e]);
                     sum += w;
-                    but += v0 + i * DV_THREADS * N + e == guess ? 0. : w;
+                    but += v0 + i * THREADS * N + e == guess ? 0. : w;
                 }
             but = group_sum<64>(but);
         } else if (law.k > 0.) {
@@ -175,7 +181,7 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_stats(const SvVerify a, DvRec
     if (threadIdx.x == 0) {
         sum = but = 0.;
 #pragma unroll
-        for (int w = 0; w < DV_THREADS / 64; w++) {
+        for (int w = 0; w < THREADS / 64; w++) {
             sum += sums[w];
             but += buts[w];
             first = min(first, at[w]);
@@ -497,7 +503,13 @@ static hipError_t verify(const SvVerify &a, void *ws, hipStream_t st) {
     if (wgs > (1ll << 32) / DV_THREADS - 1 || (long long)a.n_seqs * a.chunks > (1ll << 32) / DV_THREADS - 1)
         return hipErrorInvalidConfiguration;
     const DvWs w = verify_ws(ws, a.n_seqs, a.n_rows, a.vocab, a.draft != nullptr);
-    if (wgs > 0) hipLaunchKernelGGL(k_dv_stats<T>, dim3((unsigned)wgs), dim3(DV_THREADS), 0, st, a, w.rec, w.drafted, w.others);
+    // Many chunks: 32 logits a thread, for fewer instructions a logit (218 + 154 rows of 151936, fp32: 59 -> 53.5 us; 64 logits
+    // 55).  Few are spread further (5 rows 4.4 us, in 32 logits 5.3).
+    if (wgs >= DV_MANY)
+        hipLaunchKernelGGL((k_dv_stats<T, DV_WIDE>), dim3((unsigned)wgs), dim3(DV_WIDE), 0, st, a, w.rec, w.drafted, w.others);
+    else if (wgs > 0)
+        hipLaunchKernelGGL((k_dv_stats<T, DV_THREADS>), dim3((unsigned)wgs), dim3(DV_THREADS), 0, st, a, w.rec, w.drafted,
+                           w.others);
     if (a.draft) {
         hipLaunchKernelGGL(k_dv_choose, dim3(a.n_seqs), dim3(DV_CHOOSE), 0, st, a, w.rec, w.drafted, w.choice);
         hipLaunchKernelGGL(k_dv_rest<T>, dim3((unsigned)(a.n_seqs * a.chunks)), dim3(DV_THREADS), 0, st, a, w.choice,
