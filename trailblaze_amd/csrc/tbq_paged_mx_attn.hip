@@ -337,7 +337,7 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(3
 // come to registers two tiles ahead and to LDS as halves one tile ahead, each wave
 // those of one 16-position block.
 //
-// 2048 tokens after 8192, 32 / 8 heads of 128, fp16: 335 us, 0.92 PFLOP/s, where power
+// 2048 tokens after 8192, 32 / 8 heads of 128, fp16: 335-353 us, 0.9 PFLOP/s, where power
 // bounds it, as over fp16 pages (337); shorter chunks take 3-10% longer than over those,
 // for the codes' conversions.  Nine mixed sequences under a window of 1024 + 4, heads of 64,
 // bf16: 39, about 19 tiles one after the other in 304 workgroups on 256 CUs.  Not kept for
