@@ -500,6 +500,46 @@ def test_streams_and_repeats():
     assert torch.equal(b["out"], want) and torch.equal(b["K"], a["K"])
 
 
+def test_offsets_beyond_32_bits():
+    """Pages more than 4 GiB into a layer: prompts, single tokens, a page copied, rows moved and values read back as with
+    the same pages at the front of a small cache."""
+    torch = _torch()
+    NQ, NKV, D, page = 16, 8, 128, 256
+    big = 2 ** 32 // (NKV * paged.kv_head_bytes(page, D)) + 2
+    assert big * NKV * paged.kv_head_bytes(page, D) > 2 ** 32
+    rope, got = paged.rope(D, 1e6), []
+    for P, ids in ((8, [0, 1, 2, 3, 4, 5]), (big + 8, [big, big + 1, 2, big + 5, big + 3, big + 7])):
+        K, V = (torch.empty(1, P, NKV, paged.kv_head_bytes(page, D), dtype=torch.uint8, device="cuda") for _ in range(2))
+        for t in (K, V):
+            t[0, ids] = 255
+        c, out = paged.kv_cache(K, V, head_dim=D), []
+        table = [[ids[0], ids[1]], [ids[2], ids[3]]]
+        g = torch.Generator().manual_seed(1)
+        at = [0, 0]
+        for new in ([300, 20], [1, 1], [5, 240]):
+            at = [x + n for x, n in zip(at, new)]
+            T = sum(new)
+            x = torch.randn(T, NQ + 2 * NKV, D, generator=g).half().cuda()
+            b = make_batch(new, at, table, max_q=max(new), max_kv=512)
+            q, o = (torch.empty(T, NQ, D, dtype=torch.float16, device="cuda") for _ in range(2))
+            paged.kv_append(c, 0, b, x[:, :NQ], x[:, NQ:NQ + NKV], x[:, NQ + NKV:], q, rope=rope)
+            paged.attn_paged(c, 0, b, q, o)
+            out += [q.cpu(), o.cpu()]
+        paged.kv_copy_pages(c, [ids[1], ids[2]], [ids[4], ids[5]])
+        paged.kv_compact(c, ints([[ids[4]], [ids[5]]]), ints([0, 3, 7]), ints([2, 5, 30, 0, 7, 8, 100]))
+        kv = [torch.empty(6, NKV, page, D, device="cuda") for _ in range(2)]
+        paged.kv_dequant(c, 0, *kv, pages=ints(ids))
+        out += [t.cpu().nan_to_num(1e30) for t in kv]
+        for t in (K, V):
+            out.append(t[0, ids].cpu())
+        got.append(out)
+        del K, V, c
+        torch.cuda.empty_cache()
+    assert bool(torch.isfinite(got[0][1]).all())
+    for x, y in zip(*got):
+        assert torch.equal(x, y)
+
+
 def test_two_steps_at_once():
     """Two caches' steps on two streams, none waiting for the other."""
     torch = _torch()

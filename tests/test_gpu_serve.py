@@ -399,6 +399,32 @@ def test_verify_is_captured_and_repeats():
     assert [x.tolist() for x in b["o"]] == [x.tolist() for x in e["o"]]
 
 
+@pytest.mark.parametrize("draft", [False, True])
+def test_verify_rows_beyond_32_bits(draft):
+    """Rows more than 2^32 bytes apart, and 2^32 elements of 16 bits, as those of a small tensor."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(9)
+    V, R = 9001, 3
+    for act, apart in (("f32", 2 ** 30 + 7), ("bf16", 2 ** 31 + 5)):
+        ta = TYPES[act]
+        near = [3 * torch.randn(R, V, generator=g) for _ in range(2)]
+        near = [x.to(ta).cuda() for x in near]
+        buf = torch.empty((R - 1) * apart + 2 * V + 3, dtype=ta, device="cuda")
+        far = [buf.as_strided((R, V), (apart, 1), storage_offset=i * (V + 1)) for i in range(2)]
+        for x, y in zip(far, near):
+            x.copy_(y)
+        tok = ints([0, int(near[0][0].float().argmax()), 17])
+        u = torch.tensor([0.3, 0.999999, 0.5], device="cuda")
+        res = []
+        for x in (near, far):
+            o = [ints([77]) for _ in range(3)]
+            paged.draft_verify(ints([0, 3]), tok, x[0], u, u[:1], o[0], o[1], n_drop=o[2], draft_logits=x[1] if draft else None)
+            res.append([t.item() for t in o])
+        assert res[0] == res[1] and 0 <= res[0][1] < V
+        del buf, far
+        torch.cuda.empty_cache()
+
+
 def test_two_verifications_and_tables_at_once():
     """Calls on two streams with workspaces and outputs of their own, none waiting for the other."""
     torch = _torch()
