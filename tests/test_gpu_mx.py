@@ -321,6 +321,18 @@ def test_attention_drafts(act, wide):
                       spoil=widen if wide else None)
 
 
+@pytest.mark.parametrize("wide", [0, 20, 100, 900])
+@pytest.mark.parametrize("act", ACTS)
+def test_attention_longer_drafts(act, wide):
+    """Rows around the 48 and the 64 that a sequence of few rows has at most in short batches, and the same in batches
+    that may hold more (tables up to every limit)."""
+    def widen(table, P):
+        for r in table:
+            r.extend([-1] * wide)
+    run_attention(act, 64, 16, 8, 256, [24, 25, 32, 33, 1, 3], [300, 20, 0, 511, 250, 600], spoil=widen)
+    run_attention(act, 128, 32, 8, 64, [12, 13, 16, 17], [70, 5, 100, 200], window=90, sinks=3, spoil=widen)
+
+
 def test_attention_bounds_leave_out_what_lies_beyond():
     """Lengths above max_q and max_kv: as over 16-bit pages, what lies beyond is left out."""
     torch = _torch()

@@ -1083,15 +1083,16 @@ static StepWs step_ws(const tbq_dense_model *m, int n_seqs, int T, int max_pages
     return w;
 }
 
-static size_t step_attn_bytes(const tbq_dense_model *m, int n_seqs, int T, long long max_kv) {
+static size_t step_attn_bytes(const tbq_dense_model *m, int n_seqs, int T, long long max_kv, int c_type) {
     const int kv = (int)std::min(max_kv, 0x7FFFFFFFll), NKV = m->n_kv_heads, D = m->head_dim, NQ = m->n_heads;
-    return std::max(pg_attn_workspace_upto(n_seqs, T, kv, NKV, D, NQ, false), pg_attn_workspace_upto(1, 1, kv, NKV, D, NQ, true));
+    return std::max(pg_attn_workspace_upto(n_seqs, T, kv, NKV, D, NQ, false, c_type),
+                    pg_attn_workspace_upto(1, 1, kv, NKV, D, NQ, true, c_type));
 }
 
 size_t dense_step_workspace_bytes(const tbq_dense_model *m, const tbq_kv_cache *c, int n_seqs, int T, int max_pages) {
     size_t t = 0;
     const StepWs w = step_ws(m, n_seqs, T, max_pages, nullptr, 0, &t);
-    return t + pf_up(step_attn_bytes(m, n_seqs, T, (long long)max_pages * c->page_size)) +
+    return t + pf_up(step_attn_bytes(m, n_seqs, T, (long long)max_pages * c->page_size, c->type)) +
            std::max(pf_partials(m, T), step_lm_partials(m, n_seqs, w.pf.wh_halves));
 }
 
@@ -1106,7 +1107,7 @@ bool dense_step_attn_fits(const tbq_dense_model *m, const tbq_kv_cache *c, int n
         a.max_q = std::max(a.max_q, n_new[s]);
         a.max_kv = std::max(a.max_kv, kv_len[s]);
     }
-    const size_t room = step_attn_bytes(m, n_seqs, a.n_tokens, (long long)max_pages * c->page_size);
+    const size_t room = step_attn_bytes(m, n_seqs, a.n_tokens, (long long)max_pages * c->page_size, c->type);
     if (dense_prefill_batched(m) && a.n_tokens >= 2) {
         a.n_seqs = n_seqs;
         return pg_attn_workspace_bytes(a, m->head_dim, m->n_heads, false, c->type) <= room;
@@ -1131,7 +1132,7 @@ hipError_t launch_dense_step(const tbq_dense_model *m, const tbq_kv_cache *c, in
     size_t off = 0;
     StepWs w = step_ws(m, n_seqs, T, max_pages, ws, ws_bytes, &off);
     w.attn = (char *)ws + off;
-    off += pf_up(step_attn_bytes(m, n_seqs, T, (long long)max_pages * c->page_size));
+    off += pf_up(step_attn_bytes(m, n_seqs, T, (long long)max_pages * c->page_size, c->type));
     w.pf = pf_ws(m, T, ws, ws_bytes, nullptr, true);
     w.pf.gpart_bytes = ws_bytes > off ? ws_bytes - off : 0;
     w.pf.gpart = w.pf.gpart_bytes ? (float *)((char *)ws + off) : nullptr;

@@ -149,7 +149,8 @@ hipError_t launch_pg_compact(void *k, void *v, int n_layers, long long lelems, i
                              const int *keep, hipStream_t st);
 size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32, int c_type);
 // at least that of every batch of up to n_seqs sequences, n_tokens tokens and max_kv positions
-size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int D, int NQ, bool f32);
+size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int D, int NQ, bool f32,
+                              int c_type);
 // One token of one sequence (tbq_dense.hip), a batch of sequences (tbq_dense_prefill.hip).
 hipError_t launch_dense_decode_paged(const tbq_dense_model *m, int token, const PgArgs &pg, int c_type, size_t layer_bytes,
                                      const PgRope &rope, int window, int sinks, float *logits, void *ws, void *attn_ws,

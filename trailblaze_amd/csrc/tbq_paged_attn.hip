@@ -408,7 +408,7 @@ __device__ __forceinline__ void pg_join_rows(const PgAttn &a, int nrb, int tps, 
     constexpr int RB = HL ? 8 : 16;
     const int kvh = x % a.pg.NKV, r = x / a.pg.NKV, G = a.NQ / a.pg.NKV;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
-    if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
+    if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MOST) return;
     const int rows = qn * G;
     if (rows > a.few || r >= rows) return;
     const int base = a.pg.kv_len[s] - qn, r0 = r / RB * RB;
@@ -803,10 +803,18 @@ __global__ __launch_bounds__(PJ_THREADS) void k_pg_join(const PgAttn a, int nrb,
 // ---------------------------------------------------------------------------
 // Host side: the splits, by what the host knows (max_q, max_kv, n_tokens).
 // ---------------------------------------------------------------------------
-PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, int pos_bytes) {
+static int pg_few(const PgArgs &a, int D, bool f32, int c_type) {
+    const double positions = (double)a.n_seqs * a.max_kv * a.NKV;   // of kv heads
+    const bool mx = c_type == TBQ_KV_MXFP4;
+    if (mx && positions <= (f32 ? PR_SHORT32 : PR_SHORT)) return PR_MOST;
+    if (positions * 2 * pg_row_bytes(c_type, D) > 256 << 20) return PR_MAX / 2;
+    return mx && !f32 ? PR_MAX + PR_MAX / 2 : PR_MAX;
+}
+
+PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, int c_type) {
     PgPlan p{};
     const int G = NQ / a.NKV, RB = f32 ? 8 : 16, cu = 256;
-    p.few = (double)a.n_seqs * a.max_kv * a.NKV * pos_bytes > 256 << 20 ? PR_MAX / 2 : PR_MAX;
+    p.few = pg_few(a, D, f32, c_type);
     p.most = (int)std::min((long long)a.max_q * G, (long long)p.few);
     p.nrb = (p.most + RB - 1) / RB;
     // positions that one block can see
@@ -866,14 +874,15 @@ PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, 
 // the chunks' splits only fall with it.
 size_t pg_attn_workspace_bytes(const PgArgs &a, int D, int NQ, bool f32, int c_type) {
     if (a.n_seqs == 0 || a.n_tokens == 0) return 0;
-    return pg_plan(a, D, NQ, 0, 0, f32, 2 * pg_row_bytes(c_type, D)).bytes;
+    return pg_plan(a, D, NQ, 0, 0, f32, c_type).bytes;
 }
 
 // Rows: a batch of w workgroups a split has at most 512 / w + 1 splits to fill the
 // chip, or one for each `longest` tiles, where w / longest <= 2 PR_MANY / PR_LONG;
 // chunks: more than one split only while all of them fill three workgroups a CU.
-size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int D, int NQ, bool f32) {
-    const long long RB = f32 ? 8 : 16, w = (long long)NKV * (PR_MAX / RB) * n_seqs;
+size_t pg_attn_workspace_upto(int n_seqs, int n_tokens, int max_kv, int NKV, int D, int NQ, bool f32,
+                              int c_type) {
+    const long long RB = f32 ? 8 : 16, w = (long long)NKV * ((c_type == TBQ_KV_MXFP4 ? PR_MOST : PR_MAX) / RB) * n_seqs;
     const long long all = ((long long)max_kv + PR_TS - 1) / PR_TS + 1;
     const long long rows = std::max(512 + w, std::max(std::min(w, 2ll * PR_MANY) * ((all + PR_LONG - 1) / PR_LONG),
                                                       2ll * PR_MANY * all / PR_LONG + w));
@@ -913,7 +922,7 @@ hipError_t launch_mx_join(const PgAttn &a, int D, const PgPlan &p, bool f32, int
 
 template <typename TC, int D, bool HL>
 static hipError_t pg_attn(PgAttn a, float *ws, hipStream_t st) {
-    const PgPlan p = pg_plan(a.pg, D, a.NQ, a.window, a.sinks, HL, 4 * D);
+    const PgPlan p = pg_plan(a.pg, D, a.NQ, a.window, a.sinks, HL, TBQ_KV_F16);
     a.few = p.few;
     float *part = ws + p.rows_bytes / 4;
     if (!p.chunks) {

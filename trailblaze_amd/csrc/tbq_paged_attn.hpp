@@ -106,6 +106,13 @@ constexpr int PR_WAVES = 4, PR_TS = 32;
 // 5 over 65536 202 / 172, of 9 over 16384 142 / 156; 17 heads of 64 over 2000 114 / 120;
 // fp32 (four blocks) 32 heads of 64 over 4096 362 / 280, of 9 over 16384 207 / 182.
 constexpr int PR_MAX = 32;
+// Over 4-bit pages the row blocks' bytes are a quarter, so up to PR_MOST rows of a batch of PR_SHORT positions of kv
+// heads (fp32: PR_SHORT32), and half as many again as PR_MAX of 16-bit rows while the last cache holds the batch.  As
+// row blocks / as many rows, fp16, 16 tokens of 4 heads a kv head: 1 sequence after 500 positions 9.5 / 14.3 us, after
+// 4096 12.9 / 19.8, 4 after 4096 20.2 / 28.4, 4 after 32768 84 / 91, 16 after 4096 53 / 52, 32 after 500 17.8 / 30.8; 12
+// tokens, 32 after 4096 74 / 93, 64 after 4096 158 / 160.  fp32, 16 tokens: 1 after 4096 16.0 / 23.9, 4 after 4096 31.6 /
+// 35.6, 32 after 500 35 / 37.5, 64 after 500 60 / 43, 16 after 4096 99 / 75; 12 tokens, 16 after 4096 80 / 75.
+constexpr int PR_MOST = 64, PR_SHORT = 1 << 19, PR_SHORT32 = 1 << 17;
 constexpr int PR_MIN = 4, PR_LONG = 64;   // tiles of a split: one a wave at least, 2048 positions at most
 constexpr int PR_MANY = 1024;              // (in batches of up to twice so many workgroups)
 
@@ -222,8 +229,7 @@ struct PgPlan {
     size_t rows_bytes, bytes;             // workspace: the few rows' records, then the others'
 };
 
-// pos_bytes: of a kv head's keys and values at one position.
-PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, int pos_bytes);
+PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, int c_type);
 
 constexpr long long PG_WGS = (1ll << 32) / 256 - 1;   // a launch's threads along x stay below 2^32
 

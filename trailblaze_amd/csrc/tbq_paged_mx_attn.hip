@@ -137,7 +137,7 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
     const int lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), li = lane & 15, h = lane >> 4;
     const int kvh = x % a.pg.NKV, r0 = x / a.pg.NKV * RB, G = a.NQ / a.pg.NKV;
     const int q0 = a.pg.q_start[s], qn = a.pg.q_start[s + 1] - q0;
-    if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MAX) return;
+    if (qn <= 0 || q0 < 0 || qn > a.pg.n_tokens - q0 || qn > PR_MOST) return;
     const int rows = qn * G;
     if (rows > a.few || r0 >= rows) return;
     const int base = a.pg.kv_len[s] - qn;   // position of the first token
@@ -621,7 +621,7 @@ __global__ __launch_bounds__(64 * PC_WAVES)
 template <typename TA, int D>
 static hipError_t mx_attn(PgAttn a, int out_type, float *ws, hipStream_t st) {
     constexpr bool HL = std::is_same<TA, float>::value;
-    const PgPlan p = pg_plan(a.pg, D, a.NQ, a.window, a.sinks, HL, 2 * pg_row_bytes(TBQ_KV_MXFP4, D));
+    const PgPlan p = pg_plan(a.pg, D, a.NQ, a.window, a.sinks, HL, TBQ_KV_MXFP4);
     a.few = p.few;
     float *part = ws + p.rows_bytes / 4;
     if (!p.chunks) {
