@@ -341,8 +341,10 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(3
 // bounds it, as over fp16 pages (337); shorter chunks take 3-10% longer than over those,
 // for the codes' conversions.  Nine mixed sequences under a window of 1024 + 4, heads of 64,
 // bf16: 39, about 19 tiles one after the other in 304 workgroups on 256 CUs.  Not kept for
-// it: three waves a SIMD (no change), codes two tiles ahead in two sets of registers (no
-// change), the positions in two ranges (32, and 9.5 the join).
+// it: three waves a SIMD, codes two tiles ahead in two sets of registers, all of a tile's LDS reads
+// ahead of its products (no change each), the positions in two ranges (32, and 9.5 the join), two
+// groups of four waves that share a block's tiles and add at the end (44, with registers spilled;
+// heads of 128, where none are: 2048 tokens after none 66 -> 60, but 512 after 4096 64 -> 72).
 // ---------------------------------------------------------------------------
 template <int D>
 struct McLds {

@@ -372,7 +372,7 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
                                                      const float *__restrict__ drafted,
                                                      const DvChoice *__restrict__ choice, const double *__restrict__ rest,
                                                      const double *__restrict__ others) {
-    constexpr int EACH = DV_CHUNK / DV_PICK, WAVES = DV_PICK / 64, N = 16 / sizeof(T);
+    constexpr int EACH = DV_CHUNK / DV_PICK, WAVES = DV_PICK / 64;
     __shared__ double red[WAVES];
     __shared__ int who[WAVES];
     const int s = blockIdx.x, tid = threadIdx.x;
@@ -391,16 +391,13 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
         auto weights = [&](int ck) {
             const int v0 = ck * DV_CHUNK + tid * EACH;
             double sum = 0.;
+            float x[EACH], y[EACH];
+            dv_load(l, v0, a.vocab, x);
+            if (d && c.rest) dv_load(d, v0, a.vocab, y);
 #pragma unroll
-            for (int i = 0; i < EACH; i += N) {
-                float x[N], y[N];
-                dv_load(l, v0 + i, a.vocab, x);
-                if (d && c.rest) dv_load(d, v0 + i, a.vocab, y);
-#pragma unroll
-                for (int e = 0; e < N; e++) {
-                    w[i + e] = dv_rest(c, p, q, pi, qi, d != nullptr, x[e], y[e], v0 + i + e);
-                    sum += w[i + e];
-                }
+            for (int e = 0; e < EACH; e++) {
+                w[e] = dv_rest(c, p, q, pi, qi, d != nullptr, x[e], y[e], v0 + e);
+                sum += w[e];
             }
             return sum;
         };
