@@ -323,12 +323,11 @@ __global__ __launch_bounds__(DV_THREADS) void k_dv_rest(const SvVerify a, const 
     }
 }
 
-// Inclusive sum over the workgroup of WAVES waves, and the whole one.
+// Inclusive sum over the workgroup of WAVES waves, and the whole one; lds: of this call only.
 template <int WAVES>
 __device__ __forceinline__ double dv_scan(double v, double *lds, double *total) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     v = wave_scan(v);
-    __syncthreads();
     if (lane == 63) lds[wave] = v;
     __syncthreads();
     double before = 0., all = 0.;
@@ -340,28 +339,30 @@ __device__ __forceinline__ double dv_scan(double v, double *lds, double *total) 
     *total = all;
     return before + v;
 }
-// The first thread that says yes: its value (and x); -1 where none does.  Of the last one with LAST.
+// The first thread that says yes (LAST: the last one): its value (and x); -1 where none does.  lds: of this call only,
+// and of one with LAST behind it.
+template <int WAVES>
+struct DvWho {
+    int v[WAVES];
+    double x[WAVES];
+};
 template <int WAVES, bool LAST>
-__device__ __forceinline__ int dv_which(bool yes, int v, double x, int *li, double *ld, double *out) {
+__device__ __forceinline__ int dv_which(bool yes, int v, double x, DvWho<WAVES> *lds, double *out) {
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const uint64_t b = __builtin_amdgcn_ballot_w64(yes);
     const int l = b ? LAST ? 63 - __builtin_clzll(b) : __builtin_ctzll(b) : 0;
-    __syncthreads();
+    if (LAST) __syncthreads();
     if (lane == l) {
-        li[wave] = b ? v : -1;
-        ld[wave] = x;
+        lds->v[wave] = b ? v : -1;
+        lds->x[wave] = x;
     }
     __syncthreads();
-    int found = -1;
-#pragma unroll
-    for (int i = 0; i < WAVES; i++) {
-        const int w = LAST ? WAVES - 1 - i : i;
-        if (found < 0 && li[w] >= 0) {
-            found = li[w];
-            *out = ld[w];
-        }
-    }
-    return found;
+    const int found = lds->v[lane % WAVES];
+    const uint64_t w = __builtin_amdgcn_ballot_w64(lane < WAVES && found >= 0);
+    if (!w) return -1;   // uniform
+    const int at = LAST ? 63 - __builtin_clzll(w) : __builtin_ctzll(w);
+    *out = lds->x[at];
+    return __builtin_amdgcn_readlane(found, at);
 }
 
 // The draw, a workgroup a sequence: a chain of records, the scan of the chunks, one chunk's logits and
@@ -373,8 +374,8 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
                                                      const DvChoice *__restrict__ choice, const double *__restrict__ rest,
                                                      const double *__restrict__ others) {
     constexpr int EACH = DV_CHUNK / DV_PICK, WAVES = DV_PICK / 64;
-    __shared__ double red[WAVES];
-    __shared__ int who[WAVES];
+    __shared__ double red[3][WAVES];
+    __shared__ DvWho<WAVES> who[2];
     const int s = blockIdx.x, tid = threadIdx.x;
     DvChoice c = choice ? choice[s] : dv_choose<WAVES>(a, rec, drafted, s);
     const bool is = c.n > 0;
@@ -416,7 +417,7 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
         for (int round = 0; round < 2; round++) {   // (nothing left of p - q: p itself)
             mine = 0.;
             for (int k = k0; k < k1; k++) mine += mass(k);
-            run = dv_scan<WAVES>(mine, red, &total) - mine;
+            run = dv_scan<WAVES>(mine, red[round], &total) - mine;
             if (total > 0.) break;
             c.rest = 0;
         }
@@ -436,12 +437,12 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
             }
             run += m;
         }
-        int ck = dv_which<WAVES, false>(f >= 0, f, at, who, red, &before);
-        if (ck < 0) ck = dv_which<WAVES, true>(z >= 0, z, end, who, red, &before);
+        int ck = dv_which<WAVES, false>(f >= 0, f, at, &who[0], &before);
+        if (ck < 0) ck = dv_which<WAVES, true>(z >= 0, z, end, &who[0], &before);
         if (ck >= 0) {
             mine = weights(ck);
             double all;
-            run = before + (dv_scan<WAVES>(mine, red, &all) - mine);
+            run = before + (dv_scan<WAVES>(mine, red[2], &all) - mine);
             f = z = -1;
 #pragma unroll
             for (int e = 0; e < EACH; e++) {
@@ -452,8 +453,8 @@ __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvR
                 }
             }
             const int v0 = ck * DV_CHUNK + tid * EACH;
-            next = dv_which<WAVES, false>(f >= 0, v0 + f, 0., who, red, &before);
-            if (next < 0) next = dv_which<WAVES, true>(z >= 0, v0 + z, 0., who, red, &before);
+            next = dv_which<WAVES, false>(f >= 0, v0 + f, 0., &who[1], &before);
+            if (next < 0) next = dv_which<WAVES, true>(z >= 0, v0 + z, 0., &who[1], &before);
         }
     }
     if (tid == 0) {
