@@ -857,6 +857,11 @@ PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, 
     // mixed sequences with a window of 1024 41.3 -> 37.1 us.
     if (p.chunks) tps = std::max(tps, (seen + PC_TS - 1) / PC_TS * 4 / p.chunk_splits);
     tps = std::max((long long)PR_MIN, std::min(longest, (tps + 3) / 4 * 4));
+    // Over 4-bit pages a wave's tile takes 0.6 us, so a short range in one split is done before a join (and its launch)
+    // would be: single tokens, 32 / 8 heads of 128, fp16, in one split / in several, in a graph: 1 sequence after 250
+    // positions 4.9 / 7.2 us, after 750 7.4 / 7.4, after 1000 8.6 / 7.4; 8 after 500 6.4 / 8.3, after 1000 8.8 / 9.4, after
+    // 1500 11.4 / 9.6; 32 after 500 6.9 / 11.2, after 2000 15.4 / 17.3, after 3000 21.6 / 21.9.
+    if (c_type == TBQ_KV_MXFP4 && !p.chunks && tiles <= std::min((long long)PR_LONG, 22 + wgs / 6)) tps = (tiles + 3) / 4 * 4;
     if ((tiles + tps - 1) / tps > PJ_MAX) tps = (tiles + PJ_MAX - 1) / PJ_MAX;
     p.row_tps = (int)tps;
     p.row_splits = (int)((tiles + tps - 1) / tps);
