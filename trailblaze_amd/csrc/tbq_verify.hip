@@ -366,7 +366,7 @@ __device__ __forceinline__ int dv_which(bool yes, int v, double x, DvWho<WAVES> 
 }
 
 // The draw, a workgroup a sequence: a chain of records, the scan of the chunks, one chunk's logits and
-// the scan of its weights (5 rows of 151936, the choice within: 6.8 us; with sums by shuffles and the
+// the scan of its weights (5 rows of 151936, the choice within: 6.6 us; with sums by shuffles and the
 // guess's chunk formed again 9.4).
 template <typename T>
 __global__ __launch_bounds__(DV_PICK) void k_dv_pick(const SvVerify a, const DvRec *__restrict__ rec,
