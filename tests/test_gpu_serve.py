@@ -516,3 +516,59 @@ def test_speculative_steps_on_the_device():
     want = server(0)
     for k in (1, drafts):
         assert server(k, want) == want
+
+
+def test_a_step_in_one_graph():
+    """Tables, append, attention and verification, whose drops the next tables take, captured once and replayed, against the
+    same calls made eagerly; the pages' bytes, the tables and the tokens of each step."""
+    torch = _torch()
+    S, NQ, NKV, D, V, page, P, k = 4, 8, 2, 64, 5000, 16, 48, 3
+    rows, rope = S * (1 + k), paged.rope(64, 1e4)
+
+    def server():
+        s = dict(kv_len=ints([0] * S), table=ints([[-1] * 10] * S), free=ints(list(range(P))), n_free=ints([P]), drop=ints([0] * S),
+                 new=ints([1 + k] * S), q_start=ints([0] * (S + 1)), slots=ints([0] * rows), accept=ints([0] * S), next=ints([0] * S),
+                 tok=ints([0] * rows), served=ints([0]))
+        s["K"], s["V"] = (torch.full((1, P, NKV, paged.kv_head_bytes(page, D)), 255, dtype=torch.uint8, device="cuda") for _ in range(2))
+        s["x"], s["q"], s["out"] = (torch.zeros(rows, n, D, device="cuda", dtype=torch.float16) for n in (NQ + 2 * NKV, NQ, NQ))
+        s["logits"], s["draft"] = (torch.zeros(rows, V, device="cuda") for _ in range(2))
+        s["ua"], s["un"] = torch.zeros(rows, device="cuda"), torch.zeros(S, device="cuda")
+        h = paged.kv_tables(page, s["kv_len"], s["new"], s["table"], s["free"], s["n_free"], q_start=s["q_start"], n_drop=s["drop"],
+                            slots=s["slots"], served=s["served"])
+        c = paged.kv_cache(s["K"], s["V"], head_dim=D)
+        b = paged.kv_batch(s["q_start"], s["kv_len"], s["table"], rows, max_q=1 + k, max_kv=160)
+        ws = [torch.empty(max(n, 16), dtype=torch.uint8, device="cuda") for n in
+              (paged.attn_workspace_size(c, b, NQ, torch.float16), paged.draft_verify_workspace_size(S, rows, V, torch.float32, True))]
+
+        def step():
+            paged.kv_build_tables(h)
+            x = s["x"]
+            paged.kv_append(c, 0, b, x[:, :NQ], x[:, NQ:NQ + NKV], x[:, NQ + NKV:], s["q"], rope=rope)
+            paged.attn_paged(c, 0, b, s["q"], s["out"], workspace=ws[0])
+            paged.draft_verify(s["q_start"], s["tok"], s["logits"], s["ua"], s["un"], s["accept"], s["next"], n_drop=s["drop"],
+                               draft_logits=s["draft"], workspace=ws[1])
+        return s, step
+    (a, replayed), (e, eager) = server(), server()
+    start = {n: t.clone() for n, t in a.items()}
+    graph = torch.cuda.CUDAGraph()
+    replayed()   # (what a first call sets up)
+    torch.cuda.synchronize()
+    with torch.cuda.graph(graph):
+        replayed()
+    for n, t in a.items():
+        t.copy_(start[n])
+    for r in range(8):
+        g = torch.Generator().manual_seed(r)
+        l = 3 * torch.randn(rows, V, generator=g)
+        new = dict(x=torch.randn(rows, NQ + 2 * NKV, D, generator=g), logits=l, draft=l + 0.4 * torch.randn(rows, V, generator=g),
+                   tok=torch.cat([torch.zeros(1), l.argmax(-1)[:-1].float()]), ua=torch.rand(rows, generator=g),
+                   un=torch.rand(S, generator=g), new=torch.randint(1, 2 + k, (S,), generator=g))
+        for s in (a, e):
+            for n, t in new.items():
+                s[n].copy_(t)
+        graph.replay()
+        eager()
+        torch.cuda.synchronize()
+        assert a["served"].item() == S
+        for n in a:
+            assert torch.equal(a[n], e[n]), (r, n)
