@@ -350,6 +350,41 @@ def test_attention_bounds_leave_out_what_lies_beyond():
     assert bool(torch.isfinite(out[61:]).all())
 
 
+def rounds_only_its_output(o, spread, size, ta, V, keys):
+    """tolerance() without the rounding of the probabilities: they are pairs of halves, each off by half a step of what
+    it rounds, so what is left of them is half a step squared; then the one rounding of the output."""
+    torch = _torch()
+    tol = tolerance(o, spread, size, torch.float32, V, keys) + half_step(torch.float16) ** 2 * spread
+    return tol + half_step(ta) * (o.abs() + tol) + least(ta)
+
+
+@pytest.mark.parametrize("act", ["f16", "bf16"])
+@pytest.mark.parametrize("D,heads,kv,q_lens,past", [
+    (128, 32, 8, [1, 1, 1], [299, 999, 8]), (64, 8, 1, [1, 1], [2000, 3]), (64, 4, 2, [4, 3, 1], [70, 0, 500]),
+    (64, 9, 1, [1, 1], [700, 40]), (128, 17, 1, [1], [900]), (64, 4, 1, [8, 3, 1], [700, 40, 500]),
+    (64, 16, 8, [24, 1], [300, 9]),   # few rows
+    (128, 4, 2, [70, 1, 3], [150, 77, 5]), (64, 6, 2, [129, 20], [10, 400]), (64, 4, 1, [33], [3000])])   # many rows
+def test_attention_of_16_bit_rows_rounds_only_its_output(act, D, heads, kv, q_lens, past):
+    """Scores near each other and values of alternating sign, whose average is small beside them, so that the rounding of
+    the output hides no other; and random values."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(D + heads)
+    ta, page, kvl = TYPES[act], 64, [n + p for n, p in zip(q_lens, past)]
+    table, P = make_table(kvl, page, g)
+    K, V = (torch.randn(1, P, kv, page, D, generator=g) for _ in range(2))
+    V[..., :D // 2] = torch.where(torch.arange(page) % 2 == 0, 1.0, -1.0)[:, None]
+    T = sum(q_lens)
+    Q = torch.randn(T, heads, D, generator=g).to(ta)
+    out = torch.empty(T, heads, D, dtype=ta, device="cuda")
+    c = paged.kv_cache(mx_ref.pool(K, False).cuda(), mx_ref.pool(V, True).cuda(), head_dim=D)
+    paged.attn_paged(c, 0, make_batch(q_lens, kvl, table), Q.cuda(), out, scale=0.01)
+    K, V = mx_ref.rounded(K), mx_ref.rounded(V)
+    ref = attention(K, V, 0, starts(q_lens), kvl, table, Q, scale=0.01)
+    for r in ref:
+        o, spread, size = ref[r]
+        assert bool(((out[r].cpu().double() - o).abs() <= rounds_only_its_output(o, spread, size, ta, V, max(kvl))).all()), r
+
+
 def test_attention_bad_pages_are_not_seen():
     def spoil(table, P):
         table[0][1] = -1                 # a hole

@@ -7,7 +7,10 @@
 // on their way to LDS (many rows); the values are halves exactly, so this rounds
 // nothing.  16-bit rows of q: fp16 as they are, bf16 scaled by a power of two into
 // fp16's range (elements below 2^-38 of a row's largest are lost); fp32 rows as two
-// halves each.
+// halves each.  Probabilities are two halves each for every type (2^-22 of one, or 2^-39 of
+// the largest, is lost), so a 16-bit row is rounded once, at the output.  As one half
+// they would add 17% (few rows, fp16, 64 sequences of up to 8192) and 29% (2048 tokens
+// after 8192) to the output's own rounding, 2.1e-4 against 64 bits.
 #include <algorithm>
 #include <type_traits>
 
@@ -112,11 +115,10 @@ __device__ __forceinline__ void mx_load_q(const TA *q, Spread spread, mx_h8 (&hi
 // Bound by HBM where there are many positions: 64 ragged sequences to 8192, 32 / 8 heads
 // of 128, fp16 rows 60 us, 5.3 TB/s.  What that took (a first form: 81):
 //   codes of one row block loaded past the caches: 73 -> 67.5;
-//   16-bit rows' probabilities as halves, one product a tile of V (fp32 rows: two columns'
-//   worth, at no cost): 67.5 -> 62.5.  Over 16-bit pages, four times the bytes hide the
-//   second product; here it is the longer part.  It costs 2^-11 of a probability;
-//   loads without a condition, so that a whole tile stays in flight, and three waves a
-//   SIMD: 62.5 -> 60.
+//   loads without a condition, so that a whole tile stays in flight, and three waves a SIMD.
+// The lo halves' product (fp32 rows': columns of the same one) takes 2 to 5%, up to 11% with
+// heads of 64: 64 sequences of 4096 62-65 -> 64-68, of 8192 107 -> 111, of 4096 with 16 / 8 heads of
+// 64 44 -> 49 us.
 // One sequence of 131072: 16 us (4.5 TB/s), of 4096: 6, a chain of page, codes, products and
 // the workgroup's own join.
 // ---------------------------------------------------------------------------
@@ -248,15 +250,18 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
 #pragma unroll
             for (int j = 0; j < ND; j++) o[j] *= corr;
         }
-        mx_h8 pf;   // (fp32 rows' lo halves are columns of their own)
+        mx_h8 pf, pl;   // (fp32 rows' lo halves are columns of their own)
         const float mb = MX_SH - m;
 #pragma unroll
         for (int e = 0; e < 8; e++) {
             const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 4][e % 4], cs, mb));
             l += p;
-            const pg_f16 hi = (pg_f16)p;
-            if constexpr (HL) pf[e] = li < 8 ? hi : (pg_f16)(p - (float)hi);
-            else pf[e] = hi;
+            const pg_f16 hi = (pg_f16)p, lo = (pg_f16)(p - (float)hi);
+            if constexpr (HL) pf[e] = li < 8 ? hi : lo;
+            else {
+                pf[e] = hi;
+                pl[e] = lo;
+            }
         }
         auto two = [&](auto S) {   // dims 2 S and 2 S + 1 of the lane's ND
             constexpr int I = decltype(S)::value;
@@ -270,6 +275,10 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
             }
             o[2 * I] = pg_mfma16(va, pf, o[2 * I]);
             o[2 * I + 1] = pg_mfma16(vb, pf, o[2 * I + 1]);
+            if constexpr (!HL) {
+                o[2 * I] = pg_mfma16(va, pl, o[2 * I]);
+                o[2 * I + 1] = pg_mfma16(vb, pl, o[2 * I + 1]);
+            }
         };
         two(std::integral_constant<int, 0>{});
         two(std::integral_constant<int, 1>{});
@@ -521,7 +530,7 @@ __device__ __forceinline__ void mx_chunk(const PgAttn &a, int nsplit, float *__r
 #pragma unroll
                 for (int j = 0; j < NT; j++) o[j] *= corr;
             }
-            mx_h8 pf[NP][4];
+            mx_h8 pf[2][4];   // hi and lo halves
             const float mb = MX_SH - m;
             float sum = 0.f;
 #pragma unroll
@@ -529,7 +538,7 @@ __device__ __forceinline__ void mx_chunk(const PgAttn &a, int nsplit, float *__r
                 const float p = __builtin_amdgcn_exp2f(fmaf(sc[e / 16][e % 16], cs, mb));
                 sum += p;
                 pf[0][e / 8][e % 8] = (pg_f16)p;
-                if constexpr (HL) pf[NP - 1][e / 8][e % 8] = (pg_f16)(p - (float)pf[0][e / 8][e % 8]);
+                pf[1][e / 8][e % 8] = (pg_f16)(p - (float)pf[0][e / 8][e % 8]);
             }
             l += sum;
             const uint32_t vb = lv + buf * (PC_TS * D * 2);
@@ -543,7 +552,7 @@ __device__ __forceinline__ void mx_chunk(const PgAttn &a, int nsplit, float *__r
                 for (int j = 0; j < NT; j++) {
                     const mx_h8 y = __builtin_bit_cast(mx_h8, vfrag(u, j));
 #pragma unroll
-                    for (int p = 0; p < NP; p++) o[j] = pg_mfma32(y, pf[p][u], o[j]);
+                    for (int p = 0; p < 2; p++) o[j] = pg_mfma32(y, pf[p][u], o[j]);
                 }
         }
         none = none1;
