@@ -145,8 +145,7 @@ int tbq_kv_append(const tbq_kv_cache *c, int layer, const tbq_kv_batch *b, int n
  * 256 MiB of keys and values) are rounded once, at the output; with more rows the
  * probabilities are rounded to the cache's type too.  Over an MXFP4 cache 16-bit
  * rows are rounded once, at the output, however many there are (of a probability 2^-22
- * is lost, or 2^-39 of the row's largest); BF16 elements of q below 2^-38 of its row's
- * largest are lost.  F32 takes q and the probabilities as pairs of
+ * is lost, or 2^-39 of the row's largest).  F32 takes q and the probabilities as pairs of
  * halves (~22 bits, relative to a row's largest element), so its rows are exact to
  * about 1e-6.
  * workspace: tbq_attn_paged_workspace_size() bytes, 16-byte aligned, no

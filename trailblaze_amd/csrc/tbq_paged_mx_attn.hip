@@ -6,8 +6,8 @@
 // products take halves that the codes and scales become in registers (few rows) or
 // on their way to LDS (many rows); the values are halves exactly, so this rounds
 // nothing.  16-bit rows of q: fp16 as they are, bf16 scaled by a power of two into
-// fp16's range (elements below 2^-38 of a row's largest are lost); fp32 rows as two
-// halves each.  Probabilities are two halves each for every type (2^-22 of one, or 2^-39 of
+// fp16's range (a row with elements that a half then cannot hold, below 2^-31 of its largest
+// one, is formed alone, from q as it is); fp32 rows as two halves each.  Probabilities are two halves each for every type (2^-22 of one, or 2^-39 of
 // the largest, is lost), so a 16-bit row is rounded once, at the output.  As one half
 // they would add 17% (few rows, fp16, 64 sequences of up to 8192) and 29% (2048 tokens
 // after 8192) to the output's own rounding, 2.1e-4 against 64 bits.
@@ -70,12 +70,14 @@ __device__ __forceinline__ void mx_slow_row(const PgArgs &pg, const TA *q, float
 
 // N dims of row tok's head (from element `at` of q) at `step` elements apart, as halves:
 // fp16 as it is, bf16 and fp32 scaled by 2^sh so that the row's largest element (over the
-// lanes that share it: spread) lies in [2^13, 2^14); fp32 as hi and lo.
+// lanes that share it: spread) lies in [2^13, 2^14); fp32 as hi and lo.  Returns whether a
+// bf16 row has an element that is no half then.
 template <typename TA, int NS, typename Spread>
-__device__ __forceinline__ void mx_load_q(const TA *q, Spread spread, mx_h8 (&hi)[NS], mx_h8 (&lo)[NS], float *cs) {
+__device__ __forceinline__ bool mx_load_q(const TA *q, Spread spread, mx_h8 (&hi)[NS], mx_h8 (&lo)[NS], float *cs) {
     if constexpr (std::is_same<TA, pg_f16>::value) {
 #pragma unroll
         for (int i = 0; i < NS; i++) hi[i] = *reinterpret_cast<const mx_h8 *>(q + 8 * i);
+        return false;
     } else {
         float x[NS][8], mx = 0.f;
 #pragma unroll
@@ -90,16 +92,19 @@ __device__ __forceinline__ void mx_load_q(const TA *q, Spread spread, mx_h8 (&hi
                 mx = fmaxf(mx, fmaxf(fmaxf(fabsf(v.x), fabsf(v.y)), fmaxf(fabsf(v.z), fabsf(v.w))));
             }
         const int sh = pg_row_shift(spread(mx));
-        const float f = ldexpf(1.f, sh);
-        *cs = fmaxf(*cs * ldexpf(1.f, -sh), PG_TINY);
+        const float f = ldexpf(1.f, sh), back = ldexpf(1.f, -sh);
+        *cs = fmaxf(*cs * back, PG_TINY);
+        bool lost = false;
 #pragma unroll
         for (int i = 0; i < NS; i++)
 #pragma unroll
             for (int e = 0; e < 8; e++) {
                 const float v = x[i][e] * f;
                 hi[i][e] = (pg_f16)v;
-                lo[i][e] = (pg_f16)(v - (float)hi[i][e]);
+                if constexpr (std::is_same<TA, float>::value) lo[i][e] = (pg_f16)(v - (float)hi[i][e]);
+                else lost |= (float)hi[i][e] * back != x[i][e];
             }
+        return spread(lost ? 1.f : 0.f) > 0.f;
     }
 }
 
@@ -152,10 +157,11 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
     const int row = r0 + (HL ? li & 7 : li), rc = min(row, rows - 1), tok = rc / G, pos = base + tok;
     mx_h8 qf[NS];
     float cs = fmaxf(a.scale, PG_TINY);
+    uint64_t lost;   // of the lanes' rows
     {
         mx_h8 lo[NS];
-        mx_load_q((const TA *)a.q + (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + D / 4 * h,
-                  [](float v) { return swap32_max(swap16_max(v)); }, qf, lo, &cs);
+        lost = __builtin_amdgcn_ballot_w64(mx_load_q((const TA *)a.q + (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + D / 4 * h,
+                  [](float v) { return swap32_max(swap16_max(v)); }, qf, lo, &cs));
         if constexpr (HL) {
 #pragma unroll
             for (int i = 0; i < NS; i++)
@@ -301,11 +307,11 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
             if (n + 2 >= nt) break;
         }
     }
-    // rows with an output that is not finite are formed again, one at a time
+    // rows with an output that is not finite, and those whose q lost something, are formed again, one at a time
     float odd = 0.f;   // NaN where an output is NaN or infinite
 #pragma unroll
     for (int j = 0; j < ND; j++) odd += (o[j][0] - o[j][0]) + (o[j][1] - o[j][1]) + (o[j][2] - o[j][2]) + (o[j][3] - o[j][3]);
-    const bool again = row < rows && !(odd == 0.f);
+    const bool again = row < rows && (!(odd == 0.f) || (lost >> lane & 1));
     pg_rows_out<TA, D, HL>(a, o, m, l, r0, rows, G, kvh, q0, s, z, nz, nrb, nsplit, part, lds, [&] {
         uint64_t left = __builtin_amdgcn_ballot_w64(again);   // lane bits: a row's are li (HL: and li + 8) of each 16
         left |= left >> 32;
@@ -385,10 +391,11 @@ __device__ __forceinline__ void mx_chunk(const PgAttn &a, int nsplit, float *__r
     // Q^T's columns: dim step i, lane half h has dims 8 NS h + 8 i .. + 8 (the keys' in that order too)
     mx_h8 qf[NP][NS];
     float cs = fmaxf(a.scale, PG_TINY);
+    uint64_t lost;   // of the lanes' rows
     {
         mx_h8 lo[NS];
-        mx_load_q((const TA *)a.q + (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * NS * h,
-                  [](float v) { return swap32_max(v); }, qf[0], lo, &cs);
+        lost = __builtin_amdgcn_ballot_w64(mx_load_q((const TA *)a.q + (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * NS * h,
+                  [](float v) { return swap32_max(v); }, qf[0], lo, &cs));
         if constexpr (HL) {
 #pragma unroll
             for (int i = 0; i < NS; i++) qf[NP - 1][i] = lo[i];
@@ -560,14 +567,14 @@ __device__ __forceinline__ void mx_chunk(const PgAttn &a, int nsplit, float *__r
         barrier();
     }
     l = swap32_sum(l);
-    // rows with an output that is not finite are formed again, one at a time
+    // rows with an output that is not finite, and those whose q lost something, are formed again, one at a time
     float odd = 0.f;   // NaN where an output is NaN or infinite
 #pragma unroll
     for (int j = 0; j < NT; j++)
 #pragma unroll
         for (int r = 0; r < 16; r++) odd += o[j][r] - o[j][r];
     odd += __builtin_bit_cast(float, __builtin_amdgcn_ds_bpermute(4 * (lane ^ 32), __builtin_bit_cast(int, odd)));
-    const bool again = row < rows && !(odd == 0.f);
+    const bool again = row < rows && (!(odd == 0.f) || (lost >> lane & 1));
     auto put = [&](long long at, float v) {
         if (HL || a.f32_out) ((float *)a.out)[at] = v;
         else ((TA *)a.out)[at] = (TA)v;
