@@ -21,8 +21,8 @@ struct SvVerify {
     const float *temperature, *u_accept, *u_next;
     int *n_accept, *next, *n_drop;
 };
-// Elements of a row that a workgroup takes at a time.  (218 + 154 rows of 151936, fp32, all kernels: 88 us in 8192,
-// 86 in 4096, 103 in 2048; 146 + 113 rows of 50257, bf16: 40, 34 and 34; 5 rows of 151936 13 in all.)
+// Elements of a row that a workgroup takes at a time.  (Calls, on one card: 218 + 154 rows of 151936, fp32, 93 us in 8192,
+// 85 in 4096, 91 in 2048; 146 + 113 rows of 50257, bf16, 38.6, 33.5 and 31.4; 5 rows of 151936 14.6, 13 and 12.)
 constexpr int DV_CHUNK = 4096;
 size_t verify_workspace_bytes(int n_seqs, int n_rows, int vocab, bool draft);
 hipError_t launch_verify(const SvVerify &a, int type, void *ws, hipStream_t st);

@@ -5,8 +5,8 @@
 // does not, the next token is drawn from max(p - q, 0), behind the last draft from
 // p: the first token whose cumulative weight, in the order of the vocabulary, is above u times the
 // whole.  Which token that is changes at as many borders as there are tokens, so
-// weights and sums are fp64: with fp32's 1e-7 one draw in thirty over 150000 tokens
-// would depend on the order of a sum, with fp64 one in 10^10.
+// weights and sums are fp64, and the weights exact to it: with fp32's 1e-7 one draw in
+// thirty over 150000 tokens would depend on roundings, with fp64 one in 10^10.
 //
 // Three launches: a chunk's largest logit and sum of exponentials, for all rows;
 // with a draft model, the sums of max(p - q, 0) a chunk for the one row of a
@@ -30,12 +30,13 @@ typedef DvRec DvRow;   // of a row: the same
 
 // The weights exp((l - m) / T) of a row whose largest logit is m, by k = log2(e) / T: 2^t, t = k (l - m).
 // t is split into the nearest whole number, which adding 1.5 * 2^52 leaves in the low bits, and r, |r| <= 1/2;
-// 2^r is the polynomial of degree 8 that meets it at the nine Chebyshev points, off by 1.1e-12 of it at most; the
-// whole number goes to the exponent.  Logits from none on have no weight (2^-1000 of the largest, -infinity, NaN); where
+// 2^r is the polynomial of degree 10 that meets it at the eleven Chebyshev points, off by 4e-16 of it at most with the
+// roundings (degree 8: 1.1e-12, which moves the borders by up to 4e-9 of the whole in all, and 1 to 3 us less in the case
+// below); the whole number goes to the exponent.  Logits from none on have no weight (2^-1000 of the largest, -infinity, NaN); where
 // m is infinite, all below it; k is 0 where only m itself has weight.  Those below low count as low: it is none, but for
 // temperatures so high that every finite logit has weight (all).  With Least set, logits without weight have up to
 // 2^-999, for sums alone (k > 0 and not all).
-// (218 + 154 rows of 151936: 113 us with the library's exp, 53 with this.)
+// (218 + 154 rows of 151936: 113 us with the library's exp, 55 with this.)
 struct DvLaw {
     double k, m;
     float low, none;
@@ -57,14 +58,16 @@ template <bool Least = false>
 __device__ __forceinline__ double dv_weight(const DvLaw &w, float l) {
     const double t = ((double)__builtin_amdgcn_fmed3f(l, w.low, 3.402823466e38f) - w.m) * w.k, magic = 6755399441055744.;
     const double n = t + magic, r = t - (n - magic);
-    double p = 1.3255179556479267e-6;
-    p = fma(p, r, 1.5310080611926545e-5);
-    p = fma(p, r, 1.5403456082633648e-4);
-    p = fma(p, r, 1.3333450563173552e-3);
-    p = fma(p, r, 9.618129159053034e-3);
-    p = fma(p, r, 5.5504109412108156e-2);
-    p = fma(p, r, 2.4022650695814518e-1);
-    p = fma(p, r, 6.931471805459332e-1);
+    double p = 7.072585949269223e-9;
+    p = fma(p, r, 1.0208690299958306e-7);
+    p = fma(p, r, 1.321544258792169e-6);
+    p = fma(p, r, 1.5252657260200837e-5);
+    p = fma(p, r, 1.540353044173605e-4);
+    p = fma(p, r, 1.3333558230164974e-3);
+    p = fma(p, r, 9.618129107606888e-3);
+    p = fma(p, r, 5.550410866444772e-2);
+    p = fma(p, r, 2.4022650695910097e-1);
+    p = fma(p, r, 6.9314718055995e-1);
     p = fma(p, r, 1.);
     const uint64_t b = __builtin_bit_cast(uint64_t, p) + ((uint64_t)(uint32_t)__builtin_bit_cast(uint64_t, n) << 52);
     return Least || l > w.none ? __builtin_bit_cast(double, b) : 0.;
@@ -99,9 +102,9 @@ __device__ __forceinline__ double dv_rate(const SvVerify &a, int s) {
     return t > 0. ? fmax(1.4426950408889634 / t, 1e-60) : 0.;   // (1e-60 of any two finite ones is alike)
 }
 
-// Block x: chunk, row, and (draft) whose logits.  Bound by the vector units, which have 18 instructions a
-// logit to do, 14 of them fp64, and about 170 a wave (218 + 154 rows of 151936, fp32: 53.5 us, 4.2 TB/s; with 16
-// logits a thread 59, where they were busy for 88% of the cycles; loads past the caches changed nothing).
+// Block x: chunk, row, and (draft) whose logits.  Bound by the vector units, which have 20 instructions a
+// logit to do, 16 of them fp64, and about 170 a wave (218 + 154 rows of 151936, fp32: 55-58 us, 4.0 TB/s, busy for
+// 85% of the cycles; with 16 logits a thread and two instructions a logit fewer 59; loads past the caches changed nothing).
 template <typename T, int THREADS>
 __global__ __launch_bounds__(THREADS) void k_dv_stats(const SvVerify a, DvRec *__restrict__ rec,
                                                          float *__restrict__ drafted, double *__restrict__ others) {
@@ -501,8 +504,8 @@ static hipError_t verify(const SvVerify &a, void *ws, hipStream_t st) {
     if (wgs > (1ll << 32) / DV_THREADS - 1 || (long long)a.n_seqs * a.chunks > (1ll << 32) / DV_THREADS - 1)
         return hipErrorInvalidConfiguration;
     const DvWs w = verify_ws(ws, a.n_seqs, a.n_rows, a.vocab, a.draft != nullptr);
-    // Many chunks: 32 logits a thread, for fewer instructions a logit (218 + 154 rows of 151936, fp32: 59 -> 53.5 us; 64 logits
-    // 55).  Few are spread further (5 rows 4.4 us, in 32 logits 5.3).
+    // Many chunks: 32 logits a thread, for fewer instructions a logit (218 + 154 rows of 151936, fp32, with weights of degree 8:
+    // 59 -> 53.5 us; 64 logits 55).  Few are spread further (5 rows 4.4 us, in 32 logits 5.3).
     if (wgs >= DV_MANY)
         hipLaunchKernelGGL((k_dv_stats<T, DV_WIDE>), dim3((unsigned)wgs), dim3(DV_WIDE), 0, st, a, w.rec, w.drafted, w.others);
     else if (wgs > 0)
