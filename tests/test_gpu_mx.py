@@ -154,6 +154,20 @@ def test_append_many_sequences():
     run_append("f16", "f16", 64, 1, 1, 16, [(i * 7) % 4 for i in range(200)], [i % 20 for i in range(200)], layers=1, layer=0)
 
 
+@pytest.mark.parametrize("layout", ["half", "interleaved"])
+@pytest.mark.parametrize("act,qact", [("f32", "f16"), ("f32", "f32"), ("bf16", "bf16")])
+@pytest.mark.parametrize("heads,kv,D,T", [(32, 8, 128, 700), (16, 4, 128, 1100), (50, 5, 128, 600), (32, 8, 64, 1100),
+                                          (64, 16, 64, 700), (100, 10, 64, 600)])
+def test_append_long_prompts_of_many_heads(heads, kv, D, T, act, qact, layout):
+    """Prompts and heads enough for two and for three heads a lane, the last workgroup of a token full, partly and all but
+    empty."""
+    run_append(act, qact, D, heads, kv, 64, [T, 3], [100, 9], layout=layout, rot=D if T > 700 else D // 2, layers=1, layer=0,
+               pad=2)
+
+def test_append_many_sequences():
+    run_append("f16", "f16", 64, 1, 1, 16, [(i * 7) % 4 for i in range(200)], [i % 20 for i in range(200)], layers=1, layer=0)
+
+
 @pytest.mark.parametrize("act", ACTS)
 def test_append_sizes_of_values(act):
     """Blocks of zeros, of values below every scale and beyond the largest one, on the borders between two
