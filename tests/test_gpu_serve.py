@@ -356,68 +356,6 @@ def test_verify_draws_next_to_borders(V, at, draft):
                        draft_logits=l if draft else None, temperature=f32(T))
     assert out[0].tolist() == [0] * S and out[1].tolist() == want.tolist()
 
-@pytest.mark.parametrize("draft", [False, True])
-@pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
-def test_verify_of_more_than_4096_parts(act, draft):
-    """Hundreds of rows of several parts each and an odd vocabulary, in the launch of many parts: guesses at the parts' ends
-    that are rejected, that are nearly all of their part or its only weight, greedy rows, masked rows, rows of nothing."""
-    at = [0, 4095, 4096, 8191, 49151, 49152, 50256, 20000]
-    inf = float("inf")
-
-    def change(logits, dl, tokens, ua, un):
-        R = len(tokens)
-        ua[::4] = 1 - 2.0 ** -24
-        for i, r in enumerate(range(0, R - 1, 3)):
-            x = at[i % 8]
-            tokens[r + 1] = x
-            if i % 3 == 1:
-                logits[r, x] = 14.0
-            if i % 5 == 2:
-                logits[r, x // 4096 * 4096:(x // 4096 + 1) * 4096] = -inf
-                logits[r, x] = 9.0
-        for t in (logits,) if dl is None else (logits, dl):
-            t[1::17, ::2] = -inf
-            t[2::23, :8192] = -inf
-            t[4::29, 100:30000] = float("nan")
-            t[7, :] = -inf
-            t[8, 40000] = inf
-    rng = np.random.default_rng(21)
-    rows = rng.integers(1, 9, 80).tolist()
-    assert sum(rows) * 13 >= 4096
-    for T in ("mixed", [0.9] * 80):
-        run_verify(rng, rows, 50257, act, draft, T, change=change, wide=3)
-
-@pytest.mark.parametrize("draft", [False, True])
-def test_verify_more_chunks_than_threads(draft):
-    """A vocabulary of 537 parts."""
-    run_verify(np.random.default_rng(8), [2, 1], 2200003, draft=draft, T=[0.8, 1.0], u=(1 - 2.0 ** -24, 0.75))
-
-
-@pytest.mark.parametrize("V,at", [(2, (0, 1)), (9000, (3, 8200)), (4096, (4000, 4095))])
-@pytest.mark.parametrize("draft", [False, True])
-def test_verify_draws_next_to_borders(V, at, draft):
-    """Two tokens with weight, 1 and w, of which the first ends within 1e-14 to 1e-13 of the random number: fp64's weights
-    (off by a few 1e-16, and 2e-16 times the exponent) decide such a draw as the formula does."""
-    torch = _torch()
-    rng = np.random.default_rng(V)
-    d, T = (rng.uniform(a, b, 20000000).astype(np.float32) for a, b in ((0.1, 3.0), (0.3, 2.0)))
-    ends = 1 / (1 + np.exp(-d.astype(np.float64) / T)) * 2.0 ** 24
-    near = np.abs(ends - np.rint(ends)) < 1.1e-13 * 2 ** 24
-    d, T = d[near], T[near]
-    ends = 1 / (1 + np.exp(-d.astype(np.longdouble) / T.astype(np.longdouble)))
-    u = np.rint(ends * 2 ** 24) / 2 ** 24
-    keep = (np.abs(ends - u) > 1e-14) & (np.abs(ends - u) < 1e-13)
-    d, T, u, want = d[keep], T[keep], u[keep].astype(np.float32), np.where(u < ends, *at)[keep]
-    S = len(d)
-    assert S > 30 and len(set(want.tolist())) == 2
-    logits = torch.full((S, V), -float("inf"))
-    logits[:, at[0]], logits[:, at[1]] = 0.0, torch.tensor(-d)
-    f32 = lambda v: torch.tensor(v, device="cuda")   # noqa: E731
-    out = [torch.full((S,), 77, dtype=torch.int32, device="cuda") for _ in range(2)]
-    l = logits.cuda()
-    paged.draft_verify(ints(list(range(S + 1))), ints([0] * S), l, torch.zeros(S, device="cuda"), f32(u), out[0], out[1],
-                       draft_logits=l if draft else None, temperature=f32(T))
-    assert out[0].tolist() == [0] * S and out[1].tolist() == want.tolist()
 
 @pytest.mark.parametrize("draft", [False, True])
 @pytest.mark.parametrize("act", ["f32", "f16", "bf16"])
@@ -449,11 +387,6 @@ def test_verify_of_more_than_4096_parts(act, draft):
     assert sum(rows) * 13 >= 4096
     for T in ("mixed", [0.9] * 80):
         run_verify(rng, rows, 50257, act, draft, T, change=change, wide=3)
-
-@pytest.mark.parametrize("draft", [False, True])
-def test_verify_more_chunks_than_threads(draft):
-    """A vocabulary of 537 parts."""
-    run_verify(np.random.default_rng(8), [2, 1], 2200003, draft=draft, T=[0.8, 1.0], u=(1 - 2.0 ** -24, 0.75))
 
 
 def test_verify_draft_equal_to_the_target():
