@@ -217,6 +217,33 @@ def test_dequant(page, D, NKV, out):
     assert torch.equal(few[1].cpu().double().nan_to_num(1e30), mx_ref.values(pages[1][0, :2], page, D, True).nan_to_num(1e30))
 
 
+@pytest.mark.parametrize("out", ACTS)
+@pytest.mark.parametrize("page,D,NKV", [(16, 64, 3), (16, 128, 2), (32, 64, 1), (32, 128, 2), (64, 64, 1), (64, 128, 4), (128, 64, 2),
+                                        (256, 64, 1), (256, 128, 2)])
+def test_dequant_of_many_pages(page, D, NKV, out):
+    """Enough rows for several of them a thread; a list of pages with invalid ones, and all pages."""
+    torch = _torch()
+    g = torch.Generator().manual_seed(page + D)
+    n = 32768 // (page * NKV) + 3
+    P = n + 2
+    pages, want = [], []
+    for is_v in (False, True):
+        code = torch.randint(0, 16, (1, P, NKV, page, D), generator=g)
+        scale = torch.randint(104, 142, (1, P, NKV, page, D // 32), generator=g)
+        pages.append(mx_ref.pack(code, torch.where(scale == 141, 255, scale), is_v))
+        want.append(mx_ref.values(pages[-1][0], page, D, is_v).nan_to_num(1e30))
+    c = paged.kv_cache(pages[0].cuda(), pages[1].cuda(), head_dim=D)
+    ids = torch.randint(0, P, (n,), generator=g)
+    ids[5], ids[7], ids[n - 1] = -1, P, 2 ** 31 - 1
+    there = (ids >= 0) & (ids < P)
+    for list_ in (ids, None):
+        o = [torch.full((n, NKV, page, D), 7.0, dtype=TYPES[out], device="cuda") for _ in range(2)]
+        paged.kv_dequant(c, 0, *o, pages=None if list_ is None else ints(ids.tolist()))
+        for t, w in zip(o, want):
+            w = w[:n] if list_ is None else torch.where(there[:, None, None, None], w[torch.where(there, ids, 0)], 0.0)
+            assert torch.equal(t.cpu().double().nan_to_num(1e30), w)
+
+
 # ---- attention ----------------------------------------------------------------------
 def fill_seen(L, P, NKV, page, D, table, kv, g):
     """Pools of 0xFF with random rows at every sequence's positions: bytes, and the values they hold."""

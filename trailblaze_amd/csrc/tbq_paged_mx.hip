@@ -261,21 +261,32 @@ static void mx_dequant(const PgArgs &a, const int *pages, int n, void *k, void *
 
 hipError_t launch_mx_dequant(const PgArgs &a, int D, const int *pages, int n, int out_type, void *k, void *v,
                              hipStream_t st) {
-    // Four rounds a workgroup, their loads in flight together, where there are many rows: 8192 positions of 8 heads of 128
-    // 12.5 -> 9.4 us (8.9 MB in, 33.6 out: 4.5 TB/s).  One round where there are few: 64 positions 2.6-2.9 us, a chain of a
-    // page's number, codes and stores.
-    const bool many = (long long)n * a.NKV << a.shift >= 1 << 15;
-#define TBQ_MD(TO)                                                                                                       \
-    if (D == 128) many ? mx_dequant<TO, 128, 4>(a, pages, n, k, v, st) : mx_dequant<TO, 128, 1>(a, pages, n, k, v, st);  \
-    else many ? mx_dequant<TO, 64, 4>(a, pages, n, k, v, st) : mx_dequant<TO, 64, 1>(a, pages, n, k, v, st)
+    // Up to four rounds a workgroup, their loads in flight together, where there are many rows and a page has as many: fp16,
+    // 8192 positions of 8 heads of 128 in one / two / four: pages of 64 9.2 / 8.0 / 8.2 us (8.9 MB in, 33.6 out: 5.2 TB/s), of
+    // 32 9.05 / 8.1 / 8.7, of 16 9.0 / 9.4 / 10.4; heads of 64, pages of 64 5.8 / 5.7 / 6.0, of 16 6.05 / 6.3 / 6.9, 40000
+    // positions in pages of 256 17.9 in one, 15.5 in four.  One round where there are few: 64 positions 2.6-2.9 us, a chain of
+    // a page's number, codes and stores.
+    const int of_page = (1 << a.shift) / (MD_THREADS / (D / 8));
+    const int rounds = (long long)n * a.NKV << a.shift >= 1 << 15 ? std::min(of_page, 4) : 1;
+#define TBQ_MD_D(TO, D)                                                   \
+    if (rounds == 4) mx_dequant<TO, D, 4>(a, pages, n, k, v, st);         \
+    else if (rounds == 2) mx_dequant<TO, D, 2>(a, pages, n, k, v, st);    \
+    else mx_dequant<TO, D, 1>(a, pages, n, k, v, st)
+#define TBQ_MD(TO)              \
+    if (D == 128) {             \
+        TBQ_MD_D(TO, 128);      \
+    } else {                    \
+        TBQ_MD_D(TO, 64);       \
+    }
     if (out_type == TBQ_KV_F32) {
-        TBQ_MD(float);
+        TBQ_MD(float)
     } else if (out_type == TBQ_KV_F16) {
-        TBQ_MD(pg_f16);
+        TBQ_MD(pg_f16)
     } else {
-        TBQ_MD(pg_bf16);
+        TBQ_MD(pg_bf16)
     }
 #undef TBQ_MD
+#undef TBQ_MD_D
     return hipGetLastError();
 }
 
