@@ -108,3 +108,36 @@ def test_python_cache_refusals():
                             (t, t[:, :1], dict(head_dim=128), "alike"), (t[..., :500], t[..., :500], dict(head_dim=128), "alike")):
         with pytest.raises(ValueError, match=words):
             paged.kv_cache(k, v, **kw)
+
+
+def test_steps_attention_has_its_room_over_mxfp4():
+    """The bound that sets aside the attention's part of a step's workspace, whatever the batch: the call compares it with
+    what the batch's plan writes before it looks at the whole workspace's size."""
+    import random
+    import numpy as np
+    from test_paged_cpu import _dense
+    from trailblaze_amd import formats as fm
+    from trailblaze_amd.dense import DenseModel
+    rng, m = random.Random(7), _dense()
+    ptr = lambda a: a.ctypes.data_as(C.c_void_p)   # noqa: E731
+    for i in range(400):
+        D, G = rng.choice([64, 128]), rng.choice([1, 2, 4, 8])
+        NKV = rng.choice([n for n in (1, 2, 4, 8, 16, 32) if n * G * D % 256 == 0])
+        hidden = 8448 if i % 10 == 0 else 512    # beyond the batched rows: one token after the other
+        mod = DenseModel(2, hidden, NKV * G, NKV, D, 512, 1000, 0, 1e-6, 1e6, fm.Q4_K, fm.Q6_K, FAKE, FAKE, FAKE,
+                         m._layers, None, None)
+        n = 1 if rng.random() < 0.2 else int(2 ** rng.uniform(0, 10))
+        page = rng.choice([16, 64, 256])
+        most = max(1, int(2 ** rng.uniform(0, min(14, 20 - np.log2(n)))))   # pages of a sequence
+        q = min(rng.choice([1, rng.randrange(1, 65), rng.randrange(1, 2 + 6000 // n)]), most * page)
+        n_new = np.array([rng.randrange(1, q + 1) for _ in range(n)], np.int32)
+        kv_len = np.array([rng.randrange(k, most * page + 1) for k in n_new], np.int32)
+        kv_len[0] = most * page
+        table = np.arange(n * most, dtype=np.int32).reshape(n, most)
+        if n * most * NKV * page > 0x7FFFFFFF:
+            continue
+        c = cache(n_pages=n * most, n_kv_heads=NKV, page_size=page, head_dim=D)
+        tokens = np.zeros(int(n_new.sum()), np.int32)
+        ok = tb.lib().tbq_dense_step(C.byref(mod), C.byref(c), n, ptr(n_new), ptr(kv_len), ptr(table), most, ptr(tokens),
+                                     None, rng.choice([0, 100]), 0, FAKE, FAKE, 100, None)
+        refused(ok, "workspace 100 <")

@@ -803,10 +803,15 @@ __global__ __launch_bounds__(PJ_THREADS) void k_pg_join(const PgAttn a, int nrb,
 // ---------------------------------------------------------------------------
 // Host side: the splits, by what the host knows (max_q, max_kv, n_tokens).
 // ---------------------------------------------------------------------------
-static int pg_few(const PgArgs &a, int D, bool f32, int c_type) {
+static int pg_few(const PgArgs &a, int D, int G, bool f32, int c_type) {
     const double positions = (double)a.n_seqs * a.max_kv * a.NKV;   // of kv heads
     const bool mx = c_type == TBQ_KV_MXFP4;
-    if (mx && positions <= (f32 ? PR_SHORT32 : PR_SHORT)) return PR_MOST;
+    if (mx) {
+        const long long rows = (long long)a.max_q * G;
+        if (rows <= PR_MAX) return PR_MOST;
+        if (rows <= PR_MOST && (!f32 || (positions <= PR_SHORT32 && (long long)a.n_seqs * a.NKV < 256))) return PR_MOST;
+        if (rows > PR_MOST && positions <= (f32 ? PR_SHORT32 : PR_SHORT)) return PR_MOST;
+    }
     if (positions * 2 * pg_row_bytes(c_type, D) > 256 << 20) return PR_MAX / 2;
     return mx && !f32 ? PR_MAX + PR_MAX / 2 : PR_MAX;
 }
@@ -814,7 +819,7 @@ static int pg_few(const PgArgs &a, int D, bool f32, int c_type) {
 PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, int c_type) {
     PgPlan p{};
     const int G = NQ / a.NKV, RB = f32 ? 8 : 16, cu = 256;
-    p.few = pg_few(a, D, f32, c_type);
+    p.few = pg_few(a, D, G, f32, c_type);
     p.most = (int)std::min((long long)a.max_q * G, (long long)p.few);
     p.nrb = (p.most + RB - 1) / RB;
     // positions that one block can see
@@ -857,10 +862,12 @@ PgPlan pg_plan(const PgArgs &a, int D, int NQ, int window, int sinks, bool f32, 
     // mixed sequences with a window of 1024 41.3 -> 37.1 us.
     if (p.chunks) tps = std::max(tps, (seen + PC_TS - 1) / PC_TS * 4 / p.chunk_splits);
     tps = std::max((long long)PR_MIN, std::min(longest, (tps + 3) / 4 * 4));
-    // Over 4-bit pages a wave's tile takes 0.6 us, so a short range in one split is done before a join (and its launch)
-    // would be: single tokens, 32 / 8 heads of 128, fp16, in one split / in several, in a graph: 1 sequence after 250
-    // positions 4.9 / 7.2 us, after 750 7.4 / 7.4, after 1000 8.6 / 7.4; 8 after 500 6.4 / 8.3, after 1000 8.8 / 9.4, after
-    // 1500 11.4 / 9.6; 32 after 500 6.9 / 11.2, after 2000 15.4 / 17.3, after 3000 21.6 / 21.9.
+    // Over 4-bit pages a wave's tile takes 0.7 us (heads of 64: 0.55), so a short range in one split is done before a join (and
+    // its launch) would be: single tokens in one split / in several, in a graph, 32 / 8 heads of 128, fp16: 1 sequence after 350
+    // positions 6.8 / 8.5 us, after 750 8.8 / 8.5, after 1000 10.1 / 8.5; 8 after 500 8.1 / 9.8, after 1000 10.7 / 11.1, after
+    // 1500 13.3 / 11.3; 32 after 500 8.1 / 12.7, after 2000 16.9 / 18.9.  fp32: 1 after 500 8.2 / 9.3, after 750 9.8 / 9.3; 8 after
+    // 750 10.0 / 11.2, after 1500 14.0 / 12.1.  16 / 8 heads of 64, fp16: 1 after 500 6.5 / 8.1, after 1000 8.7 / 8.2; 8 after 750
+    // 8.0 / 9.3, after 1500 11.2 / 10.3.
     if (c_type == TBQ_KV_MXFP4 && !p.chunks && tiles <= std::min((long long)PR_LONG, 22 + wgs / 6)) tps = (tiles + 3) / 4 * 4;
     if ((tiles + tps - 1) / tps > PJ_MAX) tps = (tiles + PJ_MAX - 1) / PJ_MAX;
     p.row_tps = (int)tps;

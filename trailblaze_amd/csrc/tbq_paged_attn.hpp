@@ -106,12 +106,19 @@ constexpr int PR_WAVES = 4, PR_TS = 32;
 // 5 over 65536 202 / 172, of 9 over 16384 142 / 156; 17 heads of 64 over 2000 114 / 120;
 // fp32 (four blocks) 32 heads of 64 over 4096 362 / 280, of 9 over 16384 207 / 182.
 constexpr int PR_MAX = 32;
-// Over 4-bit pages the row blocks' bytes are a quarter, so up to PR_MOST rows of a batch of PR_SHORT positions of kv
-// heads (fp32: PR_SHORT32), and half as many again as PR_MAX of 16-bit rows while the last cache holds the batch.  As
-// row blocks / as many rows, fp16, 16 tokens of 4 heads a kv head: 1 sequence after 500 positions 9.5 / 14.3 us, after
-// 4096 12.9 / 19.8, 4 after 4096 20.2 / 28.4, 4 after 32768 84 / 91, 16 after 4096 53 / 52, 32 after 500 17.8 / 30.8; 12
-// tokens, 32 after 4096 74 / 93, 64 after 4096 158 / 160.  fp32, 16 tokens: 1 after 4096 16.0 / 23.9, 4 after 4096 31.6 /
-// 35.6, 32 after 500 35 / 37.5, 64 after 500 60 / 43, 16 after 4096 99 / 75; 12 tokens, 16 after 4096 80 / 75.
+// Over 4-bit pages a row block's codes become halves in registers, where many rows wait for them in LDS.  So where no
+// sequence has more than PR_MOST rows, 16-bit ones are few whatever the batch, and fp32 ones up to PR_MAX, or up to PR_MOST in
+// batches of up to PR_SHORT32 positions of kv heads that, as many rows, would be less than a block a CU.  As row blocks / as
+// many rows, fp16, 32 / 8 heads of 128: 20 rows a kv head, 1 sequence after 300 positions 7.4 / 15.2 us, 64 after 4096 100 /
+// 191, after 32768 708 / 1494, 1000 after 300 163 / 351; 48 rows, 64 after 4096 150 / 198; 64 rows, 32 after 4096 101 / 109,
+// 64 after 300 24.2 / 23.1, after 32768 1274 / 1553; 16 / 8 heads of 64, 64 rows, 64 after 300 18.7 / 19.9, 32 after 4096 75 / 83.
+// fp32, 32 / 8 heads of 128: 20 rows, 64 after 4096 143 / 233; 32 rows, 64 after 4096 188 / 236; 64 rows, 1 after 16384 and 4
+// after 4096 32 / 37, 32 after 300 26.8 / 20.4, 64 after 1000 90 / 67; 16 / 8 heads of 64: 32 rows, 64 after 300 20.9 / 19.1,
+// after 4096 144 / 150, 64 rows, 16 after 1000 22.6 / 26.6, 4 after 16384 73 / 51.
+// Beside longer prompts the blocks that a short sequence does not have are workgroups all the same, so there it is PR_MOST in
+// batches of PR_SHORT positions only (fp32: PR_SHORT32), else half as many again as over 16-bit pages for 16-bit rows: 64
+// single tokens to 8192 beside a prompt of 1000, fp16, up to 16 rows as few 126 us, up to 64 215; 32 x 5 tokens beside one of
+// 500 up to 48 80, up to 64 102.
 constexpr int PR_MOST = 64, PR_SHORT = 1 << 19, PR_SHORT32 = 1 << 17;
 constexpr int PR_MIN = 4, PR_LONG = 64;   // tiles of a split: one a wave at least, 2048 positions at most
 constexpr int PR_MANY = 1024;              // (in batches of up to twice so many workgroups)
