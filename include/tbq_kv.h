@@ -215,8 +215,12 @@ int tbq_kv_pool_defrag(tbq_kv_pool *p, int max, int *src, int *dst);
  * host, on the device: lengths that a kernel produced (tbq_draft_verify's n_drop)
  * become the next batch without a copy to the host.  The free list is device
  * memory: free_pages[0 .. n_free[0] - 1] are pages with no holder, for instance
- * those of a tbq_kv_pool_alloc that the host lends (pages with several holders stay
- * in the host's books).
+ * those of a tbq_kv_pool_alloc that the host lends.  The device counts no holders:
+ * a page that a sequence drops is free, whoever else has it in a table, and is listed
+ * once for each that drops it.  So a sequence whose first pages are shared (a prefix
+ * that tbq_kv_pool_share or tbq_kv_pool_fork gave to several) drops no position of them;
+ * when it ends, the host takes it out of the batch (kv_len 0, n_drop 0) and gives its
+ * shared pages back to the pool, and its own ones to the list.
  * First every sequence s drops its last n_drop[s] positions (NULL: none; at most
  * kv_len[s]): pages behind the last position kept go to the list's end, in the order of
  * sequences and positions (entries that name no page do not).  Then each gets

@@ -129,6 +129,31 @@ def test_tables_of_odd_inputs(place):
         check(16, 64, lens, [2 ** 31 - 1, -2 ** 31] * 6, a, table, free, odd, place=place)
 
 
+@pytest.mark.parametrize("place", ["apart", "in place"])
+def test_tables_of_sequences_that_share_a_prefix(place):
+    """Sequences whose first pages are the same ones drop and add behind them, and one leaves with length and drop 0: the
+    shared pages stay where they are and never come to the list."""
+    rng = np.random.default_rng(8)
+    page, S, own = 16, 5, 4
+    shared = [3, 0, 11]
+    rest = [p for p in rng.permutation(12 + S * own).tolist() if p not in shared]
+    lens = [48 + int(n) for n in rng.integers(1, 50, S)]
+    table = [shared + rest[s * own:(s + 1) * own] + [-1] * 3 for s in range(S)]
+    free, n = rest[S * own:] + [-1] * (12 + S * own - len(rest) + S * own), len(rest) - S * own
+    for s, m in enumerate(lens):
+        table[s][-(-m // page):] = [-1] * (10 - -(-m // page))
+    for step in range(6):
+        drop = [int(rng.integers(0, m - 48 + 1)) if m else 0 for m in lens]
+        new = [int(rng.integers(0, 20)) if m else 0 for m in lens]
+        want = check(page, 200, lens, drop, new, table, free, n, place=place)
+        lens, table, free, n = want["kv_len"], want["table"], want["free"], want["n_free"][0]
+        assert not set(shared) & set(free[:n])
+        if step == 2:
+            lens[1] = 0
+        for s, m in enumerate(lens):
+            assert table[s][:3] == shared or not m
+
+
 def test_tables_without_rows_and_without_sequences():
     torch = _torch()
     rng = np.random.default_rng(6)

@@ -364,7 +364,8 @@ def kv_tables(page_size: int, kv_len, n_new, page_table, free_pages, n_free, *, 
 
 def kv_build_tables(tables: KvTables, stream=None):
     """Pages of dropped positions go back, pages for new ones are taken; the batch's q_start, lengths, page
-    table, slots and positions (tbq_kv_build_tables)."""
+    table, slots and positions (tbq_kv_build_tables).  Pages that several sequences hold (PagePool.share, fork) must
+    not be dropped here: they would be free while the others read them."""
     dev = _here(tables)
     _check(lib().tbq_kv_build_tables(C.byref(tables), _to(stream, dev)), "tbq_kv_build_tables")
 
