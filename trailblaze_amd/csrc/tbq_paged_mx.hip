@@ -295,6 +295,10 @@ hipError_t launch_mx_dequant(const PgArgs &a, int D, const int *pages, int n, in
 // ascending.  A workgroup has one sequence, layer, kv head and K or V (no other
 // touches its rows) and moves MC_ROWS rows a step: all of them have arrived in every
 // wave before any is stored, and no later step loads a row that this one stores.
+// Bound by a step's chain of lookups, loads and stores: in 36 layers, 16000 rows of one sequence to 9001,
+// 4 heads of 128, 321 us (fp16 pages, four times the bytes: 315; the bytes alone 75), 16 x 24 to 9, 8 heads,
+// 17 (14); HBM where sequences are many: 64 x 1000 to 600, 8 heads of 128 903 us (2182), heads of 64 in
+// pages of 16 569 (1169).
 // ---------------------------------------------------------------------------
 constexpr int MC_THREADS = 256, MC_ROWS = 64;
 template <int D>

@@ -6,11 +6,12 @@
 // products take halves that the codes and scales become in registers (few rows) or
 // on their way to LDS (many rows); the values are halves exactly, so this rounds
 // nothing.  16-bit rows of q: fp16 as they are, bf16 scaled by a power of two into
-// fp16's range (a row with elements that a half then cannot hold, below 2^-31 of its largest
-// one, is formed alone, from q as it is); fp32 rows as two halves each.  Probabilities are two halves each for every type (2^-22 of one, or 2^-39 of
-// the largest, is lost), so a 16-bit row is rounded once, at the output.  As one half
-// they would add 17% (few rows, fp16, 64 sequences of up to 8192) and 29% (2048 tokens
-// after 8192) to the output's own rounding, 2.1e-4 against 64 bits.
+// fp16's range (a row with elements that a half then cannot hold, below 2^-31 of its
+// largest one, is formed alone, from q as it is); fp32 rows as two halves each.
+// Probabilities are two halves each for every type (2^-22 of one, or 2^-39 of the
+// largest, is lost), so a 16-bit row is rounded once, at the output.  As one half they
+// would add 17% (few rows, fp16, 64 sequences of up to 8192) and 29% (2048 tokens after
+// 8192) to the output's own rounding, 2.1e-4 against 64 bits.
 #include <algorithm>
 #include <type_traits>
 
@@ -118,13 +119,13 @@ __device__ __forceinline__ bool mx_load_q(const TA *q, Spread spread, mx_h8 (&hi
 // registers.
 //
 // Bound by HBM where there are many positions: 64 ragged sequences to 8192, 32 / 8 heads
-// of 128, fp16 rows 60 us, 5.3 TB/s.  What that took (a first form: 81):
+// of 128, fp16 rows 62-64 us, 5.0 TB/s.  What that took (a first form: 81):
 //   codes of one row block loaded past the caches: 73 -> 67.5;
 //   loads without a condition, so that a whole tile stays in flight, and three waves a SIMD.
 // The lo halves' product (fp32 rows': columns of the same one) takes 2 to 5%, up to 11% with
 // heads of 64: 64 sequences of 4096 62-65 -> 64-68, of 8192 107 -> 111, of 4096 with 16 / 8 heads of
 // 64 44 -> 49 us.
-// One sequence of 131072: 16 us (4.5 TB/s), of 4096: 6, a chain of page, codes, products and
+// One sequence of 131072: 18 us (4.0 TB/s), of 4096: 6, a chain of page, codes, products and
 // the workgroup's own join.
 // ---------------------------------------------------------------------------
 template <int D>
@@ -160,8 +161,9 @@ __device__ __forceinline__ void mx_rows(const PgAttn &a, int nrb, int tps, int n
     uint64_t lost;   // of the lanes' rows
     {
         mx_h8 lo[NS];
-        lost = __builtin_amdgcn_ballot_w64(mx_load_q((const TA *)a.q + (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + D / 4 * h,
-                  [](float v) { return swap32_max(swap16_max(v)); }, qf, lo, &cs));
+        const TA *q = (const TA *)a.q + (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + D / 4 * h;
+        lost = __builtin_amdgcn_ballot_w64(
+            mx_load_q(q, [](float v) { return swap32_max(swap16_max(v)); }, qf, lo, &cs));
         if constexpr (HL) {
 #pragma unroll
             for (int i = 0; i < NS; i++)
@@ -352,14 +354,17 @@ __global__ __launch_bounds__(64 * PR_WAVES) __attribute__((amdgpu_waves_per_eu(3
 // come to registers two tiles ahead and to LDS as halves one tile ahead, each wave
 // those of one 16-position block.
 //
-// 2048 tokens after 8192, 32 / 8 heads of 128, fp16: 335-353 us, 0.9 PFLOP/s, where power
-// bounds it, as over fp16 pages (337); shorter chunks take 3-10% longer than over those,
-// for the codes' conversions.  Nine mixed sequences under a window of 1024 + 4, heads of 64,
-// bf16: 39, about 19 tiles one after the other in 304 workgroups on 256 CUs.  Not kept for
-// it: three waves a SIMD, codes two tiles ahead in two sets of registers, all of a tile's LDS reads
-// ahead of its products (no change each), the positions in two ranges (32, and 9.5 the join), two
-// groups of four waves that share a block's tiles and add at the end (44, with registers spilled;
-// heads of 128, where none are: 2048 tokens after none 66 -> 60, but 512 after 4096 64 -> 72).
+// 2048 tokens after 8192, 32 / 8 heads of 128: 16-bit rows 445-471 us over several cards (0.67 PFLOP/s
+// of the attention's, 1.0 with the lo halves' product), fp32 ones, a product of q more, 573; over fp16
+// pages 348 and 572.  Matrix units busy for 45% of the cycles, vector units (softmax, halves, the
+// codes' conversions) for 53%, at 1.97 GHz: two waves a SIMD overlap little of the two.  With the
+// probabilities as one half 348-391, 38% and 47% at 2.07 GHz; 512 after 4096 64 -> 76.  Nine mixed sequences under a
+// window of 1024 + 4, heads of 64, bf16: 47-49 (one half: 39), about 19 tiles one after the other in 304
+// workgroups on 256 CUs.  Not kept for it, measured with one half: three waves a SIMD, codes two tiles
+// ahead in two sets of registers, all of a tile's LDS reads ahead of its products (no change each), the
+// positions in two ranges (32, and 9.5 the join), two groups of four waves that share a block's tiles
+// and add at the end (44, with registers spilled; heads of 128, where none are: 2048 tokens after none
+// 66 -> 60, but 512 after 4096 64 -> 72).
 // ---------------------------------------------------------------------------
 template <int D>
 struct McLds {
@@ -394,8 +399,8 @@ __device__ __forceinline__ void mx_chunk(const PgAttn &a, int nsplit, float *__r
     uint64_t lost;   // of the lanes' rows
     {
         mx_h8 lo[NS];
-        lost = __builtin_amdgcn_ballot_w64(mx_load_q((const TA *)a.q + (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * NS * h,
-                  [](float v) { return swap32_max(v); }, qf[0], lo, &cs));
+        const TA *q = (const TA *)a.q + (long long)(q0 + tok) * a.qs + (long long)(kvh * G + rc % G) * D + 8 * NS * h;
+        lost = __builtin_amdgcn_ballot_w64(mx_load_q(q, [](float v) { return swap32_max(v); }, qf[0], lo, &cs));
         if constexpr (HL) {
 #pragma unroll
             for (int i = 0; i < NS; i++) qf[NP - 1][i] = lo[i];
